@@ -15,6 +15,7 @@ checked by the C library.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 
 import torch  # imported first: its HIP runtime is the one libops3d_fda.so binds to
@@ -58,6 +59,10 @@ EXPORTED_SYMBOLS = (
     "ops3d_roi_align3d_channels_last_supported",
     "ops3d_roi_align3d_forward_channels_last",
     "ops3d_roi_align3d_to_channels_last",
+    "ops3d_linear_forward_workspace_bytes",
+    "ops3d_linear_forward",
+    "ops3d_linear_backward_workspace_bytes",
+    "ops3d_linear_backward",
     "ops3d_fda_profile_enable",
     "ops3d_fda_profile_read",
 )
@@ -122,6 +127,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ops3d_roi_align3d_forward_channels_last.argtypes = [_vp] * 3 + [_i] * 10 + [ctypes.c_float, _i, _i, _vp]
     lib.ops3d_roi_align3d_to_channels_last.restype = _i
     lib.ops3d_roi_align3d_to_channels_last.argtypes = [_vp] * 2 + [_i] * 6 + [_vp]
+    lib.ops3d_linear_forward_workspace_bytes.restype = _sz
+    lib.ops3d_linear_forward_workspace_bytes.argtypes = [_i, _i, _i64, _i, _i, _i, _i]
+    lib.ops3d_linear_forward.restype = _i
+    lib.ops3d_linear_forward.argtypes = ([_vp, _i64, _vp, _vp, _vp, _i64, _vp, _i, _vp, _vp, _vp, _sz]
+                                         + [_i] * 3 + [_i64] + [_i] * 3 + [_vp])
+    lib.ops3d_linear_backward_workspace_bytes.restype = _sz
+    lib.ops3d_linear_backward_workspace_bytes.argtypes = [_i, _i, _i64, _i, _i, _i, _i]
+    lib.ops3d_linear_backward.restype = _i
+    lib.ops3d_linear_backward.argtypes = ([_vp, _i64, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz]
+                                          + [_i] * 2 + [_i64] + [_i] * 3 + [_vp])
     lib.ops3d_fda_backward_offsets.argtypes = [_vp] * 6 + [_i] + [_vp] * 5 + [_sz] + [_i] * 9 + [_vp]
 
 
@@ -148,7 +163,8 @@ class _NativeFDA:
             for name in ("flash_deform_attn_forward", "flash_deform_attn_backward",
                          "forward_keep_head_major", "backward_with_head_major",
                          "forward_offsets", "backward_offsets", "nms_3d", "roi_align_3d_forward",
-                         "roi_align_3d_backward", "dcnv4_forward", "dcnv4_backward"):
+                         "roi_align_3d_backward", "dcnv4_forward", "dcnv4_backward", "linear_forward",
+                         "linear_backward"):
                 setattr(self, name, getattr(ext, name))
 
     # -- helpers ---------------------------------------------------------------------------
@@ -207,6 +223,139 @@ class _NativeFDA:
             )
         Q = sampling_loc_attn.shape[1]
         return B, S, G, D, L, Q
+
+    # -- linear operators (include/ops3d_linear.h) --------------------------------------------
+    @staticmethod
+    def _linear_check(name: str, t: torch.Tensor, x: torch.Tensor) -> None:
+        if not t.is_cuda:
+            raise RuntimeError(f"Not implemented on the CPU ({name} is on the CPU)")
+        if t.layout != torch.strided:
+            raise ValueError(f"{name} must be a dense tensor")
+        if t.device != x.device:
+            raise RuntimeError(f"{name} is on another device than x")
+        if t.dtype != x.dtype:
+            raise ValueError(f"{name} dtype differs from x dtype")
+
+    @staticmethod
+    def _as_rows(t: torch.Tensor):
+        """t as rows of its last axis and their distance in elements; a copy where it is not."""
+        t = t.resolve_neg()
+        n = t.shape[-1]
+        step, count, rows = None, 1, t.stride(-1) == 1 or n == 1
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if step is None:
+                step = stride
+            elif stride != step * count:
+                rows = False
+            count *= size
+        return (t, n if step is None else step) if rows else (t.contiguous(), n)
+
+    @staticmethod
+    def _linear_sizes(rows: torch.Tensor, group_start, groups: int):
+        """(batch, rows per item, groups, group_start, entries)."""
+        if rows.dtype not in _DTYPE_CODE:
+            raise ValueError(f"unsupported value dtype {rows.dtype}")
+        if group_start is None:
+            return 1, math.prod(rows.shape[:-1]), 1, None, 0
+        if not group_start.is_cuda:
+            raise RuntimeError("Not implemented on the CPU (group_start is on the CPU)")
+        if group_start.device != rows.device:
+            raise RuntimeError("group_start is on another device than x")
+        if group_start.dtype != torch.int64 or group_start.dim() != 1 or not group_start.is_contiguous():
+            raise ValueError("group_start must be a contiguous int64 tensor of one axis")
+        count = group_start.shape[0]
+        if count not in (groups, groups + 1):
+            raise ValueError(f"group_start must have {groups} or {groups + 1} entries, got {count}")
+        return rows.shape[0] if rows.dim() == 3 else 1, rows.shape[-2], groups, group_start, count
+
+    def linear_forward(self, x, weight, bias, residual, group_start, act, keep):
+        """(y, act_grad); act_grad (None without an activation) when ``keep``."""
+        self._linear_check("x", x, x)
+        self._linear_check("weight", weight, x)
+        grouped = group_start is not None
+        if weight.dim() != (3 if grouped else 2):
+            raise ValueError("weight must be [groups, out_features, in_features]" if grouped
+                             else "weight must be [out_features, in_features]")
+        N, K = weight.shape[-2:]
+        if x.dim() not in (2, 3) if grouped else x.dim() < 1:
+            raise ValueError("x must be [rows, in_features] or [batch, rows, in_features]")
+        if x.shape[-1] != K:
+            raise ValueError(f"x has {x.shape[-1]} features, weight {K}")
+        if bias is not None:
+            self._linear_check("bias", bias, x)
+            if bias.shape != weight.shape[:-1]:
+                raise ValueError("bias must be [groups, out_features]" if grouped else "bias must be [out_features]")
+        shape = (*x.shape[:-1], N)
+        if residual is not None:
+            self._linear_check("residual", residual, x)
+            if residual.shape != shape:
+                raise ValueError("residual must have the output's shape")
+        B, S, E, start, count = self._linear_sizes(x, group_start, weight.shape[0])
+        xr, ldx = self._as_rows(x)
+        r, ldr = (None, 0) if residual is None else self._as_rows(residual)
+        w = weight.resolve_neg().contiguous()
+        b = None if bias is None else bias.resolve_neg().contiguous()
+        y = torch.empty(shape, dtype=x.dtype, device=x.device)
+        act_grad = None
+        if keep and act:
+            act_grad = torch.empty(shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16,
+                                   device=x.device)
+        code = _DTYPE_CODE[x.dtype]
+        n = self._lib.ops3d_linear_forward_workspace_bytes(code, B, S, E, N, K, int(grouped))
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        with torch.cuda.device(x.device):
+            rc = self._lib.ops3d_linear_forward(
+                _ptr(xr), ldx, _ptr(w), _ptr(b), _ptr(r), ldr, _ptr(start), count, _ptr(y), _ptr(act_grad), _ptr(ws), n,
+                code, int(act), B, S, E, N, K, torch.cuda.current_stream(x.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "linear_forward failed")
+        return y, act_grad
+
+    def linear_backward(self, x, weight, group_start, act_grad, grad_y, in_features, groups, need_w, need_b):
+        """(grad_x when weight is given, grad_weight, grad_bias), None where not wanted."""
+        self._linear_check("grad_output", grad_y, grad_y)
+        grouped = group_start is not None
+        if grad_y.dim() not in (2, 3) if grouped else grad_y.dim() < 1:
+            raise ValueError("grad_output must be [rows, out_features] or [batch, rows, out_features]")
+        N, K = grad_y.shape[-1], in_features
+        shape = (*grad_y.shape[:-1], K)
+        if (need_w or need_b) and x is None:
+            raise ValueError("x is needed for the gradients of weight and bias")
+        if x is not None:
+            self._linear_check("x", x, grad_y)
+            if x.shape != shape:
+                raise ValueError("x and grad_output differ in their rows")
+        wshape = (groups, N, K) if grouped else (N, K)
+        if weight is not None:
+            self._linear_check("weight", weight, grad_y)
+            if weight.shape != wshape:
+                raise ValueError("weight does not fit grad_output")
+        want = torch.float32 if grad_y.dtype == torch.float32 else torch.int16
+        if act_grad is not None and (act_grad.device != grad_y.device or not act_grad.is_contiguous()
+                                     or act_grad.shape != grad_y.shape or act_grad.dtype != want):
+            raise ValueError("act_grad is not a forward's of this shape")
+        B, S, E, start, count = self._linear_sizes(grad_y, group_start, groups)
+        g, ldg = self._as_rows(grad_y)
+        xr, ldx = (None, 0) if x is None else self._as_rows(x)
+        w = None if weight is None else weight.resolve_neg().contiguous()
+
+        def empty(want, sizes):
+            return torch.empty(sizes, dtype=grad_y.dtype, device=grad_y.device) if want else None
+
+        gx, gw, gb = empty(weight is not None, shape), empty(need_w, wshape), empty(need_b, wshape[:-1])
+        code = _DTYPE_CODE[grad_y.dtype]
+        n = (self._lib.ops3d_linear_backward_workspace_bytes(code, B, S, E, N, K, int(grouped))
+             if need_w or need_b else 0)
+        ws = torch.empty(n, dtype=torch.uint8, device=grad_y.device) if n else None
+        with torch.cuda.device(grad_y.device):
+            rc = self._lib.ops3d_linear_backward(
+                _ptr(xr), ldx, _ptr(w), _ptr(start), count, _ptr(act_grad), _ptr(g), ldg, _ptr(gx), _ptr(gw), _ptr(gb),
+                _ptr(ws), n, code, B, S, E, N, K, torch.cuda.current_stream(grad_y.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "linear_backward failed")
+        return gx, gw, gb
 
     # -- entry points (reference csrc/flash_deform_attn.h) -----------------------------------
     def flash_deform_attn_forward(

@@ -482,6 +482,14 @@ void *scratch_address() {
 }
 }  // namespace
 
+namespace ops3d_fda {
+// the other files' entry points report through the same ops3d_fda_last_error
+int set_last_error(int code, const char *text) {
+  g_last_error = text;
+  return code;
+}
+}  // namespace ops3d_fda
+
 extern "C" {
 
 int ops3d_fda_abi_version(void) { return 7; }

@@ -1,0 +1,10 @@
+// Linear operators: kernel instantiations for element type __bf16.
+#include "linear_kernels.h"
+
+namespace ops3d_linear {
+
+template hipError_t forward<__bf16>(const RowsArgs &, hipStream_t);
+template hipError_t grad_x<__bf16>(const RowsArgs &, hipStream_t);
+template hipError_t grad_weight<__bf16>(const WeightArgs &, bool, hipStream_t);
+
+}  // namespace ops3d_linear

@@ -1,0 +1,192 @@
+// C entry points of the linear operators (include/ops3d_linear.h).
+#include "linear_kernels.h"
+
+#include <stdarg.h>
+#include <stdio.h>
+
+#include "../../include/ops3d_linear.h"
+
+namespace ops3d_fda {
+int set_last_error(int code, const char *text);   // fda_capi.hip
+}
+
+namespace {
+
+using namespace ops3d_linear;
+
+int fail(int code, const char *fmt, ...) {
+  char buf[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return ops3d_fda::set_last_error(code, buf);
+}
+
+int elem_size(int dtype) {
+  return dtype == OPS3D_FDA_F32 ? 4 : dtype == OPS3D_FDA_F16 || dtype == OPS3D_FDA_BF16 ? 2 : 0;
+}
+
+constexpr int64_t kMaxRows = 0x7fffffff - 4096;   // rows of all items and tile counts stay 32-bit
+constexpr int kMaxFeatures = 1 << 24;
+
+int check_sizes(int dtype, int batch, int64_t rows, int groups, int out_features, int in_features) {
+  if (elem_size(dtype) == 0) return fail(OPS3D_FDA_EINVAL, "unsupported dtype code %d", dtype);
+  if (batch < 0 || rows < 0 || (batch > 0 && rows > kMaxRows / batch))
+    return fail(OPS3D_FDA_EINVAL, "invalid or too many rows: %d items of %lld", batch, (long long)rows);
+  if (out_features < 1 || in_features < 1 || out_features > kMaxFeatures || in_features > kMaxFeatures)
+    return fail(OPS3D_FDA_EINVAL, "out_features and in_features must be in 1..%d, got %d and %d", kMaxFeatures, out_features,
+                in_features);
+  if (groups < 1 || groups > OPS3D_LINEAR_MAX_GROUPS)
+    return fail(OPS3D_FDA_EINVAL, "groups must be in 1..%d, got %d", OPS3D_LINEAR_MAX_GROUPS, groups);
+  // every segment may end inside a tile of 16 rows or a chunk
+  if ((int64_t)batch * (groups + 2) + (int64_t)batch * rows / 16 > kMaxRows)
+    return fail(OPS3D_FDA_EINVAL, "too many groups for %d items", batch);
+  return OPS3D_FDA_OK;
+}
+
+int make_groups(const int64_t *start, int count, int batch, int64_t rows, int groups, Groups &g) {
+  if (!start) {
+    if (groups != 1) return fail(OPS3D_FDA_EINVAL, "group_start is NULL but there are %d groups", groups);
+    g = Groups{nullptr, 0, 1, 1, (int)(batch * rows)};
+    return OPS3D_FDA_OK;
+  }
+  if (count != groups && count != groups + 1)
+    return fail(OPS3D_FDA_EINVAL, "group_start must have groups or groups + 1 entries (%d), got %d", groups, count);
+  if (reinterpret_cast<uintptr_t>(start) & 7u) return fail(OPS3D_FDA_EINVAL, "group_start must be 8-byte aligned");
+  g = Groups{start, count, groups, batch, (int)rows};
+  return OPS3D_FDA_OK;
+}
+
+// The plan of the weights' gradients; batch and rows as the caller gave them.
+ChunkPlan plan_of(int dtype, bool grouped, int batch, int64_t rows, int groups, int N, int K) {
+  return grouped ? ChunkPlan(elem_size(dtype), true, batch, rows, groups, N, K)
+                 : ChunkPlan(elem_size(dtype), false, 1, batch * rows, 1, N, K);
+}
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+template <typename F> int run(int dtype, const char *what, F f) {
+  hipError_t e = dtype == OPS3D_FDA_F32 ? f(float()) : dtype == OPS3D_FDA_F16 ? f(_Float16()) : f(__bf16());
+  if (e == hipSuccess) return OPS3D_FDA_OK;
+  return fail(OPS3D_FDA_ERUNTIME, "%s: kernel launch failed: %s", what, hipGetErrorString(e));
+}
+
+bool misaligned(const void *p, int esize) { return reinterpret_cast<uintptr_t>(p) & (uintptr_t)(esize - 1); }
+
+}  // namespace
+
+extern "C" {
+
+size_t ops3d_linear_forward_workspace_bytes(int, int, int64_t, int, int, int, int) { return 0; }
+
+int ops3d_linear_forward(const void *x, int64_t ld_x, const void *weight, const void *bias, const void *residual,
+                         int64_t ld_residual, const int64_t *group_start, int group_start_count, void *y, void *act_grad,
+                         void *, size_t, int dtype, int act, int batch, int64_t rows, int groups, int out_features,
+                         int in_features, void *stream) {
+  ops3d_fda::set_last_error(OPS3D_FDA_OK, "");
+  int rc = check_sizes(dtype, batch, rows, groups, out_features, in_features);
+  if (rc) return rc;
+  if (act < OPS3D_LINEAR_ACT_NONE || act > OPS3D_LINEAR_ACT_SILU) return fail(OPS3D_FDA_EINVAL, "unknown activation %d", act);
+  if (act_grad && act == OPS3D_LINEAR_ACT_NONE)
+    return fail(OPS3D_FDA_EINVAL, "act_grad must be NULL without an activation");
+  if (ld_x < 0 || (residual && ld_residual < 0)) return fail(OPS3D_FDA_EINVAL, "row distances must not be negative");
+  if (batch * rows == 0) return OPS3D_FDA_OK;
+  RowsArgs p{};
+  if ((rc = make_groups(group_start, group_start_count, batch, rows, groups, p.g))) return rc;
+  if (!x || !weight || !y) return fail(OPS3D_FDA_EINVAL, "NULL pointer argument");
+  const int es = elem_size(dtype);
+  if (misaligned(x, es) || misaligned(weight, es) || misaligned(y, es) || misaligned(bias, es) || misaligned(residual, es) ||
+      misaligned(act_grad, es))
+    return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
+  p.a = x;
+  p.lda = ld_x;
+  p.w = weight;
+  p.w_group = (int64_t)out_features * in_features;
+  p.bias = bias;
+  p.res = residual;
+  p.ld_res = ld_residual;
+  p.c = y;
+  p.act_grad = act_grad;
+  p.act = act;
+  p.N = out_features;
+  p.K = in_features;
+  return run(dtype, "linear forward", [&](auto t) { return forward<decltype(t)>(p, static_cast<hipStream_t>(stream)); });
+}
+
+size_t ops3d_linear_backward_workspace_bytes(int dtype, int batch, int64_t rows, int groups, int out_features,
+                                             int in_features, int grouped) {
+  if (elem_size(dtype) == 0 || batch < 1 || rows < 1 || rows > kMaxRows / batch || groups < 1 ||
+      groups > OPS3D_LINEAR_MAX_GROUPS || out_features < 1 || in_features < 1 || out_features > kMaxFeatures ||
+      in_features > kMaxFeatures || (!grouped && groups != 1))
+    return 0;
+  const ChunkPlan c = plan_of(dtype, grouped != 0, batch, rows, groups, out_features, in_features);
+  if (!c.joined) return 0;
+  return align256((size_t)c.slots * out_features * in_features * 4) + align256((size_t)c.slots * out_features * 4);
+}
+
+int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const int64_t *group_start,
+                          int group_start_count, const void *act_grad, const void *grad_y, int64_t ld_grad_y,
+                          void *grad_x, void *grad_weight_out, void *grad_bias, void *workspace, size_t workspace_bytes,
+                          int dtype, int batch, int64_t rows, int groups, int out_features, int in_features,
+                          void *stream) {
+  ops3d_fda::set_last_error(OPS3D_FDA_OK, "");
+  int rc = check_sizes(dtype, batch, rows, groups, out_features, in_features);
+  if (rc) return rc;
+  if (ld_x < 0 || ld_grad_y < 0) return fail(OPS3D_FDA_EINVAL, "row distances must not be negative");
+  const bool wants_w = grad_weight_out || grad_bias, empty = batch * rows == 0;
+  Groups g{};
+  if ((rc = make_groups(group_start, group_start_count, batch, rows, groups, g))) return rc;
+  if (!empty && (!grad_y || (grad_x && !weight) || (wants_w && !x))) return fail(OPS3D_FDA_EINVAL, "NULL pointer argument");
+  const int es = elem_size(dtype);
+  if (misaligned(x, es) || misaligned(weight, es) || misaligned(act_grad, es) || misaligned(grad_y, es) ||
+      misaligned(grad_x, es) || misaligned(grad_weight_out, es) || misaligned(grad_bias, es))
+    return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (wants_w) {
+    const ChunkPlan c = plan_of(dtype, group_start != nullptr, batch, empty ? 0 : rows, groups, out_features, in_features);
+    const size_t need = empty ? 0
+                              : ops3d_linear_backward_workspace_bytes(dtype, batch, rows, groups, out_features,
+                                                                      in_features, group_start != nullptr);
+    if (need && (!workspace || workspace_bytes < need))
+      return fail(OPS3D_FDA_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
+    if (need && (reinterpret_cast<uintptr_t>(workspace) & 255u))
+      return fail(OPS3D_FDA_EINVAL, "workspace must be 256-byte aligned");
+    WeightArgs p{};
+    p.u = grad_y;
+    p.ldu = ld_grad_y;
+    p.scale = act_grad;
+    p.x = x;
+    p.ldx = ld_x;
+    p.gw = grad_weight_out;
+    p.gb = grad_bias;
+    p.N = out_features;
+    p.K = in_features;
+    p.chunk = c.chunk;
+    p.slots = empty ? 0 : (int)c.slots;
+    if (need) {
+      p.part = static_cast<float *>(workspace);
+      p.part_b = reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                           align256((size_t)c.slots * out_features * in_features * 4));
+    }
+    p.g = g;
+    rc = run(dtype, "linear weight gradient", [&](auto t) { return ops3d_linear::grad_weight<decltype(t)>(p, need != 0, st); });
+    if (rc) return rc;
+  }
+  if (grad_x && !empty) {
+    RowsArgs p{};
+    p.a = grad_y;
+    p.lda = ld_grad_y;
+    p.scale = act_grad;
+    p.w = weight;
+    p.w_group = (int64_t)out_features * in_features;
+    p.c = grad_x;
+    p.N = in_features;
+    p.K = out_features;
+    p.g = g;
+    rc = run(dtype, "linear input gradient", [&](auto t) { return ops3d_linear::grad_x<decltype(t)>(p, st); });
+  }
+  return rc;
+}
+
+}  // extern "C"

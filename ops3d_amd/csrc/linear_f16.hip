@@ -1,0 +1,10 @@
+// Linear operators: kernel instantiations for element type _Float16.
+#include "linear_kernels.h"
+
+namespace ops3d_linear {
+
+template hipError_t forward<_Float16>(const RowsArgs &, hipStream_t);
+template hipError_t grad_x<_Float16>(const RowsArgs &, hipStream_t);
+template hipError_t grad_weight<_Float16>(const WeightArgs &, bool, hipStream_t);
+
+}  // namespace ops3d_linear

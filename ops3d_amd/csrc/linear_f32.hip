@@ -1,0 +1,10 @@
+// Linear operators: kernel instantiations for element type float.
+#include "linear_kernels.h"
+
+namespace ops3d_linear {
+
+template hipError_t forward<float>(const RowsArgs &, hipStream_t);
+template hipError_t grad_x<float>(const RowsArgs &, hipStream_t);
+template hipError_t grad_weight<float>(const WeightArgs &, bool, hipStream_t);
+
+}  // namespace ops3d_linear

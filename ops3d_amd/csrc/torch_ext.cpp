@@ -17,9 +17,11 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/ops3d_fda.h"
 #include "../../include/ops3d_dcnv4.h"
+#include "../../include/ops3d_linear.h"
 #include "../../include/ops3d_nms3d.h"
 #include "../../include/ops3d_roi_align3d.h"
 
@@ -456,6 +458,172 @@ std::vector<at::Tensor> dcnv4_backward(const at::Tensor &value, const at::Tensor
   return {grad_value, grad_offset};
 }
 
+// Linear operators (include/ops3d_linear.h).  Tensors may have any row distance; what cannot be seen
+// as rows of consecutive elements is copied.
+const at::Tensor &linear_check(const at::Tensor &t, const char *name, const at::Tensor &x) {
+  if (!t.is_cuda()) throw std::runtime_error(std::string("Not implemented on the CPU (") + name + " is on the CPU)");
+  if (t.layout() != at::kStrided) throw std::invalid_argument(std::string(name) + " must be a dense tensor");
+  if (t.device() != x.device()) throw std::runtime_error(std::string(name) + " is on another device than x");
+  if (t.scalar_type() != x.scalar_type())
+    throw std::invalid_argument(std::string(name) + " dtype differs from x dtype");
+  return t;
+}
+
+// t as rows of its last axis, `ld` elements apart; a copy where it is not.
+at::Tensor as_rows(const at::Tensor &t_, int64_t &ld) {
+  at::Tensor t = t_.is_neg() ? t_.resolve_neg() : t_;
+  const int64_t d = t.dim(), n = t.size(d - 1);
+  bool rows = t.stride(d - 1) == 1 || n == 1;
+  int64_t step = -1, count = 1;   // of the axes seen so far, from the last but one outwards
+  for (int64_t i = d - 2; i >= 0 && rows; --i) {
+    if (t.size(i) == 1) continue;
+    if (step < 0) step = t.stride(i);
+    else rows = t.stride(i) == step * count;
+    count *= t.size(i);
+  }
+  if (!rows) {
+    ld = n;
+    return t.contiguous();
+  }
+  ld = step < 0 ? n : step;
+  return t;
+}
+
+at::Tensor dense(const at::Tensor &t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+
+struct LinearSizes {
+  int code, batch, groups, N, K;
+  int64_t rows;
+  const int64_t *start;
+  int count;
+};
+
+int linear_int(int64_t v, const char *what) {
+  if (v < 0 || v > 0x7fffffff) throw std::invalid_argument(std::string(what) + " is too large");
+  return (int)v;
+}
+
+// rows: x or grad_y, whose last axis is not looked at; groups 0: one weight.
+LinearSizes linear_sizes(const at::Tensor &rows, const c10::optional<at::Tensor> &group_start, int64_t groups, int64_t N,
+                         int64_t K) {
+  LinearSizes z{};
+  z.code = dtype_code(rows);
+  z.N = linear_int(N, "out_features");
+  z.K = linear_int(K, "in_features");
+  if (!group_start) {
+    int64_t n = 1;
+    for (int64_t i = 0; i + 1 < rows.dim(); ++i) n *= rows.size(i);
+    z.batch = z.groups = 1;
+    z.rows = n;
+    return z;
+  }
+  const at::Tensor &g = *group_start;
+  if (!g.is_cuda()) throw std::runtime_error("Not implemented on the CPU (group_start is on the CPU)");
+  if (g.device() != rows.device()) throw std::runtime_error("group_start is on another device than x");
+  if (g.scalar_type() != at::kLong || g.dim() != 1 || !g.is_contiguous())
+    throw std::invalid_argument("group_start must be a contiguous int64 tensor of one axis");
+  z.groups = linear_int(groups, "the number of groups");
+  if (g.size(0) != groups && g.size(0) != groups + 1)
+    throw std::invalid_argument("group_start must have " + std::to_string(groups) + " or " + std::to_string(groups + 1) +
+                                " entries, got " + std::to_string(g.size(0)));
+  z.count = (int)g.size(0);
+  z.start = g.data_ptr<int64_t>();
+  z.batch = rows.dim() == 3 ? linear_int(rows.size(0), "the batch") : 1;
+  z.rows = rows.size(rows.dim() - 2);
+  return z;
+}
+
+// [y, act_grad]; act_grad (None without an activation) when keep.
+std::tuple<at::Tensor, c10::optional<at::Tensor>> linear_forward(
+    const at::Tensor &x, const at::Tensor &weight, const c10::optional<at::Tensor> &bias,
+    const c10::optional<at::Tensor> &residual, const c10::optional<at::Tensor> &group_start, int64_t act, bool keep) {
+  linear_check(x, "x", x);
+  linear_check(weight, "weight", x);
+  const bool grouped = group_start.has_value();
+  if (grouped ? weight.dim() != 3 : weight.dim() != 2)
+    throw std::invalid_argument(grouped ? "weight must be [groups, out_features, in_features]"
+                                        : "weight must be [out_features, in_features]");
+  const int64_t N = weight.size(-2), K = weight.size(-1);
+  if (grouped ? x.dim() != 2 && x.dim() != 3 : x.dim() < 1)
+    throw std::invalid_argument("x must be [rows, in_features] or [batch, rows, in_features]");
+  if (x.size(-1) != K)
+    throw std::invalid_argument("x has " + std::to_string(x.size(-1)) + " features, weight " + std::to_string(K));
+  if (bias) {
+    linear_check(*bias, "bias", x);
+    if (grouped ? bias->dim() != 2 || bias->size(0) != weight.size(0) || bias->size(1) != N
+                : bias->dim() != 1 || bias->size(0) != N)
+      throw std::invalid_argument(grouped ? "bias must be [groups, out_features]" : "bias must be [out_features]");
+  }
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  if (residual) {
+    linear_check(*residual, "residual", x);
+    if (residual->sizes().vec() != shape) throw std::invalid_argument("residual must have the output's shape");
+  }
+  const LinearSizes z = linear_sizes(x, group_start, grouped ? weight.size(0) : 0, N, K);
+  const DeviceGuard guard(x.device());
+  int64_t ldx = 0, ldr = 0;
+  const at::Tensor xr = as_rows(x, ldx), w = dense(weight);
+  const at::Tensor b = bias ? dense(*bias) : at::Tensor(), r = residual ? as_rows(*residual, ldr) : at::Tensor();
+  at::Tensor y = at::empty(shape, x.options());
+  c10::optional<at::Tensor> act_grad;
+  if (keep && act != OPS3D_LINEAR_ACT_NONE)
+    act_grad = at::empty(shape, x.scalar_type() == at::kFloat ? x.options() : x.options().dtype(at::kShort));
+  const size_t n = ops3d_linear_forward_workspace_bytes(z.code, z.batch, z.rows, z.groups, z.N, z.K, grouped);
+  at::Tensor ws;
+  if (n) ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
+  const int rc = ops3d_linear_forward(ptr(xr), ldx, ptr(w), ptr(b), ptr(r), ldr, z.start, z.count, ptr(y),
+                                      act_grad ? ptr(*act_grad) : nullptr, ptr(ws), n, z.code, (int)act, z.batch, z.rows,
+                                      z.groups, z.N, z.K, stream_of(x));
+  if (rc != OPS3D_FDA_OK) raise(rc, "linear_forward failed");
+  return {y, act_grad};
+}
+
+// [grad_x (with weight), grad_weight, grad_bias], None where not wanted.  groups 0: one weight.
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<at::Tensor>> linear_backward(
+    const c10::optional<at::Tensor> &x, const c10::optional<at::Tensor> &weight,
+    const c10::optional<at::Tensor> &group_start, const c10::optional<at::Tensor> &act_grad, const at::Tensor &grad_y,
+    int64_t in_features, int64_t groups, bool need_w, bool need_b) {
+  linear_check(grad_y, "grad_output", grad_y);
+  const bool grouped = group_start.has_value();
+  if (grouped ? grad_y.dim() != 2 && grad_y.dim() != 3 : grad_y.dim() < 1)
+    throw std::invalid_argument("grad_output must be [rows, out_features] or [batch, rows, out_features]");
+  const int64_t N = grad_y.size(-1), K = in_features;
+  auto shape = grad_y.sizes().vec();
+  shape.back() = K;
+  if ((need_w || need_b) && !x) throw std::invalid_argument("x is needed for the gradients of weight and bias");
+  if (x) {
+    linear_check(*x, "x", grad_y);
+    if (x->sizes().vec() != shape) throw std::invalid_argument("x and grad_output differ in their rows");
+  }
+  const std::vector<int64_t> wshape = grouped ? std::vector<int64_t>{groups, N, K} : std::vector<int64_t>{N, K};
+  if (weight) {
+    linear_check(*weight, "weight", grad_y);
+    if (weight->sizes().vec() != wshape) throw std::invalid_argument("weight does not fit grad_output");
+  }
+  if (act_grad && (!act_grad->is_cuda() || act_grad->device() != grad_y.device() || !act_grad->is_contiguous() ||
+                   act_grad->sizes() != grad_y.sizes() ||
+                   act_grad->scalar_type() != (grad_y.scalar_type() == at::kFloat ? at::kFloat : at::kShort)))
+    throw std::invalid_argument("act_grad is not a forward's of this shape");
+  const LinearSizes z = linear_sizes(grad_y, group_start, groups, N, K);
+  const DeviceGuard guard(grad_y.device());
+  int64_t ldx = 0, ldg = 0;
+  const at::Tensor g = as_rows(grad_y, ldg), xr = x ? as_rows(*x, ldx) : at::Tensor();
+  const at::Tensor w = weight ? dense(*weight) : at::Tensor();
+  c10::optional<at::Tensor> gx, gw, gb;
+  if (weight) gx = at::empty(shape, grad_y.options());
+  if (need_w) gw = at::empty(wshape, grad_y.options());
+  if (need_b) gb = at::empty(grouped ? std::vector<int64_t>{groups, N} : std::vector<int64_t>{N}, grad_y.options());
+  const size_t n = need_w || need_b ? ops3d_linear_backward_workspace_bytes(z.code, z.batch, z.rows, z.groups, z.N, z.K, grouped) : 0;
+  at::Tensor ws;
+  if (n) ws = at::empty({(int64_t)n}, grad_y.options().dtype(at::kByte));
+  const int rc = ops3d_linear_backward(ptr(xr), ldx, ptr(w), z.start, z.count, act_grad ? ptr(*act_grad) : nullptr, ptr(g),
+                                       ldg, gx ? ptr(*gx) : nullptr, gw ? ptr(*gw) : nullptr, gb ? ptr(*gb) : nullptr,
+                                       ptr(ws), n, z.code, z.batch, z.rows, z.groups, z.N, z.K, stream_of(grad_y));
+  if (rc != OPS3D_FDA_OK) raise(rc, "linear_backward failed");
+  return {gx, gw, gb};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -474,6 +642,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("nms_3d", &nms_3d, "non-maximum suppression for 3d");
   m.def("dcnv4_forward", &dcnv4_forward, "dcnv4_forward");
   m.def("dcnv4_backward", &dcnv4_backward, "dcnv4_backward");
+  m.def("linear_forward", &linear_forward, "act(x W^T + b) + residual, one weight or one per group of rows");
+  m.def("linear_backward", &linear_backward, "gradients of linear_forward");
   m.def("roi_align_3d_forward", &roi_align_3d_forward, "roi_align_3d_forward");
   m.def("roi_align_3d_backward", &roi_align_3d_backward, "roi_align_3d_backward");
 }
