@@ -60,9 +60,11 @@ OPS3D_FDA_API int ops3d_linear_forward(const void *x, int64_t ld_x, const void *
                                        size_t workspace_bytes, int dtype, int act, int batch, int64_t rows, int groups,
                                        int out_features, int in_features, void *stream);
 
-/* Bytes of device workspace (256-byte aligned) the backward needs. */
+/* Bytes of device workspace (256-byte aligned) the backward needs when it gives grad_weight or
+ * grad_bias (otherwise none): dz (with an act_grad) and the partial sums over chunks of rows. */
 OPS3D_FDA_API size_t ops3d_linear_backward_workspace_bytes(int dtype, int batch, int64_t rows, int groups,
-                                                           int out_features, int in_features, int grouped);
+                                                           int out_features, int in_features, int grouped,
+                                                           int with_act_grad);
 
 /*
  * Backward.  With dz = grad_y * act_grad (grad_y where act_grad is NULL):

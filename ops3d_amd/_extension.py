@@ -133,7 +133,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ops3d_linear_forward.argtypes = ([_vp, _i64, _vp, _vp, _vp, _i64, _vp, _i, _vp, _vp, _vp, _sz]
                                          + [_i] * 3 + [_i64] + [_i] * 3 + [_vp])
     lib.ops3d_linear_backward_workspace_bytes.restype = _sz
-    lib.ops3d_linear_backward_workspace_bytes.argtypes = [_i, _i, _i64, _i, _i, _i, _i]
+    lib.ops3d_linear_backward_workspace_bytes.argtypes = [_i, _i, _i64, _i, _i, _i, _i, _i]
     lib.ops3d_linear_backward.restype = _i
     lib.ops3d_linear_backward.argtypes = ([_vp, _i64, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz]
                                           + [_i] * 2 + [_i64] + [_i] * 3 + [_vp])
@@ -346,7 +346,7 @@ class _NativeFDA:
 
         gx, gw, gb = empty(weight is not None, shape), empty(need_w, wshape), empty(need_b, wshape[:-1])
         code = _DTYPE_CODE[grad_y.dtype]
-        n = (self._lib.ops3d_linear_backward_workspace_bytes(code, B, S, E, N, K, int(grouped))
+        n = (self._lib.ops3d_linear_backward_workspace_bytes(code, B, S, E, N, K, int(grouped), int(act_grad is not None))
              if need_w or need_b else 0)
         ws = torch.empty(n, dtype=torch.uint8, device=grad_y.device) if n else None
         with torch.cuda.device(grad_y.device):

@@ -66,6 +66,19 @@ ChunkPlan plan_of(int dtype, bool grouped, int batch, int64_t rows, int groups, 
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// Workspace of the backward: dz (behind an activation) and the chunks' partial sums.
+struct Layout {
+  ChunkPlan plan;
+  size_t dz, part, part_b, bytes;
+  Layout(int dtype, bool grouped, int batch, int64_t rows, int groups, int N, int K, bool with_dz)
+      : plan(plan_of(dtype, grouped, batch, rows, groups, N, K)) {
+    dz = 0;
+    part = with_dz ? align256((size_t)batch * rows * N * elem_size(dtype)) : 0;
+    part_b = part + (plan.joined ? align256((size_t)plan.slots * N * K * 4) : 0);
+    bytes = part_b + (plan.joined ? align256((size_t)plan.slots * N * 4) : 0);
+  }
+};
+
 template <typename F> int run(int dtype, const char *what, F f) {
   hipError_t e = dtype == OPS3D_FDA_F32 ? f(float()) : dtype == OPS3D_FDA_F16 ? f(_Float16()) : f(__bf16());
   if (e == hipSuccess) return OPS3D_FDA_OK;
@@ -111,73 +124,51 @@ int ops3d_linear_forward(const void *x, int64_t ld_x, const void *weight, const 
   p.act = act;
   p.N = out_features;
   p.K = in_features;
-  return run(dtype, "linear forward", [&](auto t) { return forward<decltype(t)>(p, static_cast<hipStream_t>(stream)); });
+  return run(dtype, "linear forward", [&](auto t) { return ops3d_linear::forward<decltype(t)>(p, static_cast<hipStream_t>(stream)); });
 }
 
 size_t ops3d_linear_backward_workspace_bytes(int dtype, int batch, int64_t rows, int groups, int out_features,
-                                             int in_features, int grouped) {
+                                             int in_features, int grouped, int with_act_grad) {
   if (elem_size(dtype) == 0 || batch < 1 || rows < 1 || rows > kMaxRows / batch || groups < 1 ||
       groups > OPS3D_LINEAR_MAX_GROUPS || out_features < 1 || in_features < 1 || out_features > kMaxFeatures ||
       in_features > kMaxFeatures || (!grouped && groups != 1))
     return 0;
-  const ChunkPlan c = plan_of(dtype, grouped != 0, batch, rows, groups, out_features, in_features);
-  if (!c.joined) return 0;
-  return align256((size_t)c.slots * out_features * in_features * 4) + align256((size_t)c.slots * out_features * 4);
+  return Layout(dtype, grouped != 0, batch, rows, groups, out_features, in_features, with_act_grad != 0).bytes;
 }
 
 int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const int64_t *group_start,
                           int group_start_count, const void *act_grad, const void *grad_y, int64_t ld_grad_y,
-                          void *grad_x, void *grad_weight_out, void *grad_bias, void *workspace, size_t workspace_bytes,
+                          void *grad_x, void *grad_weight, void *grad_bias, void *workspace, size_t workspace_bytes,
                           int dtype, int batch, int64_t rows, int groups, int out_features, int in_features,
                           void *stream) {
   ops3d_fda::set_last_error(OPS3D_FDA_OK, "");
   int rc = check_sizes(dtype, batch, rows, groups, out_features, in_features);
   if (rc) return rc;
   if (ld_x < 0 || ld_grad_y < 0) return fail(OPS3D_FDA_EINVAL, "row distances must not be negative");
-  const bool wants_w = grad_weight_out || grad_bias, empty = batch * rows == 0;
+  const bool wants_w = grad_weight || grad_bias, empty = batch * rows == 0;
   Groups g{};
   if ((rc = make_groups(group_start, group_start_count, batch, rows, groups, g))) return rc;
   if (!empty && (!grad_y || (grad_x && !weight) || (wants_w && !x))) return fail(OPS3D_FDA_EINVAL, "NULL pointer argument");
   const int es = elem_size(dtype);
   if (misaligned(x, es) || misaligned(weight, es) || misaligned(act_grad, es) || misaligned(grad_y, es) ||
-      misaligned(grad_x, es) || misaligned(grad_weight_out, es) || misaligned(grad_bias, es))
+      misaligned(grad_x, es) || misaligned(grad_weight, es) || misaligned(grad_bias, es))
     return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (wants_w) {
-    const ChunkPlan c = plan_of(dtype, group_start != nullptr, batch, empty ? 0 : rows, groups, out_features, in_features);
-    const size_t need = empty ? 0
-                              : ops3d_linear_backward_workspace_bytes(dtype, batch, rows, groups, out_features,
-                                                                      in_features, group_start != nullptr);
-    if (need && (!workspace || workspace_bytes < need))
-      return fail(OPS3D_FDA_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
-    if (need && (reinterpret_cast<uintptr_t>(workspace) & 255u))
-      return fail(OPS3D_FDA_EINVAL, "workspace must be 256-byte aligned");
-    WeightArgs p{};
-    p.u = grad_y;
-    p.ldu = ld_grad_y;
-    p.scale = act_grad;
-    p.x = x;
-    p.ldx = ld_x;
-    p.gw = grad_weight_out;
-    p.gb = grad_bias;
-    p.N = out_features;
-    p.K = in_features;
-    p.chunk = c.chunk;
-    p.slots = empty ? 0 : (int)c.slots;
-    if (need) {
-      p.part = static_cast<float *>(workspace);
-      p.part_b = reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                           align256((size_t)c.slots * out_features * in_features * 4));
-    }
-    p.g = g;
-    rc = run(dtype, "linear weight gradient", [&](auto t) { return ops3d_linear::grad_weight<decltype(t)>(p, need != 0, st); });
-    if (rc) return rc;
-  }
+  const Layout lay(dtype, group_start != nullptr, batch, empty ? 0 : rows, groups, out_features, in_features,
+                   act_grad != nullptr);
+  const size_t need = wants_w && !empty ? lay.bytes : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(OPS3D_FDA_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return fail(OPS3D_FDA_EINVAL, "workspace must be 256-byte aligned");
+  char *const ws = static_cast<char *>(workspace);
+  void *const dz = wants_w && act_grad && !empty ? ws + lay.dz : nullptr;
   if (grad_x && !empty) {
     RowsArgs p{};
     p.a = grad_y;
     p.lda = ld_grad_y;
     p.scale = act_grad;
+    p.dz = dz;
     p.w = weight;
     p.w_group = (int64_t)out_features * in_features;
     p.c = grad_x;
@@ -185,8 +176,31 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
     p.K = out_features;
     p.g = g;
     rc = run(dtype, "linear input gradient", [&](auto t) { return ops3d_linear::grad_x<decltype(t)>(p, st); });
+  } else if (dz) {
+    rc = run(dtype, "linear gradient", [&](auto t) {
+      return ops3d_linear::scale<decltype(t)>(grad_y, ld_grad_y, act_grad, dz, batch * rows, out_features, st);
+    });
   }
-  return rc;
+  if (rc || !wants_w) return rc;
+  WeightArgs p{};
+  p.u = dz ? dz : grad_y;
+  p.ldu = dz ? out_features : ld_grad_y;
+  p.x = x;
+  p.ldx = ld_x;
+  p.gw = grad_weight;
+  p.gb = grad_bias;
+  p.N = out_features;
+  p.K = in_features;
+  p.chunk = lay.plan.chunk;
+  p.slots = empty ? 0 : (int)lay.plan.slots;
+  if (need && lay.plan.joined) {
+    p.part = reinterpret_cast<float *>(ws + lay.part);
+    p.part_b = reinterpret_cast<float *>(ws + lay.part_b);
+  }
+  p.g = g;
+  return run(dtype, "linear weight gradient", [&](auto t) {
+    return ops3d_linear::grad_weight<decltype(t)>(p, lay.plan.tile, !empty && lay.plan.joined, st);
+  });
 }
 
 }  // extern "C"

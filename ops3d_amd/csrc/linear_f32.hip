@@ -5,6 +5,7 @@ namespace ops3d_linear {
 
 template hipError_t forward<float>(const RowsArgs &, hipStream_t);
 template hipError_t grad_x<float>(const RowsArgs &, hipStream_t);
-template hipError_t grad_weight<float>(const WeightArgs &, bool, hipStream_t);
+template hipError_t grad_weight<float>(const WeightArgs &, int, bool, hipStream_t);
+template hipError_t scale<float>(const void *, int64_t, const void *, void *, int64_t, int, hipStream_t);
 
 }  // namespace ops3d_linear

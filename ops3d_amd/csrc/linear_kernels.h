@@ -11,8 +11,8 @@
 // lane; the others lie as they are in memory, sum axis outermost, and are read transposed
 // (ds_read_tr16_b64; single words for fp32).  16-byte chunks are XOR-swizzled so that the lanes of a
 // read fall on different banks.
-// The weight is the first operand of the MFMA, so a lane holds 4 consecutive output columns of a row;
-// the epilogue passes them through LDS, 16 rows at a time, to write whole 16-byte chunks.
+// The weight is the first operand of the MFMA, so a lane holds 4 consecutive output columns of a row, or
+// 8 of two results (column_of): whole 16-byte chunks, and the epilogue stays in registers.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -40,6 +40,7 @@ struct RowsArgs {
   const void *res;        // residual or nullptr
   void *c;                // [rows, N]
   void *act_grad;         // forward: act'(z) out, [rows, N], or nullptr
+  void *dz;               // backward with scale: a * scale out, [rows, K], or nullptr
   int64_t lda, ld_res;
   int64_t w_group;        // elements from one group's weight to the next
   int N, K;               // columns of c, length of the sum
@@ -51,8 +52,7 @@ struct RowsArgs {
 };
 
 struct WeightArgs {
-  const void *u;          // grad_y
-  const void *scale;      // act_grad or nullptr, [rows, N]
+  const void *u;          // dz: grad_y, or grad_y * act_grad
   const void *x;
   void *gw, *gb;          // [E, N, K], [E, N] or nullptr
   float *part, *part_b;   // partial sums [slots, N, K], [slots, N] (nullptr: one chunk per group)
@@ -114,25 +114,67 @@ __device__ __forceinline__ void store16(void *p, uint4 v) {
   *static_cast<Packed16 *>(p) = Packed16{v.x, v.y, v.z, v.w};
 }
 
+// the same past the caches, for what is next read a whole backward pass away
+__device__ __forceinline__ void store16_streaming(void *p, uint4 v) {
+  typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+  __builtin_nontemporal_store(words{v.x, v.y, v.z, v.w}, static_cast<words *>(p));
+}
+
 template <typename T> union Chunk {
   uint4 raw;
   T e[16 / sizeof(T)];
   __device__ __forceinline__ Chunk() {}
 };
 
+// The first n elements of the chunk at p, zeros behind them; not unrolled: the rare end of a row.
+template <typename T> __device__ __forceinline__ uint4 load_part(const T *p, int n) {
+  Chunk<T> c;
+  c.raw = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int i = n - 1; i >= 0; --i) {
+    if (sizeof(T) == 2) {
+      c.raw.w = (c.raw.w << 16) | (c.raw.z >> 16);
+      c.raw.z = (c.raw.z << 16) | (c.raw.y >> 16);
+      c.raw.y = (c.raw.y << 16) | (c.raw.x >> 16);
+      c.raw.x <<= 16;
+    } else {
+      c.raw = make_uint4(0, c.raw.x, c.raw.y, c.raw.z);
+    }
+    c.raw.x |= sizeof(T) == 2 ? *reinterpret_cast<const uint16_t *>(p + i) : *reinterpret_cast<const uint32_t *>(p + i);
+  }
+  return c.raw;
+}
+// The first n elements of a chunk to p.
+template <typename T> __device__ __forceinline__ void store_part(T *p, uint4 v, int n) {
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    if (sizeof(T) == 2) {
+      *reinterpret_cast<uint16_t *>(p + i) = (uint16_t)v.x;
+      v.x = (v.x >> 16) | (v.y << 16);
+      v.y = (v.y >> 16) | (v.z << 16);
+      v.z = (v.z >> 16) | (v.w << 16);
+      v.w >>= 16;
+    } else {
+      *reinterpret_cast<uint32_t *>(p + i) = v.x;
+      v = make_uint4(v.y, v.z, v.w, 0);
+    }
+  }
+}
+
 // The 16-byte chunk at (row, col) of a matrix of nrows x ncols; zeros outside it.
 template <typename T>
 __device__ __forceinline__ uint4 fetch(const T *base, int64_t ld, int row, int col, int nrows, int ncols) {
-  constexpr int CH = 16 / sizeof(T);
+  constexpr int CH = 16 / (int)sizeof(T);
   if (row >= nrows || col >= ncols) return make_uint4(0, 0, 0, 0);
   const T *p = base + (int64_t)row * ld + col;
-  if (col + CH <= ncols) return load16(p);
-  Chunk<T> c;
-  c.raw = make_uint4(0, 0, 0, 0);
-#pragma unroll
-  for (int i = 0; i < CH; ++i)
-    if (col + i < ncols) c.e[i] = p[i];
-  return c.raw;
+  return col + CH <= ncols ? load16(p) : load_part(p, ncols - col);
+}
+
+// A chunk of a row with `left` elements left.
+template <typename T, bool STREAM = false> __device__ __forceinline__ void store_chunk(T *p, uint4 v, int left) {
+  if (left < 16 / (int)sizeof(T)) store_part(p, v, left);
+  else if (STREAM) store16_streaming(p, v);
+  else store16(p, v);
 }
 
 // act_grad: fp32 beside fp32, otherwise 16-bit fixed point in steps of 2^-14 (act' lies in
@@ -140,7 +182,27 @@ __device__ __forceinline__ uint4 fetch(const T *base, int64_t ld, int row, int c
 // INT16_MIN for NaN.
 template <typename T> struct Deriv {
   typedef int16_t type;
-  static __device__ __forceinline__ type encode(float d) {
+  static __device__ __forceinline__ uint4 encode(const float (&d)[8]) {
+    // v_cvt_pknorm takes [-1, 1] to [-32767, 32767], rounded to nearest, and NaN to 0
+    typedef short pair __attribute__((ext_vector_type(2)));
+    constexpr float c = 16384.f / 32767.f;
+    uint32_t w[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(pair, __builtin_amdgcn_cvt_pknorm_i16(c * d[2 * i], c * d[2 * i + 1])));
+      sum += d[2 * i] + d[2 * i + 1];
+    }
+    if (sum != sum) {   // derivatives are finite otherwise, and so is their sum
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (d[2 * i] != d[2 * i]) w[i] = (w[i] & 0xffff0000u) | 0x8000u;
+        if (d[2 * i + 1] != d[2 * i + 1]) w[i] = (w[i] & 0xffffu) | 0x80000000u;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ type encode1(float d) {
     return d != d ? (int16_t)-32768 : (int16_t)__float2int_rn(d * 16384.f);
   }
   // u * derivative, element by element of a 16-byte chunk
@@ -163,7 +225,10 @@ template <typename T> struct Deriv {
 };
 template <> struct Deriv<float> {
   typedef float type;
-  static __device__ __forceinline__ type encode(float d) { return d; }
+  static __device__ __forceinline__ uint4 encode(const float (&d)[4]) {
+    return make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]), __float_as_uint(d[3]));
+  }
+  static __device__ __forceinline__ type encode1(float d) { return d; }
   static __device__ __forceinline__ uint4 apply(uint4 u, uint4 d) {
     return make_uint4(__float_as_uint(__uint_as_float(u.x) * __uint_as_float(d.x)),
                       __float_as_uint(__uint_as_float(u.y) * __uint_as_float(d.y)),
@@ -187,20 +252,21 @@ template <bool FAST> __device__ __forceinline__ float activate(int act, float z,
       return z <= 0.f ? 0.f : z;
     }
     case kGelu: {
-      float phi, cdf;   // sqrt(2 pi) times the normal density, and its distribution
       if (FAST) {
-        phi = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+        // tail = P(X > |z|), w = |z| times the density: act = max(z, 0) - |z| tail, and act' is
+        // tail - w below zero and 1 minus that above
+        const float e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
         const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
-        float p = fmaf(1.061405429f, t, -1.453152027f);
-        p = fmaf(p, t, 1.421413741f);
-        p = fmaf(p, t, -0.284496736f);
-        p = fmaf(p, t, 0.254829592f);
-        const float tail = 0.5f * p * t * phi;
-        cdf = z > 0.f ? 1.f - tail : tail;
-      } else {
-        phi = expf(-0.5f * z * z);
-        cdf = 0.5f * erfcf(-0.70710678f * z);
+        float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+        p = fmaf(p, t, 0.5f * 1.421413741f);
+        p = fmaf(p, t, 0.5f * -0.284496736f);
+        p = fmaf(p, t, 0.5f * 0.254829592f);
+        const float tail = p * t * e;
+        const float g = fmaf(-0.39894228f * fabsf(z), e, tail);
+        d = z > 0.f ? 1.f - g : g;
+        return fmaf(-fabsf(z), tail, z > 0.f ? z : (z != z ? z : 0.f));
       }
+      const float phi = expf(-0.5f * z * z), cdf = 0.5f * erfcf(-0.70710678f * z);
       d = fmaf(z * 0.39894228f, phi, cdf);
       return z * cdf;
     }
@@ -359,51 +425,83 @@ __device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, bo
 // ---------------------------------------------------------------------------------------------
 // A stage of an operand tile of R rows (of the output's side): loaded to registers, then to LDS.
 // STRIDED: the sum's axis is the matrix's row axis.
-template <typename T, int R, int NT, bool STRIDED, bool SCALE> struct Stage {
+template <typename T, int R, int NT, bool STRIDED> struct Stage {
   static constexpr int CH = 16 / (int)sizeof(T);      // elements of a chunk
   static constexpr int KC = 128 / (int)sizeof(T);     // sum elements of a stage
   static constexpr int NC = R / CH;                   // chunks of a matrix row (STRIDED)
   static constexpr int NL = R * 8 / NT;               // chunks per thread
   static constexpr int kBytes = R * 128;
   static_assert(R * 8 % NT == 0, "chunks divide over the threads");
-  uint4 v[NL], d[SCALE ? NL : 1];
 
-  // base: the tile's first element; rows, cols: what is left of the matrix from there
-  __device__ __forceinline__ void load(const T *base, int64_t ld, const void *scale, int64_t ld_scale, int rows, int cols,
-                                       int k0) {
-    typedef typename Deriv<T>::type D;
+  // matrix row and column of chunk i of this thread, from the tile's first element, in stage 0
+  static __device__ __forceinline__ int row_of(int i) {
+    const int c = threadIdx.x + i * NT;
+    return STRIDED ? c / NC : c >> 3;
+  }
+  static __device__ __forceinline__ int col_of(int i) {
+    const int c = threadIdx.x + i * NT;
+    return STRIDED ? c % NC * CH : (c & 7) * CH;
+  }
+  static constexpr int kRowStep = STRIDED ? NT / NC : NT / 8;   // matrix rows between a thread's chunks
+  static constexpr int kRowBytes = STRIDED ? R * (int)sizeof(T) : 128;
+
+  // Chunks of one stage.  base: the tile's first element; rows, cols: what is left of the matrix from
+  // there; k0: sum elements before this stage.  A stage of a whole tile takes 16-byte loads at one
+  // 32-bit offset a thread and scalar bases; one that lacks rows of the output's side reads the last
+  // row for them (their results are not stored); others go chunk by chunk with zeros outside.
+  template <typename E>
+  static __device__ __forceinline__ void load(uint4 (&v)[NL], const E *base, int64_t ld, int rows, int cols, int k0) {
+    const bool inside = (STRIDED ? k0 + KC <= rows && cols >= R : k0 + KC <= cols) && ld < (1 << 22);
+    const E *at = base + (STRIDED ? (int64_t)k0 * ld : (int64_t)k0);
+    if (inside && (STRIDED || rows >= R)) {
+      const uint32_t off = row_of(0) * (int)ld + col_of(0);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int c = threadIdx.x + i * NT;
-      const int row = STRIDED ? k0 + c / NC : c >> 3, col = STRIDED ? c % NC * CH : k0 + (c & 7) * CH;
-      v[i] = fetch(base, ld, row, col, rows, cols);
-      if (SCALE) d[i] = fetch(static_cast<const D *>(scale), ld_scale, row, col, rows, cols);
+      for (int i = 0; i < NL; ++i) v[i] = load16(at + (int64_t)i * kRowStep * ld + off);
+    } else if (inside) {
+      int last = rows - 1;
+      asm volatile("" : "+s"(last));   // the offsets are formed here, not in every block before its loop
+#pragma unroll
+      for (int i = 0; i < NL; ++i) v[i] = load16(at + (uint32_t)(min(row_of(i), last) * (int)ld + col_of(i)));
+    } else {
+      int zero = 0;
+      asm volatile("" : "+s"(zero));
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        v[i] = fetch(base, ld, row_of(i) + (STRIDED ? k0 : zero), col_of(i) + (STRIDED ? zero : k0), rows, cols);
     }
   }
-  __device__ __forceinline__ void store(char *lds) const {
+  static __device__ __forceinline__ void store(char *lds, const uint4 (&v)[NL]) {
+    if constexpr (kRowStep % 16 == 0) {   // the swizzle looks at the row's lower 4 bits
+      char *at = lds + address(row_of(0), col_of(0) / CH);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int c = threadIdx.x + i * NT;
-      const int row = STRIDED ? c / NC : c >> 3, col = STRIDED ? c % NC : c & 7;
-      *reinterpret_cast<uint4 *>(lds + address(row, col)) = SCALE ? Deriv<T>::apply(v[i], d[i]) : v[i];
+      for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4 *>(at + i * kRowStep * kRowBytes) = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4 *>(lds + address(row_of(i), col_of(i) / CH)) = v[i];
     }
   }
-  // byte address of a 16-byte chunk
+  // Byte address of a 16-byte chunk.  Rows of 128 bytes: 8 rows that follow each other, and 8 that a lane
+  // octet reads in the order of column_of (4 h + 0 .. 3 of two groups of 8), fall on 8 different chunks.
+  // STRIDED: the 4 matrix rows that 16 lanes read (fp32: the rows that the lane quarters read) fall on
+  // different chunks, for columns that follow each other and for those of column_of.
   static __device__ __forceinline__ int address(int row, int col) {
-    if (!STRIDED) return row * 128 + ((col ^ (row & 7)) << 4);
-    return row * (R * (int)sizeof(T)) + ((col ^ (sizeof(T) == 2 ? (row & 3) << 1 : ((row >> 2) & 3) << 2)) << 4);
+    if (!STRIDED) return row * 128 + ((col ^ ((row & 3) | (((row >> 2) ^ (row >> 3)) & 1) << 2)) << 4);
+    constexpr int kShift = sizeof(T) == 4 || NC >= 16 ? 2 : 1;
+    return row * (R * (int)sizeof(T)) + ((col ^ (sizeof(T) == 2 ? row & 3 : (row >> 2) & 3) << kShift) << 4);
   }
-  // MFMA operand of output rows r0 .. r0 + 15, half `step` of the stage
-  static __device__ __forceinline__ typename Type<T>::frag frag(const char *lds, int r0, int step) {
-    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  // MFMA operand, half `step` of the stage, of 16 output rows: r0 + row(i) for lane index i
+  template <typename F> static __device__ __forceinline__ typename Type<T>::frag frag(const char *lds, int step, F row, int lane) {
+    const int i = lane & 15, q = lane >> 4;
     if constexpr (!STRIDED) {
-      return __builtin_bit_cast(typename Type<T>::frag, *reinterpret_cast<const uint4 *>(lds + address(r0 + i, step * 4 + q)));
+      return __builtin_bit_cast(typename Type<T>::frag, *reinterpret_cast<const uint4 *>(lds + address(row(i), step * 4 + q)));
     } else if constexpr (sizeof(T) == 2) {
-      // 16 lanes read 4 matrix rows of 16 elements and get them transposed: lane i column r0 + i
+      // 16 lanes read 4 matrix rows of 16 elements, 4 elements a lane, and get them transposed: lane i
+      // has the elements that lanes i / 4, 4 + i / 4, .. read at place i % 4
       s16x4 h[2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const char *at = lds + address(step * 32 + q * 8 + p * 4 + (i >> 2), (r0 >> 3) + ((i & 3) >> 1)) + (i & 1) * 8;
+        const int c = row((i & 3) * 4);
+        const char *at = lds + address(step * 32 + q * 8 + p * 4 + (i >> 2), c >> 3) + (c & 7) * 2;
         h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) s16x4 *)(const_cast<char *>(at)));
       }
@@ -412,11 +510,19 @@ template <typename T, int R, int NT, bool STRIDED, bool SCALE> struct Stage {
       f32x4 f;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        f[j] = *reinterpret_cast<const float *>(lds + address(step * 16 + q * 4 + j, (r0 + i) >> 2) + (i & 3) * 4);
+        f[j] = *reinterpret_cast<const float *>(lds + address(step * 16 + q * 4 + j, row(i) >> 2) + (row(i) & 3) * 4);
       return __builtin_bit_cast(typename Type<T>::frag, f);
     }
   }
 };
+
+// The output columns of the MFMA rows: a lane holds rows 4 q .. 4 q + 3 of each 16-row result.  In 16
+// bits results 2 t and 2 t + 1 take columns 32 t + 8 q .. + 3 and .. + 4 .. + 7, so that a lane holds 8
+// consecutive columns, a 16-byte chunk; in fp32 4 columns are one already.
+template <typename T> __device__ __forceinline__ int column_of(int n, int i) {
+  if (sizeof(T) == 4) return n * 16 + i;
+  return (n >> 1) * 32 + (i >> 2) * 8 + (n & 1) * 4 + (i & 3);
+}
 
 // blockIdx -> (row tile, column tile).  spread: the column tiles of a row tile run one after another
 // on one XCD, whose L2 then holds the row tile (blocks go to XCD blockIdx % 8); used from 64 row tiles
@@ -432,35 +538,89 @@ __device__ __forceinline__ void block_tile(int bid, int col_tiles, int spread, i
   }
 }
 
-// Cross-lane traffic through LDS inside one wave: LDS accesses of a wave stay in order; this keeps
-// the compiler from moving them.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+// The results of a wave: rows r0 + 16 m + lane & 15 of the tile, columns col0 + column_of of acc[m][..],
+// with activation and residual.  FULL: all inside.  A row's chunks follow one another, so that the
+// 64-byte pieces of a line are stored together (and 22 % faster than column by column, 73728 x 1024
+// bf16 with act_grad); act_grad goes past the caches (120 -> 95 us there).
+template <typename T, int MI, int NI, bool EPI, int ACT, bool FULL>
+__device__ __forceinline__ void store_results(const RowsArgs &p, const f32x4 (&acc)[MI][NI], const RowTile &tile, int r0,
+                                              int col0, int lane) {
+  constexpr int CH = 16 / (int)sizeof(T), NP = CH / 4;   // MFMA results that make up a chunk of columns
+  typedef typename Deriv<T>::type D;
+  const int row0 = r0 + (lane & 15), c0 = (lane >> 4) * CH;
+  const int64_t at = tile.first * p.N + col0;                    // uniform
+  const uint32_t off = (uint32_t)(row0 * p.N + c0);              // the rest: below 256 rows of 2^24
+  const T *res = EPI && p.res ? static_cast<const T *>(p.res) + tile.first * p.ld_res + col0 : nullptr;
+  const int64_t off_res = row0 * p.ld_res + c0;
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    if (!FULL && row0 + m * 16 >= tile.rows) continue;
+#pragma unroll
+    for (int t = 0; t < NI / NP; ++t) {
+      const int cols = t * NP * 16, left = FULL ? CH : p.N - col0 - c0 - cols;
+      if (!FULL && left <= 0) continue;
+      const int64_t to = at + (int64_t)m * 16 * p.N + cols;      // uniform
+      float z[CH], d[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        z[i] = acc[m][t * NP + i / 4][i & 3];
+        if (EPI) z[i] = activate<sizeof(T) == 2>(ACT, z[i], d[i]);
+      }
+      if (EPI && ACT != kNone && p.act_grad) store_chunk<D, true>(static_cast<D *>(p.act_grad) + to + off, Deriv<T>::encode(d), left);
+      if (EPI && res) {
+        const T *rp = res + (int64_t)m * 16 * p.ld_res + cols + off_res;
+        Chunk<T> r;
+        r.raw = left >= CH ? load16(rp) : load_part(rp, left);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) z[i] += (float)r.e[i];
+      }
+      Chunk<T> out;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) out.e[i] = (T)z[i];
+      store_chunk<T>(static_cast<T *>(p.c) + to + off, out.raw, left);
+    }
+  }
+}
+template <typename T, int MI, int NI, bool EPI, bool FULL>
+__device__ __forceinline__ void finish_tile(const RowsArgs &p, const f32x4 (&acc)[MI][NI], const RowTile &tile, int r0, int col0,
+                                            int lane) {
+  if constexpr (!EPI) {
+    store_results<T, MI, NI, false, kNone, FULL>(p, acc, tile, r0, col0, lane);
+  } else if (tile.e < 0) {
+    store_results<T, MI, NI, false, kNone, FULL>(p, acc, tile, r0, col0, lane);
+  } else {
+    switch (p.act) {
+      case kRelu: store_results<T, MI, NI, true, kRelu, FULL>(p, acc, tile, r0, col0, lane); break;
+      case kGelu: store_results<T, MI, NI, true, kGelu, FULL>(p, acc, tile, r0, col0, lane); break;
+      case kGeluTanh: store_results<T, MI, NI, true, kGeluTanh, FULL>(p, acc, tile, r0, col0, lane); break;
+      case kSilu: store_results<T, MI, NI, true, kSilu, FULL>(p, acc, tile, r0, col0, lane); break;
+      default: store_results<T, MI, NI, true, kNone, FULL>(p, acc, tile, r0, col0, lane); break;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
 // c = epilogue(a w^T) (WSTR = false, w [N, K]) or a w (WSTR = true, w [K, N]) over tiles of BM rows
-// and BN columns, WR x WC waves.
-template <typename T, int BM, int BN, int WR, int WC, bool WSTR, bool SCALE, bool EPI>
-__global__ __launch_bounds__(64 * WR *WC) void rows_kernel(RowsArgs p) {
+// and BN columns, WR x WC waves.  SCALE: a is grad_y * act_grad, and the first column's tiles store
+// it for the weights' gradients.
+template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI>
+__global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void rows_kernel(RowsArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
-  constexpr int CH = 16 / (int)sizeof(T);
-  typedef Stage<T, BM, NT, false, SCALE> SA;
-  typedef Stage<T, BN, NT, WSTR, false> SB;
-  constexpr int kPad = TN + 4;   // floats of a row of the epilogue's buffer: rows 16 bytes off each other's banks
-  constexpr int kEpi = WR * WC * 16 * kPad * 4;
-  __shared__ __attribute__((aligned(16))) char lds[SA::kBytes + SB::kBytes > kEpi ? SA::kBytes + SB::kBytes : kEpi];
+  typedef Stage<T, BM, NT, false> SA;
+  typedef Stage<T, BN, NT, WSTR> SB;
+  typedef typename Deriv<T>::type D;
+  constexpr int kStage = SA::kBytes + SB::kBytes;
+  __shared__ __attribute__((aligned(16))) char lds[BUFS * kStage];
 
   int rt, ct;
   block_tile(blockIdx.x, p.col_tiles, p.spread, rt, ct);
   if (rt >= p.row_tiles) return;
   RowTile tile;
   if (!find_row_tile(p.g, rt, BM, tile)) return;
-  const int n0 = ct * BN, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int n0 = ct * BN, wave = threadIdx.x >> 6, q = (threadIdx.x & 63) >> 4;
   const int wr = wave / WC, wc = wave % WC;
 
-  f32x4 acc[MI][NI];
+  f32x4 acc[MI][NI];   // lane (i, q) of [m][n]: row 16 m + i, columns column_of(n, 4 q) .. + 3
 #pragma unroll
   for (int m = 0; m < MI; ++m)
 #pragma unroll
@@ -468,111 +628,66 @@ __global__ __launch_bounds__(64 * WR *WC) void rows_kernel(RowsArgs p) {
 
   if (tile.e >= 0) {
     const T *a = static_cast<const T *>(p.a) + tile.first * p.lda;
-    const void *scale = SCALE ? static_cast<const typename Deriv<T>::type *>(p.scale) + tile.first * p.K : nullptr;
+    const D *scale = SCALE ? static_cast<const D *>(p.scale) + tile.first * p.K : nullptr;
+    T *dz = SCALE && ct == 0 && p.dz ? static_cast<T *>(p.dz) + tile.first * p.K : nullptr;
     const T *w = static_cast<const T *>(p.w) + tile.e * p.w_group + (WSTR ? (int64_t)n0 : (int64_t)n0 * p.K);
     const int64_t ldw = WSTR ? p.N : p.K;
     const int wrows = WSTR ? p.K : p.N - n0, wcols = WSTR ? p.N - n0 : p.K;
-    SA sa;
-    SB sb;
-    sa.load(a, p.lda, scale, p.K, tile.rows, p.K, 0);
-    sb.load(w, ldw, nullptr, 0, wrows, wcols, 0);
+    uint4 va[SA::NL], vd[SA::NL], vb[SB::NL];
+    SA::load(va, a, p.lda, tile.rows, p.K, 0);
+    if (SCALE) SA::load(vd, scale, p.K, tile.rows, p.K, 0);
+    SB::load(vb, w, ldw, wrows, wcols, 0);
+    int buf = 0;
     for (int k0 = 0; k0 < p.K; k0 += SA::KC) {
-      __syncthreads();
-      sa.store(lds);
-      sb.store(lds + SA::kBytes);
-      __syncthreads();
-      if (k0 + SA::KC < p.K) {
-        sa.load(a, p.lda, scale, p.K, tile.rows, p.K, k0 + SA::KC);
-        sb.load(w, ldw, nullptr, 0, wrows, wcols, k0 + SA::KC);
+      if (BUFS == 1) __syncthreads();
+      char *const at = lds + (BUFS == 1 ? 0 : buf * kStage);
+      if (SCALE) {
+#pragma unroll
+        for (int i = 0; i < SA::NL; ++i) {
+          va[i] = Deriv<T>::apply(va[i], vd[i]);
+          const int row = SA::row_of(i), left = p.K - k0 - SA::col_of(i);
+          if (dz && row < tile.rows && left > 0) store_chunk<T>(dz + (int64_t)row * p.K + k0 + SA::col_of(i), va[i], left);
+        }
       }
+      SA::store(at, va);
+      SB::store(at + SA::kBytes, vb);
+      if (k0 + SA::KC < p.K) {
+        SA::load(va, a, p.lda, tile.rows, p.K, k0 + SA::KC);
+        if (SCALE) SA::load(vd, scale, p.K, tile.rows, p.K, k0 + SA::KC);
+        SB::load(vb, w, ldw, wrows, wcols, k0 + SA::KC);
+      }
+      __syncthreads();
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         typename Type<T>::frag fb[NI];
 #pragma unroll
-        for (int n = 0; n < NI; ++n) fb[n] = SB::frag(lds + SA::kBytes, wc * TN + n * 16, s);
+        for (int n = 0; n < NI; ++n)
+          fb[n] = SB::frag(at + SA::kBytes, s, [&](int i) { return wc * TN + column_of<T>(n, i); }, threadIdx.x & 63);
 #pragma unroll
         for (int m = 0; m < MI; ++m) {
-          const typename Type<T>::frag fa = SA::frag(lds, wr * TM + m * 16, s);
+          const typename Type<T>::frag fa = SA::frag(at, s, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
 #pragma unroll
           for (int n = 0; n < NI; ++n) acc[m][n] = Type<T>::mma(fb[n], fa, acc[m][n]);
         }
       }
+      buf ^= 1;
     }
-    __syncthreads();
   }
 
-  // lane (i, q) of acc[m][n]: row m * 16 + i, columns n * 16 + 4 q .. + 3
-  float *buf = reinterpret_cast<float *>(lds) + wave * 16 * kPad;
-  constexpr int PC = TN / CH;                     // chunks of a row
-  constexpr int PN = 16 * PC / 64;                // chunks per lane and 16 rows
-  static_assert(64 % PC == 0 && 16 * PC % 64 == 0, "a lane keeps its columns");
-  const int c0 = lane % PC * CH, col = n0 + wc * TN + c0, left = p.N - col;
-  float bias[CH];
+  if (EPI && p.bias && tile.e >= 0) {
+    constexpr int CH = 16 / (int)sizeof(T), NP = CH / 4;
 #pragma unroll
-  for (int i = 0; i < CH; ++i) bias[i] = 0.f;
-  if (EPI && p.bias && tile.e >= 0 && left > 0) {
-    Chunk<T> b;
-    b.raw = fetch(static_cast<const T *>(p.bias) + (int64_t)tile.e * p.N, 0, 0, col, 1, p.N);
+    for (int t = 0; t < NI / NP; ++t) {
+      Chunk<T> b;
+      b.raw = fetch(static_cast<const T *>(p.bias) + (int64_t)tile.e * p.N, 0, 0, n0 + wc * TN + t * NP * 16 + q * CH, 1, p.N);
 #pragma unroll
-    for (int i = 0; i < CH; ++i) bias[i] = (float)b.e[i];
-  }
+      for (int m = 0; m < MI; ++m)
 #pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    if (m) wave_fence();
-#pragma unroll
-    for (int n = 0; n < NI; ++n) *reinterpret_cast<f32x4 *>(buf + (lane & 15) * kPad + n * 16 + (lane >> 4) * 4) = acc[m][n];
-    wave_fence();
-#pragma unroll
-    for (int t = 0; t < PN; ++t) {
-      const int r = t * (64 / PC) + lane / PC, row = wr * TM + m * 16 + r;
-      if (row >= tile.rows || left <= 0) continue;
-      const int64_t grow = tile.first + row;
-      float z[CH];
-#pragma unroll
-      for (int i = 0; i < CH; i += 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(buf + r * kPad + c0 + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) z[i + j] = v[j];
-      }
-      Chunk<T> out;
-      if (EPI && tile.e >= 0) {
-        typedef typename Deriv<T>::type D;
-        D der[CH];
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          float d;
-          z[i] = activate<sizeof(T) == 2>(p.act, z[i] + bias[i], d);
-          der[i] = Deriv<T>::encode(d);
-        }
-        if (p.act_grad) {
-          D *dp = static_cast<D *>(p.act_grad) + grow * p.N + col;
-          if (left >= CH) {
-            store16(dp, __builtin_bit_cast(uint4, der));
-          } else {
-#pragma unroll
-            for (int i = 0; i < CH; ++i)
-              if (i < left) dp[i] = der[i];
-          }
-        }
-        if (p.res) {
-          Chunk<T> rr;
-          rr.raw = fetch(static_cast<const T *>(p.res) + grow * p.ld_res, 0, 0, col, 1, p.N);
-#pragma unroll
-          for (int i = 0; i < CH; ++i) z[i] += (float)rr.e[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < CH; ++i) out.e[i] = (T)z[i];
-      T *cp = static_cast<T *>(p.c) + grow * p.N + col;
-      if (left >= CH) {
-        store16(cp, out.raw);
-      } else {
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if (i < left) cp[i] = out.e[i];
-      }
+        for (int i = 0; i < CH; ++i) acc[m][t * NP + i / 4][i & 3] += (float)b.e[i];
     }
   }
+  if (tile.rows >= BM && n0 + BN <= p.N) finish_tile<T, MI, NI, EPI, true>(p, acc, tile, wr * TM, n0 + wc * TN, threadIdx.x & 63);
+  else finish_tile<T, MI, NI, EPI, false>(p, acc, tile, wr * TM, n0 + wc * TN, threadIdx.x & 63);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -630,7 +745,7 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
         if (p.bias) y += (float)static_cast<const T *>(p.bias)[(int64_t)tile.e * p.N + col + j];
         float d;
         y = activate<sizeof(T) == 2>(p.act, y, d);
-        if (p.act_grad) static_cast<typename Deriv<T>::type *>(p.act_grad)[grow * p.N + col + j] = Deriv<T>::encode(d);
+        if (p.act_grad) static_cast<typename Deriv<T>::type *>(p.act_grad)[grow * p.N + col + j] = Deriv<T>::encode1(d);
         if (p.res) y += (float)static_cast<const T *>(p.res)[grow * p.ld_res + col + j];
       }
       static_cast<T *>(p.c)[grow * p.N + col + j] = (T)y;
@@ -641,12 +756,13 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
 // ---------------------------------------------------------------------------------------------
 // gw = dz^T x, gb = sum of dz over the rows of a chunk; a chunk that is its group's only one writes
 // the results, the others their partial sums.
-template <typename T, int BM, int BN, int WR, int WC, bool SCALE>
-__global__ __launch_bounds__(64 * WR *WC) void weight_kernel(WeightArgs p) {
+template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC>
+__global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void weight_kernel(WeightArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
-  typedef Stage<T, BM, NT, true, SCALE> SU;
-  typedef Stage<T, BN, NT, true, false> SX;
-  __shared__ __attribute__((aligned(16))) char lds[SU::kBytes + SX::kBytes];
+  typedef Stage<T, BM, NT, true> SU;
+  typedef Stage<T, BN, NT, true> SX;
+  constexpr int kStage = SU::kBytes + SX::kBytes;
+  __shared__ __attribute__((aligned(16))) char lds[BUFS * kStage];
   int slot, ct;
   block_tile(blockIdx.x, p.n_tiles * p.k_tiles, 1, slot, ct);
   if (slot >= p.slots) return;
@@ -664,34 +780,35 @@ __global__ __launch_bounds__(64 * WR *WC) void weight_kernel(WeightArgs p) {
     for (int n = 0; n < NI; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const T *u = static_cast<const T *>(p.u) + ch.first * p.ldu + n0;
-  const void *scale = SCALE ? static_cast<const typename Deriv<T>::type *>(p.scale) + ch.first * p.N + n0 : nullptr;
   const T *x = static_cast<const T *>(p.x) + ch.first * p.ldx + k0;
-  SU su;
-  SX sx;
-  su.load(u, p.ldu, scale, p.N, ch.rows, p.N - n0, 0);
-  sx.load(x, p.ldx, nullptr, 0, ch.rows, p.K - k0, 0);
+  uint4 vu[SU::NL], vx[SX::NL];
+  SU::load(vu, u, p.ldu, ch.rows, p.N - n0, 0);
+  SX::load(vx, x, p.ldx, ch.rows, p.K - k0, 0);
+  int buf = 0;
   for (int r0 = 0; r0 < ch.rows; r0 += SU::KC) {
-    __syncthreads();
-    su.store(lds);
-    sx.store(lds + SU::kBytes);
-    __syncthreads();
+    if (BUFS == 1) __syncthreads();
+    char *const at = lds + (BUFS == 1 ? 0 : buf * kStage);
+    SU::store(at, vu);
+    SX::store(at + SU::kBytes, vx);
     if (r0 + SU::KC < ch.rows) {
-      su.load(u, p.ldu, scale, p.N, ch.rows, p.N - n0, r0 + SU::KC);
-      sx.load(x, p.ldx, nullptr, 0, ch.rows, p.K - k0, r0 + SU::KC);
+      SU::load(vu, u, p.ldu, ch.rows, p.N - n0, r0 + SU::KC);
+      SX::load(vx, x, p.ldx, ch.rows, p.K - k0, r0 + SU::KC);
     }
+    __syncthreads();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       typename Type<T>::frag fx[NI];
 #pragma unroll
-      for (int n = 0; n < NI; ++n) fx[n] = SX::frag(lds + SU::kBytes, wc * TN + n * 16, s);
+      for (int n = 0; n < NI; ++n) fx[n] = SX::frag(at + SU::kBytes, s, [&](int i) { return wc * TN + n * 16 + i; }, threadIdx.x & 63);
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
-        const typename Type<T>::frag fu = SU::frag(lds, wr * TM + m * 16, s);
+        const typename Type<T>::frag fu = SU::frag(at, s, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[m][n] = Type<T>::mma(fx[n], fu, acc[m][n]);
         if (with_b) accb[m] = Type<T>::mma(Type<T>::ones(), fu, accb[m]);
       }
     }
+    buf ^= 1;
   }
   // lane (i, q) of acc[m][n]: row n0 + m * 16 + i of gw, columns k0 + n * 16 + 4 q .. + 3
   const bool direct = ch.chunks == 1;
@@ -702,18 +819,35 @@ __global__ __launch_bounds__(64 * WR *WC) void weight_kernel(WeightArgs p) {
     if (row >= p.N) continue;
 #pragma unroll
     for (int n = 0; n < NI && p.gw; ++n) {
-      const int col = k0 + wc * TN + n * 16 + q * 4;
+      const int col = k0 + wc * TN + n * 16 + q * 4, left = p.K - col;
+      if (left <= 0) continue;
+      if (direct) {
+        T *at = static_cast<T *>(p.gw) + ((int64_t)ch.e * p.N + row) * p.K + col;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (col + j >= p.K) continue;
-        if (direct) static_cast<T *>(p.gw)[((int64_t)ch.e * p.N + row) * p.K + col + j] = (T)acc[m][n][j];
-        else p.part[((int64_t)slot * p.N + row) * p.K + col + j] = acc[m][n][j];
+        for (int j = 0; j < 4; ++j)
+          if (j < left) at[j] = (T)acc[m][n][j];
+      } else {
+        store_chunk<float>(p.part + ((int64_t)slot * p.N + row) * p.K + col, __builtin_bit_cast(uint4, acc[m][n]), left);
       }
     }
     if (with_b && q == 0) {
       if (direct) static_cast<T *>(p.gb)[(int64_t)ch.e * p.N + row] = (T)accb[m][0];
       else p.part_b[(int64_t)slot * p.N + row] = accb[m][0];
     }
+  }
+}
+
+// dz = grad_y * act_grad, where no input gradient's kernel forms it
+template <typename T> __global__ __launch_bounds__(256) void scale_kernel(const T *u, int64_t ldu, const void *scale, T *dz, int64_t rows, int N) {
+  constexpr int CH = 16 / (int)sizeof(T);
+  typedef typename Deriv<T>::type D;
+  const int per = (N + CH - 1) / CH;
+  for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < rows * per; c += (int64_t)gridDim.x * 256) {
+    const int64_t row = c / per;
+    const int col = (int)(c - row * per) * CH;
+    const uint4 v = Deriv<T>::apply(fetch(u + row * ldu, 0, 0, col, 1, N),
+                                    fetch(static_cast<const D *>(scale) + row * N, 0, 0, col, 1, N));
+    store_chunk<T>(dz + row * N + col, v, N - col);
   }
 }
 
@@ -767,14 +901,14 @@ template <typename K> inline hipError_t launch(K kernel, int64_t grid, int threa
   return hipGetLastError();
 }
 
-template <typename T, int BM, int BN, int WR, int WC, bool WSTR, bool SCALE, bool EPI>
+template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI>
 inline hipError_t launch_rows(RowsArgs p, hipStream_t st) {
   const int64_t rt = max_row_tiles(p.g, BM);
   p.row_tiles = (int)rt;
   p.col_tiles = ceil_div(p.N, BN);
   p.spread = rt >= 64;
   const int64_t grid = (p.spread ? (rt + 7) / 8 * 8 : rt) * p.col_tiles;
-  return launch(rows_kernel<T, BM, BN, WR, WC, WSTR, SCALE, EPI>, grid, 64 * WR * WC, st, p);
+  return launch(rows_kernel<T, BM, BN, WR, WC, BUFS, OCC, WSTR, SCALE, EPI>, grid, 64 * WR * WC, st, p);
 }
 
 template <typename T, int RT, int NW> inline hipError_t launch_few(RowsArgs p, hipStream_t st) {
@@ -786,8 +920,20 @@ template <typename T, int RT, int NW> inline hipError_t launch_few(RowsArgs p, h
 
 template <typename T, bool WSTR, bool SCALE, bool EPI> inline hipError_t launch_tiles(const RowsArgs &p, hipStream_t st) {
   const int64_t rows = (int64_t)p.g.B * p.g.S;
-  if ((rows + 127) / 128 * ceil_div(p.N, 128) >= 256) return launch_rows<T, 128, 128, 2, 2, WSTR, SCALE, EPI>(p, st);
-  return launch_rows<T, 64, 64, 2, 2, WSTR, SCALE, EPI>(p, st);
+  if constexpr (sizeof(T) == 2 && !SCALE) {
+    // one block of 256 x 256 a CU: long sums (4096^3 bf16 145 us, 195 with 128 x 128), or outputs of many
+    // tiles, where the operands' second and third reading costs most (598016 x 256 -> 1024 590 and 680 us,
+    // but 73728 rows, 1152 tiles, 116 and 98)
+    const int64_t tiles = (rows + 255) / 256 * ceil_div(p.N, 256);
+    if (rows / p.g.E >= 512 && p.N >= 256 && ((p.K >= 512 && tiles >= 192) || tiles >= 4096))
+      return launch_rows<T, 256, 256, 2, 4, 2, 2, WSTR, SCALE, EPI>(p, st);
+  }
+  if ((rows + 127) / 128 * ceil_div(p.N, 128) >= 256) {
+    // with act_grad 64 x 128, whose registers fit four blocks a CU (73728 x 1024 -> 256 142 us, 157)
+    if constexpr (SCALE) return launch_rows<T, 64, 128, 1, 4, 1, 4, WSTR, SCALE, EPI>(p, st);
+    else return launch_rows<T, 128, 128, 2, 2, 1, 3, WSTR, SCALE, EPI>(p, st);
+  }
+  return launch_rows<T, 64, 64, 2, 2, 1, 4, WSTR, SCALE, EPI>(p, st);
 }
 
 template <typename T> hipError_t forward(const RowsArgs &p, hipStream_t st) {
@@ -802,18 +948,20 @@ template <typename T> hipError_t grad_x(const RowsArgs &p, hipStream_t st) {
   return p.scale ? launch_tiles<T, true, true, false>(p, st) : launch_tiles<T, true, false, false>(p, st);
 }
 
-constexpr int kWeightTile = 128;
-
-// Rows per chunk of the weight kernel and the number of chunks; the workspace follows from it.
+// Tile, rows per chunk and number of chunks of the weight kernel; the workspace follows from it.
+// 512 blocks of 128 x 128 fill the 256 CUs once (two blocks each); where the tiles times chunks of 256
+// rows do not make 256 blocks, tiles of 64 x 64 and chunks of 64 rows do better.
 struct ChunkPlan {
-  int chunk;
+  int tile, chunk;
   int64_t slots;
   bool joined;   // a group may have several chunks
   ChunkPlan(int esize, bool grouped, int B, int64_t S, int E, int N, int K) {
     const int kc = 128 / esize;
-    const int64_t tiles = (int64_t)ceil_div(N, kWeightTile) * ceil_div(K, kWeightTile), rows = (int64_t)B * S;
+    const int64_t rows = (int64_t)B * S, big = (int64_t)ceil_div(N, 128) * ceil_div(K, 128);
+    tile = big * (rows / 256 > E ? rows / 256 : E) >= 256 ? 128 : 64;
+    const int64_t tiles = (int64_t)ceil_div(N, tile) * ceil_div(K, tile), least = tile == 128 ? 256 : 64;
     int64_t want = 512 / tiles;
-    if (want > rows / 256) want = rows / 256;
+    if (want > rows / least) want = rows / least;
     if (want <= E) want = 1;
     chunk = (int)((S + kc - 1) / kc * kc);
     if (want > 1) chunk = (int)((rows / want + kc - 1) / kc * kc);
@@ -823,15 +971,23 @@ struct ChunkPlan {
   }
 };
 
-template <typename T> hipError_t grad_weight(const WeightArgs &q, bool joined, hipStream_t st) {
+template <typename T>
+hipError_t scale(const void *u, int64_t ldu, const void *act_grad, void *dz, int64_t rows, int N, hipStream_t st) {
+  const int64_t chunks = rows * ceil_div(N, 16 / (int)sizeof(T)), blocks = (chunks + 255) / 256;
+  hipLaunchKernelGGL((scale_kernel<T>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st,
+                     static_cast<const T *>(u), ldu, act_grad, static_cast<T *>(dz), rows, N);
+  return hipGetLastError();
+}
+
+template <typename T> hipError_t grad_weight(const WeightArgs &q, int tile, bool joined, hipStream_t st) {
   WeightArgs p = q;
-  p.n_tiles = ceil_div(p.N, kWeightTile);
-  p.k_tiles = p.gw ? ceil_div(p.K, kWeightTile) : 1;
+  p.n_tiles = ceil_div(p.N, tile);
+  p.k_tiles = p.gw ? ceil_div(p.K, tile) : 1;
   const int64_t grid = ((int64_t)p.slots + 7) / 8 * 8 * p.n_tiles * p.k_tiles;
   if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
   if (grid > 0) {
-    if (p.scale) hipLaunchKernelGGL((weight_kernel<T, kWeightTile, kWeightTile, 2, 2, true>), dim3((unsigned)grid), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((weight_kernel<T, kWeightTile, kWeightTile, 2, 2, false>), dim3((unsigned)grid), dim3(256), 0, st, p);
+    if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, 1, 2>), dim3((unsigned)grid), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, 1, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
   }
   if (joined || p.g.start || !p.slots) {
     const int64_t total = (p.gw ? (int64_t)p.N * p.K : 0) + (p.gb ? p.N : 0);
@@ -848,8 +1004,11 @@ extern template hipError_t forward<__bf16>(const RowsArgs &, hipStream_t);
 extern template hipError_t grad_x<float>(const RowsArgs &, hipStream_t);
 extern template hipError_t grad_x<_Float16>(const RowsArgs &, hipStream_t);
 extern template hipError_t grad_x<__bf16>(const RowsArgs &, hipStream_t);
-extern template hipError_t grad_weight<float>(const WeightArgs &, bool, hipStream_t);
-extern template hipError_t grad_weight<_Float16>(const WeightArgs &, bool, hipStream_t);
-extern template hipError_t grad_weight<__bf16>(const WeightArgs &, bool, hipStream_t);
+extern template hipError_t grad_weight<float>(const WeightArgs &, int, bool, hipStream_t);
+extern template hipError_t scale<float>(const void *, int64_t, const void *, void *, int64_t, int, hipStream_t);
+extern template hipError_t grad_weight<_Float16>(const WeightArgs &, int, bool, hipStream_t);
+extern template hipError_t scale<_Float16>(const void *, int64_t, const void *, void *, int64_t, int, hipStream_t);
+extern template hipError_t grad_weight<__bf16>(const WeightArgs &, int, bool, hipStream_t);
+extern template hipError_t scale<__bf16>(const void *, int64_t, const void *, void *, int64_t, int, hipStream_t);
 
 }  // namespace ops3d_linear

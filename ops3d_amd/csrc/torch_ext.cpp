@@ -614,7 +614,9 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
   if (weight) gx = at::empty(shape, grad_y.options());
   if (need_w) gw = at::empty(wshape, grad_y.options());
   if (need_b) gb = at::empty(grouped ? std::vector<int64_t>{groups, N} : std::vector<int64_t>{N}, grad_y.options());
-  const size_t n = need_w || need_b ? ops3d_linear_backward_workspace_bytes(z.code, z.batch, z.rows, z.groups, z.N, z.K, grouped) : 0;
+  const size_t n = need_w || need_b ? ops3d_linear_backward_workspace_bytes(z.code, z.batch, z.rows, z.groups, z.N, z.K,
+                                                                            grouped, act_grad.has_value())
+                                    : 0;
   at::Tensor ws;
   if (n) ws = at::empty({(int64_t)n}, grad_y.options().dtype(at::kByte));
   const int rc = ops3d_linear_backward(ptr(xr), ldx, ptr(w), z.start, z.count, act_grad ? ptr(*act_grad) : nullptr, ptr(g),

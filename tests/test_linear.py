@@ -198,7 +198,7 @@ def test_c_refusals_before_device_work(lib):
     refused(_forward, "NULL", y=None)
     refused(_backward, "NULL", x=None)
     refused(_backward, "NULL", u=None)
-    need = lib.ops3d_linear_backward_workspace_bytes(2, 1, 100000, 1, 256, 256, 0)
+    need = lib.ops3d_linear_backward_workspace_bytes(2, 1, 100000, 1, 256, 256, 0, 0)
     assert need > 0 and need % 256 == 0
     refused(_backward, "workspace too small", rows=100000, N=256, K=256)
     refused(_backward, "workspace too small", rows=100000, N=256, K=256, ws=p, ws_bytes=need - 1)
@@ -208,7 +208,10 @@ def test_c_refusals_before_device_work(lib):
 
 
 def test_workspace_sizes(lib):
-    f = lib.ops3d_linear_backward_workspace_bytes
+    def f(*args, act=0):
+        return lib.ops3d_linear_backward_workspace_bytes(*args, act)
+
+    assert f(2, 1, 4, 1, 8, 8, 0, act=1) == 256            # dz
     assert f(2, 1, 4, 1, 8, 8, 0) == 0                     # one chunk: results are written at once
     assert f(2, 1, 0, 1, 8, 8, 0) == 0 and f(9, 1, 4, 1, 8, 8, 0) == 0 and f(2, 1, 4, 2, 8, 8, 0) == 0
     assert f(2, 1, 16384, 64, 1024, 512, 1) == 0           # as many groups as chunks are wanted
