@@ -48,8 +48,8 @@ extern "C" {
 #define OPS3D_LINEAR_ACT_SILU 4      /* z / (1 + exp(-z)) */
 #define OPS3D_LINEAR_MAX_GROUPS 4096
 
-/* Bytes of device workspace (256-byte aligned) the forward needs: 0 for most sizes and for invalid
- * ones. */
+/* Bytes of device workspace (256-byte aligned) the forward needs: parts of long sums over few tiles; 0
+ * for other sizes and for invalid ones. */
 OPS3D_FDA_API size_t ops3d_linear_forward_workspace_bytes(int dtype, int batch, int64_t rows, int groups,
                                                           int out_features, int in_features, int grouped);
 
@@ -60,8 +60,8 @@ OPS3D_FDA_API int ops3d_linear_forward(const void *x, int64_t ld_x, const void *
                                        size_t workspace_bytes, int dtype, int act, int batch, int64_t rows, int groups,
                                        int out_features, int in_features, void *stream);
 
-/* Bytes of device workspace (256-byte aligned) the backward needs when it gives grad_weight or
- * grad_bias (otherwise none): dz (with an act_grad) and the partial sums over chunks of rows. */
+/* Bytes of device workspace (256-byte aligned) the backward needs: dz (with an act_grad) and partial
+ * sums, of grad_x over parts of long sums and of grad_weight over chunks of rows. */
 OPS3D_FDA_API size_t ops3d_linear_backward_workspace_bytes(int dtype, int batch, int64_t rows, int groups,
                                                            int out_features, int in_features, int grouped,
                                                            int with_act_grad);

@@ -163,7 +163,7 @@ class _NativeFDA:
             for name in ("flash_deform_attn_forward", "flash_deform_attn_backward",
                          "forward_keep_head_major", "backward_with_head_major",
                          "forward_offsets", "backward_offsets", "nms_3d", "roi_align_3d_forward",
-                         "roi_align_3d_backward", "dcnv4_forward", "dcnv4_backward", "linear_forward",
+                         "roi_align_3d_backward", "dcnv4_forward", "dcnv4_backward", "linear", "linear_forward",
                          "linear_backward"):
                 setattr(self, name, getattr(ext, name))
 
@@ -270,6 +270,14 @@ class _NativeFDA:
             raise ValueError(f"group_start must have {groups} or {groups + 1} entries, got {count}")
         return rows.shape[0] if rows.dim() == 3 else 1, rows.shape[-2], groups, group_start, count
 
+    def linear(self, x, weight, bias, residual, group_start, act):
+        """The operator through autograd (LinearFunction where a gradient is wanted)."""
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+            from .linear import LinearFunction
+
+            return LinearFunction.apply(x, weight, bias, residual, group_start, act, self)
+        return self.linear_forward(x, weight, bias, residual, group_start, act, False)[0]
+
     def linear_forward(self, x, weight, bias, residual, group_start, act, keep):
         """(y, act_grad); act_grad (None without an activation) when ``keep``."""
         self._linear_check("x", x, x)
@@ -346,8 +354,7 @@ class _NativeFDA:
 
         gx, gw, gb = empty(weight is not None, shape), empty(need_w, wshape), empty(need_b, wshape[:-1])
         code = _DTYPE_CODE[grad_y.dtype]
-        n = (self._lib.ops3d_linear_backward_workspace_bytes(code, B, S, E, N, K, int(grouped), int(act_grad is not None))
-             if need_w or need_b else 0)
+        n = self._lib.ops3d_linear_backward_workspace_bytes(code, B, S, E, N, K, int(grouped), int(act_grad is not None))
         ws = torch.empty(n, dtype=torch.uint8, device=grad_y.device) if n else None
         with torch.cuda.device(grad_y.device):
             rc = self._lib.ops3d_linear_backward(

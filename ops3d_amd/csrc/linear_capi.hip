@@ -66,16 +66,48 @@ ChunkPlan plan_of(int dtype, bool grouped, int batch, int64_t rows, int groups, 
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Workspace of the backward: dz (behind an activation) and the chunks' partial sums.
+bool sizes_ok(int dtype, int batch, int64_t rows, int groups, int N, int K, bool grouped) {
+  return elem_size(dtype) != 0 && batch >= 1 && rows >= 1 && rows <= kMaxRows / batch && groups >= 1 &&
+         groups <= OPS3D_LINEAR_MAX_GROUPS && N >= 1 && K >= 1 && N <= kMaxFeatures && K <= kMaxFeatures &&
+         (grouped || groups == 1);
+}
+
+// Bytes of the parts of a rows kernel's split sums.
+size_t split_bytes(int dtype, int64_t rows, int groups, int N, int K) {
+  const int n = split_count(elem_size(dtype), rows, groups, N, K);
+  return n > 1 ? align256((size_t)n * rows * N * 4) : 0;
+}
+void set_split(RowsArgs &p, bool on, void *part, int dtype, int64_t rows, int groups) {
+  p.rows = rows;
+  p.splits = 1;
+  if (!on) return;
+  const int kc = 128 / elem_size(dtype);
+  p.splits = split_count(elem_size(dtype), rows, groups, p.N, p.K);
+  p.per_split = ceil_div(ceil_div(p.K, kc), p.splits) * kc;
+  p.part = static_cast<float *>(part);
+}
+
+int check_workspace(const void *workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need))
+    return fail(OPS3D_FDA_EINVAL, "workspace too small: %zu bytes given, %zu needed", bytes, need);
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return fail(OPS3D_FDA_EINVAL, "workspace must be 256-byte aligned");
+  return OPS3D_FDA_OK;
+}
+
+// Workspace of the backward: dz (behind an activation), then the parts of the input gradient's split
+// sums and, after it and in the same place, the chunks' partial sums.
 struct Layout {
   ChunkPlan plan;
-  size_t dz, part, part_b, bytes;
+  size_t dz, part, part_b, split, bytes;
   Layout(int dtype, bool grouped, int batch, int64_t rows, int groups, int N, int K, bool with_dz)
       : plan(plan_of(dtype, grouped, batch, rows, groups, N, K)) {
     dz = 0;
     part = with_dz ? align256((size_t)batch * rows * N * elem_size(dtype)) : 0;
     part_b = part + (plan.joined ? align256((size_t)plan.slots * N * K * 4) : 0);
     bytes = part_b + (plan.joined ? align256((size_t)plan.slots * N * 4) : 0);
+    split = rows > 0 && batch > 0 ? split_bytes(dtype, batch * rows, groups, K, N) : 0;
+    if (bytes < part + split) bytes = part + split;
   }
 };
 
@@ -91,11 +123,16 @@ bool misaligned(const void *p, int esize) { return reinterpret_cast<uintptr_t>(p
 
 extern "C" {
 
-size_t ops3d_linear_forward_workspace_bytes(int, int, int64_t, int, int, int, int) { return 0; }
+size_t ops3d_linear_forward_workspace_bytes(int dtype, int batch, int64_t rows, int groups, int out_features,
+                                            int in_features, int grouped) {
+  if (!sizes_ok(dtype, batch, rows, groups, out_features, in_features, grouped != 0) || batch * rows / groups <= kFewRows)
+    return 0;
+  return split_bytes(dtype, batch * rows, groups, out_features, in_features);
+}
 
 int ops3d_linear_forward(const void *x, int64_t ld_x, const void *weight, const void *bias, const void *residual,
                          int64_t ld_residual, const int64_t *group_start, int group_start_count, void *y, void *act_grad,
-                         void *, size_t, int dtype, int act, int batch, int64_t rows, int groups, int out_features,
+                         void *workspace, size_t workspace_bytes, int dtype, int act, int batch, int64_t rows, int groups, int out_features,
                          int in_features, void *stream) {
   ops3d_fda::set_last_error(OPS3D_FDA_OK, "");
   int rc = check_sizes(dtype, batch, rows, groups, out_features, in_features);
@@ -124,15 +161,16 @@ int ops3d_linear_forward(const void *x, int64_t ld_x, const void *weight, const 
   p.act = act;
   p.N = out_features;
   p.K = in_features;
+  const size_t need = ops3d_linear_forward_workspace_bytes(dtype, batch, rows, groups, out_features, in_features,
+                                                           group_start != nullptr);
+  if ((rc = check_workspace(workspace, workspace_bytes, need))) return rc;
+  set_split(p, need != 0, workspace, dtype, batch * rows, groups);
   return run(dtype, "linear forward", [&](auto t) { return ops3d_linear::forward<decltype(t)>(p, static_cast<hipStream_t>(stream)); });
 }
 
 size_t ops3d_linear_backward_workspace_bytes(int dtype, int batch, int64_t rows, int groups, int out_features,
                                              int in_features, int grouped, int with_act_grad) {
-  if (elem_size(dtype) == 0 || batch < 1 || rows < 1 || rows > kMaxRows / batch || groups < 1 ||
-      groups > OPS3D_LINEAR_MAX_GROUPS || out_features < 1 || in_features < 1 || out_features > kMaxFeatures ||
-      in_features > kMaxFeatures || (!grouped && groups != 1))
-    return 0;
+  if (!sizes_ok(dtype, batch, rows, groups, out_features, in_features, grouped != 0)) return 0;
   return Layout(dtype, grouped != 0, batch, rows, groups, out_features, in_features, with_act_grad != 0).bytes;
 }
 
@@ -156,11 +194,7 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Layout lay(dtype, group_start != nullptr, batch, empty ? 0 : rows, groups, out_features, in_features,
                    act_grad != nullptr);
-  const size_t need = wants_w && !empty ? lay.bytes : 0;
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(OPS3D_FDA_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
-  if (need && (reinterpret_cast<uintptr_t>(workspace) & 255u))
-    return fail(OPS3D_FDA_EINVAL, "workspace must be 256-byte aligned");
+  if ((rc = check_workspace(workspace, workspace_bytes, empty || (!grad_x && !wants_w) ? 0 : lay.bytes))) return rc;
   char *const ws = static_cast<char *>(workspace);
   void *const dz = wants_w && act_grad && !empty ? ws + lay.dz : nullptr;
   if (grad_x && !empty) {
@@ -175,6 +209,7 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
     p.N = in_features;
     p.K = out_features;
     p.g = g;
+    set_split(p, lay.split != 0, ws + lay.part, dtype, batch * rows, groups);
     rc = run(dtype, "linear input gradient", [&](auto t) { return ops3d_linear::grad_x<decltype(t)>(p, st); });
   } else if (dz) {
     rc = run(dtype, "linear gradient", [&](auto t) {
@@ -193,7 +228,7 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
   p.K = in_features;
   p.chunk = lay.plan.chunk;
   p.slots = empty ? 0 : (int)lay.plan.slots;
-  if (need && lay.plan.joined) {
+  if (!empty && lay.plan.joined) {
     p.part = reinterpret_cast<float *>(ws + lay.part);
     p.part_b = reinterpret_cast<float *>(ws + lay.part_b);
   }

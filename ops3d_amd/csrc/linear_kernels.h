@@ -48,6 +48,9 @@ struct RowsArgs {
   int col_tiles;
   int row_tiles;          // bound on the number of row tiles
   int spread;             // row tiles over XCDs (see block_tile)
+  int splits, per_split;  // parts of the sum, and elements of each (SPLIT kernels)
+  float *part;            // their sums [splits, rows, N]
+  int64_t rows;           // of all items
   Groups g;
 };
 
@@ -599,11 +602,30 @@ __device__ __forceinline__ void finish_tile(const RowsArgs &p, const f32x4 (&acc
   }
 }
 
+// The results of a wave as one part of a split sum.
+template <typename T, int MI, int NI>
+__device__ __forceinline__ void store_parts(const RowsArgs &p, const f32x4 (&acc)[MI][NI], const RowTile &tile, int r0,
+                                            int col0, int part) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    const int row = r0 + m * 16 + (lane & 15);
+    if (row >= tile.rows) continue;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int col = col0 + column_of<T>(n, (lane >> 4) * 4);
+      if (col < p.N)
+        store_chunk<float>(p.part + (part * p.rows + tile.first + row) * p.N + col, __builtin_bit_cast(uint4, acc[m][n]), p.N - col);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // c = epilogue(a w^T) (WSTR = false, w [N, K]) or a w (WSTR = true, w [K, N]) over tiles of BM rows
 // and BN columns, WR x WC waves.  SCALE: a is grad_y * act_grad, and the first column's tiles store
-// it for the weights' gradients.
-template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI>
+// it for the weights' gradients.  SPLIT: a block sums a part of the sum's axis only and stores it for
+// split_join_kernel, where the tiles alone do not fill the CUs.
+template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void rows_kernel(RowsArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
   typedef Stage<T, BM, NT, false> SA;
@@ -612,8 +634,9 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   constexpr int kStage = SA::kBytes + SB::kBytes;
   __shared__ __attribute__((aligned(16))) char lds[BUFS * kStage];
 
+  const int part = SPLIT ? blockIdx.x % p.splits : 0;
   int rt, ct;
-  block_tile(blockIdx.x, p.col_tiles, p.spread, rt, ct);
+  block_tile(SPLIT ? blockIdx.x / p.splits : blockIdx.x, p.col_tiles, p.spread, rt, ct);
   if (rt >= p.row_tiles) return;
   RowTile tile;
   if (!find_row_tile(p.g, rt, BM, tile)) return;
@@ -633,12 +656,13 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
     const T *w = static_cast<const T *>(p.w) + tile.e * p.w_group + (WSTR ? (int64_t)n0 : (int64_t)n0 * p.K);
     const int64_t ldw = WSTR ? p.N : p.K;
     const int wrows = WSTR ? p.K : p.N - n0, wcols = WSTR ? p.N - n0 : p.K;
+    const int first = SPLIT ? part * p.per_split : 0, end = SPLIT ? min(p.K, first + p.per_split) : p.K;
     uint4 va[SA::NL], vd[SA::NL], vb[SB::NL];
-    SA::load(va, a, p.lda, tile.rows, p.K, 0);
-    if (SCALE) SA::load(vd, scale, p.K, tile.rows, p.K, 0);
-    SB::load(vb, w, ldw, wrows, wcols, 0);
+    SA::load(va, a, p.lda, tile.rows, p.K, first);
+    if (SCALE) SA::load(vd, scale, p.K, tile.rows, p.K, first);
+    SB::load(vb, w, ldw, wrows, wcols, first);
     int buf = 0;
-    for (int k0 = 0; k0 < p.K; k0 += SA::KC) {
+    for (int k0 = first; k0 < end; k0 += SA::KC) {
       if (BUFS == 1) __syncthreads();
       char *const at = lds + (BUFS == 1 ? 0 : buf * kStage);
       if (SCALE) {
@@ -651,7 +675,7 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
       }
       SA::store(at, va);
       SB::store(at + SA::kBytes, vb);
-      if (k0 + SA::KC < p.K) {
+      if (k0 + SA::KC < end) {
         SA::load(va, a, p.lda, tile.rows, p.K, k0 + SA::KC);
         if (SCALE) SA::load(vd, scale, p.K, tile.rows, p.K, k0 + SA::KC);
         SB::load(vb, w, ldw, wrows, wcols, k0 + SA::KC);
@@ -674,6 +698,10 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
     }
   }
 
+  if constexpr (SPLIT) {
+    if (tile.e >= 0) store_parts<T, MI, NI>(p, acc, tile, wr * TM, n0 + wc * TN, part);
+    return;
+  }
   if (EPI && p.bias && tile.e >= 0) {
     constexpr int CH = 16 / (int)sizeof(T), NP = CH / 4;
 #pragma unroll
@@ -688,6 +716,58 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   }
   if (tile.rows >= BM && n0 + BN <= p.N) finish_tile<T, MI, NI, EPI, true>(p, acc, tile, wr * TM, n0 + wc * TN, threadIdx.x & 63);
   else finish_tile<T, MI, NI, EPI, false>(p, acc, tile, wr * TM, n0 + wc * TN, threadIdx.x & 63);
+}
+
+// Joins the parts of split sums in order, with the epilogue; zeros for rows of no group.  A block has 64
+// rows and 64 columns.
+template <typename T, bool EPI> __global__ __launch_bounds__(256) void split_join_kernel(RowsArgs p) {
+  constexpr int CH = 16 / (int)sizeof(T), PC = 64 / CH;
+  typedef typename Deriv<T>::type D;
+  RowTile tile;
+  if (!find_row_tile(p.g, blockIdx.x / p.col_tiles, 64, tile)) return;
+  const int n0 = blockIdx.x % p.col_tiles * 64;
+  for (int c = threadIdx.x; c < 64 * PC; c += 256) {
+    const int row = c / PC, col = n0 + c % PC * CH, left = p.N - col;
+    if (row >= tile.rows || left <= 0) continue;
+    const int64_t at = (tile.first + row) * p.N + col;
+    float z[CH], d[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) z[i] = 0.f;
+    if (tile.e >= 0) {
+      for (int s = 0; s < p.splits; ++s) {
+        const float *src = p.part + s * p.rows * p.N + at;
+#pragma unroll
+        for (int i = 0; i < CH; i += 4) {
+          const uint4 v = fetch(src + i, 0, 0, 0, 1, left - i);
+          z[i] += __uint_as_float(v.x);
+          z[i + 1] += __uint_as_float(v.y);
+          z[i + 2] += __uint_as_float(v.z);
+          z[i + 3] += __uint_as_float(v.w);
+        }
+      }
+      if (EPI) {
+        if (p.bias) {
+          Chunk<T> b;
+          b.raw = fetch(static_cast<const T *>(p.bias) + (int64_t)tile.e * p.N, 0, 0, col, 1, p.N);
+#pragma unroll
+          for (int i = 0; i < CH; ++i) z[i] += (float)b.e[i];
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) z[i] = activate<sizeof(T) == 2>(p.act, z[i], d[i]);
+        if (p.act_grad) store_chunk<D, true>(static_cast<D *>(p.act_grad) + at, Deriv<T>::encode(d), left);
+        if (p.res) {
+          Chunk<T> r;
+          r.raw = fetch(static_cast<const T *>(p.res) + (tile.first + row) * p.ld_res, 0, 0, col, 1, p.N);
+#pragma unroll
+          for (int i = 0; i < CH; ++i) z[i] += (float)r.e[i];
+        }
+      }
+    }
+    Chunk<T> out;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) out.e[i] = (T)z[i];
+    store_chunk<T>(static_cast<T *>(p.c) + at, out.raw, left);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -901,14 +981,25 @@ template <typename K> inline hipError_t launch(K kernel, int64_t grid, int threa
   return hipGetLastError();
 }
 
-template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI>
+template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT = false>
 inline hipError_t launch_rows(RowsArgs p, hipStream_t st) {
   const int64_t rt = max_row_tiles(p.g, BM);
   p.row_tiles = (int)rt;
   p.col_tiles = ceil_div(p.N, BN);
   p.spread = rt >= 64;
-  const int64_t grid = (p.spread ? (rt + 7) / 8 * 8 : rt) * p.col_tiles;
-  return launch(rows_kernel<T, BM, BN, WR, WC, BUFS, OCC, WSTR, SCALE, EPI>, grid, 64 * WR * WC, st, p);
+  const int64_t grid = (p.spread ? (rt + 7) / 8 * 8 : rt) * p.col_tiles * (SPLIT ? p.splits : 1);
+  return launch(rows_kernel<T, BM, BN, WR, WC, BUFS, OCC, WSTR, SCALE, EPI, SPLIT>, grid, 64 * WR * WC, st, p);
+}
+
+// How many parts a sum of K elements is cut into, by tiles of 64 x 64: none where the tiles make 256
+// blocks or there are less than 8 stages; otherwise parts of 4 stages or more, up to 512 blocks.
+// (bf16, one row of dz, 3301 -> 1856: 16 us, 100 in one part.)
+inline int split_count(int esize, int64_t rows, int E, int N, int K) {
+  const int stages = ceil_div(K, 128 / esize);
+  const int64_t tiles = (ceil_div(rows, 64) + (E > 1 ? E : 0)) * (int64_t)ceil_div(N, 64);
+  if (tiles >= 256 || stages < 8) return 1;
+  int64_t parts = 512 / tiles < stages / 4 ? 512 / tiles : stages / 4;
+  return parts < 2 ? 1 : ceil_div(stages, ceil_div(stages, parts));
 }
 
 template <typename T, int RT, int NW> inline hipError_t launch_few(RowsArgs p, hipStream_t st) {
@@ -919,7 +1010,7 @@ template <typename T, int RT, int NW> inline hipError_t launch_few(RowsArgs p, h
 }
 
 template <typename T, bool WSTR, bool SCALE, bool EPI> inline hipError_t launch_tiles(const RowsArgs &p, hipStream_t st) {
-  const int64_t rows = (int64_t)p.g.B * p.g.S;
+  const int64_t rows = p.rows;
   if constexpr (sizeof(T) == 2 && !SCALE) {
     // one block of 256 x 256 a CU: long sums (4096^3 bf16 145 us, 195 with 128 x 128), or outputs of many
     // tiles, where the operands' second and third reading costs most (598016 x 256 -> 1024 590 and 680 us,
@@ -933,14 +1024,24 @@ template <typename T, bool WSTR, bool SCALE, bool EPI> inline hipError_t launch_
     if constexpr (SCALE) return launch_rows<T, 64, 128, 1, 4, 1, 4, WSTR, SCALE, EPI>(p, st);
     else return launch_rows<T, 128, 128, 2, 2, 1, 3, WSTR, SCALE, EPI>(p, st);
   }
+  if (p.splits > 1) {
+    const hipError_t e = launch_rows<T, 64, 64, 2, 2, 1, 4, WSTR, SCALE, EPI, true>(p, st);
+    if (e != hipSuccess) return e;
+    RowsArgs j = p;
+    j.col_tiles = ceil_div(p.N, 64);
+    return launch(split_join_kernel<T, EPI>, max_row_tiles(p.g, 64) * j.col_tiles, 256, st, j);
+  }
   return launch_rows<T, 64, 64, 2, 2, 1, 4, WSTR, SCALE, EPI>(p, st);
 }
 
+// Rows a group up to which the forward takes the kernel for few rows.
+constexpr int kFewRows = 64;
+
 template <typename T> hipError_t forward(const RowsArgs &p, hipStream_t st) {
-  const int64_t per_group = (int64_t)p.g.B * p.g.S / p.g.E;
+  const int64_t per_group = p.rows / p.g.E;
   if (per_group <= 16) return p.K >= 2048 ? launch_few<T, 1, 8>(p, st) : launch_few<T, 1, 4>(p, st);
   if (per_group <= 32) return p.K >= 2048 ? launch_few<T, 2, 8>(p, st) : launch_few<T, 2, 4>(p, st);
-  if (per_group <= 64) return p.K >= 2048 ? launch_few<T, 4, 8>(p, st) : launch_few<T, 4, 4>(p, st);
+  if (per_group <= kFewRows) return p.K >= 2048 ? launch_few<T, 4, 8>(p, st) : launch_few<T, 4, 4>(p, st);
   return launch_tiles<T, false, false, true>(p, st);
 }
 

@@ -8,6 +8,7 @@
 // Errors: a failed check or an OPS3D_FDA_EINVAL from the library raises ValueError
 // (std::invalid_argument, as the reference's), OPS3D_FDA_ERUNTIME raises RuntimeError.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 // torch's current HIP stream of a device (c10's native HIP API); the device is made current
 // with HIP's own calls (DeviceGuard below)
@@ -614,9 +615,8 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
   if (weight) gx = at::empty(shape, grad_y.options());
   if (need_w) gw = at::empty(wshape, grad_y.options());
   if (need_b) gb = at::empty(grouped ? std::vector<int64_t>{groups, N} : std::vector<int64_t>{N}, grad_y.options());
-  const size_t n = need_w || need_b ? ops3d_linear_backward_workspace_bytes(z.code, z.batch, z.rows, z.groups, z.N, z.K,
-                                                                            grouped, act_grad.has_value())
-                                    : 0;
+  const size_t n = ops3d_linear_backward_workspace_bytes(z.code, z.batch, z.rows, z.groups, z.N, z.K, grouped,
+                                                         act_grad.has_value());
   at::Tensor ws;
   if (n) ws = at::empty({(int64_t)n}, grad_y.options().dtype(at::kByte));
   const int rc = ops3d_linear_backward(ptr(xr), ldx, ptr(w), z.start, z.count, act_grad ? ptr(*act_grad) : nullptr, ptr(g),
@@ -624,6 +624,65 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
                                        ptr(ws), n, z.code, z.batch, z.rows, z.groups, z.N, z.K, stream_of(grad_y));
   if (rc != OPS3D_FDA_OK) raise(rc, "linear_backward failed");
   return {gx, gw, gb};
+}
+
+// The operator with its autograd node here: a training step on a small crop is bound by host time, of
+// which a node in Python costs several times as much.  Once differentiable: with create_graph the
+// gradients raise when they are differentiated.
+class LinearNode : public torch::autograd::Function<LinearNode> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight,
+                            const c10::optional<at::Tensor> &bias, const c10::optional<at::Tensor> &residual,
+                            const c10::optional<at::Tensor> &group_start, int64_t act) {
+    const bool need_x = x.requires_grad(), need_w = weight.requires_grad(), need_b = bias && bias->requires_grad();
+    auto [y, act_grad] = linear_forward(x, weight, bias, residual, group_start, act, need_x || need_w || need_b);
+    ctx->save_for_backward({need_w || need_b ? x : at::Tensor(), need_x ? weight : at::Tensor(),
+                            group_start ? *group_start : at::Tensor(), act_grad ? *act_grad : at::Tensor()});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{weight.size(-1), weight.dim() == 3 ? weight.size(0) : 0, need_x,
+                                                    need_w, need_b, residual && residual->requires_grad()};
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const at::Tensor &grad = grads[0];
+    torch::autograd::variable_list out(6);
+    const auto some = [](const at::Tensor &t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+    const bool once = at::GradMode::is_enabled() && grad.requires_grad();
+    {
+      const at::NoGradGuard no_grad;
+      if (sizes[2] || sizes[3] || sizes[4]) {
+        auto [gx, gw, gb] = linear_backward(some(saved[0]), some(saved[1]), some(saved[2]), some(saved[3]), grad, sizes[0],
+                                            sizes[1], sizes[3], sizes[4]);
+        if (gx) out[0] = *gx;
+        if (gw) out[1] = *gw;
+        if (gb) out[2] = *gb;
+      }
+      if (sizes[5]) out[3] = grad;
+    }
+    if (once) {
+      torch::autograd::variable_list given;
+      for (const auto &t : out)
+        if (t.defined()) given.push_back(t.detach().set_requires_grad(true));
+      const auto error = std::make_shared<torch::autograd::DelayedError>(
+          "trying to differentiate twice a linear operator that is differentiable once", (int64_t)given.size());
+      given = (*error)(std::move(given));
+      size_t i = 0;
+      for (auto &t : out)
+        if (t.defined()) t = given[i++];
+    }
+    return out;
+  }
+};
+
+at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const c10::optional<at::Tensor> &bias,
+                  const c10::optional<at::Tensor> &residual, const c10::optional<at::Tensor> &group_start, int64_t act) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
+                                     (residual && residual->requires_grad())))
+    return LinearNode::apply(x, weight, bias, residual, group_start, act);
+  return std::get<0>(linear_forward(x, weight, bias, residual, group_start, act, false));
 }
 
 }  // namespace
@@ -645,6 +704,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dcnv4_forward", &dcnv4_forward, "dcnv4_forward");
   m.def("dcnv4_backward", &dcnv4_backward, "dcnv4_backward");
   m.def("linear_forward", &linear_forward, "act(x W^T + b) + residual, one weight or one per group of rows");
+  m.def("linear", &linear, "linear_forward with its gradients through autograd");
   m.def("linear_backward", &linear_backward, "gradients of linear_forward");
   m.def("roi_align_3d_forward", &roi_align_3d_forward, "roi_align_3d_forward");
   m.def("roi_align_3d_backward", &roi_align_3d_backward, "roi_align_3d_backward");

@@ -24,22 +24,17 @@ from . import _extension
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
-def _native(what):
-    if _extension._C is None:
-        raise RuntimeError(f"ops3d_amd native library (libops3d_fda.so) not built; {what} requires it.")
-    return _extension._C
-
-
 class LinearFunction(Function):
-    """Autograd of both operators; ``group_start`` None is the plain product."""
+    """Autograd of both operators for the binding without the extension module (which has its own node);
+    ``group_start`` None is the plain product, ``native`` the binding."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, group_start, act):
+    def forward(ctx, x, weight, bias, residual, group_start, act, native):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        y, act_grad = _native("linear").linear_forward(x, weight, bias, residual, group_start, act,
-                                                       need_x or need_w or need_b)
+        y, act_grad = native.linear_forward(x, weight, bias, residual, group_start, act, need_x or need_w or need_b)
         ctx.save_for_backward(x if need_w or need_b else None, weight if need_x else None, group_start, act_grad)
         ctx.in_features, ctx.groups = weight.shape[-1], weight.shape[0] if weight.dim() == 3 else 0
+        ctx.native = native
         return y
 
     @staticmethod
@@ -49,9 +44,9 @@ class LinearFunction(Function):
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         grad_x = grad_w = grad_b = None
         if need_x or need_w or need_b:
-            grad_x, grad_w, grad_b = _native("linear").linear_backward(
+            grad_x, grad_w, grad_b = ctx.native.linear_backward(
                 x, weight, group_start, act_grad, grad_output, ctx.in_features, ctx.groups, need_w, need_b)
-        return grad_x, grad_w, grad_b, grad_output if need_r else None, None, None
+        return grad_x, grad_w, grad_b, grad_output if need_r else None, None, None, None
 
 
 def _apply(x, weight, bias, residual, group_start, activation):
@@ -70,11 +65,9 @@ def _apply(x, weight, bias, residual, group_start, activation):
 
 
 def _run(x, weight, bias, residual, group_start, act):
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        return LinearFunction.apply(x, weight, bias, residual, group_start, act)
-    return _native("linear").linear_forward(x, weight, bias, residual, group_start, act, False)[0]
+    if _extension._C is None:
+        raise RuntimeError("ops3d_amd native library (libops3d_fda.so) not built; the linear operators require it.")
+    return _extension._C.linear(x, weight, bias, residual, group_start, act)
 
 
 def fused_linear(x, weight, bias=None, activation=None, residual=None):

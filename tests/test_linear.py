@@ -267,6 +267,16 @@ def test_linear_large(gpu_device, dtype, rows, K, N):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,K,N", [(1, 1856, 3301), (70, 3000, 100), (130, 1111, 72), (300, 640, 1100), (65, 129, 2000)])
+def test_linear_long_sums(gpu_device, rows, K, N, dtype):
+    """Sums that are cut into parts, of the forward or of the input gradient, and joined."""
+    log(f"[case] linear long sums {rows}x{K}->{N} {dtype}")
+    linear_case(rows, K, N, DTYPES[dtype], "gelu", with_residual=True)
+    linear_case(rows, K, N, DTYPES[dtype], None, with_bias=False)
+
+
+@gpu
 @pytest.mark.parametrize("want", ["x", "w", "b", "r", "xb"])
 def test_linear_some_gradients(gpu_device, want):
     """Only the gradients that are asked for, each as it is with the others."""
@@ -438,6 +448,7 @@ GROUPS = [
     (900, [min(i * i // 10, 880) for i in range(130)], 130, 2),
     (40000, [0, 34990, 39400], 3, 0),
     (30000, [100, 25000, 25001, 29999], 3, 2),
+    (150, [3, 70, 70, 149], 3, 2),                  # with 1500 features: sums in parts
 ]
 
 
@@ -446,7 +457,7 @@ GROUPS = [
 @pytest.mark.parametrize("case", range(len(GROUPS)))
 def test_grouped_sizes(gpu_device, case, dtype):
     S, start, groups, batch = GROUPS[case]
-    K, N = [(40, 24), (64, 64), (33, 70), (136, 129)][case % 4]
+    K, N = (1500, 900) if case == 11 else [(40, 24), (64, 64), (33, 70), (136, 129)][case % 4]
     act = list(ACTIVATIONS)[case % 5]
     log(f"[case] grouped {case}: {S} rows, {groups} groups, batch {batch}, {K}->{N} {act} {dtype}")
     grouped_case(S, start, groups, K, N, DTYPES[dtype], act, batch, with_bias=case != 5, with_residual=case % 2 == 0)
@@ -540,6 +551,7 @@ def test_refusals(gpu_device):
 def test_ctypes_binding_gives_the_same(gpu_device, dtype):
     """The binding without the extension module: the same bits."""
     C, N = _extension._C, type(_extension._C)
+    bare = N(C._lib, C.__file__)   # without the extension module's functions
     gen = torch.Generator(device="cuda").manual_seed(13)
     dt = DTYPES[dtype]
     x, w, b = make(gen, (2, 300, 40), dt), make(gen, (3, 24, 40), dt), make(gen, (3, 24), dt)
@@ -554,6 +566,16 @@ def test_ctypes_binding_gives_the_same(gpu_device, dtype):
         back = (x, args[1], args[4], want[1], u, 40, 3 if args[4] is not None else 0, True, True)
         for g, e in zip(N.linear_backward(C, *back), C.linear_backward(*back)):
             assert torch.equal(g, e)
+        grads = []
+        for f in (C.linear, lambda *a: N.linear(bare, *a)):
+            leaves = [t.detach().requires_grad_(True) for t in args[:4]]
+            y = f(*leaves, args[4], 2)
+            assert torch.equal(y, want[0])
+            grads.append(torch.autograd.grad(y, leaves, u.clone().requires_grad_(True), create_graph=True))
+            with pytest.raises(RuntimeError, match="differentiate twice"):
+                grads[-1][0].sum().backward()
+        for a, e in zip(*grads):
+            assert torch.equal(a, e)
 
 
 @gpu
