@@ -192,7 +192,7 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
       misaligned(grad_x, es) || misaligned(grad_weight, es) || misaligned(grad_bias, es))
     return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const Layout lay(dtype, group_start != nullptr, batch, empty ? 0 : rows, groups, out_features, in_features,
+  const Layout lay(dtype, group_start != nullptr, empty ? 1 : batch, empty ? 0 : rows, groups, out_features, in_features,
                    act_grad != nullptr);
   if ((rc = check_workspace(workspace, workspace_bytes, empty || (!grad_x && !wants_w) ? 0 : lay.bytes))) return rc;
   char *const ws = static_cast<char *>(workspace);
@@ -227,12 +227,13 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
   p.N = out_features;
   p.K = in_features;
   p.chunk = lay.plan.chunk;
-  p.slots = empty ? 0 : (int)lay.plan.slots;
+  p.slots = (int)lay.plan.slots;
   if (!empty && lay.plan.joined) {
     p.part = reinterpret_cast<float *>(ws + lay.part);
     p.part_b = reinterpret_cast<float *>(ws + lay.part_b);
   }
   p.g = g;
+  if (empty) p.g.B = 1, p.g.S = 0;   // one chunk of no rows a group
   return run(dtype, "linear weight gradient", [&](auto t) {
     return ops3d_linear::grad_weight<decltype(t)>(p, lay.plan.tile, !empty && lay.plan.joined, st);
   });

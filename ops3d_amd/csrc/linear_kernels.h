@@ -385,11 +385,12 @@ struct RowChunk {
   int slot;         // of this group's first chunk
 };
 
-// Chunk t of `chunk` rows, counted over groups, items and steps.  by_group: the chunks of group t
-// instead (first and rows not set; false never).
+// Chunk t of `chunk` rows, counted over groups, items and steps; a group without rows has one of no rows
+// in each item, which writes its zeros.  by_group: the chunks of group t instead (first and rows not
+// set; false never).
 __device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, bool by_group, RowChunk &out) {
   if (!g.start) {
-    const int n = (g.S + chunk - 1) / chunk;
+    const int n = max(1, (g.S + chunk - 1) / chunk);
     out.e = 0;
     out.chunks = n;
     out.slot = 0;
@@ -404,7 +405,7 @@ __device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, bo
   for (int base = 0; base < g.E + 2; base += 64) {
     const int j = base + lane;
     const Segment s = segment_at(g, j, carry);
-    const int per = j >= 1 && j <= g.E ? (s.upper - s.lower + chunk - 1) / chunk : 0;   // per item
+    const int per = j >= 1 && j <= g.E ? max(1, (s.upper - s.lower + chunk - 1) / chunk) : 0;   // per item
     const int n = per * g.B;
     const int incl = before + scan_add(n);
     const uint64_t m = __ballot(by_group ? j == t + 1 : incl > t);
@@ -487,10 +488,41 @@ template <typename T, int R, int NT, bool STRIDED> struct Stage {
   // octet reads in the order of column_of (4 h + 0 .. 3 of two groups of 8), fall on 8 different chunks.
   // STRIDED: the 4 matrix rows that 16 lanes read (fp32: the rows that the lane quarters read) fall on
   // different chunks, for columns that follow each other and for those of column_of.
-  static __device__ __forceinline__ int address(int row, int col) {
-    if (!STRIDED) return row * 128 + ((col ^ ((row & 3) | (((row >> 2) ^ (row >> 3)) & 1) << 2)) << 4);
-    constexpr int kShift = sizeof(T) == 4 || NC >= 16 ? 2 : 1;
-    return row * (R * (int)sizeof(T)) + ((col ^ (sizeof(T) == 2 ? row & 3 : (row >> 2) & 3) << kShift) << 4);
+  static __device__ __forceinline__ int swizzle(int row) {
+    if (!STRIDED) return (row & 3) | (((row >> 2) ^ (row >> 3)) & 1) << 2;
+    return (sizeof(T) == 2 ? row & 3 : (row >> 2) & 3) << (sizeof(T) == 4 || NC >= 16 ? 2 : 1);
+  }
+  static __device__ __forceinline__ int address(int row, int col) { return row * kRowBytes + ((col ^ swizzle(row)) << 4); }
+
+  // A stage inside the matrix straight to LDS, without registers between: an instruction of a wave fills
+  // 1024 bytes in lane order, so the lane at a place loads the chunk that the swizzle puts there.  Needs
+  // rows that start at 16-byte boundaries and, STRIDED, cols a multiple of CH; sides beyond the matrix
+  // read its last row or chunk (their results are not stored).
+  static __device__ __forceinline__ void load_lds(char *lds, const T *base, int64_t ld, int rows, int cols, int k0) {
+    constexpr int kRowChunks = kRowBytes / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const T *at = base + (STRIDED ? (int64_t)k0 * ld : (int64_t)k0);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int slot = (wave * NL + j) * 64 + lane, row = slot / kRowChunks, col = ((slot % kRowChunks) ^ swizzle(row)) * CH;
+      const uint32_t off = STRIDED ? (uint32_t)(row * (int)ld + min(col, cols - CH))
+                                   : (uint32_t)(min(row, rows - 1) * (int)ld + col);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(at + off),
+                                       (__attribute__((address_space(3))) void *)(lds + (wave * NL + j) * 1024), 16, 0, 0);
+    }
+  }
+  // A stage that ends inside the matrix, chunk by chunk with zeros behind it.
+  static __device__ __forceinline__ void load_end(char *lds, const T *base, int64_t ld, int rows, int cols, int k0) {
+#pragma unroll 1
+    for (int c = threadIdx.x; c < R * 8; c += NT) {
+      const int row = STRIDED ? c / NC : c >> 3, col = STRIDED ? c % NC : c & 7;
+      *reinterpret_cast<uint4 *>(lds + address(row, col)) =
+          fetch(base, ld, row + (STRIDED ? k0 : 0), col * CH + (STRIDED ? 0 : k0), rows, cols);
+    }
+  }
+  static __device__ __forceinline__ void load_either(char *lds, const T *base, int64_t ld, int rows, int cols, int k0) {
+    if (k0 + KC <= (STRIDED ? rows : cols)) load_lds(lds, base, ld, rows, cols, k0);
+    else load_end(lds, base, ld, rows, cols, k0);
   }
   // MFMA operand, half `step` of the stage, of 16 output rows: r0 + row(i) for lane index i
   template <typename F> static __device__ __forceinline__ typename Type<T>::frag frag(const char *lds, int step, F row, int lane) {
@@ -625,14 +657,19 @@ __device__ __forceinline__ void store_parts(const RowsArgs &p, const f32x4 (&acc
 // and BN columns, WR x WC waves.  SCALE: a is grad_y * act_grad, and the first column's tiles store
 // it for the weights' gradients.  SPLIT: a block sums a part of the sum's axis only and stores it for
 // split_join_kernel, where the tiles alone do not fill the CUs.
-template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT>
+// U stages are loaded and multiplied at a time.  DMA: loads go straight to LDS (rows at 16-byte
+// boundaries); nothing is loaded ahead, but without registers for it more blocks fit a CU, which wait in
+// turn (4096^3 bf16: 128 x 256 120 us, 128 x 128 128; through registers and a stage ahead 192 and 181,
+// 256 x 256 152).  Otherwise loads go through registers, the next stages' while these are multiplied; so
+// does the scaled operand always.
+template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void rows_kernel(RowsArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
   typedef Stage<T, BM, NT, false> SA;
   typedef Stage<T, BN, NT, WSTR> SB;
   typedef typename Deriv<T>::type D;
   constexpr int kStage = SA::kBytes + SB::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[BUFS * kStage];
+  __shared__ __attribute__((aligned(16))) char lds[U * kStage];
 
   const int part = SPLIT ? blockIdx.x % p.splits : 0;
   int rt, ct;
@@ -657,44 +694,61 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
     const int64_t ldw = WSTR ? p.N : p.K;
     const int wrows = WSTR ? p.K : p.N - n0, wcols = WSTR ? p.N - n0 : p.K;
     const int first = SPLIT ? part * p.per_split : 0, end = SPLIT ? min(p.K, first + p.per_split) : p.K;
-    uint4 va[SA::NL], vd[SA::NL], vb[SB::NL];
-    SA::load(va, a, p.lda, tile.rows, p.K, first);
-    if (SCALE) SA::load(vd, scale, p.K, tile.rows, p.K, first);
-    SB::load(vb, w, ldw, wrows, wcols, first);
-    int buf = 0;
-    for (int k0 = first; k0 < end; k0 += SA::KC) {
-      if (BUFS == 1) __syncthreads();
-      char *const at = lds + (BUFS == 1 ? 0 : buf * kStage);
-      if (SCALE) {
+    constexpr int kStep = U * SA::KC;
+    constexpr bool kRegA = !DMA || SCALE;
+    uint4 va[kRegA ? U : 1][kRegA ? SA::NL : 1], vd[SCALE ? U : 1][SCALE ? SA::NL : 1], vb[DMA ? 1 : U][DMA ? 1 : SB::NL];
+    const auto load = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < SA::NL; ++i) {
-          va[i] = Deriv<T>::apply(va[i], vd[i]);
-          const int row = SA::row_of(i), left = p.K - k0 - SA::col_of(i);
-          if (dz && row < tile.rows && left > 0) store_chunk<T>(dz + (int64_t)row * p.K + k0 + SA::col_of(i), va[i], left);
+      for (int u = 0; u < U; ++u) {
+        if (u && k0 + u * SA::KC >= end) break;
+        if constexpr (kRegA) SA::load(va[u], a, p.lda, tile.rows, p.K, k0 + u * SA::KC);
+        if constexpr (SCALE) SA::load(vd[u], scale, p.K, tile.rows, p.K, k0 + u * SA::KC);
+        if constexpr (!DMA) SB::load(vb[u], w, ldw, wrows, wcols, k0 + u * SA::KC);
+      }
+    };
+    if (kRegA) load(first);
+    for (int k0 = first; k0 < end; k0 += kStep) {
+      if (k0 > first) __syncthreads();
+      if constexpr (DMA) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (u && k0 + u * SA::KC >= end) break;
+          if constexpr (!SCALE) SA::load_either(lds + u * kStage, a, p.lda, tile.rows, p.K, k0 + u * SA::KC);
+          SB::load_either(lds + u * kStage + SA::kBytes, w, ldw, wrows, wcols, k0 + u * SA::KC);
         }
       }
-      SA::store(at, va);
-      SB::store(at + SA::kBytes, vb);
-      if (k0 + SA::KC < end) {
-        SA::load(va, a, p.lda, tile.rows, p.K, k0 + SA::KC);
-        if (SCALE) SA::load(vd, scale, p.K, tile.rows, p.K, k0 + SA::KC);
-        SB::load(vb, w, ldw, wrows, wcols, k0 + SA::KC);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u && k0 + u * SA::KC >= end) break;
+        if constexpr (SCALE) {
+#pragma unroll
+          for (int i = 0; i < SA::NL; ++i) {
+            va[u][i] = Deriv<T>::apply(va[u][i], vd[u][i]);
+            const int row = SA::row_of(i), col = k0 + u * SA::KC + SA::col_of(i), left = p.K - col;
+            if (dz && row < tile.rows && left > 0) store_chunk<T>(dz + (int64_t)row * p.K + col, va[u][i], left);
+          }
+        }
+        if constexpr (kRegA) SA::store(lds + u * kStage, va[u]);
+        if constexpr (!DMA) SB::store(lds + u * kStage + SA::kBytes, vb[u]);
       }
+      if (DMA) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
+      if (kRegA && k0 + kStep < end) load(k0 + kStep);
       __syncthreads();
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < 2 * U; ++s) {
+        if (s >= 2 && k0 + (s >> 1) * SA::KC >= end) break;
+        const char *const la = lds + (s >> 1) * kStage, *const lb = la + SA::kBytes;
         typename Type<T>::frag fb[NI];
 #pragma unroll
         for (int n = 0; n < NI; ++n)
-          fb[n] = SB::frag(at + SA::kBytes, s, [&](int i) { return wc * TN + column_of<T>(n, i); }, threadIdx.x & 63);
+          fb[n] = SB::frag(lb, s & 1, [&](int i) { return wc * TN + column_of<T>(n, i); }, threadIdx.x & 63);
 #pragma unroll
         for (int m = 0; m < MI; ++m) {
-          const typename Type<T>::frag fa = SA::frag(at, s, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
+          const typename Type<T>::frag fa = SA::frag(la, s & 1, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
 #pragma unroll
           for (int n = 0; n < NI; ++n) acc[m][n] = Type<T>::mma(fb[n], fa, acc[m][n]);
         }
       }
-      buf ^= 1;
     }
   }
 
@@ -718,15 +772,16 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   else finish_tile<T, MI, NI, EPI, false>(p, acc, tile, wr * TM, n0 + wc * TN, threadIdx.x & 63);
 }
 
-// Joins the parts of split sums in order, with the epilogue; zeros for rows of no group.  A block has 64
+// Joins the parts of split sums in order, with the epilogue; zeros for rows of no group.  A block has 16
 // rows and 64 columns.
-template <typename T, bool EPI> __global__ __launch_bounds__(256) void split_join_kernel(RowsArgs p) {
+constexpr int kJoinThreads = 128;
+template <typename T, bool EPI> __global__ __launch_bounds__(kJoinThreads) void split_join_kernel(RowsArgs p) {
   constexpr int CH = 16 / (int)sizeof(T), PC = 64 / CH;
   typedef typename Deriv<T>::type D;
   RowTile tile;
-  if (!find_row_tile(p.g, blockIdx.x / p.col_tiles, 64, tile)) return;
+  if (!find_row_tile(p.g, blockIdx.x / p.col_tiles, 16, tile)) return;
   const int n0 = blockIdx.x % p.col_tiles * 64;
-  for (int c = threadIdx.x; c < 64 * PC; c += 256) {
+  for (int c = threadIdx.x; c < 16 * PC; c += kJoinThreads) {
     const int row = c / PC, col = n0 + c % PC * CH, left = p.N - col;
     if (row >= tile.rows || left <= 0) continue;
     const int64_t at = (tile.first + row) * p.N + col;
@@ -734,6 +789,7 @@ template <typename T, bool EPI> __global__ __launch_bounds__(256) void split_joi
 #pragma unroll
     for (int i = 0; i < CH; ++i) z[i] = 0.f;
     if (tile.e >= 0) {
+#pragma unroll 4
       for (int s = 0; s < p.splits; ++s) {
         const float *src = p.part + s * p.rows * p.N + at;
 #pragma unroll
@@ -836,13 +892,13 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
 // ---------------------------------------------------------------------------------------------
 // gw = dz^T x, gb = sum of dz over the rows of a chunk; a chunk that is its group's only one writes
 // the results, the others their partial sums.
-template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC>
+template <typename T, int BM, int BN, int WR, int WC, bool DMA, int OCC>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void weight_kernel(WeightArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
   typedef Stage<T, BM, NT, true> SU;
   typedef Stage<T, BN, NT, true> SX;
   constexpr int kStage = SU::kBytes + SX::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[BUFS * kStage];
+  __shared__ __attribute__((aligned(16))) char lds[kStage];
   int slot, ct;
   block_tile(blockIdx.x, p.n_tiles * p.k_tiles, 1, slot, ct);
   if (slot >= p.slots) return;
@@ -861,36 +917,42 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   }
   const T *u = static_cast<const T *>(p.u) + ch.first * p.ldu + n0;
   const T *x = static_cast<const T *>(p.x) + ch.first * p.ldx + k0;
-  uint4 vu[SU::NL], vx[SX::NL];
-  SU::load(vu, u, p.ldu, ch.rows, p.N - n0, 0);
-  SX::load(vx, x, p.ldx, ch.rows, p.K - k0, 0);
-  int buf = 0;
+  uint4 vu[DMA ? 1 : SU::NL], vx[DMA ? 1 : SX::NL];
+  if constexpr (!DMA) {
+    SU::load(vu, u, p.ldu, ch.rows, p.N - n0, 0);
+    SX::load(vx, x, p.ldx, ch.rows, p.K - k0, 0);
+  }
   for (int r0 = 0; r0 < ch.rows; r0 += SU::KC) {
-    if (BUFS == 1) __syncthreads();
-    char *const at = lds + (BUFS == 1 ? 0 : buf * kStage);
-    SU::store(at, vu);
-    SX::store(at + SU::kBytes, vx);
-    if (r0 + SU::KC < ch.rows) {
-      SU::load(vu, u, p.ldu, ch.rows, p.N - n0, r0 + SU::KC);
-      SX::load(vx, x, p.ldx, ch.rows, p.K - k0, r0 + SU::KC);
+    if (r0) __syncthreads();
+    if constexpr (DMA) {
+      SU::load_either(lds, u, p.ldu, ch.rows, p.N - n0, r0);
+      SX::load_either(lds + SU::kBytes, x, p.ldx, ch.rows, p.K - k0, r0);
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
+    } else {
+      SU::store(lds, vu);
+      SX::store(lds + SU::kBytes, vx);
+      if (r0 + SU::KC < ch.rows) {
+        SU::load(vu, u, p.ldu, ch.rows, p.N - n0, r0 + SU::KC);
+        SX::load(vx, x, p.ldx, ch.rows, p.K - k0, r0 + SU::KC);
+      }
     }
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       typename Type<T>::frag fx[NI];
 #pragma unroll
-      for (int n = 0; n < NI; ++n) fx[n] = SX::frag(at + SU::kBytes, s, [&](int i) { return wc * TN + n * 16 + i; }, threadIdx.x & 63);
+      for (int n = 0; n < NI; ++n) fx[n] = SX::frag(lds + SU::kBytes, s, [&](int i) { return wc * TN + column_of<T>(n, i); }, threadIdx.x & 63);
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
-        const typename Type<T>::frag fu = SU::frag(at, s, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
+        const typename Type<T>::frag fu = SU::frag(lds, s, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[m][n] = Type<T>::mma(fx[n], fu, acc[m][n]);
         if (with_b) accb[m] = Type<T>::mma(Type<T>::ones(), fu, accb[m]);
       }
     }
-    buf ^= 1;
   }
-  // lane (i, q) of acc[m][n]: row n0 + m * 16 + i of gw, columns k0 + n * 16 + 4 q .. + 3
+  // lane (i, q) of acc[m][n]: row n0 + m * 16 + i of gw, columns k0 + column_of(n, 4 q) .. + 3
+  constexpr int CH = 16 / (int)sizeof(T), NP = CH / 4;
   const bool direct = ch.chunks == 1;
   const int i = lane & 15, q = lane >> 4;
 #pragma unroll
@@ -898,16 +960,20 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
     const int row = n0 + wr * TM + m * 16 + i;
     if (row >= p.N) continue;
 #pragma unroll
-    for (int n = 0; n < NI && p.gw; ++n) {
-      const int col = k0 + wc * TN + n * 16 + q * 4, left = p.K - col;
+    for (int t = 0; t < NI / NP && p.gw; ++t) {
+      const int col = k0 + wc * TN + t * NP * 16 + q * CH, left = p.K - col;
       if (left <= 0) continue;
       if (direct) {
-        T *at = static_cast<T *>(p.gw) + ((int64_t)ch.e * p.N + row) * p.K + col;
+        Chunk<T> out;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < left) at[j] = (T)acc[m][n][j];
+        for (int j = 0; j < CH; ++j) out.e[j] = (T)acc[m][t * NP + j / 4][j & 3];
+        store_chunk<T>(static_cast<T *>(p.gw) + ((int64_t)ch.e * p.N + row) * p.K + col, out.raw, left);
       } else {
-        store_chunk<float>(p.part + ((int64_t)slot * p.N + row) * p.K + col, __builtin_bit_cast(uint4, acc[m][n]), left);
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+          if (left > j * 4)
+            store_chunk<float>(p.part + ((int64_t)slot * p.N + row) * p.K + col + j * 4,
+                               __builtin_bit_cast(uint4, acc[m][t * NP + j]), left - j * 4);
       }
     }
     if (with_b && q == 0) {
@@ -931,7 +997,7 @@ template <typename T> __global__ __launch_bounds__(256) void scale_kernel(const 
   }
 }
 
-// Sums the chunks' partial results in order; zeros for groups without rows.  Blocks of 64 elements,
+// Sums the chunks' partial results in order.  Blocks of 64 elements,
 // four threads an element, each a quarter of the slots.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(WeightArgs p) {
@@ -981,23 +1047,24 @@ template <typename K> inline hipError_t launch(K kernel, int64_t grid, int threa
   return hipGetLastError();
 }
 
-template <typename T, int BM, int BN, int WR, int WC, int BUFS, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT = false>
+template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT = false>
 inline hipError_t launch_rows(RowsArgs p, hipStream_t st) {
   const int64_t rt = max_row_tiles(p.g, BM);
   p.row_tiles = (int)rt;
   p.col_tiles = ceil_div(p.N, BN);
   p.spread = rt >= 64;
   const int64_t grid = (p.spread ? (rt + 7) / 8 * 8 : rt) * p.col_tiles * (SPLIT ? p.splits : 1);
-  return launch(rows_kernel<T, BM, BN, WR, WC, BUFS, OCC, WSTR, SCALE, EPI, SPLIT>, grid, 64 * WR * WC, st, p);
+  return launch(rows_kernel<T, BM, BN, WR, WC, U, DMA, OCC, WSTR, SCALE, EPI, SPLIT>, grid, 64 * WR * WC, st, p);
 }
 
 // How many parts a sum of K elements is cut into, by tiles of 64 x 64: none where the tiles make 256
-// blocks or there are less than 8 stages; otherwise parts of 4 stages or more, up to 512 blocks.
-// (bf16, one row of dz, 3301 -> 1856: 16 us, 100 in one part.)
+// blocks or there are less than 16 stages (four rounds of loads in one part, which two launches do not
+// beat); otherwise parts of 4 stages or more, up to 512 blocks.  One row of dz, 3301 -> 1856 in bf16:
+// 11 us, about 100 in one part; 576 x 256 -> 256 in fp32 (8 stages): 13 us in two parts, 9 in one.
 inline int split_count(int esize, int64_t rows, int E, int N, int K) {
   const int stages = ceil_div(K, 128 / esize);
   const int64_t tiles = (ceil_div(rows, 64) + (E > 1 ? E : 0)) * (int64_t)ceil_div(N, 64);
-  if (tiles >= 256 || stages < 8) return 1;
+  if (tiles >= 256 || stages < 16) return 1;
   int64_t parts = 512 / tiles < stages / 4 ? 512 / tiles : stages / 4;
   return parts < 2 ? 1 : ceil_div(stages, ceil_div(stages, parts));
 }
@@ -1009,29 +1076,38 @@ template <typename T, int RT, int NW> inline hipError_t launch_few(RowsArgs p, h
   return launch(few_rows_kernel<T, RT, NW>, rt * p.col_tiles, 64 * NW, st, p);
 }
 
-template <typename T, bool WSTR, bool SCALE, bool EPI> inline hipError_t launch_tiles(const RowsArgs &p, hipStream_t st) {
-  const int64_t rows = p.rows;
-  if constexpr (sizeof(T) == 2 && !SCALE) {
-    // one block of 256 x 256 a CU: long sums (4096^3 bf16 145 us, 195 with 128 x 128), or outputs of many
-    // tiles, where the operands' second and third reading costs most (598016 x 256 -> 1024 590 and 680 us,
-    // but 73728 rows, 1152 tiles, 116 and 98)
-    const int64_t tiles = (rows + 255) / 256 * ceil_div(p.N, 256);
-    if (rows / p.g.E >= 512 && p.N >= 256 && ((p.K >= 512 && tiles >= 192) || tiles >= 4096))
-      return launch_rows<T, 256, 256, 2, 4, 2, 2, WSTR, SCALE, EPI>(p, st);
+// Whether every row of a matrix starts at a 16-byte boundary, within the offsets of Stage::load_lds.
+inline bool rows_aligned(const void *p, int64_t ld, int esize) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * esize)) & 15u) == 0 && ld < (1 << 22);
+}
+
+template <typename T, bool DMA, bool WSTR, bool SCALE, bool EPI> inline hipError_t launch_tiles(const RowsArgs &p, hipStream_t st) {
+  if constexpr (DMA && !SCALE) {
+    // long sums: wider tiles read their operands less often (4096^3 bf16 120 us, 128 in tiles of 128; at
+    // sums of 256 those are as fast or faster)
+    if (p.K >= 1024 && p.N >= 256 && p.rows / p.g.E >= 512 && (p.rows + 127) / 128 * ceil_div(p.N, 256) >= 384)
+      return launch_rows<T, 128, 256, 2, 4, 1, true, 4, WSTR, SCALE, EPI>(p, st);
   }
-  if ((rows + 127) / 128 * ceil_div(p.N, 128) >= 256) {
-    // with act_grad 64 x 128, whose registers fit four blocks a CU (73728 x 1024 -> 256 142 us, 157)
-    if constexpr (SCALE) return launch_rows<T, 64, 128, 1, 4, 1, 4, WSTR, SCALE, EPI>(p, st);
-    else return launch_rows<T, 128, 128, 2, 2, 1, 3, WSTR, SCALE, EPI>(p, st);
+  if ((p.rows + 127) / 128 * ceil_div(p.N, 128) >= 256) {
+    // act_grad through registers takes a block a CU more off the unaligned 128 x 128 (73728 x 1024 -> 256:
+    // 64 x 128 142 us, 157; aligned 128 x 128 121, 64 x 128 137)
+    if constexpr (SCALE && !DMA) return launch_rows<T, 64, 128, 1, 4, 1, DMA, 4, WSTR, SCALE, EPI>(p, st);
+    else return launch_rows<T, 128, 128, 2, 2, 1, DMA, DMA && !SCALE ? 4 : 3, WSTR, SCALE, EPI>(p, st);
   }
+  constexpr int U = SCALE ? 2 : 4, OCC = SCALE ? 4 : 2;
   if (p.splits > 1) {
-    const hipError_t e = launch_rows<T, 64, 64, 2, 2, 1, 4, WSTR, SCALE, EPI, true>(p, st);
+    const hipError_t e = launch_rows<T, 64, 64, 2, 2, U, DMA, OCC, WSTR, SCALE, EPI, true>(p, st);
     if (e != hipSuccess) return e;
     RowsArgs j = p;
     j.col_tiles = ceil_div(p.N, 64);
-    return launch(split_join_kernel<T, EPI>, max_row_tiles(p.g, 64) * j.col_tiles, 256, st, j);
+    return launch(split_join_kernel<T, EPI>, max_row_tiles(p.g, 16) * j.col_tiles, kJoinThreads, st, j);
   }
-  return launch_rows<T, 64, 64, 2, 2, 1, 4, WSTR, SCALE, EPI>(p, st);
+  return launch_rows<T, 64, 64, 2, 2, U, DMA, OCC, WSTR, SCALE, EPI>(p, st);
+}
+
+template <typename T, bool WSTR, bool SCALE, bool EPI> inline hipError_t launch_rows_of(const RowsArgs &p, hipStream_t st) {
+  const bool aligned = (SCALE || rows_aligned(p.a, p.lda, sizeof(T))) && rows_aligned(p.w, WSTR ? p.N : p.K, sizeof(T));
+  return aligned ? launch_tiles<T, true, WSTR, SCALE, EPI>(p, st) : launch_tiles<T, false, WSTR, SCALE, EPI>(p, st);
 }
 
 // Rows a group up to which the forward takes the kernel for few rows.
@@ -1042,11 +1118,11 @@ template <typename T> hipError_t forward(const RowsArgs &p, hipStream_t st) {
   if (per_group <= 16) return p.K >= 2048 ? launch_few<T, 1, 8>(p, st) : launch_few<T, 1, 4>(p, st);
   if (per_group <= 32) return p.K >= 2048 ? launch_few<T, 2, 8>(p, st) : launch_few<T, 2, 4>(p, st);
   if (per_group <= kFewRows) return p.K >= 2048 ? launch_few<T, 4, 8>(p, st) : launch_few<T, 4, 4>(p, st);
-  return launch_tiles<T, false, false, true>(p, st);
+  return launch_rows_of<T, false, false, true>(p, st);
 }
 
 template <typename T> hipError_t grad_x(const RowsArgs &p, hipStream_t st) {
-  return p.scale ? launch_tiles<T, true, true, false>(p, st) : launch_tiles<T, true, false, false>(p, st);
+  return p.scale ? launch_rows_of<T, true, true, false>(p, st) : launch_rows_of<T, true, false, false>(p, st);
 }
 
 // Tile, rows per chunk and number of chunks of the weight kernel; the workspace follows from it.
@@ -1067,7 +1143,7 @@ struct ChunkPlan {
     chunk = (int)((S + kc - 1) / kc * kc);
     if (want > 1) chunk = (int)((rows / want + kc - 1) / kc * kc);
     if (chunk < kc) chunk = kc;
-    slots = grouped ? (int64_t)B * (S / chunk + E) : ceil_div(S, chunk);
+    slots = grouped ? (int64_t)B * (S / chunk + E) : S > chunk ? ceil_div(S, chunk) : 1;
     joined = grouped ? B > 1 || chunk < S : slots > 1;
   }
 };
@@ -1086,14 +1162,16 @@ template <typename T> hipError_t grad_weight(const WeightArgs &q, int tile, bool
   p.k_tiles = p.gw ? ceil_div(p.K, tile) : 1;
   const int64_t grid = ((int64_t)p.slots + 7) / 8 * 8 * p.n_tiles * p.k_tiles;
   if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
-  if (grid > 0) {
-    if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, 1, 2>), dim3((unsigned)grid), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, 1, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
-  }
-  if (joined || p.g.start || !p.slots) {
-    const int64_t total = (p.gw ? (int64_t)p.N * p.K : 0) + (p.gb ? p.N : 0);
-    const int64_t want = (total + 63) / 64, most = joined ? 2048 : 64;
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(want < most ? want : most), p.g.E), dim3(256), 0, st, p);
+  const bool aligned = rows_aligned(p.u, p.ldu, sizeof(T)) && rows_aligned(p.x, p.ldx, sizeof(T)) &&
+                       p.N % (16 / sizeof(T)) == 0 && p.K % (16 / sizeof(T)) == 0;
+  const dim3 blocks((unsigned)grid), threads(256);
+  if (tile == 128 && aligned) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, 2>), blocks, threads, 0, st, p);
+  else if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, false, 2>), blocks, threads, 0, st, p);
+  else if (aligned) hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, true, 4>), blocks, threads, 0, st, p);
+  else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, false, 4>), blocks, threads, 0, st, p);
+  if (joined) {
+    const int64_t total = (p.gw ? (int64_t)p.N * p.K : 0) + (p.gb ? p.N : 0), want = (total + 63) / 64;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(want < 2048 ? want : 2048), p.g.E), dim3(256), 0, st, p);
   }
   return hipGetLastError();
 }
