@@ -18,6 +18,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace ops3d_linear {
 
 enum Act { kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4 };
@@ -332,19 +334,22 @@ struct RowTile {
   int rows;
 };
 
-// Row tile t, counted over items, segments and steps of BM rows; false: there is none.  Every wave
-// walks the table by itself: E + 2 loads and two scans, no barrier and no kernel before this one.
-__device__ __forceinline__ bool find_row_tile(const Groups &g, int t, int BM, RowTile &out) {
+// The row tiles of one segment of one item: tiles lo .. hi - 1, of `rows` rows from `first` on.
+struct SegmentTiles {
+  int e, lo, hi, rows;
+  int64_t first;
+};
+
+// The segment of row tile t, counted over items, segments and steps of BM rows; false: there is none.
+// Every wave walks the table by itself: E + 2 loads and two scans, no barrier and no kernel before
+// this one.
+__device__ __forceinline__ bool find_segment(const Groups &g, int t, int BM, SegmentTiles &out) {
   if (!g.start) {
-    const int64_t first = (int64_t)t * BM;
-    if (first >= g.S) return false;
-    out.e = 0;
-    out.first = first;
-    out.rows = min(BM, (int)(g.S - first));
-    return true;
+    out = SegmentTiles{0, 0, (g.S + BM - 1) / BM, g.S, 0};
+    return t < out.hi;
   }
   const int lane = threadIdx.x & 63;
-  int b = 0;
+  int b = 0, skipped = 0;
   if (g.B > 1) {
     int carry = 0, total = 0;
     for (int base = 0; base < g.E + 2; base += 64) {
@@ -353,28 +358,36 @@ __device__ __forceinline__ bool find_row_tile(const Groups &g, int t, int BM, Ro
     }
     if (total == 0) return false;
     b = t / total;
-    t -= b * total;
+    skipped = b * total;
     if (b >= g.B) return false;
   }
-  int carry = 0, before = 0;
+  int carry = 0, before = skipped;
   for (int base = 0; base < g.E + 2; base += 64) {
     const Segment s = segment_at(g, base + lane, carry);
     const int tiles = (s.upper - s.lower + BM - 1) / BM;
     const int incl = before + scan_add(tiles);
     const uint64_t m = __ballot(incl > t);
     if (m) {
-      const int src = __builtin_ctzll(m);
-      const int lower = __builtin_amdgcn_readlane(s.lower, src), upper = __builtin_amdgcn_readlane(s.upper, src);
-      const int step = t - (__builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane(tiles, src));
-      const int at = lower + step * BM, j = base + src;
+      const int src = __builtin_ctzll(m), j = base + src;
+      const int lower = __builtin_amdgcn_readlane(s.lower, src);
       out.e = j <= g.E ? j - 1 : -1;
-      out.first = (int64_t)b * g.S + at;
-      out.rows = min(BM, upper - at);
+      out.hi = __builtin_amdgcn_readlane(incl, src);
+      out.lo = out.hi - __builtin_amdgcn_readlane(tiles, src);
+      out.rows = __builtin_amdgcn_readlane(s.upper, src) - lower;
+      out.first = (int64_t)b * g.S + lower;
       return true;
     }
     before = __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
+}
+
+__device__ __forceinline__ bool find_row_tile(const Groups &g, int t, int BM, RowTile &out) {
+  SegmentTiles s;
+  if (!find_segment(g, t, BM, s)) return false;
+  const int at = (t - s.lo) * BM;
+  out = RowTile{s.e, s.first + at, min(BM, s.rows - at)};
+  return true;
 }
 
 struct RowChunk {
@@ -581,17 +594,26 @@ template <typename T, int MI, int NI, bool EPI, int ACT, bool FULL>
 __device__ __forceinline__ void store_results(const RowsArgs &p, const f32x4 (&acc)[MI][NI], const RowTile &tile, int r0,
                                               int col0, int lane) {
   constexpr int CH = 16 / (int)sizeof(T), NP = CH / 4;   // MFMA results that make up a chunk of columns
+  constexpr int NC = NI / NP;
   typedef typename Deriv<T>::type D;
   const int row0 = r0 + (lane & 15), c0 = (lane >> 4) * CH;
   const int64_t at = tile.first * p.N + col0;                    // uniform
   const uint32_t off = (uint32_t)(row0 * p.N + c0);              // the rest: below 256 rows of 2^24
   const T *res = EPI && p.res ? static_cast<const T *>(p.res) + tile.first * p.ld_res + col0 : nullptr;
   const int64_t off_res = row0 * p.ld_res + c0;
+  uint4 r[NC];
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
     if (!FULL && row0 + m * 16 >= tile.rows) continue;
+    if (EPI && res) {   // of these 16 rows, all on their way before the first is waited for
 #pragma unroll
-    for (int t = 0; t < NI / NP; ++t) {
+      for (int t = 0; t < NC; ++t) {
+        const T *from = res + (int64_t)m * 16 * p.ld_res + t * NP * 16 + off_res;
+        r[t] = FULL ? load16(from) : fetch(from, 0, 0, 0, 1, p.N - col0 - c0 - t * NP * 16);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NC; ++t) {
       const int cols = t * NP * 16, left = FULL ? CH : p.N - col0 - c0 - cols;
       if (!FULL && left <= 0) continue;
       const int64_t to = at + (int64_t)m * 16 * p.N + cols;      // uniform
@@ -603,16 +625,16 @@ __device__ __forceinline__ void store_results(const RowsArgs &p, const f32x4 (&a
       }
       if (EPI && ACT != kNone && p.act_grad) store_chunk<D, true>(static_cast<D *>(p.act_grad) + to + off, Deriv<T>::encode(d), left);
       if (EPI && res) {
-        const T *rp = res + (int64_t)m * 16 * p.ld_res + cols + off_res;
-        Chunk<T> r;
-        r.raw = left >= CH ? load16(rp) : load_part(rp, left);
+        Chunk<T> c;
+        c.raw = r[t];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) z[i] += (float)r.e[i];
+        for (int i = 0; i < CH; ++i) z[i] += (float)c.e[i];
       }
       Chunk<T> out;
 #pragma unroll
       for (int i = 0; i < CH; ++i) out.e[i] = (T)z[i];
       store_chunk<T>(static_cast<T *>(p.c) + to + off, out.raw, left);
+      __builtin_amdgcn_sched_barrier(0);   // chunk by chunk: together they would not fit the registers
     }
   }
 }
@@ -770,6 +792,146 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   }
   if (tile.rows >= BM && n0 + BN <= p.N) finish_tile<T, MI, NI, EPI, true>(p, acc, tile, wr * TM, n0 + wc * TN, threadIdx.x & 63);
   else finish_tile<T, MI, NI, EPI, false>(p, acc, tile, wr * TM, n0 + wc * TN, threadIdx.x & 63);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many rows, a short sum (16-bit types, K = 64 KS, no scale), as projections of whole volumes are: bound by
+// the rows' bytes.  The tile kernel reads its operands through LDS once for every 128 columns or rows,
+// waits for every stage of every tile and has no more than its LDS's bytes under way (598016 x 256 ->
+// 1024 570 to 690 us).  Here a block of 8 waves stays on its CU with 256 columns of the weight in
+// registers (64 a wave: 32 KS registers) and walks over tiles of 64 rows: loads to a ring of four tiles in
+// LDS run two to three tiles ahead of the products, one barrier a tile, and results go out meanwhile
+// (414 us; with 256 columns 121, 171, where the bytes alone take 118).
+// A segment's last tile is its last 64 rows, and the last columns are the last 256: what two blocks
+// compute they write alike, and every tile is whole.
+//
+// Order of a wave's memory operations, which complete in order: loads of tile i (KS of them), results of
+// tile i - 3, loads of tile i + 1, results of i - 2, loads of i + 2, results of i - 1.  So when all but the
+// newest 2 KS operations are done, the loads of tile i are, with results to store or without.  Behind the
+// barrier every wave's are, and every wave has read tile i - 1 (the reads' results are waited for where
+// they are read), whose place tile i + 3 takes.  Behind the last tile it is loaded again, so the counts
+// hold, and all loads are waited for before a segment ends.
+// The operands are read in assembly with the wait in the same statement: for its own reads of LDS the
+// compiler waits for all loads to LDS under way.
+template <int OFF> __device__ __forceinline__ void read_rows(f32x4 (&x)[4], uint32_t even, uint32_t odd) {
+  asm volatile(
+      "ds_read_b128 %0, %4 offset:%6\n\tds_read_b128 %1, %4 offset:%7\n\t"
+      "ds_read_b128 %2, %5 offset:%6\n\tds_read_b128 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+      : "v"(even), "v"(odd), "n"(OFF), "n"(OFF + 16 * 128)
+      : "memory");
+}
+
+template <typename T, int KS, bool WSTR, bool EPI, int ACT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void stream_kernel(RowsArgs p) {
+  constexpr int BM = 64, NB = 256, NI = 4, ST = 2 * KS;
+  typedef Stage<T, NB, 512, WSTR> SB;
+  typedef Stage<T, BM, 512, false> SA;
+  constexpr int kTile = KS * SA::kBytes;
+  static_assert(KS * SB::kBytes == 4 * kTile, "the weight's columns pass through the ring");
+  static_assert(SA::NL == 1, "a stage of rows is one load a thread");
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTile];
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, ct = slot % p.col_tiles;
+  const int groups = gridDim.x / 8 / p.col_tiles * 8;
+  const int n0 = min(ct * NB, p.N - NB);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+  const int wr = wave >> 2, col0 = n0 + (wave & 3) * 64;   // the wave has 32 rows and 64 columns of a tile
+  const int64_t ldw = WSTR ? p.N : p.K;
+  // LDS addresses of this lane's operands of tile 0: even and odd steps of 32
+  const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+  const uint32_t even = ring + SA::address(wr * 32 + li, q), odd = ring + SA::address(wr * 32 + li, 4 + q);
+
+  int rt = slot / p.col_tiles * 8 + xcd;
+  while (rt < p.row_tiles) {
+    SegmentTiles seg;
+    if (!find_segment(p.g, rt, BM, seg)) return;
+    // first row of tile t of the segment
+    const auto first_row = [&](int t) { return seg.first + max(0, min((t - seg.lo) * BM, seg.rows - BM)); };
+    const auto load_tile = [&](int t, int buf) {
+      const T *a = static_cast<const T *>(p.a) + first_row(t) * p.lda;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) SA::load_lds(lds + buf * kTile + k * SA::kBytes, a, p.lda, min(seg.rows, BM), p.K, k * 64);
+    };
+    if (seg.e < 0) {
+      for (; rt < seg.hi; rt += groups) {
+        f32x4 zero[2][NI];
+#pragma unroll
+        for (int n = 0; n < NI; ++n) zero[0][n] = zero[1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const RowTile tile{-1, first_row(rt), min(seg.rows, BM)};
+        store_results<T, 2, NI, false, kNone, false>(p, zero, tile, wr * 32, col0, lane);
+      }
+      continue;
+    }
+
+    // the weight's columns, through the ring, and the bias
+    const T *w = static_cast<const T *>(p.w) + seg.e * p.w_group + (WSTR ? (int64_t)n0 : (int64_t)n0 * p.K);
+    typename Type<T>::frag fw[NI][ST];
+    uint4 bias[2];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) SB::load_lds(lds + k * SB::kBytes, w, ldw, WSTR ? p.K : NB, WSTR ? NB : p.K, k * 64);
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+      for (int s = 0; s < ST; ++s)
+        fw[n][s] = SB::frag(lds + (s >> 1) * SB::kBytes, s & 1, [&](int i) { return (wave & 3) * 64 + column_of<T>(n, i); }, lane);
+    if constexpr (EPI)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        bias[t] = p.bias ? load16(static_cast<const T *>(p.bias) + (int64_t)seg.e * p.N + col0 + t * 32 + q * 8) : make_uint4(0, 0, 0, 0);
+    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): the weight is read, the ring free
+    __syncthreads();
+
+    const int last = rt + (seg.hi - 1 - rt) / groups * groups;   // this block's last tile of the segment
+#pragma unroll
+    for (int j = 0; j < 3; ++j) load_tile(min(rt + j * groups, last), j);
+    for (int buf = 0; rt < seg.hi; rt += groups, buf = (buf + 1) & 3) {
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * KS));   // vmcnt(2 KS)
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      load_tile(min(rt + 3 * groups, last), (buf + 3) & 3);
+      f32x4 acc[2][NI];
+#pragma unroll
+      for (int n = 0; n < NI; ++n) acc[0][n] = acc[1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const auto products = [&](auto stage) {
+        constexpr int S = decltype(stage)::value;
+        f32x4 x[4];
+        read_rows<S * SA::kBytes>(x, even + buf * kTile, odd + buf * kTile);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+              acc[m][n] = Type<T>::mma(fw[n][S * 2 + s], __builtin_bit_cast(typename Type<T>::frag, x[s * 2 + m]), acc[m][n]);
+      };
+      products(std::integral_constant<int, 0>());
+      if constexpr (KS > 1) products(std::integral_constant<int, 1>());
+      if constexpr (KS > 2) products(std::integral_constant<int, 2>());
+      if constexpr (KS > 3) products(std::integral_constant<int, 3>());
+      if constexpr (EPI)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Chunk<T> b;
+          b.raw = bias[t];
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[m][t * 2 + i / 4][i & 3] += (float)b.e[i];
+        }
+      // what depends on the lane is formed again for every tile: kept over the loop it would not fit
+      // beside the weight
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      const RowTile tile{seg.e, first_row(rt), min(seg.rows, BM)};
+      if (seg.rows >= BM) store_results<T, 2, NI, EPI, ACT, true>(p, acc, tile, wr * 32, col0, l);
+      else store_results<T, 2, NI, EPI, ACT, false>(p, acc, tile, wr * 32, col0, l);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): no load to LDS is under way
+  }
 }
 
 // Joins the parts of split sums in order, with the epilogue; zeros for rows of no group.  A block has 16
@@ -1069,6 +1231,34 @@ inline int split_count(int esize, int64_t rows, int E, int N, int K) {
   return parts < 2 ? 1 : ceil_div(stages, ceil_div(stages, parts));
 }
 
+template <typename T, int KS, bool WSTR, bool EPI, int ACT> inline hipError_t launch_stream_of(RowsArgs p, hipStream_t st) {
+  p.row_tiles = (int)max_row_tiles(p.g, 64);
+  p.col_tiles = ceil_div(p.N, 256);
+  const int per_xcd = p.col_tiles < 32 ? 32 / p.col_tiles : 1;   // groups of row tiles on each XCD's 32 CUs
+  return launch(stream_kernel<T, KS, WSTR, EPI, ACT>, (int64_t)8 * p.col_tiles * per_xcd, 512, st, p);
+}
+template <typename T, int KS, bool WSTR, bool EPI> inline hipError_t launch_stream(const RowsArgs &p, hipStream_t st) {
+  if constexpr (EPI) {
+    switch (p.act) {
+      case kRelu: return launch_stream_of<T, KS, WSTR, EPI, kRelu>(p, st);
+      case kGelu: return launch_stream_of<T, KS, WSTR, EPI, kGelu>(p, st);
+      case kGeluTanh: return launch_stream_of<T, KS, WSTR, EPI, kGeluTanh>(p, st);
+      case kSilu: return launch_stream_of<T, KS, WSTR, EPI, kSilu>(p, st);
+      default: break;
+    }
+  }
+  return launch_stream_of<T, KS, WSTR, EPI, kNone>(p, st);
+}
+
+// What the streaming kernel takes: sums of 128 or 256, columns that fill their slices of 256 for the most
+// part, and 8 tiles of 64 rows or more for each block and segment, which starts by loading the weight
+// (73728 rows: 1024 columns 46 us, 61 in tiles, 256 columns 21 and 20).  Not smooth activations that keep
+// act_grad: their arithmetic needs more waves than two a SIMD (73728 x 256 -> 1024 gelu 101 us, 93).
+inline bool streams(const RowsArgs &p) {
+  return (p.K == 128 || p.K == 256) && p.N >= 256 && p.N % 8 == 0 && p.N * 4 >= ceil_div(p.N, 256) * 768 &&
+         p.rows * ceil_div(p.N, 256) >= (int64_t)131072 * p.g.E * p.g.B && (!p.act_grad || p.act == kRelu);
+}
+
 template <typename T, int RT, int NW> inline hipError_t launch_few(RowsArgs p, hipStream_t st) {
   const int64_t rt = max_row_tiles(p.g, 16 * RT);
   p.row_tiles = (int)rt;
@@ -1082,6 +1272,9 @@ inline bool rows_aligned(const void *p, int64_t ld, int esize) {
 }
 
 template <typename T, bool DMA, bool WSTR, bool SCALE, bool EPI> inline hipError_t launch_tiles(const RowsArgs &p, hipStream_t st) {
+  if constexpr (DMA && !SCALE && sizeof(T) == 2) {
+    if (streams(p)) return p.K == 128 ? launch_stream<T, 2, WSTR, EPI>(p, st) : launch_stream<T, 4, WSTR, EPI>(p, st);
+  }
   if constexpr (DMA && !SCALE) {
     // long sums: wider tiles read their operands less often (4096^3 bf16 120 us, 128 in tiles of 128; at
     // sums of 256 those are as fast or faster)

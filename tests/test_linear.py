@@ -267,6 +267,25 @@ def test_linear_large(gpu_device, dtype, rows, K, N):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,rows,K,N,act", [("bf16", 65607, 256, 504, "relu"), ("fp16", 70001, 128, 512, None),
+                                                ("bf16", 66001, 512, 128, None), ("fp16", 140001, 256, 256, None),
+                                                ("bf16", 140033, 256, 256, "silu")])
+def test_linear_many_rows(gpu_device, dtype, rows, K, N, act):
+    """Short sums over many rows, of the forward and of the input gradient; last tiles and slices that overlap."""
+    log(f"[case] linear many rows {rows}x{K}->{N} {dtype} {act}")
+    linear_case(rows, K, N, DTYPES[dtype], act, with_residual=True)
+    linear_case(rows, K, N, DTYPES[dtype], act, train=False, seed=1)
+
+
+@gpu
+@pytest.mark.parametrize("K,N,act", [(256, 1024, "relu"), (1024, 256, None), (128, 1016, None)])
+def test_grouped_many_rows(gpu_device, K, N, act):
+    """The same in groups: rows of none, a group shorter than a tile, two items."""
+    log(f"[case] grouped many rows {K}->{N} {act}")
+    grouped_case(100003, [70, 100, 60000, 99990], 3, K, N, torch.bfloat16, act, batch=2, with_residual=True)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,K,N", [(1, 1856, 3301), (70, 3000, 100), (130, 1111, 72), (300, 640, 1100), (65, 129, 2000)])
 def test_linear_long_sums(gpu_device, rows, K, N, dtype):
