@@ -166,13 +166,20 @@ template <typename T> __device__ __forceinline__ void store_part(T *p, uint4 v, 
   }
 }
 
-// The 16-byte chunk at (row, col) of a matrix of nrows x ncols; zeros outside it.
+// The 16-byte chunk at (row, col) of a matrix of nrows x ncols; zeros outside it.  A chunk that ends
+// outside is cut from the row's last 16 bytes.
 template <typename T>
 __device__ __forceinline__ uint4 fetch(const T *base, int64_t ld, int row, int col, int nrows, int ncols) {
   constexpr int CH = 16 / (int)sizeof(T);
   if (row >= nrows || col >= ncols) return make_uint4(0, 0, 0, 0);
-  const T *p = base + (int64_t)row * ld + col;
-  return col + CH <= ncols ? load16(p) : load_part(p, ncols - col);
+  const T *p = base + (int64_t)row * ld;
+  if (col + CH <= ncols) return load16(p + col);
+  if (ncols < CH) return load_part(p + col, ncols - col);
+  const uint4 v = load16(p + ncols - CH);
+  const int bits = (col + CH - ncols) * 8 * (int)sizeof(T);   // 16 .. 112
+  const uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
+  const uint64_t a = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64), b = bits < 64 ? hi >> bits : 0;
+  return make_uint4((uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32));
 }
 
 // A chunk of a row with `left` elements left.
@@ -260,16 +267,16 @@ template <bool FAST> __device__ __forceinline__ float activate(int act, float z,
       if (FAST) {
         // tail = P(X > |z|), w = |z| times the density: act = max(z, 0) - |z| tail, and act' is
         // tail - w below zero and 1 minus that above
-        const float e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+        const float e = __builtin_amdgcn_exp2f(-0.72134752f * z * z), a = fminf(fabsf(z), 1e4f);   // finite: e = 0 there
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, a, 1.f));
         float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
         p = fmaf(p, t, 0.5f * 1.421413741f);
         p = fmaf(p, t, 0.5f * -0.284496736f);
         p = fmaf(p, t, 0.5f * 0.254829592f);
         const float tail = p * t * e;
-        const float g = fmaf(-0.39894228f * fabsf(z), e, tail);
+        const float g = fmaf(-0.39894228f * a, e, tail);
         d = z > 0.f ? 1.f - g : g;
-        return fmaf(-fabsf(z), tail, z > 0.f ? z : (z != z ? z : 0.f));
+        return fmaf(-a, tail, z > 0.f ? z : 0.f);
       }
       const float phi = expf(-0.5f * z * z), cdf = 0.5f * erfcf(-0.70710678f * z);
       d = fmaf(z * 0.39894228f, phi, cdf);
@@ -464,24 +471,28 @@ template <typename T, int R, int NT, bool STRIDED> struct Stage {
 
   // Chunks of one stage.  base: the tile's first element; rows, cols: what is left of the matrix from
   // there; k0: sum elements before this stage.  A stage of a whole tile takes 16-byte loads at one
-  // 32-bit offset a thread and scalar bases; one that lacks rows of the output's side reads the last
-  // row for them (their results are not stored); others go chunk by chunk with zeros outside.
+  // 32-bit offset a thread and scalar bases.  One that lacks some of the output's side reads the last
+  // row for it, or, STRIDED, its columns' last chunk, whose end may lie in the next row, so not in the
+  // matrix's last row (the results of such rows and columns are not stored).  Others go chunk by chunk
+  // with zeros outside.
   template <typename E>
   static __device__ __forceinline__ void load(uint4 (&v)[NL], const E *base, int64_t ld, int rows, int cols, int k0) {
-    const bool inside = (STRIDED ? k0 + KC <= rows && cols >= R : k0 + KC <= cols) && ld < (1 << 22);
     const E *at = base + (STRIDED ? (int64_t)k0 * ld : (int64_t)k0);
-    if (inside && (STRIDED || rows >= R)) {
+    const bool inside = k0 + KC <= (STRIDED ? rows : cols) && ld < (1 << 22);
+    if (inside && (STRIDED ? cols : rows) >= R) {
       const uint32_t off = row_of(0) * (int)ld + col_of(0);
 #pragma unroll
       for (int i = 0; i < NL; ++i) v[i] = load16(at + (int64_t)i * kRowStep * ld + off);
-    } else if (inside) {
-      int last = rows - 1;
-      asm volatile("" : "+s"(last));   // the offsets are formed here, not in every block before its loop
+    } else if (inside && (!STRIDED || (k0 + KC < rows && ld >= CH))) {
+      int last = STRIDED ? (cols - 1) / CH * CH : rows - 1;
+      asm volatile("" : "+v"(last));   // the offsets are formed here, not in every block before its loop
 #pragma unroll
-      for (int i = 0; i < NL; ++i) v[i] = load16(at + (uint32_t)(min(row_of(i), last) * (int)ld + col_of(i)));
+      for (int i = 0; i < NL; ++i)
+        v[i] = STRIDED ? load16(at + (uint32_t)(row_of(i) * (int)ld + min(col_of(i), last)))
+                       : load16(at + (uint32_t)(min(row_of(i), last) * (int)ld + col_of(i)));
     } else {
       int zero = 0;
-      asm volatile("" : "+s"(zero));
+      asm volatile("" : "+v"(zero));
 #pragma unroll
       for (int i = 0; i < NL; ++i)
         v[i] = fetch(base, ld, row_of(i) + (STRIDED ? k0 : zero), col_of(i) + (STRIDED ? zero : k0), rows, cols);
@@ -598,7 +609,7 @@ __device__ __forceinline__ void store_results(const RowsArgs &p, const f32x4 (&a
   typedef typename Deriv<T>::type D;
   const int row0 = r0 + (lane & 15), c0 = (lane >> 4) * CH;
   const int64_t at = tile.first * p.N + col0;                    // uniform
-  const uint32_t off = (uint32_t)(row0 * p.N + c0);              // the rest: below 256 rows of 2^24
+  const uint32_t off = (uint32_t)row0 * (uint32_t)p.N + c0;      // the rest: below 256 rows of 2^24
   const T *res = EPI && p.res ? static_cast<const T *>(p.res) + tile.first * p.ld_res + col0 : nullptr;
   const int64_t off_res = row0 * p.ld_res + c0;
   uint4 r[NC];
@@ -1007,7 +1018,7 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
   if (tile.e >= 0) {
     const T *a = static_cast<const T *>(p.a) + tile.first * p.lda;
     const T *w = static_cast<const T *>(p.w) + tile.e * p.w_group + (int64_t)n0 * p.K;
-    constexpr int U = RT <= 2 ? 4 : 2;   // steps in flight
+    constexpr int U = RT <= 2 ? 4 : 2;   // steps in flight a wave
     for (int k0 = wave * KS; k0 < p.K; k0 += NW * KS * U) {
       uint4 fw[U], fa[U][RT];
 #pragma unroll
@@ -1281,12 +1292,22 @@ template <typename T, bool DMA, bool WSTR, bool SCALE, bool EPI> inline hipError
     if (p.K >= 1024 && p.N >= 256 && p.rows / p.g.E >= 512 && (p.rows + 127) / 128 * ceil_div(p.N, 256) >= 384)
       return launch_rows<T, 128, 256, 2, 4, 1, true, 4, WSTR, SCALE, EPI>(p, st);
   }
+  if constexpr (!DMA && !SCALE && sizeof(T) == 2) {
+    // through registers the widest tiles that fill the CUs (4096 x 4095 -> 4093 bf16 202 us, 252; its input
+    // gradient 179, 229)
+    if (p.K >= 512 && p.N >= 256 && p.rows / p.g.E >= 512 && (p.rows + 255) / 256 * ceil_div(p.N, 256) >= 192)
+      return launch_rows<T, 256, 256, 2, 4, 1, false, 2, WSTR, SCALE, EPI>(p, st);
+  }
   if ((p.rows + 127) / 128 * ceil_div(p.N, 128) >= 256) {
     // act_grad through registers takes a block a CU more off the unaligned 128 x 128 (73728 x 1024 -> 256:
     // 64 x 128 142 us, 157; aligned 128 x 128 121, 64 x 128 137)
     if constexpr (SCALE && !DMA) return launch_rows<T, 64, 128, 1, 4, 1, DMA, 4, WSTR, SCALE, EPI>(p, st);
     else return launch_rows<T, 128, 128, 2, 2, 1, DMA, DMA && !SCALE ? 4 : 3, WSTR, SCALE, EPI>(p, st);
   }
+  // 64 x 64: from two tiles a CU on the blocks wait in turn, and a stage at a time leaves room for more of
+  // them (10013 x 250 -> 333 fp32 34 us, 42 in fours); fewer tiles load four stages at once
+  if ((p.rows + 63) / 64 * ceil_div(p.N, 64) >= 512)
+    return launch_rows<T, 64, 64, 2, 2, 1, DMA, 4, WSTR, SCALE, EPI>(p, st);
   constexpr int U = SCALE ? 2 : 4, OCC = SCALE ? 4 : 2;
   if (p.splits > 1) {
     const hipError_t e = launch_rows<T, 64, 64, 2, 2, U, DMA, OCC, WSTR, SCALE, EPI, true>(p, st);
@@ -1320,7 +1341,7 @@ template <typename T> hipError_t grad_x(const RowsArgs &p, hipStream_t st) {
 
 // Tile, rows per chunk and number of chunks of the weight kernel; the workspace follows from it.
 // 512 blocks of 128 x 128 fill the 256 CUs once (two blocks each); where the tiles times chunks of 256
-// rows do not make 256 blocks, tiles of 64 x 64 and chunks of 64 rows do better.
+// rows do not make 256 blocks, tiles of 64 x 64 and chunks of 64 rows do better, up to 1024 blocks.
 struct ChunkPlan {
   int tile, chunk;
   int64_t slots;
@@ -1330,7 +1351,7 @@ struct ChunkPlan {
     const int64_t rows = (int64_t)B * S, big = (int64_t)ceil_div(N, 128) * ceil_div(K, 128);
     tile = big * (rows / 256 > E ? rows / 256 : E) >= 256 ? 128 : 64;
     const int64_t tiles = (int64_t)ceil_div(N, tile) * ceil_div(K, tile), least = tile == 128 ? 256 : 64;
-    int64_t want = 512 / tiles;
+    int64_t want = (tile == 128 ? 512 : 1024) / tiles;
     if (want > rows / least) want = rows / least;
     if (want <= E) want = 1;
     chunk = (int)((S + kc - 1) / kc * kc);

@@ -420,6 +420,9 @@ def test_linear_extreme_activations(gpu_device):
             (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
             torch.testing.assert_close(y, torch.where(x > 0, x, torch.zeros_like(x)), rtol=0, atol=1e-6)
             torch.testing.assert_close(dx, (x > 0).to(dt), rtol=0, atol=1e-6)
+            top = torch.tensor([[float("inf")], [float("nan")]], dtype=dt, device="cuda")
+            y = fused_linear(top, eye.to(dt), None, act)
+            assert torch.isposinf(y[0]).all() and torch.isnan(y[1]).all()
 
 
 @gpu
