@@ -1298,7 +1298,7 @@ template <typename T, bool DMA, bool WSTR, bool SCALE, bool EPI> inline hipError
     if (p.K >= 512 && p.N >= 256 && p.rows / p.g.E >= 512 && (p.rows + 255) / 256 * ceil_div(p.N, 256) >= 192)
       return launch_rows<T, 256, 256, 2, 4, 1, false, 2, WSTR, SCALE, EPI>(p, st);
   }
-  if ((p.rows + 127) / 128 * ceil_div(p.N, 128) >= 256) {
+  if ((p.rows + 127) / 128 * ceil_div(p.N, 128) >= 256 && p.N > 64) {
     // act_grad through registers takes a block a CU more off the unaligned 128 x 128 (73728 x 1024 -> 256:
     // 64 x 128 142 us, 157; aligned 128 x 128 121, 64 x 128 137)
     if constexpr (SCALE && !DMA) return launch_rows<T, 64, 128, 1, 4, 1, DMA, 4, WSTR, SCALE, EPI>(p, st);
@@ -1341,7 +1341,11 @@ template <typename T> hipError_t grad_x(const RowsArgs &p, hipStream_t st) {
 
 // Tile, rows per chunk and number of chunks of the weight kernel; the workspace follows from it.
 // 512 blocks of 128 x 128 fill the 256 CUs once (two blocks each); where the tiles times chunks of 256
-// rows do not make 256 blocks, tiles of 64 x 64 and chunks of 64 rows do better, up to 1024 blocks.
+// rows do not make 256 blocks, or where one side has 64 columns at most, tiles of 64 x 64 and chunks of 64
+// rows do better, up to 1024 blocks.  From
+// 64 tiles on chunks of 512 rows and more, up to 2048 blocks: a few long ones end one after another, and
+// their partial sums are little beside the products (9642 rows in two groups, 849 x 2976 fp32: 672 blocks
+// took two rounds on CUs that hold 512).
 struct ChunkPlan {
   int tile, chunk;
   int64_t slots;
@@ -1349,9 +1353,11 @@ struct ChunkPlan {
   ChunkPlan(int esize, bool grouped, int B, int64_t S, int E, int N, int K) {
     const int kc = 128 / esize;
     const int64_t rows = (int64_t)B * S, big = (int64_t)ceil_div(N, 128) * ceil_div(K, 128);
-    tile = big * (rows / 256 > E ? rows / 256 : E) >= 256 ? 128 : 64;
-    const int64_t tiles = (int64_t)ceil_div(N, tile) * ceil_div(K, tile), least = tile == 128 ? 256 : 64;
-    int64_t want = (tile == 128 ? 512 : 1024) / tiles;
+    tile = big * (rows / 256 > E ? rows / 256 : E) >= 256 && N > 64 && K > 64 ? 128 : 64;
+    const int64_t tiles = (int64_t)ceil_div(N, tile) * ceil_div(K, tile);
+    const bool many = tile == 128 && tiles >= 64;
+    const int64_t least = many ? 512 : tile == 128 ? 256 : 64;
+    int64_t want = (many ? 2048 : tile == 128 ? 512 : 1024) / tiles;
     if (want > rows / least) want = rows / least;
     if (want <= E) want = 1;
     chunk = (int)((S + kc - 1) / kc * kc);
