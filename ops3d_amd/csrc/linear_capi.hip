@@ -227,6 +227,7 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
   p.N = out_features;
   p.K = in_features;
   p.chunk = lay.plan.chunk;
+  p.items = lay.plan.items;
   p.slots = (int)lay.plan.slots;
   if (!empty && lay.plan.joined) {
     p.part = reinterpret_cast<float *>(ws + lay.part);

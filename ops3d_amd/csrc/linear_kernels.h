@@ -63,7 +63,7 @@ struct WeightArgs {
   float *part, *part_b;   // partial sums [slots, N, K], [slots, N] (nullptr: one chunk per group)
   int64_t ldu, ldx;
   int N, K;
-  int chunk;              // rows per chunk
+  int chunk, items;       // rows of an item, and items, per chunk
   int n_tiles, k_tiles;
   int slots;              // bound on the number of chunks
   Groups g;
@@ -400,15 +400,15 @@ __device__ __forceinline__ bool find_row_tile(const Groups &g, int t, int BM, Ro
 struct RowChunk {
   int e;
   int64_t first;
-  int rows;
+  int rows, items;  // rows from `first` on, and the same of the items - 1 next items
   int chunks;       // of this group, all items
   int slot;         // of this group's first chunk
 };
 
-// Chunk t of `chunk` rows, counted over groups, items and steps; a group without rows has one of no rows
-// in each item, which writes its zeros.  by_group: the chunks of group t instead (first and rows not
-// set; false never).
-__device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, bool by_group, RowChunk &out) {
+// Chunk t of `chunk` rows of each of `items` items, counted over groups, runs of items and steps; a group
+// without rows has one of no rows in each run, which writes its zeros.  by_group: the chunks of group t
+// instead (first, rows and items not set; false never).
+__device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, int items, bool by_group, RowChunk &out) {
   if (!g.start) {
     const int n = max(1, (g.S + chunk - 1) / chunk);
     out.e = 0;
@@ -418,6 +418,7 @@ __device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, bo
     if (t >= n) return false;
     out.first = (int64_t)t * chunk;
     out.rows = min(chunk, (int)(g.S - out.first));
+    out.items = 1;
     return true;
   }
   const int lane = threadIdx.x & 63;
@@ -425,8 +426,8 @@ __device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, bo
   for (int base = 0; base < g.E + 2; base += 64) {
     const int j = base + lane;
     const Segment s = segment_at(g, j, carry);
-    const int per = j >= 1 && j <= g.E ? max(1, (s.upper - s.lower + chunk - 1) / chunk) : 0;   // per item
-    const int n = per * g.B;
+    const int per = j >= 1 && j <= g.E ? max(1, (s.upper - s.lower + chunk - 1) / chunk) : 0;   // per run of items
+    const int n = per * ((g.B + items - 1) / items);
     const int incl = before + scan_add(n);
     const uint64_t m = __ballot(by_group ? j == t + 1 : incl > t);
     if (m) {
@@ -436,8 +437,9 @@ __device__ __forceinline__ bool find_chunk(const Groups &g, int t, int chunk, bo
       out.slot = __builtin_amdgcn_readlane(incl, src) - out.chunks;
       if (by_group) return true;
       const int p = __builtin_amdgcn_readlane(per, src), lower = __builtin_amdgcn_readlane(s.lower, src);
-      const int r = t - out.slot, b = r / p, at = lower + (r - b * p) * chunk;
+      const int r = t - out.slot, run = r / p, b = run * items, at = lower + (r - run * p) * chunk;
       out.first = (int64_t)b * g.S + at;
+      out.items = min(items, g.B - b);
       out.rows = min(chunk, __builtin_amdgcn_readlane(s.upper, src) - at);
       return true;
     }
@@ -1064,8 +1066,9 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
 
 // ---------------------------------------------------------------------------------------------
 // gw = dz^T x, gb = sum of dz over the rows of a chunk; a chunk that is its group's only one writes
-// the results, the others their partial sums.
-template <typename T, int BM, int BN, int WR, int WC, bool DMA, int OCC>
+// the results, the others their partial sums.  RUNS: chunks of several items, a kernel of its own as the
+// walk over them takes registers (127 -> 135 in 128 x 128, which is a wave a SIMD less).
+template <typename T, int BM, int BN, int WR, int WC, bool DMA, bool RUNS, int OCC>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void weight_kernel(WeightArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
   typedef Stage<T, BM, NT, true> SU;
@@ -1076,7 +1079,7 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   block_tile(blockIdx.x, p.n_tiles * p.k_tiles, 1, slot, ct);
   if (slot >= p.slots) return;
   RowChunk ch;
-  if (!find_chunk(p.g, slot, p.chunk, false, ch)) return;
+  if (!find_chunk(p.g, slot, p.chunk, p.items, false, ch)) return;
   const int n0 = ct / p.k_tiles * BM, k0 = ct % p.k_tiles * BN;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = wave / WC, wc = wave % WC;
   const bool with_b = p.gb && k0 == 0 && wc == 0;   // column sums as products with ones
@@ -1088,41 +1091,51 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const T *u = static_cast<const T *>(p.u) + ch.first * p.ldu + n0;
-  const T *x = static_cast<const T *>(p.x) + ch.first * p.ldx + k0;
-  uint4 vu[DMA ? 1 : SU::NL], vx[DMA ? 1 : SX::NL];
-  if constexpr (!DMA) {
-    SU::load(vu, u, p.ldu, ch.rows, p.N - n0, 0);
-    SX::load(vx, x, p.ldx, ch.rows, p.K - k0, 0);
-  }
-  for (int r0 = 0; r0 < ch.rows; r0 += SU::KC) {
-    if (r0) __syncthreads();
-    if constexpr (DMA) {
-      SU::load_either(lds, u, p.ldu, ch.rows, p.N - n0, r0);
-      SX::load_either(lds + SU::kBytes, x, p.ldx, ch.rows, p.K - k0, r0);
-      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
-    } else {
-      SU::store(lds, vu);
-      SX::store(lds + SU::kBytes, vx);
-      if (r0 + SU::KC < ch.rows) {
-        SU::load(vu, u, p.ldu, ch.rows, p.N - n0, r0 + SU::KC);
-        SX::load(vx, x, p.ldx, ch.rows, p.K - k0, r0 + SU::KC);
+  const auto add = [&](int64_t first) {
+    const T *u = static_cast<const T *>(p.u) + first * p.ldu + n0;
+    const T *x = static_cast<const T *>(p.x) + first * p.ldx + k0;
+    uint4 vu[DMA ? 1 : SU::NL], vx[DMA ? 1 : SX::NL];
+    if constexpr (!DMA) {
+      SU::load(vu, u, p.ldu, ch.rows, p.N - n0, 0);
+      SX::load(vx, x, p.ldx, ch.rows, p.K - k0, 0);
+    }
+    for (int r0 = 0; r0 < ch.rows; r0 += SU::KC) {
+      if (r0) __syncthreads();
+      if constexpr (DMA) {
+        SU::load_either(lds, u, p.ldu, ch.rows, p.N - n0, r0);
+        SX::load_either(lds + SU::kBytes, x, p.ldx, ch.rows, p.K - k0, r0);
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
+      } else {
+        SU::store(lds, vu);
+        SX::store(lds + SU::kBytes, vx);
+        if (r0 + SU::KC < ch.rows) {
+          SU::load(vu, u, p.ldu, ch.rows, p.N - n0, r0 + SU::KC);
+          SX::load(vx, x, p.ldx, ch.rows, p.K - k0, r0 + SU::KC);
+        }
+      }
+      __syncthreads();
+  #pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        typename Type<T>::frag fx[NI];
+  #pragma unroll
+        for (int n = 0; n < NI; ++n) fx[n] = SX::frag(lds + SU::kBytes, s, [&](int i) { return wc * TN + column_of<T>(n, i); }, threadIdx.x & 63);
+  #pragma unroll
+        for (int m = 0; m < MI; ++m) {
+          const typename Type<T>::frag fu = SU::frag(lds, s, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
+  #pragma unroll
+          for (int n = 0; n < NI; ++n) acc[m][n] = Type<T>::mma(fx[n], fu, acc[m][n]);
+          if (with_b) accb[m] = Type<T>::mma(Type<T>::ones(), fu, accb[m]);
+        }
       }
     }
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      typename Type<T>::frag fx[NI];
-#pragma unroll
-      for (int n = 0; n < NI; ++n) fx[n] = SX::frag(lds + SU::kBytes, s, [&](int i) { return wc * TN + column_of<T>(n, i); }, threadIdx.x & 63);
-#pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const typename Type<T>::frag fu = SU::frag(lds, s, [&](int i) { return wr * TM + m * 16 + i; }, threadIdx.x & 63);
-#pragma unroll
-        for (int n = 0; n < NI; ++n) acc[m][n] = Type<T>::mma(fx[n], fu, acc[m][n]);
-        if (with_b) accb[m] = Type<T>::mma(Type<T>::ones(), fu, accb[m]);
-      }
+  };
+  if constexpr (RUNS) {
+    for (int item = 0; item < ch.items; ++item) {
+      if (item) __syncthreads();
+      add(ch.first + (int64_t)item * p.g.S);
     }
+  } else {
+    add(ch.first);
   }
   // lane (i, q) of acc[m][n]: row n0 + m * 16 + i of gw, columns k0 + column_of(n, 4 q) .. + 3
   constexpr int CH = 16 / (int)sizeof(T), NP = CH / 4;
@@ -1177,7 +1190,7 @@ __global__ __launch_bounds__(256) void join_kernel(WeightArgs p) {
   __shared__ float red[4][64];
   const int e = blockIdx.y;
   RowChunk ch;
-  find_chunk(p.g, e, p.chunk, true, ch);
+  find_chunk(p.g, e, p.chunk, p.items, true, ch);
   if (ch.chunks == 1) return;
   const int64_t nk = p.gw ? (int64_t)p.N * p.K : 0, total = nk + (p.gb ? p.N : 0);
   const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
@@ -1346,8 +1359,11 @@ template <typename T> hipError_t grad_x(const RowsArgs &p, hipStream_t st) {
 // 64 tiles on chunks of 512 rows and more, up to 2048 blocks: a few long ones end one after another, and
 // their partial sums are little beside the products (9642 rows in two groups, 849 x 2976 fp32: 672 blocks
 // took two rounds on CUs that hold 512).
+// Many items of many groups: a chunk takes the same rows of several items, so that items times groups do
+// not make more partial sums than there are blocks to fill the CUs (64 items of 128 groups, 1024 x 4096:
+// 139 GB of them otherwise).
 struct ChunkPlan {
-  int tile, chunk;
+  int tile, chunk, items;
   int64_t slots;
   bool joined;   // a group may have several chunks
   ChunkPlan(int esize, bool grouped, int B, int64_t S, int E, int N, int K) {
@@ -1358,13 +1374,16 @@ struct ChunkPlan {
     const bool many = tile == 128 && tiles >= 64;
     const int64_t least = many ? 512 : tile == 128 ? 256 : 64;
     int64_t want = (many ? 2048 : tile == 128 ? 512 : 1024) / tiles;
+    const int64_t fill = want > E ? want : E;
+    items = (int64_t)B * E > fill ? ceil_div((int64_t)B * E, fill) : 1;
     if (want > rows / least) want = rows / least;
     if (want <= E) want = 1;
     chunk = (int)((S + kc - 1) / kc * kc);
-    if (want > 1) chunk = (int)((rows / want + kc - 1) / kc * kc);
+    if (want > 1) chunk = (int)((rows / want / items + kc - 1) / kc * kc);
     if (chunk < kc) chunk = kc;
-    slots = grouped ? (int64_t)B * (S / chunk + E) : S > chunk ? ceil_div(S, chunk) : 1;
-    joined = grouped ? B > 1 || chunk < S : slots > 1;
+    const int64_t runs = ceil_div(B, items);
+    slots = grouped ? runs * (S / chunk + E) : S > chunk ? ceil_div(S, chunk) : 1;
+    joined = grouped ? runs > 1 || chunk < S : slots > 1;
   }
 };
 
@@ -1385,10 +1404,15 @@ template <typename T> hipError_t grad_weight(const WeightArgs &q, int tile, bool
   const bool aligned = rows_aligned(p.u, p.ldu, sizeof(T)) && rows_aligned(p.x, p.ldx, sizeof(T)) &&
                        p.N % (16 / sizeof(T)) == 0 && p.K % (16 / sizeof(T)) == 0;
   const dim3 blocks((unsigned)grid), threads(256);
-  if (tile == 128 && aligned) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, 2>), blocks, threads, 0, st, p);
-  else if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, false, 2>), blocks, threads, 0, st, p);
-  else if (aligned) hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, true, 4>), blocks, threads, 0, st, p);
-  else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, false, 4>), blocks, threads, 0, st, p);
+  const auto launch = [&](auto runs) {
+    constexpr bool R = decltype(runs)::value;
+    if (tile == 128 && aligned) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, R, 2>), blocks, threads, 0, st, p);
+    else if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, false, R, 2>), blocks, threads, 0, st, p);
+    else if (aligned) hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, true, R, 4>), blocks, threads, 0, st, p);
+    else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, false, R, 4>), blocks, threads, 0, st, p);
+  };
+  if (p.items > 1) launch(std::true_type());
+  else launch(std::false_type());
   if (joined) {
     const int64_t total = (p.gw ? (int64_t)p.N * p.K : 0) + (p.gb ? p.N : 0), want = (total + 63) / 64;
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(want < 2048 ? want : 2048), p.g.E), dim3(256), 0, st, p);

@@ -220,6 +220,16 @@ def test_workspace_sizes(lib):
     assert f(2, 1, 598016, 1, 256, 256, 0) < 64 << 20
 
 
+def test_workspace_of_many_items(lib):
+    """Partial sums follow the blocks that fill the device, not items times groups."""
+    f = lib.ops3d_linear_backward_workspace_bytes
+    assert f(2, 64, 512, 128, 4096, 1024, 1, 0) == 0
+    assert f(2, 64, 512, 16, 1024, 1024, 1, 0) < 512 << 20
+    assert f(0, 1000, 50, 4, 256, 256, 1, 0) < 64 << 20
+    # 4096 groups and a million rows: below the weights' own gradients, held in fp32
+    assert f(1, 512, 2048, 4096, 256, 256, 1, 0) <= 4096 * 256 * 256 * 4
+
+
 def test_module_signatures_cpu():
     m = FlashDeformAttn3D(32, 4, 2, 4, level_value_proj=True)
     assert isinstance(m.value_proj, GroupedLinear) and m.value_proj.weight.shape == (2, 32, 32)
@@ -471,6 +481,9 @@ GROUPS = [
     (40000, [0, 34990, 39400], 3, 0),
     (30000, [100, 25000, 25001, 29999], 3, 2),
     (150, [3, 70, 70, 149], 3, 2),                  # with 1500 features: sums in parts
+    (9, [0, 2, 2, 7], 4, 700),                      # chunks of several items
+    (70, [2, 68, 69], 3, 400),                      # the same, a group of more rows than a chunk's, rows of no group
+    (33, [i // 2 for i in range(60)], 60, 150),
 ]
 
 
@@ -483,6 +496,24 @@ def test_grouped_sizes(gpu_device, case, dtype):
     act = list(ACTIVATIONS)[case % 5]
     log(f"[case] grouped {case}: {S} rows, {groups} groups, batch {batch}, {K}->{N} {act} {dtype}")
     grouped_case(S, start, groups, K, N, DTYPES[dtype], act, batch, with_bias=case != 5, with_residual=case % 2 == 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("K,N", [(512, 512), (515, 513)])
+def test_grouped_many_items(gpu_device, K, N, dtype):
+    """Weights' gradients in wide tiles, a chunk taking the same rows of several items."""
+    log(f"[case] grouped many items {K}->{N} {dtype}")
+    start = [0, 1, 1, 2, 3, 5, 8, 13, 21, 30, 31, 32, 33, 34, 35, 36, 37, 40, 50, 55]
+    grouped_case(60, start, 20, K, N, DTYPES[dtype], "silu", batch=40)
+
+
+@gpu
+@pytest.mark.parametrize("K,N,act", [(515, 1001, None), (1001, 515, "gelu"), (1024, 1032, "relu")])
+def test_grouped_large(gpu_device, K, N, act):
+    """The widest tiles in groups that end inside them, unaligned and aligned."""
+    log(f"[case] grouped large {K}->{N} {act}")
+    grouped_case(12300, [3, 700, 6007], 3, K, N, torch.bfloat16, act, batch=2, with_residual=True)
 
 
 @gpu
