@@ -28,6 +28,9 @@
  * act_grad: act'(z) for the backward, [batch * rows, out_features], written by the forward when not
  * NULL and read by the backward; fp32 for F32, otherwise int16 in steps of 2^-14 (INT16_MIN: NaN).
  * Rows in no group are not written.  It must be NULL for OPS3D_LINEAR_ACT_NONE.
+ *
+ * Outputs and workspace must overlap neither each other nor an input (a residual neither): some results
+ * are computed by two blocks, which write the same value.
  */
 #ifndef OPS3D_LINEAR_H
 #define OPS3D_LINEAR_H

@@ -6,6 +6,9 @@
 //   rows kernel     dx = dz W            rows of dz by columns of W (W is strided along the sum)
 //   weight kernel   dW = dz^T x          both strided along the sum (the rows), split over chunks of
 //                                        rows; the chunks' partial sums are joined in order
+// but for two kinds of sizes, which the bytes bound:
+//   stream kernel   y or dx              many rows, a sum of 128 or 256: the weight stays in registers
+//   few rows        y                    64 rows a group at most: the weight goes straight to registers
 // A stage of a tile is 128 bytes of the sum's axis for every row (64 elements of 16 bits, 32 of 32).
 // Operands that are contiguous along the sum lie in LDS as rows of 128 bytes and are read 16 bytes a
 // lane; the others lie as they are in memory, sum axis outermost, and are read transposed
@@ -694,8 +697,11 @@ __device__ __forceinline__ void store_parts(const RowsArgs &p, const f32x4 (&acc
 // split_join_kernel, where the tiles alone do not fill the CUs.
 // U stages are loaded and multiplied at a time.  DMA: loads go straight to LDS (rows at 16-byte
 // boundaries); nothing is loaded ahead, but without registers for it more blocks fit a CU, which wait in
-// turn (4096^3 bf16: 128 x 256 120 us, 128 x 128 128; through registers and a stage ahead 192 and 181,
-// 256 x 256 152).  Otherwise loads go through registers, the next stages' while these are multiplied; so
+// turn (4096^3 bf16, same run: 128 x 256 136 us, 128 x 128 144; through registers and a stage ahead 256 x 256
+// 159, 128 x 128 189; the whole operator 130 to 148, of which the products take 94 at a library's rate).
+// What bounds it: at long sums the wait for a stage's loads, which the blocks of a CU hide from one another
+// (half of the wave cycles wait, for 4096^3); at 73728 x 256 -> 1024 with an act_grad (97 to 125
+// us) the stores, of 300 MB, and the activation's arithmetic.  Otherwise loads go through registers, the next stages' while these are multiplied; so
 // does the scaled operand always.
 template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void rows_kernel(RowsArgs p) {
@@ -1004,7 +1010,9 @@ template <typename T, bool EPI> __global__ __launch_bounds__(kJoinThreads) void 
 // ---------------------------------------------------------------------------------------------
 // Few rows: the weight's bytes bound it.  A block takes 16 columns of up to 16 RT rows; its waves
 // share the sum, read the weight straight into MFMA operands (each byte once) and join their sums
-// through LDS.
+// through LDS.  8 x 4096 -> 4096 bf16 9 to 10 us (33.5 MB); 96 rows in 64 groups 1024 -> 2048 36 to 39 (the
+// weights of the 46 or so groups that have rows, 190 MB, at HBM's rate); one row of 256 4.2, a launch and
+// a round of loads.  16 waves a block were not faster.
 template <typename T, int RT, int NW>
 __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
   constexpr int CH = 16 / (int)sizeof(T), KS = 4 * CH;   // sum elements of a step: 16 bytes a lane, 4 lanes a row
@@ -1066,7 +1074,10 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
 
 // ---------------------------------------------------------------------------------------------
 // gw = dz^T x, gb = sum of dz over the rows of a chunk; a chunk that is its group's only one writes
-// the results, the others their partial sums.  RUNS: chunks of several items, a kernel of its own as the
+// the results, the others their partial sums.  Column sums come with the products, as one more operand of
+// ones: in fp32 registers beside the loads they were slower.  73728 rows of 256 x 256 in bf16 24 us and 6 of
+// join_kernel (75 MB: 15), 256 x 1024 75 to 82 and 7; 598016 rows in three groups 182 to 203 and 10 to 12
+// (612 MB: 118).  What bounds it: two waits a stage of 64 rows, hidden by three or four blocks a CU.  RUNS: chunks of several items, a kernel of its own as the
 // walk over them takes registers (127 -> 135 in 128 x 128, which is a wave a SIMD less).
 template <typename T, int BM, int BN, int WR, int WC, bool DMA, bool RUNS, int OCC>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void weight_kernel(WeightArgs p) {
