@@ -1073,26 +1073,48 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// RING's operands of 32 rows of a stage: results 2 t + h, H bytes apart, in halves of 4 rows of 256 bytes
+// (Stage::frag), read in assembly with the wait in the same statement, as the compiler waits for all loads
+// to LDS under way before its own reads.
+template <int OFF, int H> __device__ __forceinline__ void read_columns(s16x4 (&v)[8], const uint32_t (&at)[2], uint32_t stage) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %9 offset:%10\n\tds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %6, %9 offset:%12\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(at[0] + stage), "v"(at[1] + stage), "n"(OFF), "n"(OFF + 1024), "n"(OFF + H), "n"(OFF + 1024 + H)
+      : "memory");
+}
+
 // gw = dz^T x, gb = sum of dz over the rows of a chunk; a chunk that is its group's only one writes
 // the results, the others their partial sums.  Column sums come with the products, as one more operand of
-// ones: in fp32 registers beside the loads they were slower.  73728 rows of 256 x 256 in bf16 24 us and 6 of
-// join_kernel (75 MB: 15), 256 x 1024 75 to 82 and 7; 598016 rows in three groups 182 to 203 and 10 to 12
-// (612 MB: 118).  What bounds it: two waits a stage of 64 rows, hidden by three or four blocks a CU.  RUNS: chunks of several items, a kernel of its own as the
-// walk over them takes registers (127 -> 135 in 128 x 128, which is a wave a SIMD less).
-template <typename T, int BM, int BN, int WR, int WC, bool DMA, bool RUNS, int OCC>
+// ones: in fp32 registers beside the loads they were slower.
+// RUNS: chunks of several items, a kernel of its own as the walk over them takes registers (127 -> 135 in
+// 128 x 128, which is a wave a SIMD less).
+// RING (16-bit types, 128 x 128, chunks of 512 rows and more): two stages in LDS, the next one's loads under
+// way during the products; two blocks a CU, which is what there is of long chunks.  Order of a wave's memory
+// operations: loads of stages i, i + 1, so all but the newest kLoads done means that stage i is there; the
+// barrier behind it says so for every wave, the one behind the products that its place is free.
+// Single-buffered, with up to four blocks a CU, and with the ring: 73728 rows of 256 x 256 in bf16 24 and 21
+// us (75 MB: 15), 256 x 1024 75 and 64, 598016 rows in three groups 182 and 160 (612 MB: 118; it fetches
+// 744 MB, 4.6 TB/s, which bounds it); join_kernel adds 6, 7 and 11.  Chunks of 256 rows (16411 rows in 64
+// groups, 512 x 1024 fp16): 53 without, 56 with.
+template <typename T, int BM, int BN, int WR, int WC, bool DMA, bool RUNS, bool RING, int OCC>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void weight_kernel(WeightArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
   typedef Stage<T, BM, NT, true> SU;
   typedef Stage<T, BN, NT, true> SX;
   constexpr int kStage = SU::kBytes + SX::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[kStage];
+  static_assert(!RING || (DMA && !RUNS && sizeof(T) == 2), "whole items, 16-byte rows, transposing reads");
+  __shared__ __attribute__((aligned(16))) char lds[(RING ? 2 : 1) * kStage];
   int slot, ct;
   block_tile(blockIdx.x, p.n_tiles * p.k_tiles, 1, slot, ct);
   if (slot >= p.slots) return;
   RowChunk ch;
   if (!find_chunk(p.g, slot, p.chunk, p.items, false, ch)) return;
   const int n0 = ct / p.k_tiles * BM, k0 = ct % p.k_tiles * BN;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = wave / WC, wc = wave % WC;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wr = wave / WC, wc = wave % WC;
   const bool with_b = p.gb && k0 == 0 && wc == 0;   // column sums as products with ones
 
   f32x4 acc[MI][NI], accb[MI];
@@ -1105,6 +1127,68 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   const auto add = [&](int64_t first) {
     const T *u = static_cast<const T *>(p.u) + first * p.ldu + n0;
     const T *x = static_cast<const T *>(p.x) + first * p.ldx + k0;
+    if constexpr (RING) {
+      constexpr int kLoads = SU::NL + SX::NL;
+      static_assert(SU::kRowBytes == 256 && SX::kRowBytes == 256 && MI == 4 && NI == 4, "read_columns");
+      const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+      const int i = lane & 15, row = (lane >> 4) * 8 + (i >> 2);
+      uint32_t au[2], ax[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        au[t] = base + SU::address(row, (wr * TM + t * 32) / 8 + ((i & 3) >> 1)) + (i & 1) * 8;
+        ax[t] = base + SU::kBytes + SX::address(row, (wc * TN + t * 32) / 8 + (i & 3));
+      }
+      const auto load = [&](int st) {
+        char *const to = lds + (st & 1) * kStage;
+        SU::load_lds(to, u, p.ldu, ch.rows, p.N - n0, st * SU::KC);
+        SX::load_lds(to + SU::kBytes, x, p.ldx, ch.rows, p.K - k0, st * SU::KC);
+      };
+      const auto half = [&](auto step, uint32_t stage) {
+        constexpr int OFF = decltype(step)::value * 32 * 256;
+        typedef typename Type<T>::frag F;
+        s16x4 vx[8], vu[8];
+        read_columns<OFF, 8>(vx, ax, stage);     // column_of
+        read_columns<OFF, 32>(vu, au, stage);
+        const auto frag = [](const s16x4 (&v)[8], int n) {
+          return __builtin_bit_cast(F, __builtin_shufflevector(v[2 * n], v[2 * n + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+          const F fu = frag(vu, m);
+#pragma unroll
+          for (int n = 0; n < NI; ++n) acc[m][n] = Type<T>::mma(frag(vx, n), fu, acc[m][n]);
+          if (with_b) accb[m] = Type<T>::mma(Type<T>::ones(), fu, accb[m]);
+        }
+      };
+      const auto products = [&](int st) {
+        half(std::integral_constant<int, 0>(), (st & 1) * kStage);
+        half(std::integral_constant<int, 1>(), (st & 1) * kStage);
+      };
+      const auto barrier = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      };
+      const int whole = ch.rows / SU::KC;
+      if (whole > 0) load(0);
+      if (whole > 1) load(1);
+      for (int st = 0; st < whole; ++st) {
+        if (st + 1 < whole) __builtin_amdgcn_s_waitcnt(0x0f70 | kLoads);   // vmcnt(kLoads): stage st is here
+        else __builtin_amdgcn_s_waitcnt(0x0f70);
+        barrier();
+        products(st);
+        barrier();
+        if (st + 2 < whole) load(st + 2);
+      }
+      if (whole * SU::KC < ch.rows) {   // the rest, with zeros behind it; all loads are done
+        char *const to = lds + (whole & 1) * kStage;
+        SU::load_end(to, u, p.ldu, ch.rows, p.N - n0, whole * SU::KC);
+        SX::load_end(to + SU::kBytes, x, p.ldx, ch.rows, p.K - k0, whole * SU::KC);
+        __syncthreads();
+        products(whole);
+      }
+      return;
+    }
     uint4 vu[DMA ? 1 : SU::NL], vx[DMA ? 1 : SX::NL];
     if constexpr (!DMA) {
       SU::load(vu, u, p.ldu, ch.rows, p.N - n0, 0);
@@ -1364,7 +1448,8 @@ template <typename T> hipError_t grad_x(const RowsArgs &p, hipStream_t st) {
 }
 
 // Tile, rows per chunk and number of chunks of the weight kernel; the workspace follows from it.
-// 512 blocks of 128 x 128 fill the 256 CUs once (two blocks each); where the tiles times chunks of 256
+// 512 blocks of 128 x 128 fill the 256 CUs once (two blocks each; groups take theirs off, since each may end
+// inside a chunk: 524 blocks cost a second round, 425 -> 409 us a step for 598016 rows in three groups); where the tiles times chunks of 256
 // rows do not make 256 blocks, or where one side has 64 columns at most, tiles of 64 x 64 and chunks of 64
 // rows do better, up to 1024 blocks.  From
 // 64 tiles on chunks of 512 rows and more, up to 2048 blocks: a few long ones end one after another, and
@@ -1389,6 +1474,7 @@ struct ChunkPlan {
     items = (int64_t)B * E > fill ? ceil_div((int64_t)B * E, fill) : 1;
     if (want > rows / least) want = rows / least;
     if (want <= E) want = 1;
+    if (grouped && want > (int64_t)2 * B * E) want -= (int64_t)B * E;   // every segment may end inside a chunk
     chunk = (int)((S + kc - 1) / kc * kc);
     if (want > 1) chunk = (int)((rows / want / items + kc - 1) / kc * kc);
     if (chunk < kc) chunk = kc;
@@ -1417,13 +1503,20 @@ template <typename T> hipError_t grad_weight(const WeightArgs &q, int tile, bool
   const dim3 blocks((unsigned)grid), threads(256);
   const auto launch = [&](auto runs) {
     constexpr bool R = decltype(runs)::value;
-    if (tile == 128 && aligned) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, R, 2>), blocks, threads, 0, st, p);
-    else if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, false, R, 2>), blocks, threads, 0, st, p);
-    else if (aligned) hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, true, R, 4>), blocks, threads, 0, st, p);
-    else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, false, R, 4>), blocks, threads, 0, st, p);
+    if (tile == 128 && aligned) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, R, false, 2>), blocks, threads, 0, st, p);
+    else if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, false, R, false, 2>), blocks, threads, 0, st, p);
+    else if (aligned) hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, true, R, false, 4>), blocks, threads, 0, st, p);
+    else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, false, R, false, 4>), blocks, threads, 0, st, p);
   };
-  if (p.items > 1) launch(std::true_type());
-  else launch(std::false_type());
+  bool ring = false;
+  if constexpr (sizeof(T) == 2) {
+    ring = tile == 128 && aligned && p.items == 1 && (int64_t)p.g.B * p.g.S / p.slots >= 512;
+    if (ring) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, false, true, 2>), blocks, threads, 0, st, p);
+  }
+  if (!ring) {
+    if (p.items > 1) launch(std::true_type());
+    else launch(std::false_type());
+  }
   if (joined) {
     const int64_t total = (p.gw ? (int64_t)p.N * p.K : 0) + (p.gb ? p.N : 0), want = (total + 63) / 64;
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(want < 2048 ? want : 2048), p.g.E), dim3(256), 0, st, p);
