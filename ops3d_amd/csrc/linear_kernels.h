@@ -701,8 +701,8 @@ __device__ __forceinline__ void store_parts(const RowsArgs &p, const f32x4 (&acc
 // 159, 128 x 128 189; the whole operator 130 to 148, of which the products take 94 at a library's rate).
 // What bounds it: at long sums the wait for a stage's loads, which the blocks of a CU hide from one another
 // (half of the wave cycles wait, for 4096^3); at 73728 x 256 -> 1024 with an act_grad (97 to 125
-// us) the stores, of 300 MB, and the activation's arithmetic.  Otherwise loads go through registers, the next stages' while these are multiplied; so
-// does the scaled operand always.
+// us) the stores, of 300 MB, and the activation's arithmetic.  Otherwise loads go through registers, the
+// next stages' while these are multiplied; so does the scaled operand always.
 template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void rows_kernel(RowsArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
@@ -1449,12 +1449,12 @@ template <typename T> hipError_t grad_x(const RowsArgs &p, hipStream_t st) {
 
 // Tile, rows per chunk and number of chunks of the weight kernel; the workspace follows from it.
 // 512 blocks of 128 x 128 fill the 256 CUs once (two blocks each; groups take theirs off, since each may end
-// inside a chunk: 524 blocks cost a second round, 425 -> 409 us a step for 598016 rows in three groups); where the tiles times chunks of 256
-// rows do not make 256 blocks, or where one side has 64 columns at most, tiles of 64 x 64 and chunks of 64
-// rows do better, up to 1024 blocks.  From
-// 64 tiles on chunks of 512 rows and more, up to 2048 blocks: a few long ones end one after another, and
-// their partial sums are little beside the products (9642 rows in two groups, 849 x 2976 fp32: 672 blocks
-// took two rounds on CUs that hold 512).
+// inside a chunk: 524 blocks cost a second round, 425 -> 409 us a step for 598016 rows in three groups).
+// Where the tiles times chunks of 256 rows do not make 256 blocks, or where one side has 64 columns at most,
+// tiles of 64 x 64 and chunks of 64 rows do better, up to 1024 blocks.  From 64 tiles on chunks of 512 rows
+// and more, up to 2048 blocks: a few long ones end one after another, and their partial sums are little
+// beside the products (9642 rows in two groups, 849 x 2976 fp32: 672 blocks took two rounds on CUs that hold
+// 512).
 // Many items of many groups: a chunk takes the same rows of several items, so that items times groups do
 // not make more partial sums than there are blocks to fill the CUs (64 items of 128 groups, 1024 x 4096:
 // 139 GB of them otherwise).
