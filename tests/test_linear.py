@@ -517,6 +517,15 @@ def test_grouped_large(gpu_device, K, N, act):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,rows,K,N,act", [("bf16", 4100, 1096, 3336, "silu"), ("fp16", 12290, 1024, 1032, None),
+                                                ("bf16", 4097, 2056, 4096, "gelu")])
+def test_linear_wide_long(gpu_device, dtype, rows, K, N, act):
+    """Wide tiles of long sums: rows, columns and a stage that end inside them."""
+    log(f"[case] linear wide {rows}x{K}->{N} {dtype} {act}")
+    linear_case(rows, K, N, DTYPES[dtype], act, with_residual=True)
+
+
+@gpu
 def test_grouped_equals_plain(gpu_device):
     """One group of all rows gives the plain product's bits; equal weights give one product's rows."""
     gen = torch.Generator(device="cuda").manual_seed(11)
