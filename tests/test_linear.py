@@ -517,6 +517,27 @@ def test_grouped_large(gpu_device, K, N, act):
 
 
 @gpu
+def test_linear_leading_axes(gpu_device):
+    """One row without a leading axis and rows under three give the same bits as a matrix."""
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    x, w, b = make(gen, (2, 3, 4, 40), torch.float16), make(gen, (24, 40), torch.float16, 0.2), make(gen, (24,), torch.float16)
+    r, u = make(gen, (2, 3, 4, 24), torch.float16), make(gen, (2, 3, 4, 24), torch.float16)
+    log("[case] linear leading axes")
+
+    def step(x, r, u):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b, r)]
+        y = fused_linear(leaves[0], leaves[1], leaves[2], "gelu", leaves[3])
+        return (y.detach(), *torch.autograd.grad(y, leaves, u))
+
+    want, four = step(x.reshape(24, 40), r.reshape(24, 24), u.reshape(24, 24)), step(x, r, u)
+    assert four[0].shape == (2, 3, 4, 24) and four[1].shape == x.shape
+    assert all(torch.equal(a.reshape(e.shape), e) for a, e in zip(four, want))
+    one, row = step(x[0, 0, 0], r[0, 0, 0], u[0, 0, 0]), step(x[0, 0, :1], r[0, 0, :1], u[0, 0, :1])
+    assert one[0].shape == (24,) and one[1].shape == (40,)
+    assert all(torch.equal(a.reshape(e.shape), e) for a, e in zip(one, row))
+
+
+@gpu
 @pytest.mark.parametrize("dtype,rows,K,N,act", [("bf16", 4100, 1096, 3336, "silu"), ("fp16", 12290, 1024, 1032, None),
                                                 ("bf16", 4097, 2056, 4096, "gelu")])
 def test_linear_wide_long(gpu_device, dtype, rows, K, N, act):
