@@ -192,49 +192,53 @@ template <typename T, bool STREAM = false> __device__ __forceinline__ void store
   else store16(p, v);
 }
 
-// act_grad: fp32 beside fp32, otherwise 16-bit fixed point in steps of 2^-14 (act' lies in
-// [-0.13, 1.13]; half a step is 3.1e-5, where bf16 would round by up to 2^-9 of the value), with
-// INT16_MIN for NaN.
+// act_grad: fp32 beside fp32, otherwise 16 bits.  act' lies in [-0.13, 1.13], and a saturated unit's is
+// small in every row, so that errors of one sign add up in its gradients: below 1/8 the code is the fp16
+// number (half a step is 2^-11 of the value, 2^-25 at least), from there on steps of 2^-14 (half a step is
+// 2^-12 of the value at most, 2^-15 near 1; 0 and 1 are exact).  Codes grow with the value, 0x3000 is 1/8 in
+// both; NaN is kNan, fp16's with the sign.
 template <typename T> struct Deriv {
   typedef int16_t type;
+  static constexpr uint32_t kNan = 0xfe00;
+  // codes of two values: up to 1/8 as fp16, the steps above added.  v_cvt_pknorm_u16 takes [0, 1] to
+  // [0, 65535], rounded to nearest, and what is below to 0.
+  static __device__ __forceinline__ uint32_t encode2(float d0, float d1) {
+    typedef uint16_t codes __attribute__((ext_vector_type(2)));
+    typedef _Float16 halves __attribute__((ext_vector_type(2)));
+    constexpr float c = 16384.f / 65535.f;
+    const codes low = __builtin_bit_cast(codes, halves{(_Float16)fminf(d0, 0.125f), (_Float16)fminf(d1, 0.125f)});
+    const codes steps = __builtin_bit_cast(codes, __builtin_amdgcn_cvt_pknorm_u16(fmaf(c, d0, -0.125f * c), fmaf(c, d1, -0.125f * c)));
+    return __builtin_bit_cast(uint32_t, low + steps);
+  }
   static __device__ __forceinline__ uint4 encode(const float (&d)[8]) {
-    // v_cvt_pknorm takes [-1, 1] to [-32767, 32767], rounded to nearest, and NaN to 0
-    typedef short pair __attribute__((ext_vector_type(2)));
-    constexpr float c = 16384.f / 32767.f;
     uint32_t w[4];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(pair, __builtin_amdgcn_cvt_pknorm_i16(c * d[2 * i], c * d[2 * i + 1])));
+      w[i] = encode2(d[2 * i], d[2 * i + 1]);
       sum += d[2 * i] + d[2 * i + 1];
     }
     if (sum != sum) {   // derivatives are finite otherwise, and so is their sum
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (d[2 * i] != d[2 * i]) w[i] = (w[i] & 0xffff0000u) | 0x8000u;
-        if (d[2 * i + 1] != d[2 * i + 1]) w[i] = (w[i] & 0xffffu) | 0x80000000u;
+        if (d[2 * i] != d[2 * i]) w[i] = (w[i] & 0xffff0000u) | kNan;
+        if (d[2 * i + 1] != d[2 * i + 1]) w[i] = (w[i] & 0xffffu) | kNan << 16;
       }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  static __device__ __forceinline__ type encode1(float d) {
-    return d != d ? (int16_t)-32768 : (int16_t)__float2int_rn(d * 16384.f);
-  }
+  static __device__ __forceinline__ type encode1(float d) { return (int16_t)(d != d ? kNan : encode2(d, d) & 0xffff); }
   // u * derivative, element by element of a 16-byte chunk
   static __device__ __forceinline__ uint4 apply(uint4 u, uint4 d) {
+    typedef int16_t codes __attribute__((ext_vector_type(8)));
+    typedef _Float16 halves __attribute__((ext_vector_type(8)));
     Chunk<T> c;
-    Chunk<int16_t> s;
     c.raw = u;
-    s.raw = d;
-    // words with bit 15 set and bit 14 clear hold INT16_MIN: codes of derivatives are >= -2^12
-    const uint32_t nan = ((d.x & ~(d.x << 1)) | (d.y & ~(d.y << 1)) | (d.z & ~(d.z << 1)) | (d.w & ~(d.w << 1))) & 0x80008000u;
+    const codes s = __builtin_bit_cast(codes, d), edge = 0x3000;
+    const halves low = __builtin_bit_cast(halves, __builtin_elementwise_min(s, edge));
+    const codes steps = __builtin_elementwise_max(s, edge) - edge;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c.e[i] = (T)((float)c.e[i] * ((float)s.e[i] * (1.f / 16384.f)));
-    if (nan) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (s.e[i] == -32768) c.e[i] = (T)__builtin_nanf("");
-    }
+    for (int i = 0; i < 8; ++i) c.e[i] = (T)((float)c.e[i] * fmaf((float)steps[i], 1.f / 16384.f, (float)low[i]));
     return c.raw;
   }
 };

@@ -10,7 +10,8 @@ more term); a result rounded to a type by half a step, ``eps / 2`` of its size. 
 evaluated to ``|z| 2^-21 + 2^-24`` and their derivatives to 2^-20 (error function by a polynomial of
 error 1.5e-7, exponential and reciprocal of a few units in the last place, arguments rounded to fp32).
 Behind an activation the gradient is rounded to ``dtype`` before it is multiplied, and its factor
-act'(z) is held in steps of 2^-14 (half a step 2^-15) unless ``dtype`` is float32.
+act'(z) is held in 16 bits unless ``dtype`` is float32: above 1/8 in steps of 2^-14, below as fp16
+(``held_derivative``).
 """
 from __future__ import annotations
 
@@ -60,6 +61,14 @@ def _tiny(dtype):
     return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
 
 
+def held_derivative(d, off):
+    """How far act'(z) = d, evaluated to within ``off``, moves when it is held in 16 bits: half a step, above
+    1/8 of 2^-14, below of fp16's numbers, which have 11 significant bits down to 2^-14 and steps of 2^-24
+    below that."""
+    exponent = torch.frexp(d.abs() + off)[1].clamp(min=-13)         # |d| + off < 2^exponent
+    return torch.where(d - off >= 0.125, torch.full_like(d, 2.0 ** -15), torch.ldexp(torch.ones_like(d), exponent - 12))
+
+
 def _select(rows_group, weight, bias):
     """Per group: (group, rows, W, b)."""
     for g in range(weight.shape[0]):
@@ -100,8 +109,8 @@ def run(x, weight, bias, residual, activation, group, grad=None):
         else:
             # |act''| <= 1.13; relu's derivative is not known within ez of its step
             ed = (z.abs() <= ez).double() if activation == "relu" else 1.13 * ez + 2.0 ** -20
-            if dtype != torch.float32:
-                ed = ed + (0 if activation == "relu" else 2.0 ** -15)
+            if dtype != torch.float32 and activation != "relu":    # 0 and 1 are held exactly
+                ed = ed + held_derivative(d, ed)
             edz = us.abs() * ed
             edz = edz + step * (dz.abs() + edz) + tiny
         dx[at] = dz @ w
