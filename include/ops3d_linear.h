@@ -23,7 +23,8 @@
  * with groups + 1 entries the last is the end of the last group, with groups entries the last group
  * ends with the item.  Groups may be empty.  Entries are read on the device only: each counts as the
  * largest of itself and those before it, held to [0, rows].  Rows in no group (before the first,
- * behind the last) get y = 0 and grad_x = 0, and add nothing to the weights' gradients.
+ * behind the last) get y = 0 and grad_x = 0, whatever their residual, which has no gradient there
+ * (ops3d_linear_keep_rows), and add nothing to the weights' gradients.
  *
  * act_grad: act'(z) for the backward, [batch * rows, out_features], written by the forward when not
  * NULL and read by the backward; fp32 for F32, otherwise a 16-bit code: below 1/8 the bits of the fp16
@@ -82,6 +83,14 @@ OPS3D_FDA_API int ops3d_linear_backward(const void *x, int64_t ld_x, const void 
                                         int64_t ld_grad_y, void *grad_x, void *grad_weight, void *grad_bias,
                                         void *workspace, size_t workspace_bytes, int dtype, int batch, int64_t rows,
                                         int groups, int out_features, int in_features, void *stream);
+
+/*
+ * dst = src in rows of a group, 0 in rows of none ([batch * rows, features], contiguous): the gradient of
+ * a residual, which is grad_y in the former only, since y is 0 in the latter.  Without groups it is grad_y.
+ */
+OPS3D_FDA_API int ops3d_linear_keep_rows(const void *src, int64_t ld_src, const int64_t *group_start,
+                                         int group_start_count, void *dst, int dtype, int batch, int64_t rows,
+                                         int groups, int features, void *stream);
 
 #ifdef __cplusplus
 }

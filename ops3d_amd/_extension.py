@@ -63,6 +63,7 @@ EXPORTED_SYMBOLS = (
     "ops3d_linear_forward",
     "ops3d_linear_backward_workspace_bytes",
     "ops3d_linear_backward",
+    "ops3d_linear_keep_rows",
     "ops3d_fda_profile_enable",
     "ops3d_fda_profile_read",
 )
@@ -137,6 +138,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ops3d_linear_backward.restype = _i
     lib.ops3d_linear_backward.argtypes = ([_vp, _i64, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz]
                                           + [_i] * 2 + [_i64] + [_i] * 3 + [_vp])
+    lib.ops3d_linear_keep_rows.restype = _i
+    lib.ops3d_linear_keep_rows.argtypes = [_vp, _i64, _vp, _i, _vp, _i, _i, _i64, _i, _i, _vp]
     lib.ops3d_fda_backward_offsets.argtypes = [_vp] * 6 + [_i] + [_vp] * 5 + [_sz] + [_i] * 9 + [_vp]
 
 
@@ -164,7 +167,7 @@ class _NativeFDA:
                          "forward_keep_head_major", "backward_with_head_major",
                          "forward_offsets", "backward_offsets", "nms_3d", "roi_align_3d_forward",
                          "roi_align_3d_backward", "dcnv4_forward", "dcnv4_backward", "linear", "linear_forward",
-                         "linear_backward"):
+                         "linear_backward", "linear_keep_rows"):
                 setattr(self, name, getattr(ext, name))
 
     # -- helpers ---------------------------------------------------------------------------
@@ -363,6 +366,26 @@ class _NativeFDA:
         if rc != OPS3D_FDA_OK:
             self._raise(rc, "linear_backward failed")
         return gx, gw, gb
+
+    def linear_keep_rows(self, t, group_start, groups):
+        """t [S, N] or [B, S, N] with zeros in rows of no group, differentiable as often as wanted."""
+        from .linear import KeepRowsFunction
+
+        return KeepRowsFunction.apply(t, group_start, groups, self)
+
+    def _keep_rows(self, t, group_start, groups):
+        self._linear_check("the rows", t, t)
+        if t.dim() not in (2, 3):
+            raise ValueError("the rows must be [rows, features] or [batch, rows, features]")
+        B, S, E, start, count = self._linear_sizes(t, group_start, groups)
+        tr, ld = self._as_rows(t)
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        with torch.cuda.device(t.device):
+            rc = self._lib.ops3d_linear_keep_rows(_ptr(tr), ld, _ptr(start), count, _ptr(out), _DTYPE_CODE[t.dtype], B, S, E,
+                                                  t.shape[-1], torch.cuda.current_stream(t.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "linear_keep_rows failed")
+        return out
 
     # -- entry points (reference csrc/flash_deform_attn.h) -----------------------------------
     def flash_deform_attn_forward(

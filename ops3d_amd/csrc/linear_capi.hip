@@ -240,4 +240,22 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
   });
 }
 
+int ops3d_linear_keep_rows(const void *src, int64_t ld_src, const int64_t *group_start, int group_start_count, void *dst,
+                           int dtype, int batch, int64_t rows, int groups, int features, void *stream) {
+  ops3d_fda::set_last_error(OPS3D_FDA_OK, "");
+  int rc = check_sizes(dtype, batch, rows, groups, features, 1);
+  if (rc) return rc;
+  if (ld_src < 0) return fail(OPS3D_FDA_EINVAL, "row distances must not be negative");
+  if (!group_start) return fail(OPS3D_FDA_EINVAL, "group_start is NULL");
+  if (batch * rows == 0) return OPS3D_FDA_OK;
+  Groups g{};
+  if ((rc = make_groups(group_start, group_start_count, batch, rows, groups, g))) return rc;
+  if (!src || !dst) return fail(OPS3D_FDA_EINVAL, "NULL pointer argument");
+  if (misaligned(src, elem_size(dtype)) || misaligned(dst, elem_size(dtype)))
+    return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
+  return run(dtype, "rows of groups", [&](auto t) {
+    return ops3d_linear::keep_rows<decltype(t)>(src, ld_src, dst, batch * rows, features, g, static_cast<hipStream_t>(stream));
+  });
+}
+
 }  // extern "C"

@@ -626,6 +626,42 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
   return {gx, gw, gb};
 }
 
+// t with zeros in rows of no group.
+at::Tensor keep_rows(const at::Tensor &t, const at::Tensor &group_start, int64_t groups) {
+  linear_check(t, "the rows", t);
+  if (t.dim() != 2 && t.dim() != 3)
+    throw std::invalid_argument("the rows must be [rows, features] or [batch, rows, features]");
+  const LinearSizes z = linear_sizes(t, group_start, groups, t.size(-1), 1);
+  const DeviceGuard guard(t.device());
+  int64_t ld = 0;
+  const at::Tensor rows = as_rows(t, ld);
+  at::Tensor out = at::empty(t.sizes(), t.options());
+  const int rc = ops3d_linear_keep_rows(ptr(rows), ld, z.start, z.count, ptr(out), z.code, z.batch, z.rows, z.groups, z.N,
+                                        stream_of(t));
+  if (rc != OPS3D_FDA_OK) raise(rc, "linear_keep_rows failed");
+  return out;
+}
+
+// The same through autograd; it is its own gradient.
+class KeepRowsNode : public torch::autograd::Function<KeepRowsNode> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &t, const at::Tensor &group_start,
+                            int64_t groups) {
+    ctx->save_for_backward({group_start});
+    ctx->saved_data["groups"] = groups;
+    return keep_rows(t, group_start, groups);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    return {KeepRowsNode::apply(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["groups"].toInt()), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+at::Tensor linear_keep_rows(const at::Tensor &t, const at::Tensor &group_start, int64_t groups) {
+  return KeepRowsNode::apply(t, group_start, groups);
+}
+
 // The operator with its autograd node here: a training step on a small crop is bound by host time, of
 // which a node in Python costs several times as much.  Once differentiable: with create_graph the
 // gradients raise when they are differentiated.
@@ -660,8 +696,8 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
         if (gw) out[1] = *gw;
         if (gb) out[2] = *gb;
       }
-      if (sizes[5]) out[3] = grad;
     }
+    if (sizes[5]) out[3] = saved[2].defined() ? linear_keep_rows(grad, saved[2], sizes[1]) : grad;   // y is 0 in rows of no group
     if (once) {
       torch::autograd::variable_list given;
       for (const auto &t : out)
@@ -706,6 +742,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_forward", &linear_forward, "act(x W^T + b) + residual, one weight or one per group of rows");
   m.def("linear", &linear, "linear_forward with its gradients through autograd");
   m.def("linear_backward", &linear_backward, "gradients of linear_forward");
+  m.def("linear_keep_rows", &linear_keep_rows, "zeros in rows of no group");
   m.def("roi_align_3d_forward", &roi_align_3d_forward, "roi_align_3d_forward");
   m.def("roi_align_3d_backward", &roi_align_3d_backward, "roi_align_3d_backward");
 }

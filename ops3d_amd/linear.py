@@ -46,7 +46,25 @@ class LinearFunction(Function):
         if need_x or need_w or need_b:
             grad_x, grad_w, grad_b = ctx.native.linear_backward(
                 x, weight, group_start, act_grad, grad_output, ctx.in_features, ctx.groups, need_w, need_b)
-        return grad_x, grad_w, grad_b, grad_output if need_r else None, None, None, None
+        grad_r = None
+        if need_r:   # rows of no group are 0 whatever the residual
+            grad_r = grad_output if group_start is None else ctx.native.linear_keep_rows(grad_output, group_start, ctx.groups)
+        return grad_x, grad_w, grad_b, grad_r, None, None, None
+
+
+class KeepRowsFunction(Function):
+    """Zeros in rows of no group, for the binding without the extension module; its own gradient."""
+
+    @staticmethod
+    def forward(ctx, t, group_start, groups, native):
+        ctx.save_for_backward(group_start)
+        ctx.groups, ctx.native = groups, native
+        return native._keep_rows(t, group_start, groups)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        (group_start,) = ctx.saved_tensors
+        return KeepRowsFunction.apply(grad_output, group_start, ctx.groups, ctx.native), None, None, None
 
 
 def _apply(x, weight, bias, residual, group_start, activation):

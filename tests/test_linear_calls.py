@@ -2,12 +2,14 @@
 (whose helpers and float64 restatement are used here)."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 from oracle import linear as ref
-from ops3d_amd import fused_linear
-from test_linear import DTYPES, gpu, log
+from ops3d_amd import _extension, fused_linear, grouped_linear
+from test_linear import DTYPES, gpu, log, make
 
 
 # act' far out, small beside 1: z, and act's names
@@ -40,3 +42,89 @@ def test_saturated_units_keep_their_gradients(gpu_device, activation, z, dtype, 
         err = (got.double() / want - 1).abs().max().item()
         assert err <= rel, f"{name}: off by {err:.2e} of {want:.3e}"
     assert not dx.any()
+
+
+def bindings():
+    """The extension module's operators and those of the binding without it, under one signature."""
+    C = _extension._C
+    bare = type(C)(C._lib, C.__file__)
+    return {"module": C.linear, "ctypes": lambda *a: type(C).linear(bare, *a)}
+
+
+@gpu
+@pytest.mark.parametrize("binding", ["module", "ctypes"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("batch,N,start", [(0, 24, [10, 60, 150]), (2, 7, [10, 60, 60, 150]), (3, 1, [-5, 90, 40, 170]),
+                                           (2, 40, [0, 30, 200]), (0, 130, [200, 200, 200]), (0, 16, [5, 100])])
+def test_residual_gradient_of_rows_in_no_group(gpu_device, batch, N, start, dtype, binding):
+    """y is 0 in rows of no group whatever the residual holds, so the residual's gradient is 0 there."""
+    S, K, E = 200, 16, {2: 2, 3: 2, 4: 3}[len(start)]
+    log(f"[case] residual gradient {batch} {N} {start} {dtype} {binding}")
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    lead = (batch, S) if batch else (S,)
+    dt = DTYPES[dtype]
+    x, w, r, u = (make(gen, s, dt) for s in ((*lead, K), (E, N, K), (*lead, N), (*lead, N)))
+    inside = (ref.group_of_rows(S, start, E) >= 0).cuda()[:, None]
+    u = torch.where(inside, u, torch.full_like(u, float("nan")))
+    table = torch.tensor(start, device="cuda")
+    op = bindings()[binding]
+    want = torch.where(inside, u, torch.zeros_like(u))
+    for leaves in ((r,), (x, w, r)):
+        leaves = [t.detach().requires_grad_(True) for t in leaves]
+        y = op(*(leaves[:2] if len(leaves) == 3 else (x, w)), None, leaves[-1], table, 0)
+        assert torch.equal(torch.autograd.grad(y, leaves, u)[-1], want)
+    # rows in a wider matrix, one row for all, another order of the axes
+    for v in (torch.cat([u, u], -1)[..., :N], u[..., :1, :].nan_to_num(1.0).expand(*lead, N),
+              u.transpose(-1, -2).contiguous().transpose(-1, -2)):
+        rl = r.detach().requires_grad_(True)
+        (dr,) = torch.autograd.grad(op(x, w, None, rl, table, 0), rl, v)
+        assert torch.equal(dr, torch.where(inside, v, torch.zeros_like(v)))
+
+
+@gpu
+def test_residual_gradient_captured(gpu_device):
+    """The same in a graph, replayed with other groups between eager calls."""
+    gen = torch.Generator(device="cuda").manual_seed(32)
+    x, w, r, u = (make(gen, s, torch.bfloat16) for s in ((300, 32), (2, 48, 32), (300, 48), (300, 48)))
+    start = torch.tensor([10, 60, 150], device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w, r)]
+    log("[case] residual gradient captured")
+
+    def step():
+        return torch.autograd.grad(grouped_linear(x, w, start, None, "silu", r), leaves, u)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step()
+    for table in ([10, 60, 150], [0, 0, 300], [299, 299, 300], [0, 0, 0]):
+        start.copy_(torch.tensor(table))
+        g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(outs, want))
+        row = torch.arange(300, device="cuda")[:, None]
+        assert torch.equal(outs[2], torch.where((row >= table[0]) & (row < table[2]), u, torch.zeros_like(u)))
+
+
+def test_keep_rows_refusals():
+    if _extension._C is None:
+        pytest.skip("library not built")
+    lib, p = _extension._C._lib, ctypes.c_void_p(256)   # a stand-in: refused before any launch
+
+    def call(src=p, ld=8, start=p, count=2, dst=p, dtype=2, batch=1, rows=4, groups=2, features=8):
+        return lib.ops3d_linear_keep_rows(src, ld, start, count, dst, dtype, batch, rows, groups, features, None)
+
+    for text, kw in (("unsupported dtype", dict(dtype=9)), ("rows", dict(rows=-1)), ("out_features", dict(features=0)),
+                     ("groups must be", dict(groups=0)), ("negative", dict(ld=-1)), ("NULL", dict(start=None)),
+                     ("NULL", dict(src=None)), ("NULL", dict(dst=None)), ("must have", dict(count=4)),
+                     ("8-byte", dict(start=ctypes.c_void_p(260))), ("element size", dict(dst=ctypes.c_void_p(257)))):
+        assert call(**kw) == 1 and text in lib.ops3d_fda_last_error().decode(), (text, lib.ops3d_fda_last_error())
+    assert call(src=None, dst=None, rows=0) == 0
+    with pytest.raises(RuntimeError, match="CPU"):
+        _extension._C.linear_keep_rows(torch.zeros(4, 8), torch.zeros(2, dtype=torch.int64), 2)
