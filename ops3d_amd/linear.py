@@ -78,8 +78,19 @@ def _apply(x, weight, bias, residual, group_start, activation):
         x, weight = x.to(dt), weight.to(dt)
         bias = None if bias is None else bias.to(dt)
         if residual is not None and residual.dtype != dt:
-            return _run(x, weight, bias, None, group_start, act) + residual
+            y = _run(x, weight, bias, None, group_start, act)
+            if group_start is not None:
+                residual = _rows_of_groups(residual.expand(y.shape), group_start, weight.shape[0])
+            return y + residual
     return _run(x, weight, bias, residual, group_start, act)
+
+
+def _rows_of_groups(t, group_start, groups):
+    """t with zeros in rows of no group."""
+    if t.dtype in (torch.float32, torch.float16, torch.bfloat16):
+        return _extension._C.linear_keep_rows(t, group_start, groups)
+    ones = torch.ones((*t.shape[:-1], 1), device=t.device)
+    return torch.where(_extension._C.linear_keep_rows(ones, group_start, groups) > 0, t, t.new_zeros(()))
 
 
 def _run(x, weight, bias, residual, group_start, act):

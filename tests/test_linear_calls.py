@@ -128,3 +128,23 @@ def test_keep_rows_refusals():
     assert call(src=None, dst=None, rows=0) == 0
     with pytest.raises(RuntimeError, match="CPU"):
         _extension._C.linear_keep_rows(torch.zeros(4, 8), torch.zeros(2, dtype=torch.int64), 2)
+
+@gpu
+@pytest.mark.parametrize("wide", [torch.float32, torch.float64])
+def test_autocast_residual_of_rows_in_no_group(gpu_device, wide):
+    """Under autocast a wider residual is added outside the product: rows of no group stay 0 all the same."""
+    gen = torch.Generator(device="cuda").manual_seed(33)
+    x, w, r, u = (make(gen, s, torch.float32) for s in ((2, 50, 32), (2, 24, 32), (2, 50, 24), (2, 50, 24)))
+    r, u = r.to(wide), u.to(wide)
+    start = torch.tensor([7, 20, 41], device="cuda")
+    rl = r.requires_grad_(True)
+    log(f"[case] autocast, rows of no group {wide}")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = grouped_linear(x, w, start, None, "gelu", rl)
+        row = grouped_linear(x, w, start, None, "gelu", rl[0, 0])   # added outside, it may be broadcast
+    plain = grouped_linear(x.bfloat16(), w.bfloat16(), start, None, "gelu")
+    inside = (ref.group_of_rows(50, [7, 20, 41], 2) >= 0).cuda()[:, None]
+    assert y.dtype == wide
+    assert torch.equal(y, torch.where(inside, plain + r, torch.zeros_like(r)))
+    assert torch.equal(row, torch.where(inside, plain + r[0, 0], torch.zeros_like(r)))
+    assert torch.equal(torch.autograd.grad(y, rl, u)[0], torch.where(inside, u, torch.zeros_like(u)))
