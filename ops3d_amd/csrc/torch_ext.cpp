@@ -664,7 +664,7 @@ at::Tensor linear_keep_rows(const at::Tensor &t, const at::Tensor &group_start, 
 
 // The operator with its autograd node here: a training step on a small crop is bound by host time, of
 // which a node in Python costs several times as much.  Once differentiable: with create_graph the
-// gradients raise when they are differentiated.
+// gradients that are no constants raise when they are differentiated (a residual's may be).
 class LinearNode : public torch::autograd::Function<LinearNode> {
  public:
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight,
@@ -686,7 +686,6 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
     const at::Tensor &grad = grads[0];
     torch::autograd::variable_list out(6);
     const auto some = [](const at::Tensor &t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
-    const bool once = at::GradMode::is_enabled() && grad.requires_grad();
     {
       const at::NoGradGuard no_grad;
       if (sizes[2] || sizes[3] || sizes[4]) {
@@ -698,16 +697,14 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
       }
     }
     if (sizes[5]) out[3] = saved[2].defined() ? linear_keep_rows(grad, saved[2], sizes[1]) : grad;   // y is 0 in rows of no group
-    if (once) {
-      torch::autograd::variable_list given;
-      for (const auto &t : out)
-        if (t.defined()) given.push_back(t.detach().set_requires_grad(true));
-      const auto error = std::make_shared<torch::autograd::DelayedError>(
-          "trying to differentiate twice a linear operator that is differentiable once", (int64_t)given.size());
-      given = (*error)(std::move(given));
-      size_t i = 0;
-      for (auto &t : out)
-        if (t.defined()) t = given[i++];
+    if (at::GradMode::is_enabled()) {   // each that depends on something with a gradient
+      const bool act = saved[3].defined(), depends[3] = {sizes[3] || act, sizes[2] || act, act};
+      for (int i = 0; i < 3; ++i) {
+        if (!out[i].defined() || !(depends[i] || grad.requires_grad())) continue;
+        const auto error = std::make_shared<torch::autograd::DelayedError>(
+            "trying to differentiate twice a linear operator that is differentiable once", 1);
+        out[i] = (*error)({out[i].detach().set_requires_grad(true)})[0];
+      }
     }
     return out;
   }

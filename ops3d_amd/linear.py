@@ -17,7 +17,6 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _extension
 
@@ -38,18 +37,39 @@ class LinearFunction(Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output):
         x, weight, group_start, act_grad = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         grad_x = grad_w = grad_b = None
         if need_x or need_w or need_b:
-            grad_x, grad_w, grad_b = ctx.native.linear_backward(
-                x, weight, group_start, act_grad, grad_output, ctx.in_features, ctx.groups, need_w, need_b)
+            with torch.no_grad():
+                grad_x, grad_w, grad_b = ctx.native.linear_backward(
+                    x, weight, group_start, act_grad, grad_output, ctx.in_features, ctx.groups, need_w, need_b)
+            if torch.is_grad_enabled():   # each that depends on something with a gradient
+                act, given = act_grad is not None, grad_output.requires_grad
+                grad_x = _once(grad_x, need_w or act or given)
+                grad_w = _once(grad_w, need_x or act or given)
+                grad_b = _once(grad_b, act or given)
         grad_r = None
         if need_r:   # rows of no group are 0 whatever the residual
             grad_r = grad_output if group_start is None else ctx.native.linear_keep_rows(grad_output, group_start, ctx.groups)
         return grad_x, grad_w, grad_b, grad_r, None, None, None
+
+
+class _Once(Function):
+    """A gradient that raises when it is differentiated."""
+
+    @staticmethod
+    def forward(ctx, t):
+        return t.view_as(t)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        raise RuntimeError("trying to differentiate twice a linear operator that is differentiable once")
+
+
+def _once(grad, depends):
+    return _Once.apply(grad.detach().requires_grad_(True)) if grad is not None and depends else grad
 
 
 class KeepRowsFunction(Function):

@@ -148,3 +148,49 @@ def test_autocast_residual_of_rows_in_no_group(gpu_device, wide):
     assert torch.equal(y, torch.where(inside, plain + r, torch.zeros_like(r)))
     assert torch.equal(row, torch.where(inside, plain + r[0, 0], torch.zeros_like(r)))
     assert torch.equal(torch.autograd.grad(y, rl, u)[0], torch.where(inside, u, torch.zeros_like(u)))
+
+
+@gpu
+@pytest.mark.parametrize("binding", ["module", "ctypes"])
+@pytest.mark.parametrize("act", [0, 2])
+def test_gradient_penalty_raises(gpu_device, act, binding):
+    """A gradient that depends on something that requires one raises when it is differentiated, also where
+    grad_output is a plain tensor: a penalty on it must not be dropped."""
+    gen = torch.Generator(device="cuda").manual_seed(34)
+    op = bindings()[binding]
+    log(f"[case] penalty {act} {binding}")
+
+    def leaves(*wanted):
+        sizes = {"x": (20, 16), "w": (24, 16), "b": (24,), "r": (20, 24)}
+        return [make(gen, s, torch.float32).requires_grad_(k in wanted) for k, s in sizes.items()]
+
+    x, w, b, r = leaves("x", "w", "b", "r")
+    for wanted in (x, w, b):
+        y = op(x, w, b, r, None, act)
+        (g,) = torch.autograd.grad(y.sum(), wanted, create_graph=True)
+        if wanted is b and not act:
+            assert not g.requires_grad      # a sum of grad_output alone
+            continue
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (y.sum() + g.pow(2).sum()).backward()
+    # a weight without a gradient and no activation: x's gradient is a constant, and the penalty's is 0
+    x, w, b, r = leaves("x")
+    y = op(x, w, b, r, None, act)
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    if not act:
+        assert not g.requires_grad
+        (y.sum() + g.pow(2).sum()).backward()
+        assert torch.equal(x.grad, g)
+    else:
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (y.sum() + g.pow(2).sum()).backward()
+    # the residual's gradient is grad_output itself, as often as wanted
+    x, w, b, r = leaves("r")
+    u = make(gen, (20, 24), torch.float32).requires_grad_(True)
+    (g,) = torch.autograd.grad(op(x, w, b, r, None, act), r, u, create_graph=True)
+    assert torch.equal(torch.autograd.grad(g.pow(2).sum(), u)[0], 2 * u)
+    start = torch.tensor([3, 9, 17], device="cuda")
+    y = op(x, torch.stack([w, w]), torch.stack([b, b]), r, start, act)
+    (g,) = torch.autograd.grad(y, r, u, create_graph=True)
+    inside = (ref.group_of_rows(20, [3, 9, 17], 2) >= 0).cuda()[:, None]
+    assert torch.equal(torch.autograd.grad(g.pow(2).sum(), u)[0], torch.where(inside, 2 * u, torch.zeros_like(u)))
