@@ -114,6 +114,7 @@ struct Layout {
 template <typename F> int run(int dtype, const char *what, F f) {
   hipError_t e = dtype == OPS3D_FDA_F32 ? f(float()) : dtype == OPS3D_FDA_F16 ? f(_Float16()) : f(__bf16());
   if (e == hipSuccess) return OPS3D_FDA_OK;
+  if (e == hipErrorInvalidConfiguration) return fail(OPS3D_FDA_EINVAL, "%s: 2^31 tiles or more", what);
   return fail(OPS3D_FDA_ERUNTIME, "%s: kernel launch failed: %s", what, hipGetErrorString(e));
 }
 

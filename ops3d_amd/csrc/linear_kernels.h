@@ -56,6 +56,7 @@ struct RowsArgs {
   int splits, per_split;  // parts of the sum, and elements of each (SPLIT kernels)
   float *part;            // their sums [splits, rows, N]
   int64_t rows;           // of all items
+  unsigned block0;        // blocks in launches before this one
   Groups g;
 };
 
@@ -69,6 +70,7 @@ struct WeightArgs {
   int chunk, items;       // rows of an item, and items, per chunk
   int n_tiles, k_tiles;
   int slots;              // bound on the number of chunks
+  unsigned block0;        // as RowsArgs'
   Groups g;
 };
 
@@ -592,8 +594,8 @@ template <typename T> __device__ __forceinline__ int column_of(int n, int i) {
   return (n >> 1) * 32 + (i >> 2) * 8 + (n & 1) * 4 + (i & 3);
 }
 
-// blockIdx -> (row tile, column tile).  spread: the column tiles of a row tile run one after another
-// on one XCD, whose L2 then holds the row tile (blocks go to XCD blockIdx % 8); used from 64 row tiles
+// block -> (row tile, column tile).  spread: the column tiles of a row tile run one after another
+// on one XCD, whose L2 then holds the row tile (blocks go to XCD block % 8); used from 64 row tiles
 // on, where every XCD gets its share of them.
 __device__ __forceinline__ void block_tile(int bid, int col_tiles, int spread, int &rt, int &ct) {
   if (spread) {
@@ -716,9 +718,9 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   constexpr int kStage = SA::kBytes + SB::kBytes;
   __shared__ __attribute__((aligned(16))) char lds[U * kStage];
 
-  const int part = SPLIT ? blockIdx.x % p.splits : 0;
+  const int block = blockIdx.x + p.block0, part = SPLIT ? block % p.splits : 0;
   int rt, ct;
-  block_tile(SPLIT ? blockIdx.x / p.splits : blockIdx.x, p.col_tiles, p.spread, rt, ct);
+  block_tile(SPLIT ? block / p.splits : block, p.col_tiles, p.spread, rt, ct);
   if (rt >= p.row_tiles) return;
   RowTile tile;
   if (!find_row_tile(p.g, rt, BM, tile)) return;
@@ -964,8 +966,9 @@ template <typename T, bool EPI> __global__ __launch_bounds__(kJoinThreads) void 
   constexpr int CH = 16 / (int)sizeof(T), PC = 64 / CH;
   typedef typename Deriv<T>::type D;
   RowTile tile;
-  if (!find_row_tile(p.g, blockIdx.x / p.col_tiles, 16, tile)) return;
-  const int n0 = blockIdx.x % p.col_tiles * 64;
+  const int block = blockIdx.x + p.block0;
+  if (!find_row_tile(p.g, block / p.col_tiles, 16, tile)) return;
+  const int n0 = block % p.col_tiles * 64;
   for (int c = threadIdx.x; c < 16 * PC; c += kJoinThreads) {
     const int row = c / PC, col = n0 + c % PC * CH, left = p.N - col;
     if (row >= tile.rows || left <= 0) continue;
@@ -1022,7 +1025,7 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(RowsArgs p) {
   constexpr int CH = 16 / (int)sizeof(T), KS = 4 * CH;   // sum elements of a step: 16 bytes a lane, 4 lanes a row
   __shared__ f32x4 red[NW][RT][64];
   int rt, ct;
-  block_tile(blockIdx.x, p.col_tiles, 0, rt, ct);
+  block_tile(blockIdx.x + p.block0, p.col_tiles, 0, rt, ct);
   RowTile tile;
   if (!find_row_tile(p.g, rt, 16 * RT, tile)) return;
   const int n0 = ct * 16, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
@@ -1113,7 +1116,7 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
   static_assert(!RING || (DMA && !RUNS && sizeof(T) == 2), "whole items, 16-byte rows, transposing reads");
   __shared__ __attribute__((aligned(16))) char lds[(RING ? 2 : 1) * kStage];
   int slot, ct;
-  block_tile(blockIdx.x, p.n_tiles * p.k_tiles, 1, slot, ct);
+  block_tile(blockIdx.x + p.block0, p.n_tiles * p.k_tiles, 1, slot, ct);
   if (slot >= p.slots) return;
   RowChunk ch;
   if (!find_chunk(p.g, slot, p.chunk, p.items, false, ch)) return;
@@ -1341,16 +1344,24 @@ __global__ __launch_bounds__(256) void join_kernel(WeightArgs p) {
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Row tiles of BM rows at most: every segment may end inside one.
+// Row tiles of BM rows at most: every segment may end inside one, but an item has no more than its rows.
 inline int64_t max_row_tiles(const Groups &g, int BM) {
   if (!g.start) return ceil_div(g.S, BM);
-  return (int64_t)g.B * (g.S / BM + g.E + 2);
+  const int64_t tiles = (int64_t)g.S / BM + g.E + 2;
+  return (int64_t)g.B * (tiles < g.S ? tiles : g.S);
 }
 
-template <typename K> inline hipError_t launch(K kernel, int64_t grid, int threads, hipStream_t st, const RowsArgs &p) {
+// A launch holds less than 2^32 threads; more go in several, each a multiple of the XCDs' 8 blocks.
+template <typename K, typename A> inline hipError_t launch(K kernel, int64_t grid, int threads, hipStream_t st, A p) {
   if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), 0, st, p);
-  return hipGetLastError();
+  const int64_t most = 0xffffffff / threads & ~(int64_t)7;
+  for (int64_t at = 0; at < grid; at += most) {
+    p.block0 = (unsigned)at;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(grid - at < most ? grid - at : most)), dim3(threads), 0, st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT = false>
@@ -1532,26 +1543,23 @@ template <typename T> hipError_t grad_weight(const WeightArgs &q, int tile, bool
   p.n_tiles = ceil_div(p.N, tile);
   p.k_tiles = p.gw ? ceil_div(p.K, tile) : 1;
   const int64_t grid = ((int64_t)p.slots + 7) / 8 * 8 * p.n_tiles * p.k_tiles;
-  if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
   const bool aligned = rows_aligned(p.u, p.ldu, sizeof(T)) && rows_aligned(p.x, p.ldx, sizeof(T)) &&
                        p.N % (16 / sizeof(T)) == 0 && p.K % (16 / sizeof(T)) == 0;
-  const dim3 blocks((unsigned)grid), threads(256);
-  const auto launch = [&](auto runs) {
+  const auto start = [&](auto runs) {
     constexpr bool R = decltype(runs)::value;
-    if (tile == 128 && aligned) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, R, false, 2>), blocks, threads, 0, st, p);
-    else if (tile == 128) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, false, R, false, 2>), blocks, threads, 0, st, p);
-    else if (aligned) hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, true, R, false, 4>), blocks, threads, 0, st, p);
-    else hipLaunchKernelGGL((weight_kernel<T, 64, 64, 2, 2, false, R, false, 4>), blocks, threads, 0, st, p);
+    if (tile == 128 && aligned) return launch(weight_kernel<T, 128, 128, 2, 2, true, R, false, 2>, grid, 256, st, p);
+    if (tile == 128) return launch(weight_kernel<T, 128, 128, 2, 2, false, R, false, 2>, grid, 256, st, p);
+    if (aligned) return launch(weight_kernel<T, 64, 64, 2, 2, true, R, false, 4>, grid, 256, st, p);
+    return launch(weight_kernel<T, 64, 64, 2, 2, false, R, false, 4>, grid, 256, st, p);
   };
+  hipError_t e = hipSuccess;
   bool ring = false;
   if constexpr (sizeof(T) == 2) {
     ring = tile == 128 && aligned && p.items == 1 && (int64_t)p.g.B * p.g.S / p.slots >= 512;
-    if (ring) hipLaunchKernelGGL((weight_kernel<T, 128, 128, 2, 2, true, false, true, 2>), blocks, threads, 0, st, p);
+    if (ring) e = launch(weight_kernel<T, 128, 128, 2, 2, true, false, true, 2>, grid, 256, st, p);
   }
-  if (!ring) {
-    if (p.items > 1) launch(std::true_type());
-    else launch(std::false_type());
-  }
+  if (!ring) e = p.items > 1 ? start(std::true_type()) : start(std::false_type());
+  if (e != hipSuccess) return e;
   if (joined) {
     const int64_t total = (p.gw ? (int64_t)p.N * p.K : 0) + (p.gb ? p.N : 0), want = (total + 63) / 64;
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(want < 2048 ? want : 2048), p.g.E), dim3(256), 0, st, p);

@@ -9,7 +9,7 @@ import torch
 
 from oracle import linear as ref
 from ops3d_amd import _extension, fused_linear, grouped_linear
-from test_linear import DTYPES, gpu, log, make
+from test_linear import DTYPES, gpu, log, make, grouped_case
 
 
 # act' far out, small beside 1: z, and act's names
@@ -194,3 +194,60 @@ def test_gradient_penalty_raises(gpu_device, act, binding):
     (g,) = torch.autograd.grad(y, r, u, create_graph=True)
     inside = (ref.group_of_rows(20, [3, 9, 17], 2) >= 0).cuda()[:, None]
     assert torch.equal(torch.autograd.grad(g.pow(2).sum(), u)[0], torch.where(inside, 2 * u, torch.zeros_like(u)))
+
+
+@gpu
+def test_many_items_of_many_groups(gpu_device):
+    """More groups than an item has rows: no more tiles than rows, and no launch of 2^32 threads."""
+    S, E = 128, 1024
+    log("[case] 64 items of 1024 groups")
+    grouped_case(S, [i // 8 for i in range(E)], E, 32, 4096, torch.bfloat16, "silu", batch=64)
+
+
+@gpu
+def test_grids_beyond_one_launch(gpu_device):
+    """2^32 threads and more, in several launches: products of one term, which are exact."""
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    bf = torch.bfloat16
+    with torch.no_grad():
+        log("[case] 17 groups of one row, 2^24 columns")
+        E, N = 17, 1 << 24
+        x, w = make(gen, (E, 1), bf), make(gen, (E, N, 1), bf)
+        y = grouped_linear(x, w, torch.arange(E, device="cuda"))
+        for e in range(E):
+            assert torch.equal(y[e], (x[e].float() * w[e, :, 0].float()).to(bf))
+        del x, w, y
+    log("[case] 1.1e9 rows of one feature")
+    rows = 1_100_000_000
+    x = (torch.arange(rows, dtype=torch.int32, device="cuda") % 251).to(bf)[:, None].requires_grad_(True)
+    w = torch.full((1, 1), -2.0, dtype=bf, device="cuda")
+    y = fused_linear(x, w)
+    assert torch.equal(y, x.detach() * -2)
+    (dx,) = torch.autograd.grad(y, x, x.detach())
+    assert torch.equal(dx, y.detach())
+    del x, y, dx
+    log("[case] 4096 groups, three with a row, 262208 features")
+    E, K = 4096, 262208
+    w = torch.zeros(E, 1, K, dtype=bf, device="cuda").requires_grad_(True)
+    x, u = make(gen, (5, K), bf), make(gen, (5, 1), bf)
+    table = torch.tensor([0] + [1] * 2000 + [2] * 2094 + [3, 4], device="cuda")   # rows 0, 1, 2 and 3 each in a group
+    assert table.numel() == E + 1
+    (dw,) = torch.autograd.grad(grouped_linear(x, w, table), w, u)
+    full = {int((table[1:] > r).nonzero()[0, 0]): r for r in range(4)}
+    for e, r in full.items():
+        assert torch.equal(dw[e, 0], (u[r].float() * x[r].float()).to(bf))
+    empty = torch.ones(E, dtype=torch.bool, device="cuda")
+    empty[list(full)] = False
+    assert not dw[empty].any()
+
+
+def test_too_many_tiles_are_refused():
+    if _extension._C is None:
+        pytest.skip("library not built")
+    lib, p = _extension._C._lib, ctypes.c_void_p(256)   # a stand-in: refused before any launch
+    many = 1 << 24
+    assert lib.ops3d_linear_forward(p, 8, p, None, None, 0, None, 0, p, None, None, 0, 2, 0, 1, many, 1, many, 8, None) == 1
+    assert b"2^31 tiles" in lib.ops3d_fda_last_error()
+    assert lib.ops3d_linear_backward(p, many, p, None, 0, None, p, 8, p, None, None, p, 1 << 62, 2, 1, many, 1, 8, many,
+                                     None) == 1
+    assert b"gradient: 2^31 tiles" in lib.ops3d_fda_last_error()
