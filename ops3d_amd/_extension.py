@@ -275,6 +275,9 @@ class _NativeFDA:
 
     def linear(self, x, weight, bias, residual, group_start, act):
         """The operator through autograd (LinearFunction where a gradient is wanted)."""
+        if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+               for t in (x, weight, bias, residual)):
+            raise RuntimeError("the linear operators have no forward-mode derivatives")
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
             from .linear import LinearFunction
 

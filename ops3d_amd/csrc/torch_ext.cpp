@@ -710,8 +710,18 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
   }
 };
 
+// A tangent would be lost without a word: y comes from a kernel that knows of none.
+void refuse_tangent(const at::Tensor &t) {
+  if (t.defined() && t._fw_grad(0).defined())
+    throw std::runtime_error("the linear operators have no forward-mode derivatives");
+}
+
 at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const c10::optional<at::Tensor> &bias,
                   const c10::optional<at::Tensor> &residual, const c10::optional<at::Tensor> &group_start, int64_t act) {
+  refuse_tangent(x);
+  refuse_tangent(weight);
+  if (bias) refuse_tangent(*bias);
+  if (residual) refuse_tangent(*residual);
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
                                      (residual && residual->requires_grad())))
     return LinearNode::apply(x, weight, bias, residual, group_start, act);

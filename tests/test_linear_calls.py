@@ -251,3 +251,45 @@ def test_too_many_tiles_are_refused():
     assert lib.ops3d_linear_backward(p, many, p, None, 0, None, p, 8, p, None, None, p, 1 << 62, 2, 1, many, 1, 8, many,
                                      None) == 1
     assert b"gradient: 2^31 tiles" in lib.ops3d_fda_last_error()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+@pytest.mark.parametrize("wants", [False, True])
+def test_forward_mode_is_refused(which, wants, device):
+    """A tensor with a tangent is refused, with gradients wanted or not: y would come without one."""
+    fw = torch.autograd.forward_ad
+    t = {"x": torch.ones(5, 8), "weight": torch.ones(4, 8), "bias": torch.ones(4), "residual": torch.ones(5, 4)}
+    t = {k: v.to(device).requires_grad_(wants) for k, v in t.items()}
+    if _extension._C is None:
+        pytest.skip("library not built")
+    with fw.dual_level():
+        t[which] = fw.make_dual(t[which], torch.ones_like(t[which]))
+        for f in bindings().values():
+            for grad in (torch.enable_grad(), torch.no_grad()):
+                with grad, pytest.raises(RuntimeError, match="forward-mode"):
+                    f(t["x"], t["weight"], t["bias"], t["residual"], None, 0)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fused_linear(**t)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            grouped_linear(t["x"], t["weight"][None], torch.zeros(1, dtype=torch.int64, device=device),
+                           t["bias"][None], None, t["residual"])
+
+
+@gpu
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+def test_transforms_are_refused(gpu_device, which):
+    """torch.func and vmap wrap tensors without memory of their own: every argument raises."""
+    t = {"x": torch.ones(5, 8), "weight": torch.ones(4, 8), "bias": torch.ones(4), "residual": torch.ones(5, 4)}
+    t = {k: v.cuda() for k, v in t.items()}
+    log(f"[case] transforms of {which}")
+
+    def f(v):
+        return fused_linear(**{**t, which: v})
+
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda v: f(v).sum())(t[which])
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(f, (t[which],), (t[which],))
+    with pytest.raises(RuntimeError):
+        torch.vmap(f)(torch.stack([t[which]] * 3))
