@@ -275,6 +275,8 @@ class _NativeFDA:
 
     def linear(self, x, weight, bias, residual, group_start, act):
         """The operator through autograd (LinearFunction where a gradient is wanted)."""
+        if torch.jit.is_tracing():   # a trace would record y's allocation without the kernel that fills it
+            raise RuntimeError("the linear operators cannot be traced")
         if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
                for t in (x, weight, bias, residual)):
             raise RuntimeError("the linear operators have no forward-mode derivatives")

@@ -9,6 +9,7 @@
 // (std::invalid_argument, as the reference's), OPS3D_FDA_ERUNTIME raises RuntimeError.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 // torch's current HIP stream of a device (c10's native HIP API); the device is made current
 // with HIP's own calls (DeviceGuard below)
@@ -718,6 +719,8 @@ void refuse_tangent(const at::Tensor &t) {
 
 at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const c10::optional<at::Tensor> &bias,
                   const c10::optional<at::Tensor> &residual, const c10::optional<at::Tensor> &group_start, int64_t act) {
+  if (torch::jit::tracer::isTracing())   // a trace would record y's allocation without the kernel that fills it
+    throw std::runtime_error("the linear operators cannot be traced");
   refuse_tangent(x);
   refuse_tangent(weight);
   if (bias) refuse_tangent(*bias);

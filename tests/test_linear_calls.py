@@ -293,3 +293,18 @@ def test_transforms_are_refused(gpu_device, which):
         torch.func.jvp(f, (t[which],), (t[which],))
     with pytest.raises(RuntimeError):
         torch.vmap(f)(torch.stack([t[which]] * 3))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("wants", [False, True])
+def test_tracing_is_refused(wants, device):
+    """A trace would record the output's allocation without the kernels that fill it."""
+    if _extension._C is None:
+        pytest.skip("library not built")
+    x, w = torch.ones(5, 8, device=device), torch.ones(4, 8, device=device).requires_grad_(wants)
+    start = torch.zeros(1, dtype=torch.int64, device=device)
+    calls = [lambda t, w: fused_linear(t, w), lambda t, w: grouped_linear(t, w[None], start)]
+    calls += [lambda t, w, f=f: f(t, w, None, None, None, 0) for f in bindings().values()]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (x, w), check_trace=False)
