@@ -45,12 +45,23 @@ class GroupedLinear(nn.Module):
         return grouped_linear(x, self.weight, group_start, self.bias, self.activation, residual)
 
 
+def _plain_linear(m: nn.Module) -> bool:
+    """Whether calling m is torch's linear product of its weight and bias and nothing else: no subclass
+    (a parametrisation is one), no forward of its own, no hooks, no tensor subclasses (quantised weights)."""
+    own = type(m) is nn.Linear and "forward" not in vars(m)
+    hooks = any(getattr(m, name, None) for name in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks",
+                                                    "_backward_pre_hooks"))
+    return own and not hooks and not nn.modules.module._has_any_global_hook() and all(
+        p is None or type(p) in (torch.Tensor, nn.Parameter) for p in (m.weight, m.bias))
+
+
 class FlashDeformAttn3D(nn.Module):
     """value_proj -> deformable attention (FlashDeformAttnFromOffsets) -> output_proj.
 
     forward(query [B,Q,C], reference_points [B,Q,1 or L,3] float32 in [0,1], value [B,S,C],
     spatial_shapes [L,3] int64 (D,H,W), level_start_index [L] int64, residual [B,Q,C] or None) ->
-    [B,Q,C], the residual added to output_proj's result in its epilogue.  level_value_proj: value_proj
+    [B,Q,C], the residual added to output_proj's result (in its epilogue, where output_proj is a plain
+    nn.Linear without hooks).  level_value_proj: value_proj
     has a weight and bias of its own for each level.
     """
 
@@ -106,4 +117,6 @@ class FlashDeformAttn3D(nn.Module):
                                                reference_points.to(torch.float32), self.im2col_step, self.num_points)
         if residual is None:
             return self.output_proj(out)
-        return fused_linear(out, self.output_proj.weight, self.output_proj.bias, residual=residual)
+        if _plain_linear(self.output_proj):
+            return fused_linear(out, self.output_proj.weight, self.output_proj.bias, residual=residual)
+        return self.output_proj(out) + residual

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import linear as ref
-from ops3d_amd import _extension, fused_linear, grouped_linear
+from ops3d_amd import FlashDeformAttn3D, _extension, fused_linear, grouped_linear
 from test_linear import DTYPES, gpu, log, make, grouped_case
 
 
@@ -308,3 +308,44 @@ def test_tracing_is_refused(wants, device):
     for call in calls:
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(call, (x, w), check_trace=False)
+
+
+@gpu
+def test_module_residual_goes_through_output_proj(gpu_device):
+    """With a residual, output_proj's hooks run and what stands in its place is called, as without one."""
+    from ops3d_amd.workloads import level_meta
+
+    torch.manual_seed(0)
+    st, lsi = level_meta(((4, 4, 8), (2, 2, 4)), gpu_device)
+    m = FlashDeformAttn3D(32, 4, 2, 4).to(gpu_device)
+    q, v = torch.randn(2, 9, 32, device=gpu_device), torch.randn(2, 144, 32, device=gpu_device)
+    refp, res = torch.rand(2, 9, 1, 3, device=gpu_device), torch.randn(2, 9, 32, device=gpu_device)
+    args = (q, refp, v, st, lsi)
+    log("[case] module residual")
+
+    def check(want):
+        # one product of 32 terms, in another order: 2 * 33 * 2^-24 of a sum of |terms| below 2^6, twice
+        torch.testing.assert_close(m(*args, residual=res), want, rtol=0, atol=2 * 66 * 2.0 ** -24 * 64)
+
+    with torch.no_grad():
+        check(m(*args) + res)
+        seen = []
+        for hook in (m.output_proj.register_forward_hook(lambda mod, i, o: seen.append(o.clone())),
+                     m.output_proj.register_forward_hook(lambda mod, i, o: 2 * o),
+                     m.output_proj.register_forward_pre_hook(lambda mod, i: (i[0] * 3,))):
+            check(m(*args) + res)
+            hook.remove()
+        assert len(seen) == 2 and torch.equal(seen[0], seen[1])
+        plain = m.output_proj
+        m.output_proj = torch.nn.Sequential(plain, torch.nn.Tanh())
+        check(m(*args) + res)
+        m.output_proj = plain
+        torch.nn.utils.parametrizations.weight_norm(m.output_proj)
+        m.output_proj.parametrizations.weight.original0.mul_(2)
+        check(m(*args) + res)
+    seen = []
+    m.output_proj = torch.nn.Linear(32, 32).to(gpu_device)
+    hook = m.output_proj.register_full_backward_hook(lambda mod, gi, go: seen.append(go[0]))
+    m(*args, residual=res).sum().backward()
+    assert len(seen) == 1
+    hook.remove()
