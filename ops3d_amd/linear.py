@@ -93,10 +93,10 @@ def _apply(x, weight, bias, residual, group_start, activation):
     except (KeyError, TypeError):
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}") from None
     if torch.is_autocast_enabled("cuda"):
-        # as torch's linear does: the product in the autocast dtype; a residual of a wider type keeps it
+        # as torch's linear does: the product in the autocast dtype, float64 left alone (and refused); a
+        # residual of a wider type keeps it
         dt = torch.get_autocast_dtype("cuda")
-        x, weight = x.to(dt), weight.to(dt)
-        bias = None if bias is None else bias.to(dt)
+        x, weight, bias = (t if t is None or t.dtype == torch.float64 else t.to(dt) for t in (x, weight, bias))
         if residual is not None and residual.dtype != dt:
             y = _run(x, weight, bias, None, group_start, act)
             if group_start is not None:

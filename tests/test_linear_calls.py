@@ -349,3 +349,17 @@ def test_module_residual_goes_through_output_proj(gpu_device):
     m(*args, residual=res).sum().backward()
     assert len(seen) == 1
     hook.remove()
+
+
+@gpu
+def test_autocast_leaves_float64(gpu_device):
+    """As torch's, autocast casts no float64: refused as without it, not cut to 16 bits."""
+    x, w = torch.ones(5, 8, dtype=torch.float64, device="cuda"), torch.ones(4, 8, dtype=torch.float64, device="cuda")
+    log("[case] autocast float64")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        with pytest.raises(ValueError, match="unsupported"):
+            fused_linear(x, w)
+        with pytest.raises(ValueError, match="dtype differs"):
+            fused_linear(x.float(), w)
+        y = fused_linear(x.float(), w.float(), None, None, torch.ones(5, 4, dtype=torch.float64, device="cuda"))
+    assert y.dtype == torch.float64 and torch.equal(y, torch.full_like(y, 9.0))
