@@ -64,8 +64,18 @@ OPS3D_FDA_API int ops3d_linear_forward(const void *x, int64_t ld_x, const void *
                                        size_t workspace_bytes, int dtype, int act, int batch, int64_t rows, int groups,
                                        int out_features, int in_features, void *stream);
 
-/* Bytes of device workspace (256-byte aligned) the backward needs: dz (with an act_grad) and partial
- * sums, of grad_x over parts of long sums and of grad_weight over chunks of rows. */
+#define OPS3D_LINEAR_WANT_X 1
+#define OPS3D_LINEAR_WANT_WEIGHT 2
+#define OPS3D_LINEAR_WANT_BIAS 4
+
+/* Bytes of device workspace (256-byte aligned) the backward needs for the gradients in `want` (the
+ * outputs that are not NULL): dz (with an act_grad, for grad_weight and grad_bias) and partial sums, of
+ * grad_x over parts of long sums and of the other two over chunks of rows. */
+OPS3D_FDA_API size_t ops3d_linear_backward_workspace_bytes_for(int dtype, int batch, int64_t rows, int groups,
+                                                               int out_features, int in_features, int grouped,
+                                                               int with_act_grad, int want);
+
+/* The same for all three. */
 OPS3D_FDA_API size_t ops3d_linear_backward_workspace_bytes(int dtype, int batch, int64_t rows, int groups,
                                                            int out_features, int in_features, int grouped,
                                                            int with_act_grad);

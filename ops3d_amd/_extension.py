@@ -62,6 +62,7 @@ EXPORTED_SYMBOLS = (
     "ops3d_linear_forward_workspace_bytes",
     "ops3d_linear_forward",
     "ops3d_linear_backward_workspace_bytes",
+    "ops3d_linear_backward_workspace_bytes_for",
     "ops3d_linear_backward",
     "ops3d_linear_keep_rows",
     "ops3d_fda_profile_enable",
@@ -135,6 +136,8 @@ def _declare(lib: ctypes.CDLL) -> None:
                                          + [_i] * 3 + [_i64] + [_i] * 3 + [_vp])
     lib.ops3d_linear_backward_workspace_bytes.restype = _sz
     lib.ops3d_linear_backward_workspace_bytes.argtypes = [_i, _i, _i64, _i, _i, _i, _i, _i]
+    lib.ops3d_linear_backward_workspace_bytes_for.restype = _sz
+    lib.ops3d_linear_backward_workspace_bytes_for.argtypes = [_i, _i, _i64, _i, _i, _i, _i, _i, _i]
     lib.ops3d_linear_backward.restype = _i
     lib.ops3d_linear_backward.argtypes = ([_vp, _i64, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz]
                                           + [_i] * 2 + [_i64] + [_i] * 3 + [_vp])
@@ -362,7 +365,9 @@ class _NativeFDA:
 
         gx, gw, gb = empty(weight is not None, shape), empty(need_w, wshape), empty(need_b, wshape[:-1])
         code = _DTYPE_CODE[grad_y.dtype]
-        n = self._lib.ops3d_linear_backward_workspace_bytes(code, B, S, E, N, K, int(grouped), int(act_grad is not None))
+        n = self._lib.ops3d_linear_backward_workspace_bytes_for(
+            code, B, S, E, N, K, int(grouped), int(act_grad is not None),
+            (gx is not None) | (gw is not None) << 1 | (gb is not None) << 2)
         ws = torch.empty(n, dtype=torch.uint8, device=grad_y.device) if n else None
         with torch.cuda.device(grad_y.device):
             rc = self._lib.ops3d_linear_backward(

@@ -29,6 +29,7 @@ int elem_size(int dtype) {
 
 constexpr int64_t kMaxRows = 0x7fffffff - 4096;   // rows of all items and tile counts stay 32-bit
 constexpr int kMaxFeatures = 1 << 24;
+constexpr int kWantAll = OPS3D_LINEAR_WANT_X | OPS3D_LINEAR_WANT_WEIGHT | OPS3D_LINEAR_WANT_BIAS;
 
 int check_sizes(int dtype, int batch, int64_t rows, int groups, int out_features, int in_features) {
   if (elem_size(dtype) == 0) return fail(OPS3D_FDA_EINVAL, "unsupported dtype code %d", dtype);
@@ -95,18 +96,19 @@ int check_workspace(const void *workspace, size_t bytes, size_t need) {
   return OPS3D_FDA_OK;
 }
 
-// Workspace of the backward: dz (behind an activation), then the parts of the input gradient's split
+// Workspace of the backward, of what is wanted: dz (behind an activation), then the parts of the input gradient's split
 // sums and, after it and in the same place, the chunks' partial sums.
 struct Layout {
   ChunkPlan plan;
   size_t dz, part, part_b, split, bytes;
-  Layout(int dtype, bool grouped, int batch, int64_t rows, int groups, int N, int K, bool with_dz)
+  Layout(int dtype, bool grouped, int batch, int64_t rows, int groups, int N, int K, bool act_grad, int want)
       : plan(plan_of(dtype, grouped, batch, rows, groups, N, K)) {
+    const bool x = want & OPS3D_LINEAR_WANT_X, w = want & OPS3D_LINEAR_WANT_WEIGHT, b = want & OPS3D_LINEAR_WANT_BIAS;
     dz = 0;
-    part = with_dz ? align256((size_t)batch * rows * N * elem_size(dtype)) : 0;
-    part_b = part + (plan.joined ? align256((size_t)plan.slots * N * K * 4) : 0);
-    bytes = part_b + (plan.joined ? align256((size_t)plan.slots * N * 4) : 0);
-    split = rows > 0 && batch > 0 ? split_bytes(dtype, batch * rows, groups, K, N) : 0;
+    part = act_grad && (w || b) ? align256((size_t)batch * rows * N * elem_size(dtype)) : 0;
+    part_b = part + (plan.joined && w ? align256((size_t)plan.slots * N * K * 4) : 0);
+    bytes = part_b + (plan.joined && b ? align256((size_t)plan.slots * N * 4) : 0);
+    split = x && rows > 0 && batch > 0 ? split_bytes(dtype, batch * rows, groups, K, N) : 0;
     if (bytes < part + split) bytes = part + split;
   }
 };
@@ -169,10 +171,16 @@ int ops3d_linear_forward(const void *x, int64_t ld_x, const void *weight, const 
   return run(dtype, "linear forward", [&](auto t) { return ops3d_linear::forward<decltype(t)>(p, static_cast<hipStream_t>(stream)); });
 }
 
+size_t ops3d_linear_backward_workspace_bytes_for(int dtype, int batch, int64_t rows, int groups, int out_features,
+                                                 int in_features, int grouped, int with_act_grad, int want) {
+  if (!sizes_ok(dtype, batch, rows, groups, out_features, in_features, grouped != 0) || !(want & kWantAll)) return 0;
+  return Layout(dtype, grouped != 0, batch, rows, groups, out_features, in_features, with_act_grad != 0, want).bytes;
+}
+
 size_t ops3d_linear_backward_workspace_bytes(int dtype, int batch, int64_t rows, int groups, int out_features,
                                              int in_features, int grouped, int with_act_grad) {
-  if (!sizes_ok(dtype, batch, rows, groups, out_features, in_features, grouped != 0)) return 0;
-  return Layout(dtype, grouped != 0, batch, rows, groups, out_features, in_features, with_act_grad != 0).bytes;
+  return ops3d_linear_backward_workspace_bytes_for(dtype, batch, rows, groups, out_features, in_features, grouped,
+                                                   with_act_grad, kWantAll);
 }
 
 int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const int64_t *group_start,
@@ -193,9 +201,11 @@ int ops3d_linear_backward(const void *x, int64_t ld_x, const void *weight, const
       misaligned(grad_x, es) || misaligned(grad_weight, es) || misaligned(grad_bias, es))
     return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int want = (grad_x ? OPS3D_LINEAR_WANT_X : 0) | (grad_weight ? OPS3D_LINEAR_WANT_WEIGHT : 0) |
+                   (grad_bias ? OPS3D_LINEAR_WANT_BIAS : 0);
   const Layout lay(dtype, group_start != nullptr, empty ? 1 : batch, empty ? 0 : rows, groups, out_features, in_features,
-                   act_grad != nullptr);
-  if ((rc = check_workspace(workspace, workspace_bytes, empty || (!grad_x && !wants_w) ? 0 : lay.bytes))) return rc;
+                   act_grad != nullptr, want);
+  if ((rc = check_workspace(workspace, workspace_bytes, empty ? 0 : lay.bytes))) return rc;
   char *const ws = static_cast<char *>(workspace);
   void *const dz = wants_w && act_grad && !empty ? ws + lay.dz : nullptr;
   if (grad_x && !empty) {

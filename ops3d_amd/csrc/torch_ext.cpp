@@ -616,8 +616,9 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
   if (weight) gx = at::empty(shape, grad_y.options());
   if (need_w) gw = at::empty(wshape, grad_y.options());
   if (need_b) gb = at::empty(grouped ? std::vector<int64_t>{groups, N} : std::vector<int64_t>{N}, grad_y.options());
-  const size_t n = ops3d_linear_backward_workspace_bytes(z.code, z.batch, z.rows, z.groups, z.N, z.K, grouped,
-                                                         act_grad.has_value());
+  const int want = (gx ? OPS3D_LINEAR_WANT_X : 0) | (gw ? OPS3D_LINEAR_WANT_WEIGHT : 0) | (gb ? OPS3D_LINEAR_WANT_BIAS : 0);
+  const size_t n = ops3d_linear_backward_workspace_bytes_for(z.code, z.batch, z.rows, z.groups, z.N, z.K, grouped,
+                                                             act_grad.has_value(), want);
   at::Tensor ws;
   if (n) ws = at::empty({(int64_t)n}, grad_y.options().dtype(at::kByte));
   const int rc = ops3d_linear_backward(ptr(xr), ldx, ptr(w), z.start, z.count, act_grad ? ptr(*act_grad) : nullptr, ptr(g),
@@ -676,7 +677,7 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
     ctx->save_for_backward({need_w || need_b ? x : at::Tensor(), need_x ? weight : at::Tensor(),
                             group_start ? *group_start : at::Tensor(), act_grad ? *act_grad : at::Tensor()});
     ctx->saved_data["sizes"] = std::vector<int64_t>{weight.size(-1), weight.dim() == 3 ? weight.size(0) : 0, need_x,
-                                                    need_w, need_b, residual && residual->requires_grad()};
+                                                    need_w, need_b, residual && residual->requires_grad(), bias.has_value()};
     return y;
   }
 
@@ -689,15 +690,18 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
     const auto some = [](const at::Tensor &t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
     {
       const at::NoGradGuard no_grad;
-      if (sizes[2] || sizes[3] || sizes[4]) {
-        auto [gx, gw, gb] = linear_backward(some(saved[0]), some(saved[1]), some(saved[2]), some(saved[3]), grad, sizes[0],
-                                            sizes[1], sizes[3], sizes[4]);
+      // of the gradients that could be, those that this pass asks for
+      const bool x = sizes[2] && ctx->needs_input_grad(0), w = sizes[3] && ctx->needs_input_grad(1),
+                 b = sizes[4] && ctx->needs_input_grad(2);
+      if (x || w || b) {
+        auto [gx, gw, gb] = linear_backward(some(saved[0]), x ? some(saved[1]) : c10::nullopt, some(saved[2]), some(saved[3]),
+                                            grad, sizes[0], sizes[1], w, b);
         if (gx) out[0] = *gx;
         if (gw) out[1] = *gw;
         if (gb) out[2] = *gb;
       }
     }
-    if (sizes[5]) out[3] = saved[2].defined() ? linear_keep_rows(grad, saved[2], sizes[1]) : grad;   // y is 0 in rows of no group
+    if (sizes[5] && ctx->needs_input_grad(sizes[6] ? 3 : 2)) out[3] = saved[2].defined() ? linear_keep_rows(grad, saved[2], sizes[1]) : grad;   // y is 0 in rows of no group
     if (at::GradMode::is_enabled()) {   // each that depends on something with a gradient
       const bool act = saved[3].defined(), depends[3] = {sizes[3] || act, sizes[2] || act, act};
       for (int i = 0; i < 3; ++i) {

@@ -363,3 +363,71 @@ def test_autocast_leaves_float64(gpu_device):
             fused_linear(x.float(), w)
         y = fused_linear(x.float(), w.float(), None, None, torch.ones(5, 4, dtype=torch.float64, device="cuda"))
     assert y.dtype == torch.float64 and torch.equal(y, torch.full_like(y, 9.0))
+
+
+def test_workspace_of_the_wanted_gradients():
+    if _extension._C is None:
+        pytest.skip("library not built")
+    lib = _extension._C._lib
+    of, every = lib.ops3d_linear_backward_workspace_bytes_for, lib.ops3d_linear_backward_workspace_bytes
+    X, W, B = 1, 2, 4
+    for case in ((2, 1, 73728, 1, 1024, 256, 0), (2, 1, 598016, 3, 256, 256, 1), (0, 1, 1, 1, 1856, 3301, 0),
+                 (1, 64, 512, 16, 1024, 1024, 1), (2, 2, 4096, 64, 256, 256, 1)):
+        for act in (0, 1):
+            assert of(*case, act, X | W | B) == every(*case, act)
+            assert all(of(*case, act, w) <= every(*case, act) for w in range(8))
+            assert of(*case, act, 0) == 0 and of(*case, act, 8) == 0
+    rows, N, K = 73728, 1024, 256
+    case, dz = (2, 1, rows, 1, N, K, 0), rows * N * 2
+    assert of(*case, 1, X) == 0                       # neither dz nor partial sums
+    assert of(*case, 0, X | B) == of(*case, 0, B) and 0 < of(*case, 0, B) < 2 << 20
+    assert of(*case, 1, B) == dz + of(*case, 0, B)
+    assert of(*case, 1, W) == dz + of(*case, 0, W)
+    assert of(*case, 0, W) + of(*case, 0, B) == of(*case, 0, W | B)
+    assert of(2, 1, 1, 1, 3301, 1856, 0, 0, X) > 0    # a long sum in parts
+
+
+@gpu
+@pytest.mark.parametrize("asked", [False, True])
+@pytest.mark.parametrize("binding", ["module", "ctypes"])
+def test_memory_of_the_wanted_gradients(gpu_device, asked, binding):
+    """x's gradient alone takes its own memory and no dz or partial sums: with the other inputs frozen, or
+    (the module's node) with a backward pass that asks for nothing else."""
+    if asked and binding == "ctypes":
+        pytest.skip("a Function in Python is not told what a pass asks for")
+    rows, N, K, bf = 73728, 1024, 256, torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(51)
+    log(f"[case] memory {asked} {binding}")
+    x, w, b, u = (make(gen, s, bf) for s in ((rows, K), (N, K), (N,), (rows, N)))
+    x.requires_grad_(True)
+    for t in (w, b):
+        t.requires_grad_(asked)
+    y = bindings()[binding](x, w, b, None, None, 2)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    (dx,) = torch.autograd.grad(y, x, u)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < rows * K * 2 + (4 << 20)
+    y = bindings()[binding](x, w.detach().requires_grad_(True), b.detach().requires_grad_(True), None, None, 2)
+    assert torch.equal(torch.autograd.grad(y, x, u)[0], dx)
+
+
+@gpu
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("bias", [False, True])
+def test_each_gradient_asked_for_alone(gpu_device, bias, grouped):
+    """A pass that asks for one gradient or some gets what a pass for all gets."""
+    gen = torch.Generator(device="cuda").manual_seed(52)
+    log(f"[case] asked alone {bias} {grouped}")
+    E = (3,) if grouped else ()
+    t = [make(gen, s, torch.bfloat16).requires_grad_(True) for s in ((700, 64), (*E, 40, 64), (700, 40))]
+    b = make(gen, (*E, 40), torch.bfloat16).requires_grad_(True) if bias else None
+    u, table = make(gen, (700, 40), torch.bfloat16), torch.tensor([5, 100, 400, 650], device="cuda")
+    for act in (0, 4):
+        y = _extension._C.linear(t[0], t[1], b, t[2], table if grouped else None, act)
+        leaves = t + ([b] if bias else [])
+        every = torch.autograd.grad(y, leaves, u, retain_graph=True)
+        for pick in ([0], [1], [2], [0, 2], [1, 2], [0, 1], *([[3], [2, 3], [0, 3], [1, 3]] if bias else [])):
+            got = torch.autograd.grad(y, [leaves[i] for i in pick], u, retain_graph=True)
+            assert all(torch.equal(g, every[i]) for g, i in zip(got, pick)), pick
