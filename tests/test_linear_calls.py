@@ -431,3 +431,83 @@ def test_each_gradient_asked_for_alone(gpu_device, bias, grouped):
         for pick in ([0], [1], [2], [0, 2], [1, 2], [0, 1], *([[3], [2, 3], [0, 3], [1, 3]] if bias else [])):
             got = torch.autograd.grad(y, [leaves[i] for i in pick], u, retain_graph=True)
             assert all(torch.equal(g, every[i]) for g, i in zip(got, pick)), pick
+
+
+# Rows in thousands: a worst-case bound of their sums is wider than the sums themselves.  With small whole
+# numbers every fp32 sum is exact (below 2^24), in any order, so results are the exact ones rounded once.
+LONG = [("bf16", 40000, 256, 256, None), ("fp16", 20011, 100, 520, "relu"), ("fp32", 20011, 90, 130, "relu"),
+        ("bf16", 65607, 256, 504, "relu"), ("fp16", 70001, 128, 512, None), ("bf16", 66001, 512, 128, None),
+        ("fp16", 140001, 256, 256, None), ("bf16", 140033, 256, 256, "relu"), ("bf16", 9000, 24, 40, "relu"),
+        ("fp32", 30000, 256, 256, None), ("bf16", 73728, 250, 333, "relu")]
+
+
+def whole(gen, shape, dtype, device="cuda"):
+    return torch.randint(-2, 3, shape, generator=gen, device=device).to(dtype)
+
+
+def exact_step(x, w, b, r, u, activation, group):
+    """y and the gradients of x, w and b in 64 bits; group: of each row, -1 for none."""
+    x, w, b, r, u = (t.double() for t in (x, w, b, r, u))
+    y, dx, dw, db = torch.zeros_like(r), torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b)
+    for g in range(w.shape[0]):
+        at = (group == g).nonzero().flatten().to(x.device)
+        z, a = ref.act(x[at] @ w[g].t() + b[g], activation)[0], u[at]
+        y[at] = z + r[at]
+        if activation:
+            a = a * (z > 0)
+        dx[at], dw[g], db[g] = a @ w[g], a.t() @ x[at], a.sum(0)
+    return {"y": y, "dx": dx, "dw": dw, "db": db}
+
+
+def exact_case(start, lead, E, K, N, dtype, activation):
+    dt = DTYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(61)
+    x, w, b, r, u = (whole(gen, s, dt) for s in ((*lead, K), (E, N, K), (E, N), (*lead, N), (*lead, N)))
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    if start is None:
+        group = torch.zeros(lead[0], dtype=torch.int64)
+        y = fused_linear(x, w[0], b[0], activation, r)
+    else:
+        group = ref.group_of_rows(lead[-1], start, E).repeat(lead[0] if len(lead) > 1 else 1)
+        y = grouped_linear(x, w, torch.tensor(start, device="cuda"), b, activation, r)
+    got = dict(zip(("y", "dx", "dw", "db"), (y, *torch.autograd.grad(y, leaves, u))))
+    flat = [t.detach().reshape(-1, t.shape[-1]) for t in (x, r, u)]
+    want = exact_step(flat[0], w.detach(), b.detach(), flat[1], flat[2], activation, group)
+    for name, e in want.items():
+        assert e.abs().max() < 60000, name       # fits fp16
+        assert torch.equal(got[name].detach().reshape(e.shape), e.to(dt)), name
+
+
+@gpu
+@pytest.mark.parametrize("dtype,rows,K,N,activation", LONG)
+def test_long_sums_exact(gpu_device, dtype, rows, K, N, activation):
+    log(f"[case] exact {rows}x{K}->{N} {dtype} {activation}")
+    exact_case(None, (rows,), 1, K, N, dtype, activation)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("K,N", [(256, 256), (128, 512), (256, 504), (250, 129)])
+def test_grouped_long_sums_exact(gpu_device, K, N, dtype):
+    """Long groups of two items, a last stage that ends inside, a short group, rows of none."""
+    log(f"[case] exact grouped {K}->{N} {dtype}")
+    exact_case([70, 100, 60000, 99990], (2, 100003), 3, K, N, dtype, None)
+    exact_case([0, 34990, 39400], (40011,), 3, K, N, dtype, "relu")
+
+
+def test_exact_sums_show_a_lost_stage():
+    """The rounded gradient tells a sum without one stage of 64 rows, or without the rows behind the last
+    whole one, from the whole sum, and so it tells zeros."""
+    for dtype, rows, _, _, activation in [*LONG, ("bf16", 119800, 0, 0, None), ("fp16", 69980, 0, 0, "relu")]:
+        gen = torch.Generator().manual_seed(62)
+        dt = DTYPES[dtype]
+        x, u = (whole(gen, (rows, 16), torch.float64, "cpu") for _ in range(2))
+        if activation:
+            u = u * (torch.rand(u.shape, generator=gen) < 0.5)
+        dw, db = (u.t() @ x).to(dt), u.sum(0).to(dt)
+        last = rows - (rows % 64 or 64)
+        for a in (0, rows // 128 * 64, last):
+            b = min(a + 64, rows)
+            assert ((u.t() @ x - u[a:b].t() @ x[a:b]).to(dt) != dw).sum() > 64     # of 256
+            assert ((u.sum(0) - u[a:b].sum(0)).to(dt) != db).any()
+        assert (dw != 0).sum() > 200
