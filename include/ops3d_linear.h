@@ -28,7 +28,8 @@
  *
  * act_grad: act'(z) for the backward, [batch * rows, out_features], written by the forward when not
  * NULL and read by the backward; fp32 for F32, otherwise a 16-bit code: below 1/8 the bits of the fp16
- * number (11 significant bits), from there on 0x3000 and steps of 2^-14; 0xfe00 is NaN.  Rows in no group are not written.  It must be NULL for OPS3D_LINEAR_ACT_NONE.
+ * number (11 significant bits), from there on 0x3000 and steps of 2^-14; 0xfe00 is NaN.  Rows in no
+ * group are not written.  It must be NULL for OPS3D_LINEAR_ACT_NONE.
  *
  * Outputs and workspace must overlap neither each other nor an input (a residual neither): some results
  * are computed by two blocks, which write the same value.

@@ -704,10 +704,11 @@ __device__ __forceinline__ void store_parts(const RowsArgs &p, const f32x4 (&acc
 // U stages are loaded and multiplied at a time.  DMA: loads go straight to LDS (rows at 16-byte
 // boundaries); nothing is loaded ahead, but without registers for it more blocks fit a CU, which wait in
 // turn (4096^3 bf16, same run: 128 x 256 136 us, 128 x 128 144; through registers and a stage ahead 256 x 256
-// 159, 128 x 128 189; the whole operator 130 to 148, of which the products take 94 at a library's rate).
+// 159, 128 x 128 189; 130 to 136 from run to run, where a library's bare product takes 94).
 // What bounds it: at long sums the wait for a stage's loads, which the blocks of a CU hide from one another
 // (half of the wave cycles wait, for 4096^3); at 73728 x 256 -> 1024 with an act_grad (97 to 125
-// us) the stores, of 300 MB, and the activation's arithmetic.  Otherwise loads go through registers, the
+// us) the stores, of 300 MB, and the activation's arithmetic.  The scaled operand is rounded to T, as the
+// matrix units take no more, and stored so: dW and db sum the same dz.  Otherwise loads go through registers, the
 // next stages' while these are multiplied; so does the scaled operand always.
 template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void rows_kernel(RowsArgs p) {
@@ -826,13 +827,15 @@ __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC
 // 1024 570 to 690 us).  Here a block of 8 waves stays on its CU with 256 columns of the weight in
 // registers (64 a wave: 32 KS registers) and walks over tiles of 64 rows: loads to a ring of four tiles in
 // LDS run two to three tiles ahead of the products, one barrier a tile, and results go out meanwhile
-// (414 us; with 256 columns 121, 171, where the bytes alone take 118).
+// (390 to 450 us; with 256 columns 114 to 123, 171 in tiles, where the bytes alone take 118).
 // A segment's last tile is its last 64 rows, and the last columns are the last 256: what two blocks
 // compute they write alike, and every tile is whole.
 //
 // Order of a wave's memory operations, which complete in order: loads of tile i (KS of them), results of
 // tile i - 3, loads of tile i + 1, results of i - 2, loads of i + 2, results of i - 1.  So when all but the
-// newest 2 KS operations are done, the loads of tile i are, with results to store or without.  Behind the
+// newest 2 KS operations are done, the loads of tile i are, with results to store or without.  A residual's
+// loads come behind those of tile i + 3, so waiting for them waits for these too; it costs no more than its
+// bytes (598016 x 256 -> 256 bf16 123 us, 173 with a residual, 177 in bytes).  Behind the
 // barrier every wave's are, and every wave has read tile i - 1 (the reads' results are waited for where
 // they are read), whose place tile i + 3 takes.  Behind the last tile it is loaded again, so the counts
 // hold, and all loads are waited for before a segment ends.
@@ -1431,7 +1434,7 @@ template <typename T, bool DMA, bool WSTR, bool SCALE, bool EPI> inline hipError
     if (streams(p)) return p.K == 128 ? launch_stream<T, 2, WSTR, EPI>(p, st) : launch_stream<T, 4, WSTR, EPI>(p, st);
   }
   if constexpr (DMA && !SCALE) {
-    // long sums: wider tiles read their operands less often (4096^3 bf16 120 us, 128 in tiles of 128; at
+    // long sums: wider tiles read their operands less often (4096^3 bf16 136 us, 144 in tiles of 128; at
     // sums of 256 those are as fast or faster)
     if (p.K >= 1024 && p.N >= 256 && p.rows / p.g.E >= 512 && (p.rows + 127) / 128 * ceil_div(p.N, 256) >= 384)
       return launch_rows<T, 128, 256, 2, 4, 1, true, 4, WSTR, SCALE, EPI>(p, st);

@@ -701,7 +701,8 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
         if (gb) out[2] = *gb;
       }
     }
-    if (sizes[5] && ctx->needs_input_grad(sizes[6] ? 3 : 2)) out[3] = saved[2].defined() ? linear_keep_rows(grad, saved[2], sizes[1]) : grad;   // y is 0 in rows of no group
+    if (sizes[5] && ctx->needs_input_grad(sizes[6] ? 3 : 2))   // y is 0 in rows of no group
+      out[3] = saved[2].defined() ? linear_keep_rows(grad, saved[2], sizes[1]) : grad;
     if (at::GradMode::is_enabled()) {   // each that depends on something with a gradient
       const bool act = saved[3].defined(), depends[3] = {sizes[3] || act, sizes[2] || act, act};
       for (int i = 0; i < 3; ++i) {
