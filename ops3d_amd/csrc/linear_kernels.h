@@ -209,7 +209,8 @@ template <typename T> struct Deriv {
     typedef _Float16 halves __attribute__((ext_vector_type(2)));
     constexpr float c = 16384.f / 65535.f;
     const codes low = __builtin_bit_cast(codes, halves{(_Float16)fminf(d0, 0.125f), (_Float16)fminf(d1, 0.125f)});
-    const codes steps = __builtin_bit_cast(codes, __builtin_amdgcn_cvt_pknorm_u16(fmaf(c, d0, -0.125f * c), fmaf(c, d1, -0.125f * c)));
+    const codes steps =
+        __builtin_bit_cast(codes, __builtin_amdgcn_cvt_pknorm_u16(fmaf(c, d0, -0.125f * c), fmaf(c, d1, -0.125f * c)));
     return __builtin_bit_cast(uint32_t, low + steps);
   }
   static __device__ __forceinline__ uint4 encode(const float (&d)[8]) {
@@ -707,9 +708,9 @@ __device__ __forceinline__ void store_parts(const RowsArgs &p, const f32x4 (&acc
 // 159, 128 x 128 189; 130 to 136 from run to run, where a library's bare product takes 94).
 // What bounds it: at long sums the wait for a stage's loads, which the blocks of a CU hide from one another
 // (half of the wave cycles wait, for 4096^3); at 73728 x 256 -> 1024 with an act_grad (97 to 125
-// us) the stores, of 300 MB, and the activation's arithmetic.  The scaled operand is rounded to T, as the
-// matrix units take no more, and stored so: dW and db sum the same dz.  Otherwise loads go through registers, the
-// next stages' while these are multiplied; so does the scaled operand always.
+// us) the stores, of 300 MB, and the activation's arithmetic.  Otherwise loads go through registers, the
+// next stages' while these are multiplied; so does the scaled operand always.  That is rounded to T, as the
+// matrix units take no more, and stored so: dW and db sum the same dz.
 template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT>
 __global__ __launch_bounds__(64 * WR *WC) __attribute__((amdgpu_waves_per_eu(OCC))) void rows_kernel(RowsArgs p) {
   constexpr int NT = 64 * WR * WC, TM = BM / WR, TN = BN / WC, MI = TM / 16, NI = TN / 16;
