@@ -65,6 +65,10 @@ EXPORTED_SYMBOLS = (
     "ops3d_linear_backward_workspace_bytes_for",
     "ops3d_linear_backward",
     "ops3d_linear_keep_rows",
+    "ops3d_layer_norm_forward",
+    "ops3d_layer_norm_backward_workspace_bytes",
+    "ops3d_layer_norm_backward",
+    "ops3d_rotary",
     "ops3d_fda_profile_enable",
     "ops3d_fda_profile_read",
 )
@@ -143,6 +147,14 @@ def _declare(lib: ctypes.CDLL) -> None:
                                           + [_i] * 2 + [_i64] + [_i] * 3 + [_vp])
     lib.ops3d_linear_keep_rows.restype = _i
     lib.ops3d_linear_keep_rows.argtypes = [_vp, _i64, _vp, _i, _vp, _i, _i, _i64, _i, _i, _vp]
+    lib.ops3d_layer_norm_forward.restype = _i
+    lib.ops3d_layer_norm_forward.argtypes = [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i64, _i, ctypes.c_float, _vp]
+    lib.ops3d_layer_norm_backward_workspace_bytes.restype = _sz
+    lib.ops3d_layer_norm_backward_workspace_bytes.argtypes = [_i, _i64, _i, _i, _i]
+    lib.ops3d_layer_norm_backward.restype = _i
+    lib.ops3d_layer_norm_backward.argtypes = ([_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _i, _i, _i64, _i, _vp])
+    lib.ops3d_rotary.restype = _i
+    lib.ops3d_rotary.argtypes = ([_vp, _vp, _vp, _i, _i64, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _i, _i64, _i, _i, _vp])
     lib.ops3d_fda_backward_offsets.argtypes = [_vp] * 6 + [_i] + [_vp] * 5 + [_sz] + [_i] * 9 + [_vp]
 
 
@@ -170,7 +182,8 @@ class _NativeFDA:
                          "forward_keep_head_major", "backward_with_head_major",
                          "forward_offsets", "backward_offsets", "nms_3d", "roi_align_3d_forward",
                          "roi_align_3d_backward", "dcnv4_forward", "dcnv4_backward", "linear", "linear_forward",
-                         "linear_backward", "linear_keep_rows"):
+                         "linear_backward", "linear_keep_rows", "layer_norm", "layer_norm_forward",
+                         "layer_norm_backward", "rotary", "rotary_apply"):
                 setattr(self, name, getattr(ext, name))
 
     # -- helpers ---------------------------------------------------------------------------
@@ -396,6 +409,148 @@ class _NativeFDA:
         if rc != OPS3D_FDA_OK:
             self._raise(rc, "linear_keep_rows failed")
         return out
+
+    # -- layer norm (include/ops3d_norm.h) ----------------------------------------------------
+    @staticmethod
+    def _refuse(what: str, *tensors) -> None:
+        """What no kernel here knows of: traces and forward-mode tangents."""
+        if torch.jit.is_tracing():
+            raise RuntimeError(f"{what} cannot be traced")
+        if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError(f"{what} has no forward-mode derivatives")
+
+    @staticmethod
+    def _norm_vectors(x, weight, bias) -> int:
+        if x.dtype not in _DTYPE_CODE:
+            raise ValueError(f"unsupported value dtype {x.dtype}")
+        code, first = _DTYPE_CODE[x.dtype], None
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise RuntimeError(f"Not implemented on the CPU ({name} is on the CPU)")
+            if t.layout != torch.strided:
+                raise ValueError(f"{name} must be a dense tensor")
+            if t.device != x.device:
+                raise RuntimeError(f"{name} is on another device than x")
+            if t.dtype not in (x.dtype, torch.float32):
+                raise ValueError(f"{name} dtype must be x dtype or float32")
+            if t.shape != x.shape[-1:]:
+                raise ValueError(f"{name} must be [{x.shape[-1]}]")
+            if first is not None and first.dtype != t.dtype:
+                raise ValueError("weight and bias differ in dtype")
+            first, code = t, _DTYPE_CODE[t.dtype]
+        return code
+
+    def layer_norm(self, x, weight, bias, eps):
+        """The operator through autograd (LayerNormFunction where a gradient is wanted)."""
+        self._refuse("layer_norm", x, weight, bias)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+            from .norm import LayerNormFunction
+
+            return LayerNormFunction.apply(x, weight, bias, eps, self)
+        return self.layer_norm_forward(x, weight, bias, eps, False)[0]
+
+    def layer_norm_forward(self, x, weight, bias, eps, keep):
+        """(y, stats); stats (None otherwise) when ``keep``."""
+        self._linear_check("x", x, x)
+        if x.dim() < 1:
+            raise ValueError("x must have an axis to normalise")
+        wcode = self._norm_vectors(x, weight, bias)
+        xr, ld = self._as_rows(x)
+        w, b = (None if t is None else t.resolve_neg().contiguous() for t in (weight, bias))
+        rows, width = math.prod(x.shape[:-1]), x.shape[-1]
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty((rows, 3), dtype=torch.float32, device=x.device) if keep else None
+        with torch.cuda.device(x.device):
+            rc = self._lib.ops3d_layer_norm_forward(_ptr(xr), ld, _ptr(w), _ptr(b), _ptr(y), _ptr(stats),
+                                                    _DTYPE_CODE[x.dtype], wcode, rows, width, float(eps),
+                                                    torch.cuda.current_stream(x.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "layer_norm_forward failed")
+        return y, stats
+
+    def layer_norm_backward(self, x, weight, stats, grad_y, wide_vectors, need_x, need_w, need_b):
+        """(grad_x, grad_weight, grad_bias), None where not wanted."""
+        self._linear_check("x", x, x)
+        self._linear_check("grad_output", grad_y, x)
+        if x.dim() < 1 or grad_y.shape != x.shape:
+            raise ValueError("x and grad_output differ in shape")
+        rows, width = math.prod(x.shape[:-1]), x.shape[-1]
+        code = _DTYPE_CODE[x.dtype]
+        wcode = 0 if wide_vectors else code
+        if weight is not None and self._norm_vectors(x, weight, None) != wcode:
+            raise ValueError("weight is not the forward's")
+        if stats.device != x.device or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.shape != (rows, 3):
+            raise ValueError("stats are not a forward's of this shape")
+        (xr, ldx), (g, ldg) = self._as_rows(x), self._as_rows(grad_y)
+        w = None if weight is None else weight.resolve_neg().contiguous()
+        vector = torch.float32 if wide_vectors else x.dtype
+        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        gw, gb = (torch.empty(width, dtype=vector, device=x.device) if need else None for need in (need_w, need_b))
+        n = self._lib.ops3d_layer_norm_backward_workspace_bytes(code, rows, width, int(need_w), int(need_b))
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        with torch.cuda.device(x.device):
+            rc = self._lib.ops3d_layer_norm_backward(
+                _ptr(xr), ldx, _ptr(w), _ptr(stats), _ptr(g), ldg, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), n, code, wcode,
+                rows, width, torch.cuda.current_stream(x.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "layer_norm_backward failed")
+        return gx, gw, gb
+
+    # -- rotary positions (include/ops3d_rotary.h) ----------------------------------------------
+    @staticmethod
+    def _channels_dense(t):
+        t = t.resolve_neg()
+        return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+    @staticmethod
+    def _strides(t):
+        """{item, token, head} of [tokens, heads, dim] or [items, tokens, heads, dim]."""
+        return (ctypes.c_int64 * 3)(t.stride(0) if t.dim() == 4 else 0, t.stride(-3), t.stride(-2))
+
+    def rotary(self, x, positions, frequencies, axis_of, layout):
+        """The operator through autograd (RotaryFunction where a gradient is wanted)."""
+        self._refuse("rotary_positions", x, positions)
+        if positions.requires_grad:
+            raise ValueError("rotary_positions has no gradient of positions")
+        if torch.is_grad_enabled() and x.requires_grad:
+            from .rotary import RotaryFunction
+
+            return RotaryFunction.apply(x, positions, frequencies, axis_of, layout, False, self)
+        return self.rotary_apply(x, positions, frequencies, axis_of, layout, False)
+
+    def rotary_apply(self, x, positions, frequencies, axis_of, layout, inverse):
+        self._linear_check("x", x, x)
+        if x.dim() not in (3, 4):
+            raise ValueError("x must be [tokens, heads, dim] or [items, tokens, heads, dim]")
+        if x.dtype not in _DTYPE_CODE:
+            raise ValueError(f"unsupported value dtype {x.dtype}")
+        if not positions.is_cuda:
+            raise RuntimeError("Not implemented on the CPU (positions is on the CPU)")
+        if positions.device != x.device:
+            raise RuntimeError("positions is on another device than x")
+        if positions.layout != torch.strided:
+            raise ValueError("positions must be a dense tensor")
+        if positions.dtype not in (torch.float32, torch.int64):
+            raise ValueError("positions must be float32 or int64")
+        items, (tokens, heads, dim) = x.shape[0] if x.dim() == 4 else 1, x.shape[-3:]
+        if (positions.dim() != 2 and (positions.dim() != 3 or x.dim() != 4 or positions.shape[0] != items)) \
+                or positions.shape[-2] != tokens:
+            raise ValueError("positions must be [tokens, axes], or [items, tokens, axes] beside items")
+        if len(frequencies) != len(axis_of):
+            raise ValueError("there must be a frequency for each pair")
+        xr, pos, n = self._channels_dense(x), positions.resolve_neg().contiguous(), len(axis_of)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        with torch.cuda.device(x.device):
+            rc = self._lib.ops3d_rotary(
+                _ptr(xr), self._strides(xr), _ptr(pos), int(pos.dtype == torch.int64),
+                tokens * pos.shape[-1] if pos.dim() == 3 else 0, (ctypes.c_double * n)(*frequencies), (_i * n)(*axis_of),
+                n, pos.shape[-1], int(layout), int(inverse), _ptr(y), self._strides(y), _DTYPE_CODE[x.dtype], items, tokens,
+                heads, dim, torch.cuda.current_stream(x.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "rotary positions failed")
+        return y
 
     # -- entry points (reference csrc/flash_deform_attn.h) -----------------------------------
     def flash_deform_attn_forward(

@@ -25,6 +25,8 @@
 #include "../../include/ops3d_dcnv4.h"
 #include "../../include/ops3d_linear.h"
 #include "../../include/ops3d_nms3d.h"
+#include "../../include/ops3d_norm.h"
+#include "../../include/ops3d_rotary.h"
 #include "../../include/ops3d_roi_align3d.h"
 
 namespace {
@@ -717,9 +719,22 @@ class LinearNode : public torch::autograd::Function<LinearNode> {
 };
 
 // A tangent would be lost without a word: y comes from a kernel that knows of none.
-void refuse_tangent(const at::Tensor &t) {
+void refuse_tangent(const at::Tensor &t, const char *what = "the linear operators have") {
   if (t.defined() && t._fw_grad(0).defined())
-    throw std::runtime_error("the linear operators have no forward-mode derivatives");
+    throw std::runtime_error(std::string(what) + " no forward-mode derivatives");
+}
+
+// A trace would record y's allocation without the kernel that fills it.
+void refuse_trace(const char *what) {
+  if (torch::jit::tracer::isTracing()) throw std::runtime_error(std::string(what) + " cannot be traced");
+}
+
+// With create_graph: a gradient that depends on something with a gradient raises when it is differentiated.
+void once(at::Tensor &grad, bool depends, const char *what) {
+  if (!grad.defined() || !depends || !at::GradMode::is_enabled()) return;
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("trying to differentiate twice ") + what + " that is differentiable once", 1);
+  grad = (*error)({grad.detach().set_requires_grad(true)})[0];
 }
 
 at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const c10::optional<at::Tensor> &bias,
@@ -734,6 +749,211 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const c10::opti
                                      (residual && residual->requires_grad())))
     return LinearNode::apply(x, weight, bias, residual, group_start, act);
   return std::get<0>(linear_forward(x, weight, bias, residual, group_start, act, false));
+}
+
+// Layer norm (include/ops3d_norm.h).
+int64_t rows_of(const at::Tensor &t) {
+  int64_t n = 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
+  return n;
+}
+
+// weight or bias: [width] of x's type or float32, both of one type; returns its code.
+int norm_vectors(const at::Tensor &x, const c10::optional<at::Tensor> &weight, const c10::optional<at::Tensor> &bias) {
+  int code = dtype_code(x);
+  const at::Tensor *first = nullptr;
+  for (const auto *v : {&weight, &bias}) {
+    if (!*v) continue;
+    const at::Tensor &t = **v;
+    const char *name = v == &weight ? "weight" : "bias";
+    if (!t.is_cuda()) throw std::runtime_error(std::string("Not implemented on the CPU (") + name + " is on the CPU)");
+    if (t.layout() != at::kStrided) throw std::invalid_argument(std::string(name) + " must be a dense tensor");
+    if (t.device() != x.device()) throw std::runtime_error(std::string(name) + " is on another device than x");
+    if (t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat)
+      throw std::invalid_argument(std::string(name) + " dtype must be x dtype or float32");
+    if (t.dim() != 1 || t.size(0) != x.size(-1)) throw std::invalid_argument(std::string(name) + " must be [" + std::to_string(x.size(-1)) + "]");
+    if (first && first->scalar_type() != t.scalar_type()) throw std::invalid_argument("weight and bias differ in dtype");
+    first = &t;
+    code = dtype_code(t);
+  }
+  return code;
+}
+
+// [y, stats]; stats (for the backward) when keep.
+std::tuple<at::Tensor, c10::optional<at::Tensor>> layer_norm_forward(const at::Tensor &x, const c10::optional<at::Tensor> &weight,
+                                                                     const c10::optional<at::Tensor> &bias, double eps,
+                                                                     bool keep) {
+  linear_check(x, "x", x);
+  if (x.dim() < 1) throw std::invalid_argument("x must have an axis to normalise");
+  const int code = dtype_code(x), wcode = norm_vectors(x, weight, bias), width = linear_int(x.size(-1), "the normalised axis");
+  const DeviceGuard guard(x.device());
+  int64_t ld = 0;
+  const at::Tensor xr = as_rows(x, ld);
+  const at::Tensor w = weight ? dense(*weight) : at::Tensor(), b = bias ? dense(*bias) : at::Tensor();
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  c10::optional<at::Tensor> stats;
+  const int64_t rows = rows_of(x);
+  if (keep) stats = at::empty({rows, 3}, x.options().dtype(at::kFloat));
+  const int rc = ops3d_layer_norm_forward(ptr(xr), ld, ptr(w), ptr(b), ptr(y), stats ? (float *)ptr(*stats) : nullptr, code,
+                                          wcode, rows, width, (float)eps, stream_of(x));
+  if (rc != OPS3D_FDA_OK) raise(rc, "layer_norm_forward failed");
+  return {y, stats};
+}
+
+// [grad_x, grad_weight, grad_bias], None where not wanted; the latter two of vector_like's type.
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<at::Tensor>> layer_norm_backward(
+    const at::Tensor &x, const c10::optional<at::Tensor> &weight, const at::Tensor &stats, const at::Tensor &grad_y,
+    bool wide_vectors, bool need_x, bool need_w, bool need_b) {
+  linear_check(x, "x", x);
+  linear_check(grad_y, "grad_output", x);
+  if (x.dim() < 1 || grad_y.sizes() != x.sizes()) throw std::invalid_argument("x and grad_output differ in shape");
+  const int64_t rows = rows_of(x);
+  const int code = dtype_code(x), width = linear_int(x.size(-1), "the normalised axis");
+  const int wcode = wide_vectors ? OPS3D_FDA_F32 : code;
+  if (weight && norm_vectors(x, weight, c10::nullopt) != wcode) throw std::invalid_argument("weight is not the forward's");
+  if (stats.device() != x.device() || stats.scalar_type() != at::kFloat || !stats.is_contiguous() ||
+      stats.sizes() != at::IntArrayRef({rows, 3}))
+    throw std::invalid_argument("stats are not a forward's of this shape");
+  const DeviceGuard guard(x.device());
+  int64_t ldx = 0, ldg = 0;
+  const at::Tensor xr = as_rows(x, ldx), g = as_rows(grad_y, ldg), w = weight ? dense(*weight) : at::Tensor();
+  c10::optional<at::Tensor> gx, gw, gb;
+  const auto vector = wide_vectors ? x.options().dtype(at::kFloat) : x.options();
+  if (need_x) gx = at::empty(x.sizes(), x.options());
+  if (need_w) gw = at::empty({width}, vector);
+  if (need_b) gb = at::empty({width}, vector);
+  const size_t n = ops3d_layer_norm_backward_workspace_bytes(code, rows, width, need_w, need_b);
+  at::Tensor ws;
+  if (n) ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
+  const int rc = ops3d_layer_norm_backward(ptr(xr), ldx, ptr(w), (const float *)ptr(stats), ptr(g), ldg, gx ? ptr(*gx) : nullptr,
+                                           gw ? ptr(*gw) : nullptr, gb ? ptr(*gb) : nullptr, ptr(ws), n, code, wcode, rows, width,
+                                           stream_of(x));
+  if (rc != OPS3D_FDA_OK) raise(rc, "layer_norm_backward failed");
+  return {gx, gw, gb};
+}
+
+constexpr const char *kNormOnce = "a layer norm";
+
+class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const c10::optional<at::Tensor> &weight,
+                            const c10::optional<at::Tensor> &bias, double eps) {
+    auto [y, stats] = layer_norm_forward(x, weight, bias, eps, true);
+    ctx->save_for_backward({x, weight ? *weight : at::Tensor(), *stats});
+    const at::Tensor *v = weight ? &*weight : bias ? &*bias : nullptr;
+    ctx->saved_data["needs"] = std::vector<int64_t>{x.requires_grad(), weight && weight->requires_grad(), bias && bias->requires_grad(),
+                                                    weight.has_value(), v && v->scalar_type() == at::kFloat};
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto needs = ctx->saved_data["needs"].toIntVector();
+    torch::autograd::variable_list out(4);
+    const bool x = needs[0] && ctx->needs_input_grad(0), w = needs[1] && ctx->needs_input_grad(1),
+               b = needs[2] && ctx->needs_input_grad(needs[3] ? 2 : 1);
+    if (x || w || b) {
+      const at::NoGradGuard no_grad;
+      const bool wide = needs[4] && saved[0].scalar_type() != at::kFloat;
+      auto [gx, gw, gb] = layer_norm_backward(saved[0], needs[3] ? c10::optional<at::Tensor>(saved[1]) : c10::nullopt, saved[2],
+                                              grads[0], wide, x, w, b);
+      if (gx) out[0] = *gx;
+      if (gw) out[1] = *gw;
+      if (gb) out[2] = *gb;
+    }
+    const bool given = grads[0].requires_grad();
+    once(out[0], true, kNormOnce);
+    once(out[1], needs[0] || given, kNormOnce);
+    once(out[2], given, kNormOnce);
+    return out;
+  }
+};
+
+at::Tensor layer_norm(const at::Tensor &x, const c10::optional<at::Tensor> &weight, const c10::optional<at::Tensor> &bias,
+                      double eps) {
+  refuse_trace("layer_norm");
+  for (const at::Tensor *t : {&x, weight ? &*weight : nullptr, bias ? &*bias : nullptr})
+    if (t) refuse_tangent(*t, "layer_norm has");
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
+    return LayerNormNode::apply(x, weight, bias, eps);
+  return std::get<0>(layer_norm_forward(x, weight, bias, eps, false));
+}
+
+// Rotary positions (include/ops3d_rotary.h).  x [tokens, heads, dim] or [items, tokens, heads, dim].
+// t with consecutive channels: itself, or a copy.
+at::Tensor channels_dense(const at::Tensor &t_) {
+  const at::Tensor t = t_.is_neg() ? t_.resolve_neg() : t_;
+  return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+void strides_of(const at::Tensor &t, int64_t (&s)[3]) {   // {item, token, head}
+  s[0] = t.dim() == 4 ? t.stride(0) : 0;
+  s[1] = t.stride(-3);
+  s[2] = t.stride(-2);
+}
+
+at::Tensor rotary_apply(const at::Tensor &x, const at::Tensor &positions, const std::vector<double> &frequencies,
+                        const std::vector<int64_t> &axis_of, int64_t layout, bool inverse) {
+  linear_check(x, "x", x);
+  if (x.dim() != 3 && x.dim() != 4) throw std::invalid_argument("x must be [tokens, heads, dim] or [items, tokens, heads, dim]");
+  const int code = dtype_code(x);
+  if (!positions.is_cuda()) throw std::runtime_error("Not implemented on the CPU (positions is on the CPU)");
+  if (positions.device() != x.device()) throw std::runtime_error("positions is on another device than x");
+  if (positions.layout() != at::kStrided) throw std::invalid_argument("positions must be a dense tensor");
+  if (positions.scalar_type() != at::kFloat && positions.scalar_type() != at::kLong)
+    throw std::invalid_argument("positions must be float32 or int64");
+  const int64_t items = x.dim() == 4 ? x.size(0) : 1, tokens = x.size(-3), heads = x.size(-2), dim = x.size(-1);
+  if ((positions.dim() != 2 && (positions.dim() != 3 || x.dim() != 4 || positions.size(0) != items)) || positions.size(-2) != tokens)
+    throw std::invalid_argument("positions must be [tokens, axes], or [items, tokens, axes] beside items");
+  if (frequencies.size() != axis_of.size()) throw std::invalid_argument("there must be a frequency for each pair");
+  if (frequencies.size() > OPS3D_ROTARY_MAX_PAIRS)
+    throw std::invalid_argument("at most " + std::to_string(OPS3D_ROTARY_MAX_PAIRS) + " pairs");
+  const DeviceGuard guard(x.device());
+  const at::Tensor xr = channels_dense(x), pos = dense(positions);
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  int64_t xs[3], ys[3];
+  strides_of(xr, xs);
+  strides_of(y, ys);
+  const std::vector<int> axis(axis_of.begin(), axis_of.end());
+  const int rc = ops3d_rotary(ptr(xr), xs, ptr(pos), pos.scalar_type() == at::kFloat ? OPS3D_ROTARY_POSITION_F32 : OPS3D_ROTARY_POSITION_I64,
+                              pos.dim() == 3 ? tokens * pos.size(-1) : 0, frequencies.data(), axis.data(), (int)axis.size(),
+                              linear_int(pos.size(-1), "the number of axes"), (int)layout, inverse, ptr(y), ys, code,
+                              linear_int(items, "the number of items"), tokens, linear_int(heads, "the number of heads"),
+                              linear_int(dim, "the number of channels"), stream_of(x));
+  if (rc != OPS3D_FDA_OK) raise(rc, "rotary positions failed");
+  return y;
+}
+
+// Its gradient is the turn back, which is differentiable again.
+class RotaryNode : public torch::autograd::Function<RotaryNode> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &positions,
+                            const std::vector<double> &frequencies, const std::vector<int64_t> &axis_of, int64_t layout,
+                            bool inverse) {
+    at::Tensor y = rotary_apply(x, positions, frequencies, axis_of, layout, inverse);
+    ctx->save_for_backward({positions});
+    ctx->saved_data["frequencies"] = frequencies;
+    ctx->saved_data["axis_of"] = axis_of;
+    ctx->saved_data["layout"] = layout;
+    ctx->saved_data["inverse"] = inverse;
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(6);
+    out[0] = RotaryNode::apply(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["frequencies"].toDoubleVector(),
+                               ctx->saved_data["axis_of"].toIntVector(), ctx->saved_data["layout"].toInt(),
+                               !ctx->saved_data["inverse"].toBool());
+    return out;
+  }
+};
+
+at::Tensor rotary(const at::Tensor &x, const at::Tensor &positions, const std::vector<double> &frequencies,
+                  const std::vector<int64_t> &axis_of, int64_t layout) {
+  refuse_trace("rotary_positions");
+  refuse_tangent(x, "rotary_positions has");
+  refuse_tangent(positions, "rotary_positions has");
+  if (positions.requires_grad()) throw std::invalid_argument("rotary_positions has no gradient of positions");
+  if (at::GradMode::is_enabled() && x.requires_grad()) return RotaryNode::apply(x, positions, frequencies, axis_of, layout, false);
+  return rotary_apply(x, positions, frequencies, axis_of, layout, false);
 }
 
 }  // namespace
@@ -758,6 +978,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear, "linear_forward with its gradients through autograd");
   m.def("linear_backward", &linear_backward, "gradients of linear_forward");
   m.def("linear_keep_rows", &linear_keep_rows, "zeros in rows of no group");
+  m.def("layer_norm_forward", &layer_norm_forward, "layer norm over the last axis, and its statistics");
+  m.def("layer_norm", &layer_norm, "layer_norm_forward with its gradients through autograd");
+  m.def("layer_norm_backward", &layer_norm_backward, "gradients of layer_norm_forward");
+  m.def("rotary_apply", &rotary_apply, "pairs of channels turned by their token's position, or back");
+  m.def("rotary", &rotary, "rotary_apply with its gradient through autograd");
   m.def("roi_align_3d_forward", &roi_align_3d_forward, "roi_align_3d_forward");
   m.def("roi_align_3d_backward", &roi_align_3d_backward, "roi_align_3d_backward");
 }

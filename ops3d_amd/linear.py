@@ -60,12 +60,13 @@ class _Once(Function):
     """A gradient that raises when it is differentiated."""
 
     @staticmethod
-    def forward(ctx, t):
+    def forward(ctx, t, what="a linear operator"):
+        ctx.what = what
         return t.view_as(t)
 
     @staticmethod
     def backward(ctx, grad_output):
-        raise RuntimeError("trying to differentiate twice a linear operator that is differentiable once")
+        raise RuntimeError(f"trying to differentiate twice {ctx.what} that is differentiable once")
 
 
 def _once(grad, depends):
