@@ -19,7 +19,8 @@ LIB_NAME = "libops3d_fda.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 TORCH_EXT_NAME = "_fda_torch"
 SOURCES = ["fda_capi.hip", "fda_tiles.hip", "fda_f32.hip", "fda_f16.hip", "fda_bf16.hip", "nms3d.hip", "roi_align3d.hip",
-           "linear_capi.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip", "norm.hip", "rotary.hip"]
+           "linear_capi.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip", "norm.hip", "rotary.hip",
+           "attention_capi.hip", "attention_f32.hip", "attention_f16.hip", "attention_bf16.hip"]
 # measurement baselines (not part of the op): a library of their own
 BENCH_SOURCE = "bench_scatter.hip"
 BENCH_LIB_PATH = os.path.join(PKG_DIR, "libops3d_fda_bench.so")

@@ -65,6 +65,10 @@ EXPORTED_SYMBOLS = (
     "ops3d_linear_backward_workspace_bytes_for",
     "ops3d_linear_backward",
     "ops3d_linear_keep_rows",
+    "ops3d_attention_forward_workspace_bytes",
+    "ops3d_attention_forward",
+    "ops3d_attention_backward_workspace_bytes",
+    "ops3d_attention_backward",
     "ops3d_layer_norm_forward",
     "ops3d_layer_norm_backward_workspace_bytes",
     "ops3d_layer_norm_backward",
@@ -72,6 +76,25 @@ EXPORTED_SYMBOLS = (
     "ops3d_fda_profile_enable",
     "ops3d_fda_profile_read",
 )
+
+
+class _AttentionTensor(ctypes.Structure):
+    """ops3d_attention_tensor (include/ops3d_attention.h)."""
+
+    _fields_ = [("data", _vp), ("item", ctypes.c_int64), ("token", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class _AttentionProblem(ctypes.Structure):
+    """ops3d_attention_problem (include/ops3d_attention.h)."""
+
+    _fields_ = ([(n, _vp) for n in ("q_start", "k_start", "q_len", "k_len")]
+                + [(n, ctypes.c_int64) for n in ("q_rows", "k_rows")]
+                + [(n, ctypes.c_int32) for n in ("q_start_count", "k_start_count", "sequences", "items", "heads", "kv_heads",
+                                                 "dim", "dtype", "causal")]
+                + [("scale", ctypes.c_float)])
+
+
+MAX_SEQUENCES = 65536   # OPS3D_ATTENTION_MAX_SEQUENCES
 
 
 def _declare(lib: ctypes.CDLL) -> None:
@@ -147,6 +170,14 @@ def _declare(lib: ctypes.CDLL) -> None:
                                           + [_i] * 2 + [_i64] + [_i] * 3 + [_vp])
     lib.ops3d_linear_keep_rows.restype = _i
     lib.ops3d_linear_keep_rows.argtypes = [_vp, _i64, _vp, _i, _vp, _i, _i, _i64, _i, _i, _vp]
+    problem, tensor = ctypes.POINTER(_AttentionProblem), ctypes.POINTER(_AttentionTensor)
+    for name in ("forward", "backward"):
+        size = getattr(lib, f"ops3d_attention_{name}_workspace_bytes")
+        size.restype, size.argtypes = _sz, [problem]
+    lib.ops3d_attention_forward.restype = _i
+    lib.ops3d_attention_forward.argtypes = [problem] + [tensor] * 4 + [_vp, _vp, _sz, _vp]
+    lib.ops3d_attention_backward.restype = _i
+    lib.ops3d_attention_backward.argtypes = [problem] + [tensor] * 4 + [_vp] + [tensor] * 4 + [_vp, _sz, _vp]
     lib.ops3d_layer_norm_forward.restype = _i
     lib.ops3d_layer_norm_forward.argtypes = [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i64, _i, ctypes.c_float, _vp]
     lib.ops3d_layer_norm_backward_workspace_bytes.restype = _sz
@@ -183,7 +214,8 @@ class _NativeFDA:
                          "forward_offsets", "backward_offsets", "nms_3d", "roi_align_3d_forward",
                          "roi_align_3d_backward", "dcnv4_forward", "dcnv4_backward", "linear", "linear_forward",
                          "linear_backward", "linear_keep_rows", "layer_norm", "layer_norm_forward",
-                         "layer_norm_backward", "rotary", "rotary_apply"):
+                         "layer_norm_backward", "rotary", "rotary_apply", "attention",
+                         "attention_forward", "attention_backward"):
                 setattr(self, name, getattr(ext, name))
 
     # -- helpers ---------------------------------------------------------------------------
@@ -551,6 +583,113 @@ class _NativeFDA:
         if rc != OPS3D_FDA_OK:
             self._raise(rc, "rotary positions failed")
         return y
+
+    # -- attention over all tokens (include/ops3d_attention.h) ----------------------------------
+    def _attention_problem(self, q, k, v, q_start, k_start, q_len, k_len, causal, scale):
+        self._linear_check("q", q, q)
+        for name, t in (("k", k), ("v", v)):
+            if not t.is_cuda:
+                raise RuntimeError(f"Not implemented on the CPU ({name} is on the CPU)")
+            if t.layout != torch.strided:
+                raise ValueError(f"{name} must be a dense tensor")
+            if t.device != q.device:
+                raise RuntimeError(f"{name} is on another device than q")
+            if t.dtype != q.dtype:
+                raise ValueError(f"{name} dtype differs from q dtype")
+        if q.dim() not in (3, 4):
+            raise ValueError("q must be [tokens, heads, dim] or [items, tokens, heads, dim]")
+        if k.dim() != q.dim() or k.shape != v.shape:
+            raise ValueError("k and v must have one shape, and q's axes")
+        if k.shape[-1] != q.shape[-1]:
+            raise ValueError("q and k differ in their channels")
+        if q.dim() == 4 and k.shape[0] != q.shape[0]:
+            raise ValueError("q and k differ in their items")
+        if q.dtype not in _DTYPE_CODE:
+            raise ValueError(f"unsupported value dtype {q.dtype}")
+        p = _AttentionProblem()
+        p.dtype, p.causal, p.scale = _DTYPE_CODE[q.dtype], int(causal), scale
+        p.items = q.shape[0] if q.dim() == 4 else 1
+        (p.q_rows, p.heads, p.dim), (p.k_rows, p.kv_heads) = q.shape[-3:], k.shape[-3:-1]
+        if q_start is not None or k_start is not None:
+            if q.dim() != 3:
+                raise ValueError("packed sequences need q [tokens, heads, dim]")
+            if q_start is None or k_start is None:
+                raise ValueError("q_start and k_start go together")
+            if q_len is not None or k_len is not None:
+                raise ValueError("packed sequences have no q_len and k_len")
+        for name, t in (("q_start", q_start), ("k_start", k_start), ("q_len", q_len), ("k_len", k_len)):
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise RuntimeError(f"Not implemented on the CPU ({name} is on the CPU)")
+            if t.device != q.device:
+                raise RuntimeError(f"{name} is on another device than q")
+            if t.layout != torch.strided or t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int64 tensor of one axis")
+            if name.endswith("len") and t.shape[0] != p.items:
+                raise ValueError(f"q_len and k_len must have an entry for each of {p.items} items")
+            setattr(p, name, _ptr(t))
+        if q_start is not None:
+            n = q_start.shape[0]
+            if n < 2 or n != k_start.shape[0] or n > MAX_SEQUENCES + 1:
+                raise ValueError(f"q_start and k_start must have an entry for each of 1..{MAX_SEQUENCES} sequences and the "
+                                 f"last one's end, got {n} and {k_start.shape[0]}")
+            p.q_start_count = p.k_start_count = n
+            p.sequences = n - 1
+        return p
+
+    @classmethod
+    def _attention_tensor(cls, t):
+        return None if t is None else _AttentionTensor(_ptr(t), *cls._strides(t))
+
+    def attention(self, q, k, v, q_start, k_start, q_len, k_len, causal, scale):
+        """The operator through autograd (AttentionFunction where a gradient is wanted)."""
+        self._refuse("packed_attention", q, k, v)
+        args = (q, k, v, q_start, k_start, q_len, k_len, causal, scale)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+            from .attention import AttentionFunction
+
+            return AttentionFunction.apply(*args, self)
+        return self.attention_forward(*args, False)[0]
+
+    def attention_forward(self, q, k, v, q_start, k_start, q_len, k_len, causal, scale, keep):
+        """(out, lse); lse (None otherwise) when ``keep``."""
+        p = self._attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale)
+        qd, kd, vd = (self._channels_dense(t) for t in (q, k, v))
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((p.items, p.heads, p.q_rows), dtype=torch.float32, device=q.device) if keep else None
+        n = self._lib.ops3d_attention_forward_workspace_bytes(p)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        with torch.cuda.device(q.device):
+            rc = self._lib.ops3d_attention_forward(p, *(self._attention_tensor(t) for t in (qd, kd, vd, out)), _ptr(lse), _ptr(ws),
+                                                   n, torch.cuda.current_stream(q.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "attention_forward failed")
+        return out, lse
+
+    def attention_backward(self, q, k, v, q_start, k_start, q_len, k_len, causal, scale, out, lse, grad_out, need_q, need_kv):
+        """(grad_q, grad_k, grad_v), None where not wanted (the latter two together)."""
+        p = self._attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale)
+        self._linear_check("grad_output", grad_out, q)
+        if grad_out.shape != q.shape:
+            raise ValueError("grad_output must have the output's shape")
+        if (out.device != q.device or out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous()
+                or lse.device != q.device or lse.dtype != torch.float32 or not lse.is_contiguous()
+                or lse.shape != (p.items, p.heads, p.q_rows)):
+            raise ValueError("out and lse are not a forward's of this shape")
+        qd, kd, vd, gd = (self._channels_dense(t) for t in (q, k, v, grad_out))
+        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
+        gk, gv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_kv else None for _ in range(2))
+        n = self._lib.ops3d_attention_backward_workspace_bytes(p)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        with torch.cuda.device(q.device):
+            rc = self._lib.ops3d_attention_backward(
+                p, *(self._attention_tensor(t) for t in (qd, kd, vd, out)), _ptr(lse),
+                *(self._attention_tensor(t) for t in (gd, gq, gk, gv)), _ptr(ws), n,
+                torch.cuda.current_stream(q.device).cuda_stream)
+        if rc != OPS3D_FDA_OK:
+            self._raise(rc, "attention_backward failed")
+        return gq, gk, gv
 
     # -- entry points (reference csrc/flash_deform_attn.h) -----------------------------------
     def flash_deform_attn_forward(

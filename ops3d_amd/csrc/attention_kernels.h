@@ -1,0 +1,873 @@
+// Attention over all tokens (gfx950), forward and backward (include/ops3d_attention.h).
+//
+// One scheme for its three kernels: a block owns some columns of the logits, whose operands stay in
+// registers, and the other side's rows come by in stages through LDS:
+//   forward   owns queries, keys and values come by      S^T = K Q^T,  O^T += V^T P^T
+//   grad q    owns queries, keys and values come by      S^T, dP^T = V dO^T,  dQ^T += K^T dS^T
+//   grad k v  owns keys, queries and grad_out come by    S = Q K^T, dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS
+// The products run on 16 x 16 MFMA results: lane (i, q) (i the lane mod 16, q its quarter of the wave) holds
+// rows 4 q .. 4 q + 3 of column i.  Those are the operand elements that the next product wants from the lane
+// if its sum runs over the rows in the order 4 q .. 4 q + 3 of one result, the same of the next: so P and
+// dS go from result to operand in registers, rounded, and the other operand is read from LDS transposed in
+// that order.
+//
+// Columns of queries are pairs of a query and a head of the key head's group, c = query G + head: the heads of
+// a group share the keys that come by, in training and where one query is all there is.
+//
+// Softmax runs along: a column's reference m is raised, and its sums are rescaled, only when a logit passes
+// it by 2^kSlack; P is at most that.  Statistics are kept in log2 units.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "elements.h"
+#include "reduce.h"
+#include "segments.h"
+
+namespace ops3d_attention {
+
+using namespace ops3d_elements;
+
+struct Tensor {
+  void *p;
+  int64_t item, token, head;
+};
+
+struct Args {
+  Tensor q, k, v, o, g, gq, gk, gv;   // g: grad_out
+  const int64_t *q_start, *k_start, *q_len, *k_len;
+  int q_count, k_count, E;            // E: sequences (packed)
+  int Sq, Sk;                         // rows of an item
+  int Hk, G, D;                       // key heads, query heads of each, channels
+  uint32_t magic;                     // c / G = 2 c magic >> 32 >> shift
+  int shift;
+  int causal;
+  float scale, c;                     // c = scale log2 e
+  int tiles, tiles_item, splits;      // tiles of all items (a bound), of one, and parts of the other side
+  int heads;                          // items Hk
+  int64_t cells;                      // heads Sq G: queries times heads
+  float *lse, *delta;                 // [items, Hk, Sq G]; log2 of the sum of exponentials, and sum of o g
+  float *part, *part_ml;              // [splits, columns, DP], [splits, columns, 2]
+};
+
+// What a block works on.
+struct Work {
+  int item, q0, k0;      // first rows of the sequence
+  int nq, nk;            // queries and keys that count
+  int rows;              // rows of the owned side, all of which are written
+  int first;             // first owned column
+};
+
+// Tile t of `per` columns.  KEYS: columns are keys, otherwise queries times heads.
+template <bool KEYS> __device__ __forceinline__ bool locate(const Args &p, int t, int per, Work &w) {
+  const int unit = KEYS ? 1 : p.G;
+  if (!p.q_start) {
+    const int e = t / p.tiles_item;
+    w.item = e;
+    w.q0 = w.k0 = 0;
+    const auto held = [](const int64_t *len, int e, int rows) {
+      if (!len) return rows;
+      const int64_t v = len[e];
+      return v < 0 ? 0 : (int)(v < rows ? v : rows);
+    };
+    w.nq = held(p.q_len, e, p.Sq);
+    w.nk = held(p.k_len, e, p.Sk);
+    w.rows = KEYS ? p.Sk : p.Sq;
+    w.first = (t - e * p.tiles_item) * per;
+    return true;
+  }
+  using ops3d_segments::Segment;
+  using ops3d_segments::segment_at;
+  const int lane = threadIdx.x & 63;
+  const int64_t *own = KEYS ? p.k_start : p.q_start, *other = KEYS ? p.q_start : p.k_start;
+  const int own_count = KEYS ? p.k_count : p.q_count, other_count = KEYS ? p.q_count : p.k_count;
+  const int own_rows = KEYS ? p.Sk : p.Sq, other_rows = KEYS ? p.Sq : p.Sk;
+  int carry = 0, before = 0, j = -1, lower = 0;
+  for (int base = 0; base < p.E + 2; base += 64) {
+    const Segment s = segment_at(own, own_count, own_rows, base + lane, carry);
+    const int tiles = base + lane < p.E + 2 ? (int)(((int64_t)(s.upper - s.lower) * unit + per - 1) / per) : 0;
+    const int incl = before + ops3d_segments::scan_add(tiles);
+    const uint64_t m = __ballot(incl > t);
+    if (m) {
+      const int src = __builtin_ctzll(m);
+      j = base + src;
+      lower = __builtin_amdgcn_readlane(s.lower, src);
+      w.rows = __builtin_amdgcn_readlane(s.upper, src) - lower;
+      w.first = (t - (__builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane(tiles, src))) * per;
+      break;
+    }
+    before = __builtin_amdgcn_readlane(incl, 63);
+  }
+  if (j < 0) return false;
+  int o_lower = 0, o_rows = 0;
+  if (j >= 1 && j <= p.E) {
+    carry = 0;
+    for (int base = 0; base <= j; base += 64) {
+      const Segment s = segment_at(other, other_count, other_rows, base + lane, carry);
+      if (j < base + 64) {
+        o_lower = __builtin_amdgcn_readlane(s.lower, j - base);
+        o_rows = __builtin_amdgcn_readlane(s.upper, j - base) - o_lower;
+      }
+    }
+  }
+  const bool in = j >= 1 && j <= p.E;   // rows of no sequence: none that count
+  w.item = 0;
+  w.q0 = KEYS ? o_lower : lower;
+  w.k0 = KEYS ? lower : o_lower;
+  w.nq = KEYS ? o_rows : (in ? w.rows : 0);
+  w.nk = KEYS ? (in ? w.rows : 0) : o_rows;
+  return true;
+}
+
+__device__ __forceinline__ int divide(const Args &p, int c) { return (int)(__umulhi((uint32_t)c << 1, p.magic) >> p.shift); }
+
+// A stage of R rows of DP elements in LDS, in 16-byte chunks, XOR-swizzled: 8 rows that follow each other and
+// a chunk of each, and 4 rows and two neighbouring chunks of each, fall on different banks.
+template <typename T, int DP, int R, int NT> struct Stage {
+  static constexpr int CH = 16 / (int)sizeof(T), RC = DP / CH, NL = R * RC / NT;
+  static constexpr int kBytes = R * DP * (int)sizeof(T);
+  static_assert(R * RC % NT == 0 && RC >= 4, "chunks divide over the threads");
+
+  static __device__ __forceinline__ int address(int row, int chunk) {
+    if (RC == 4) {
+      const int line = row >> 1;
+      return (row * 4 + (chunk ^ (((line & 1) << 1) | ((line >> 1) & 1)))) << 4;
+    }
+    return (row * RC + (chunk ^ (((row & 3) << 1) | ((row >> 2) & 1)))) << 4;
+  }
+  static __device__ __forceinline__ int row_of(int i) { return (int)(threadIdx.x + i * NT) / RC; }
+  static __device__ __forceinline__ int chunk_of(int i) { return (int)(threadIdx.x + i * NT) % RC; }
+
+  // at(row): the row's first element; zeros from row n on and behind D.
+  template <typename F> static __device__ __forceinline__ void load(uint4 (&v)[NL], F at, int n, int D) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = row_of(i), col = chunk_of(i) * CH;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (row < n && col < D) v[i] = fetch(at(row), 0, 0, col, 1, D);
+    }
+  }
+  static __device__ __forceinline__ void store(char *lds, const uint4 (&v)[NL]) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4 *>(lds + address(row_of(i), chunk_of(i))) = v[i];
+  }
+
+  // MFMA operand: 16 rows from r0 on, step s of the channels
+  static __device__ __forceinline__ typename Type<T>::frag rows(const char *lds, int r0, int s, int lane) {
+    return __builtin_bit_cast(typename Type<T>::frag,
+                              *reinterpret_cast<const uint4 *>(lds + address(r0 + (lane & 15), s * 4 + (lane >> 4))));
+  }
+  // MFMA operand: 16 channels from 16 dt on, summed over rows: in 16 bits rows r0 + 4 q .. + 3 and those 16
+  // further, in 32 bits the former.  16 lanes read 4 rows of 16 channels, 4 channels a lane, and get them
+  // transposed.
+  static __device__ __forceinline__ typename Type<T>::frag columns(const char *lds, int r0, int dt, int lane) {
+    const int i = lane & 15, q = lane >> 4;
+    if constexpr (sizeof(T) == 2) {
+      s16x4 h[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const char *at = lds + address(r0 + p * 16 + q * 4 + (i >> 2), dt * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+        h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(const_cast<char *>(at)));
+      }
+      return __builtin_bit_cast(typename Type<T>::frag, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      f32x4 f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = *reinterpret_cast<const float *>(lds + address(r0 + q * 4 + j, dt * 4 + (i >> 2)) + (i & 3) * 4);
+      return __builtin_bit_cast(typename Type<T>::frag, f);
+    }
+  }
+};
+
+// Results of one (fp32) or two (16 bits) tiles of 16 rows as the operand of a product summed over them.
+template <typename T> __device__ __forceinline__ typename Type<T>::frag operand(const f32x4 *s) {
+  if constexpr (sizeof(T) == 4) {
+    return s[0];
+  } else {
+    typename Type<T>::frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)s[j >> 2][j & 3];
+    return f;
+  }
+}
+
+// The operand of a column's row of channels, from memory; zeros behind D, and everywhere without a row.
+template <typename T, int STEPS>
+__device__ __forceinline__ void load_column(typename Type<T>::frag (&f)[STEPS], const T *row, int D, int q) {
+  constexpr int CH = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+    f[s] = __builtin_bit_cast(typename Type<T>::frag, row ? fetch(row, 0, 0, (s * 4 + q) * CH, 1, D) : make_uint4(0, 0, 0, 0));
+}
+
+// 4 consecutive channels of a row; those behind D are left out.
+template <typename T> __device__ __forceinline__ void store4(T *row, int d, const f32x4 &v, int D) {
+  if (d + 4 <= D) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Four { T e[4]; } f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.e[j] = (T)v[j];
+    *reinterpret_cast<Four *>(row + d) = f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (d + j < D) row[d + j] = (T)v[j];
+  }
+}
+
+// 16-bit fractions as fp16 numbers lose precision below 2^-14, so that of P is kept 2^kShift up; with the
+// slack below, P stays under 2^15.
+template <typename T> struct Range { static constexpr float kShift = 0.f, kSlack = 8.f; };
+template <> struct Range<_Float16> { static constexpr float kShift = 10.f, kSlack = 4.f; };
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The block's place: key head, part and tile; tiles from the last on, which in causal attention have most to
+// do.
+__device__ __forceinline__ void place(const Args &p, int &h, int &part, int &tile) {
+  const int r = blockIdx.x / p.Hk;
+  h = blockIdx.x - r * p.Hk;
+  part = r % p.splits;
+  tile = p.tiles - 1 - r / p.splits;
+}
+
+// Adds the waves' results of a block whose WK waves had each a share of the rows: lane by lane through LDS,
+// wave 0 has the sum.  f(i): the i-th of n results.
+template <int WK, int N, typename F> __device__ __forceinline__ void add_waves(char *lds, int wk, int lane, F f) {
+  f32x4 *x = reinterpret_cast<f32x4 *>(lds);
+  __syncthreads();
+  if (wk) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[((wk - 1) * N + i) * 64 + lane] = f(i);
+  }
+  __syncthreads();
+  if (wk == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < WK - 1; ++k) f(i) += x[(k * N + i) * 64 + lane];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Forward: WC waves of NC x 16 columns side by side, and WK of them that share out each stage's KT keys.
+template <typename T, int DP, int NC, int WC, int WK, int KT>
+__global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
+  constexpr int NT = 64 * WC * WK, BM = WC * NC * 16, KW = KT / WK, KN = KW / 16;
+  constexpr int STEPS = DP * (int)sizeof(T) / 64, DT = DP / 16, PR = sizeof(T) == 2 ? 2 : 1;   // tiles an operand holds
+  typedef Stage<T, DP, KT, NT> ST;
+  static_assert(KN % PR == 0, "whole operands");
+  constexpr int kMerge = (WK - 1) * NC * (DT + 1) * 1024;
+  constexpr int kLds = 4 * ST::kBytes > kMerge ? 4 * ST::kBytes : kMerge;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+
+  int h, part, tile;
+  place(p, h, part, tile);
+  Work w;
+  if (!locate<false>(p, tile, BM, w)) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  const int wc = wave % WC, wk = wave / WC;
+  const int active = w.nq * p.G, off = w.nk - w.nq, c0 = w.first + wc * NC * 16;
+  const T *qb = static_cast<const T *>(p.q.p) + w.item * p.q.item + w.q0 * p.q.token + (int64_t)h * p.G * p.q.head;
+  const T *kb = static_cast<const T *>(p.k.p) + w.item * p.k.item + w.k0 * p.k.token + h * p.k.head;
+  const T *vb = static_cast<const T *>(p.v.p) + w.item * p.v.item + w.k0 * p.v.token + h * p.v.head;
+
+  typename Type<T>::frag qf[NC][STEPS];
+  int limit[NC];   // keys that the column sees; those of columns that do not count are not held back
+  int least = w.nk;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int c = c0 + n * 16 + i, t = divide(p, c);
+    load_column<T, STEPS>(qf[n], c < active ? qb + t * p.q.token + (c - t * p.G) * p.q.head : nullptr, p.D, q);
+    limit[n] = p.causal && c < active ? min(w.nk, t + off + 1) : w.nk;
+    least = min(least, limit[n]);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
+  least = __builtin_amdgcn_readfirstlane(least);
+  // keys that any column of the block sees, and this part of them
+  int keys = w.first < active ? w.nk : 0;
+  if (p.causal && keys) keys = max(0, min(keys, divide(p, min(active, w.first + BM) - 1) + off + 1));
+  int k_begin = 0, k_end = keys;
+  if (p.splits > 1) {
+    const int per = ((keys + KT - 1) / KT + p.splits - 1) / p.splits * KT;
+    k_begin = min(keys, part * per);
+    k_end = min(keys, k_begin + per);
+  }
+
+  f32x4 o[NC][DT];
+  float m[NC], mc[NC], l[NC], top[NC];   // reference, the same times c, sum (this lane's rows), what raises it
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    m[n] = top[n] = -INFINITY;
+    mc[n] = -Range<T>::kShift;
+    l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float slack = Range<T>::kSlack / p.c;
+
+  uint4 kv[ST::NL], vv[ST::NL];
+  const auto load = [&](int k0) {
+    const int left = k_end - k0;
+    ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
+    ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
+  };
+  if (k_begin < k_end) load(k_begin);
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += KT, buf ^= 1) {
+    char *const lk = lds + buf * 2 * ST::kBytes, *const lv = lk + ST::kBytes;
+    ST::store(lk, kv);
+    ST::store(lv, vv);
+    if (k0 + KT < k_end) load(k0 + KT);
+    __syncthreads();   // the other buffer's readers are past the barrier before
+
+    const int r0 = wk * KW;
+    f32x4 s[NC][KN];
+#pragma unroll
+    for (int kt = 0; kt < KN; ++kt) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) s[n][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        const auto kf = ST::rows(lk, r0 + kt * 16, st, lane);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][kt] = Type<T>::mma(kf, qf[n][st], s[n][kt]);
+      }
+    }
+    const int first = k0 + r0;
+    if (first + KW > least) {   // also keys behind the last
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int kt = 0; kt < KN; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (first + kt * 16 + q * 4 + j >= limit[n]) s[n][kt][j] = -INFINITY;
+    }
+    bool raise = false;
+    float mx[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      mx[n] = s[n][0][0];
+#pragma unroll
+      for (int kt = 0; kt < KN; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx[n] = fmaxf(mx[n], s[n][kt][j]);
+      raise |= mx[n] > top[n];
+    }
+    if (__ballot(raise)) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const float now = fmaxf(m[n], ops3d_reduce::across32<ops3d_reduce::Max>(ops3d_reduce::across16<ops3d_reduce::Max>(mx[n])));
+        if (now != m[n]) {
+          const float by = m[n] == -INFINITY ? 0.f : exp2_((m[n] - now) * p.c);
+          l[n] *= by;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[n][d] *= by;
+          m[n] = now;
+          mc[n] = now * p.c - Range<T>::kShift;
+          top[n] = now + slack;
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int kt = 0; kt < KN; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[n][kt][j] = exp2_(fmaf(s[n][kt][j], p.c, -mc[n]));
+          l[n] += s[n][kt][j];
+        }
+#pragma unroll
+    for (int kt = 0; kt < KN; kt += PR) {
+      typename Type<T>::frag pf[NC];
+#pragma unroll
+      for (int n = 0; n < NC; ++n) pf[n] = operand<T>(&s[n][kt]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const auto vf = ST::columns(lv, r0 + kt * 16, d, lane);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) o[n][d] = Type<T>::mma(vf, pf[n], o[n][d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NC; ++n) l[n] = ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(l[n]));
+
+  if constexpr (WK > 1) {   // the waves' shares, each with its own reference
+    f32x4 *x = reinterpret_cast<f32x4 *>(lds);
+    __syncthreads();
+    if (wk) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        f32x4 *y = x + (((wk - 1) * WC + wc) * NC + n) * (DT + 1) * 64 + lane;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) y[d * 64] = o[n][d];
+        y[DT * 64] = f32x4{m[n], l[n], 0.f, 0.f};
+      }
+    }
+    __syncthreads();
+    if (wk) return;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int k = 0; k < WK - 1; ++k) {
+        const f32x4 *y = x + ((k * WC + wc) * NC + n) * (DT + 1) * 64 + lane;
+        const float mk = y[DT * 64][0], now = fmaxf(m[n], mk);
+        const float a = m[n] == -INFINITY ? 0.f : exp2_((m[n] - now) * p.c), b = mk == -INFINITY ? 0.f : exp2_((mk - now) * p.c);
+        l[n] = l[n] * a + y[DT * 64][1] * b;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[n][d] = o[n][d] * a + y[d * 64] * b;
+        m[n] = now;
+      }
+  }
+
+  const int64_t cell0 = ((int64_t)(w.item * p.Hk + h) * p.Sq + w.q0) * p.G;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int c = c0 + n * 16 + i;
+    if (c >= w.rows * p.G) continue;
+    if (p.splits > 1) {
+      const int64_t at = part * p.cells + cell0 + c;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + at * DP + d * 16 + q * 4) = o[n][d];
+      if (q == 0) {   // columns that do not count saw nothing
+        p.part_ml[2 * at] = c < active ? m[n] * p.c : -INFINITY;
+        p.part_ml[2 * at + 1] = c < active ? l[n] : 0.f;
+      }
+      continue;
+    }
+    const bool none = c >= active || l[n] == 0.f;
+    const float inv = none ? 0.f : 1.f / l[n];
+    const int t = divide(p, c);
+    T *to = static_cast<T *>(p.o.p) + w.item * p.o.item + (w.q0 + t) * p.o.token + ((int64_t)h * p.G + c - t * p.G) * p.o.head;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) store4(to, d * 16 + q * 4, none ? f32x4{0.f, 0.f, 0.f, 0.f} : o[n][d] * inv, p.D);
+    if (p.lse && q == 0) p.lse[cell0 + c] = none ? INFINITY : m[n] * p.c + __builtin_amdgcn_logf(l[n]) - Range<T>::kShift;
+  }
+}
+
+// The parts of a query and head joined: a wave each.
+template <typename T, int DP> __global__ __launch_bounds__(256) void join_forward_kernel(Args p) {
+  const int64_t cell = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (cell >= p.cells) return;
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  for (int z = lane; z < p.splits; z += 64) m = fmaxf(m, p.part_ml[2 * (z * p.cells + cell)]);
+  m = ops3d_reduce::all<64, ops3d_reduce::Max>(m);
+  float l = 0.f, o[(DP + 63) / 64];
+#pragma unroll
+  for (int k = 0; k < (DP + 63) / 64; ++k) o[k] = 0.f;
+  if (m != -INFINITY) {
+    for (int z = 0; z < p.splits; ++z) {
+      const int64_t at = z * p.cells + cell;
+      const float mz = p.part_ml[2 * at];
+      const float by = mz == -INFINITY ? 0.f : exp2_(mz - m);
+      if (by == 0.f) continue;
+      l = fmaf(by, p.part_ml[2 * at + 1], l);
+#pragma unroll
+      for (int k = 0; k < (DP + 63) / 64; ++k)
+        if (k * 64 + lane < DP) o[k] = fmaf(by, p.part[at * DP + k * 64 + lane], o[k]);
+    }
+  }
+  const int per = p.Sq * p.G, ih = (int)(cell / per), c = (int)(cell - (int64_t)ih * per);
+  const int item = ih / p.Hk, h = ih - item * p.Hk, t = divide(p, c);
+  const bool none = l == 0.f;
+  T *to = static_cast<T *>(p.o.p) + item * p.o.item + t * p.o.token + ((int64_t)h * p.G + c - t * p.G) * p.o.head;
+#pragma unroll
+  for (int k = 0; k < (DP + 63) / 64; ++k)
+    if (k * 64 + lane < p.D) to[k * 64 + lane] = (T)(none ? 0.f : o[k] / l);
+  if (p.lse && lane == 0) p.lse[cell] = none ? INFINITY : m + __builtin_amdgcn_logf(l) - Range<T>::kShift;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradient of the queries, and delta = sum of o grad_out, which the keys' needs (gq NULL: that alone).
+template <typename T, int DP, int NC, int WC, int WK, int KT>
+__global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
+  constexpr int NT = 64 * WC * WK, BM = WC * NC * 16, KW = KT / WK, KN = KW / 16;
+  constexpr int STEPS = DP * (int)sizeof(T) / 64, DT = DP / 16, PR = sizeof(T) == 2 ? 2 : 1, CH = 16 / (int)sizeof(T);
+  typedef Stage<T, DP, KT, NT> ST;
+  static_assert(KN % PR == 0, "whole operands");
+  constexpr int kMerge = (WK - 1) * NC * DT * 1024;
+  constexpr int kLds = 4 * ST::kBytes > kMerge ? 4 * ST::kBytes : kMerge;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+
+  int h, part, tile;
+  place(p, h, part, tile);
+  Work w;
+  if (!locate<false>(p, tile, BM, w)) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  const int wc = wave % WC, wk = wave / WC;
+  const int active = w.nq * p.G, off = w.nk - w.nq, c0 = w.first + wc * NC * 16;
+  const T *kb = static_cast<const T *>(p.k.p) + w.item * p.k.item + w.k0 * p.k.token + h * p.k.head;
+  const T *vb = static_cast<const T *>(p.v.p) + w.item * p.v.item + w.k0 * p.v.token + h * p.v.head;
+  const int64_t cell0 = ((int64_t)(w.item * p.Hk + h) * p.Sq + w.q0) * p.G;
+
+  typename Type<T>::frag qf[NC][STEPS], gf[NC][STEPS];
+  int limit[NC], least = w.nk;
+  float lse[NC], delta[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int c = c0 + n * 16 + i, t = divide(p, c), head = h * p.G + c - t * p.G;
+    const bool in = c < active;
+    const auto row = [&](const Tensor &x) {
+      return in ? static_cast<const T *>(x.p) + w.item * x.item + (w.q0 + t) * x.token + head * x.head : nullptr;
+    };
+    load_column<T, STEPS>(qf[n], row(p.q), p.D, q);
+    load_column<T, STEPS>(gf[n], row(p.g), p.D, q);
+    typename Type<T>::frag of[STEPS];
+    load_column<T, STEPS>(of, row(p.o), p.D, q);
+    float d = 0.f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < CH; ++j) d = fmaf((float)of[s][j], (float)gf[n][s][j], d);
+    delta[n] = ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(d));
+    lse[n] = in ? p.lse[cell0 + c] : INFINITY;
+    if (c < w.rows * p.G && q == 0 && wk == 0 && part == 0) p.delta[cell0 + c] = delta[n];
+    limit[n] = p.causal && in ? min(w.nk, t + off + 1) : w.nk;
+    least = min(least, limit[n]);
+  }
+  if (!p.gq.p) return;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
+  least = __builtin_amdgcn_readfirstlane(least);
+  int keys = w.first < active ? w.nk : 0;
+  if (p.causal && keys) keys = max(0, min(keys, divide(p, min(active, w.first + BM) - 1) + off + 1));
+  int k_begin = 0, k_end = keys;
+  if (p.splits > 1) {
+    const int per = ((keys + KT - 1) / KT + p.splits - 1) / p.splits * KT;
+    k_begin = min(keys, part * per);
+    k_end = min(keys, k_begin + per);
+  }
+
+  f32x4 a[NC][DT];
+#pragma unroll
+  for (int n = 0; n < NC; ++n)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) a[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint4 kv[ST::NL], vv[ST::NL];
+  const auto load = [&](int k0) {
+    const int left = k_end - k0;
+    ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
+    ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
+  };
+  if (k_begin < k_end) load(k_begin);
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += KT, buf ^= 1) {
+    char *const lk = lds + buf * 2 * ST::kBytes, *const lv = lk + ST::kBytes;
+    ST::store(lk, kv);
+    ST::store(lv, vv);
+    if (k0 + KT < k_end) load(k0 + KT);
+    __syncthreads();
+    const int r0 = wk * KW, first = k0 + r0;
+    const bool mask = first + KW > least;
+#pragma unroll
+    for (int kt = 0; kt < KN; kt += PR) {
+      f32x4 s[NC][PR], dp[NC][PR];
+#pragma unroll
+      for (int u = 0; u < PR; ++u) {
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][u] = dp[n][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+          const auto kf = ST::rows(lk, r0 + (kt + u) * 16, st, lane), vf = ST::rows(lv, r0 + (kt + u) * 16, st, lane);
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            s[n][u] = Type<T>::mma(kf, qf[n][st], s[n][u]);
+            dp[n][u] = Type<T>::mma(vf, gf[n][st], dp[n][u]);
+          }
+        }
+      }
+      typename Type<T>::frag ds[NC];
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+#pragma unroll
+        for (int u = 0; u < PR; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float x = exp2_(fmaf(s[n][u][j], p.c, -lse[n])) * (dp[n][u][j] - delta[n]);
+            if (mask && first + (kt + u) * 16 + q * 4 + j >= limit[n]) x = 0.f;
+            s[n][u][j] = x;
+          }
+        ds[n] = operand<T>(s[n]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const auto kf = ST::columns(lk, r0 + kt * 16, d, lane);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) a[n][d] = Type<T>::mma(kf, ds[n], a[n][d]);
+      }
+    }
+  }
+  if constexpr (WK > 1) {
+    static_assert(WC == 1, "the waves' results lie one behind another");
+    add_waves<WK, NC * DT>(lds, wk, lane, [&](int k) -> f32x4 & { return a[k / DT][k % DT]; });
+    if (wk) return;
+  }
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int c = c0 + n * 16 + i, t = divide(p, c);
+    if (c >= w.rows * p.G) continue;
+    if (p.splits > 1) {
+      const int64_t at = part * p.cells + cell0 + c;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + at * DP + d * 16 + q * 4) = a[n][d];
+      continue;
+    }
+    T *to = static_cast<T *>(p.gq.p) + w.item * p.gq.item + (w.q0 + t) * p.gq.token + ((int64_t)h * p.G + c - t * p.G) * p.gq.head;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      store4(to, d * 16 + q * 4, c < active ? a[n][d] * p.scale : f32x4{0.f, 0.f, 0.f, 0.f}, p.D);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradients of keys and values.
+template <typename T, int DP, int NC, int WC, int WK, int QT>
+__global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
+  constexpr int NT = 64 * WC * WK, BN = WC * NC * 16, QW = QT / WK, QN = QW / 16;
+  constexpr int STEPS = DP * (int)sizeof(T) / 64, DT = DP / 16, PR = sizeof(T) == 2 ? 2 : 1;
+  typedef Stage<T, DP, QT, NT> ST;
+  static_assert(QN % PR == 0 && QT <= NT, "whole operands, a thread a row");
+  constexpr int kStage = 2 * ST::kBytes + QT * 8;   // and the rows' lse and delta
+  constexpr int kMerge = (WK - 1) * NC * DT * 1024;
+  constexpr int kLds = 2 * kStage > kMerge ? 2 * kStage : kMerge;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+
+  int h, part, tile;
+  place(p, h, part, tile);
+  Work w;
+  if (!locate<true>(p, p.tiles - 1 - tile, BN, w)) return;   // the first keys have most queries
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  const int wc = wave % WC, wk = wave / WC;
+  const int active = w.nq * p.G, off = w.nk - w.nq, j0 = w.first + wc * NC * 16;
+  const auto rows_of = [&](const Tensor &x) { return static_cast<const T *>(x.p) + w.item * x.item + w.q0 * x.token + (int64_t)h * p.G * x.head; };
+  const T *qb = rows_of(p.q), *gb = rows_of(p.g);
+  const int64_t cell0 = ((int64_t)(w.item * p.Hk + h) * p.Sq + w.q0) * p.G;
+
+  typename Type<T>::frag kf[NC][STEPS], vf[NC][STEPS];
+  int since[NC];   // the first column of queries that sees the key
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int j = j0 + n * 16 + i;
+    const auto row = [&](const Tensor &x) {
+      return j < w.nk ? static_cast<const T *>(x.p) + w.item * x.item + (w.k0 + j) * x.token + h * x.head : nullptr;
+    };
+    load_column<T, STEPS>(kf[n], row(p.k), p.D, q);
+    load_column<T, STEPS>(vf[n], row(p.v), p.D, q);
+    since[n] = p.causal ? (int)min((int64_t)active, max((int64_t)0, (int64_t)(j - off) * p.G)) : 0;
+  }
+  const int last = j0 + NC * 16 - 1;   // of this wave
+  const int all_see = p.causal ? (int)min((int64_t)active, max((int64_t)0, (int64_t)(last - off) * p.G)) : 0;
+  int begin = w.first < w.nk ? 0 : active;
+  if (p.causal) begin = max(begin, (int)min((int64_t)active, max((int64_t)0, (int64_t)(w.first - off) * p.G)) / QT * QT);
+  int c_begin = begin, c_end = active;
+  if (p.splits > 1) {
+    const int per = ((active - begin + QT - 1) / QT + p.splits - 1) / p.splits * QT;
+    c_begin = min(active, begin + part * per);
+    c_end = min(active, c_begin + per);
+  }
+
+  f32x4 ak[NC][DT], av[NC][DT];
+#pragma unroll
+  for (int n = 0; n < NC; ++n)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) ak[n][d] = av[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint4 qv[ST::NL], gv[ST::NL];
+  float row_lse = INFINITY, row_delta = 0.f;
+  const auto load = [&](int c0) {
+    const int left = c_end - c0;
+    const auto at = [&](const T *base, const Tensor &x, int r) {
+      const int t = divide(p, c0 + r);
+      return base + t * x.token + (c0 + r - t * p.G) * x.head;
+    };
+    ST::load(qv, [&](int r) { return at(qb, p.q, r); }, left, p.D);
+    ST::load(gv, [&](int r) { return at(gb, p.g, r); }, left, p.D);
+    if (threadIdx.x < QT) {
+      const bool in = (int)threadIdx.x < left;   // P = 0 in the others
+      row_lse = in ? p.lse[cell0 + c0 + threadIdx.x] : INFINITY;
+      row_delta = in ? p.delta[cell0 + c0 + threadIdx.x] : 0.f;
+    }
+  };
+  if (c_begin < c_end) load(c_begin);
+  int buf = 0;
+  constexpr float kDown = sizeof(T) == 2 ? 1.f / (float)(1 << (int)Range<T>::kShift) : 1.f;
+  for (int c0 = c_begin; c0 < c_end; c0 += QT, buf ^= 1) {
+    char *const lq = lds + buf * kStage, *const lg = lq + ST::kBytes;
+    float *const ll = reinterpret_cast<float *>(lg + ST::kBytes), *const ld = ll + QT;
+    ST::store(lq, qv);
+    ST::store(lg, gv);
+    if (threadIdx.x < QT) {
+      ll[threadIdx.x] = row_lse - Range<T>::kShift;
+      ld[threadIdx.x] = row_delta;
+    }
+    if (c0 + QT < c_end) load(c0 + QT);
+    __syncthreads();
+    const int r0 = wk * QW, first = c0 + r0;
+    const bool mask = first < all_see;
+#pragma unroll
+    for (int qt = 0; qt < QN; qt += PR) {
+      f32x4 s[NC][PR], dp[NC][PR];
+#pragma unroll
+      for (int u = 0; u < PR; ++u) {
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][u] = dp[n][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+          const auto qf = ST::rows(lq, r0 + (qt + u) * 16, st, lane), gf = ST::rows(lg, r0 + (qt + u) * 16, st, lane);
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            s[n][u] = Type<T>::mma(qf, kf[n][st], s[n][u]);
+            dp[n][u] = Type<T>::mma(gf, vf[n][st], dp[n][u]);
+          }
+        }
+      }
+      typename Type<T>::frag pf[NC], ds[NC];
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+#pragma unroll
+        for (int u = 0; u < PR; ++u) {
+          const int r = r0 + (qt + u) * 16 + q * 4;
+          const f32x4 lse = *reinterpret_cast<const f32x4 *>(ll + r), delta = *reinterpret_cast<const f32x4 *>(ld + r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float x = exp2_(fmaf(s[n][u][j], p.c, -lse[j])), y = x * fmaf(dp[n][u][j], kDown, -kDown * delta[j]);
+            if (mask && c0 + r + j < since[n]) x = y = 0.f;
+            s[n][u][j] = x;
+            dp[n][u][j] = y;
+          }
+        }
+        pf[n] = operand<T>(s[n]);
+        ds[n] = operand<T>(dp[n]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const auto gf = ST::columns(lg, r0 + qt * 16, d, lane), qf = ST::columns(lq, r0 + qt * 16, d, lane);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          av[n][d] = Type<T>::mma(gf, pf[n], av[n][d]);
+          ak[n][d] = Type<T>::mma(qf, ds[n], ak[n][d]);
+        }
+      }
+    }
+  }
+  if constexpr (WK > 1) {
+    static_assert(WC == 1, "the waves' results lie one behind another");
+    add_waves<WK, NC * DT>(lds, wk, lane, [&](int k) -> f32x4 & { return ak[k / DT][k % DT]; });
+    add_waves<WK, NC * DT>(lds, wk, lane, [&](int k) -> f32x4 & { return av[k / DT][k % DT]; });
+    if (wk) return;
+  }
+  const int64_t keys = (int64_t)p.heads * p.Sk;
+  const int64_t key0 = (int64_t)(w.item * p.Hk + h) * p.Sk + w.k0;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int j = j0 + n * 16 + i;
+    if (j >= w.rows) continue;
+    const bool in = j < w.nk;   // keys that do not count, whose operands are 0, have gathered exp(0) all the same
+    if (p.splits > 1) {
+      const int64_t at = (part * keys + key0 + j) * 2;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        *reinterpret_cast<f32x4 *>(p.part + at * DP + d * 16 + q * 4) = in ? ak[n][d] : f32x4{0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<f32x4 *>(p.part + (at + 1) * DP + d * 16 + q * 4) = in ? av[n][d] * kDown : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      continue;
+    }
+    const auto row = [&](const Tensor &x) { return static_cast<T *>(x.p) + w.item * x.item + (w.k0 + j) * x.token + h * x.head; };
+    T *const gk = row(p.gk), *const gv = row(p.gv);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      store4(gk, d * 16 + q * 4, in ? ak[n][d] * p.scale : f32x4{0.f, 0.f, 0.f, 0.f}, p.D);
+      store4(gv, d * 16 + q * 4, in ? av[n][d] * kDown : f32x4{0.f, 0.f, 0.f, 0.f}, p.D);
+    }
+  }
+}
+
+// Sums of parts: of grad q (KEYS false), a row a cell; of grad k and grad v, two rows a key.  A wave each.
+template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void join_sum_kernel(Args p) {
+  const int per = KEYS ? p.Sk : p.Sq * p.G;
+  const int64_t n = (int64_t)p.heads * per * (KEYS ? 2 : 1);
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= n) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = KEYS ? at >> 1 : at;
+  const int ih = (int)(row / per), c = (int)(row - (int64_t)ih * per), item = ih / p.Hk, h = ih - item * p.Hk;
+  const bool value = KEYS && (at & 1);
+  const Tensor &x = KEYS ? (value ? p.gv : p.gk) : p.gq;
+  const int t = KEYS ? c : divide(p, c), head = KEYS ? h : h * p.G + c - t * p.G;
+  T *to = static_cast<T *>(x.p) + item * x.item + t * x.token + head * x.head;
+  for (int d = lane; d < p.D; d += 64) {
+    float s = 0.f;
+    for (int z = 0; z < p.splits; ++z) s += p.part[(z * n + at) * DP + d];
+    to[d] = (T)(value ? s : s * p.scale);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Launches (attention_f32.hip and its like).  dp: the padded number of channels, 32, 64 or 128.
+enum Shape { kMany = 0, kSome = 1, kFew = 2 };   // columns of a block: 128, 64 or 16
+template <typename T, int DP, typename F> hipError_t with_shape(int shape, F f) {
+  constexpr int E = (int)sizeof(T) / 2;   // stages of as many bytes in each type
+  if (shape == kMany) return f(std::integral_constant<int, 2>(), std::integral_constant<int, 4>(), std::integral_constant<int, 1>(), std::integral_constant<int, 64 / E>());
+  if (shape == kSome) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 4>(), std::integral_constant<int, 1>(), std::integral_constant<int, 64 / E>());
+  return f(std::integral_constant<int, 1>(), std::integral_constant<int, 1>(), std::integral_constant<int, 4>(), std::integral_constant<int, 128 / E>());
+}
+template <typename F> hipError_t with_dim(int dp, F f) {
+  if (dp == 32) return f(std::integral_constant<int, 32>());
+  if (dp == 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+inline unsigned blocks_of(const Args &p) { return (unsigned)((int64_t)p.tiles * p.splits * p.Hk); }
+
+template <typename T> hipError_t forward(const Args &p, int dp, int shape, hipStream_t st) {
+  return with_dim(dp, [&](auto d) {
+    constexpr int DP = decltype(d)::value;
+    return with_shape<T, DP>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
+      constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
+      forward_kernel<T, DP, NC, WC, WK, KT><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      if (p.splits > 1) join_forward_kernel<T, DP><<<(unsigned)((p.cells + 3) / 4), 256, 0, st>>>(p);
+      return hipGetLastError();
+    });
+  });
+}
+template <typename T> hipError_t grad_q(const Args &p, int dp, int shape, hipStream_t st) {
+  return with_dim(dp, [&](auto d) {
+    constexpr int DP = decltype(d)::value;
+    return with_shape<T, DP>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
+      constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
+      grad_q_kernel<T, DP, NC, WC, WK, KT><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      if (p.splits > 1) join_sum_kernel<T, DP, false><<<(unsigned)((p.cells + 3) / 4), 256, 0, st>>>(p);
+      return hipGetLastError();
+    });
+  });
+}
+template <typename T> hipError_t grad_kv(const Args &p, int dp, int shape, hipStream_t st) {
+  return with_dim(dp, [&](auto d) {
+    constexpr int DP = decltype(d)::value;
+    return with_shape<T, DP>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
+      constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
+      grad_kv_kernel<T, DP, NC, WC, WK, KT><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      const int64_t rows = (int64_t)p.heads * p.Sk * 2;
+      if (p.splits > 1) join_sum_kernel<T, DP, true><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(p);
+      return hipGetLastError();
+    });
+  });
+}
+
+// instantiated in attention_f32.hip, attention_f16.hip and attention_bf16.hip
+#define OPS3D_ATTENTION_TYPE(EXTERN, T)                                   \
+  EXTERN template hipError_t forward<T>(const Args &, int, int, hipStream_t); \
+  EXTERN template hipError_t grad_q<T>(const Args &, int, int, hipStream_t);  \
+  EXTERN template hipError_t grad_kv<T>(const Args &, int, int, hipStream_t);
+OPS3D_ATTENTION_TYPE(extern, float)
+OPS3D_ATTENTION_TYPE(extern, _Float16)
+OPS3D_ATTENTION_TYPE(extern, __bf16)
+
+}  // namespace ops3d_attention

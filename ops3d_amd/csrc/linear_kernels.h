@@ -24,10 +24,13 @@
 #include <type_traits>
 
 #include "elements.h"
+#include "segments.h"
 
 namespace ops3d_linear {
 
 using namespace ops3d_elements;
+using ops3d_segments::scan_add;
+using ops3d_segments::Segment;
 
 enum Act { kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4 };
 
@@ -195,38 +198,9 @@ template <bool FAST> __device__ __forceinline__ float activate(int act, float z,
 // ---------------------------------------------------------------------------------------------
 // groups
 
-// Inclusive scans over a wave.
-__device__ __forceinline__ int scan_add(int v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(v, o);
-    if ((int)(threadIdx.x & 63) >= o) v += t;
-  }
-  return v;
-}
-__device__ __forceinline__ int scan_max(int v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(v, o);
-    if ((int)(threadIdx.x & 63) >= o) v = max(v, t);
-  }
-  return v;
-}
-
-// Segments of an item: 0 the rows before the first group, e + 1 group e, E + 1 the rows behind the
-// last.  One step of a walk over them, 64 at a time, a segment per lane.
-struct Segment {
-  int lower, upper;   // rows
-};
+// One step of a walk over an item's segments (segments.h).
 __device__ __forceinline__ Segment segment_at(const Groups &g, int j, int &carry) {
-  int64_t v = j < g.count ? g.start[j] : (int64_t)g.S;
-  v = v < 0 ? 0 : (v > g.S ? g.S : v);
-  Segment s;
-  s.upper = max(scan_max((int)v), carry);
-  s.lower = __shfl_up(s.upper, 1);
-  if ((threadIdx.x & 63) == 0) s.lower = carry;
-  carry = __builtin_amdgcn_readlane(s.upper, 63);
-  return s;
+  return ops3d_segments::segment_at(g.start, g.count, g.S, j, carry);
 }
 
 struct RowTile {

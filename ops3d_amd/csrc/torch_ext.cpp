@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "../../include/ops3d_fda.h"
+#include "../../include/ops3d_attention.h"
 #include "../../include/ops3d_dcnv4.h"
 #include "../../include/ops3d_linear.h"
 #include "../../include/ops3d_nms3d.h"
@@ -956,6 +957,171 @@ at::Tensor rotary(const at::Tensor &x, const at::Tensor &positions, const std::v
   return rotary_apply(x, positions, frequencies, axis_of, layout, false);
 }
 
+// Attention over all tokens (include/ops3d_attention.h).  q [items, tokens, heads, dim], or without items
+// where sequences are packed or there is one.
+typedef c10::optional<at::Tensor> Maybe;
+
+struct Attention {
+  ops3d_attention_problem p;
+  at::Tensor q_start, k_start, q_len, k_len;   // kept while p points into them
+};
+
+const int64_t *attention_table(const Maybe &t, const char *name, const at::Tensor &q, at::Tensor &keep) {
+  if (!t) return nullptr;
+  if (!t->is_cuda()) throw std::runtime_error(std::string("Not implemented on the CPU (") + name + " is on the CPU)");
+  if (t->device() != q.device()) throw std::runtime_error(std::string(name) + " is on another device than q");
+  if (t->layout() != at::kStrided || t->scalar_type() != at::kLong || t->dim() != 1 || !t->is_contiguous())
+    throw std::invalid_argument(std::string(name) + " must be a contiguous int64 tensor of one axis");
+  keep = t->is_neg() ? t->resolve_neg() : *t;
+  return keep.data_ptr<int64_t>();
+}
+
+Attention attention_problem(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const Maybe &q_start,
+                            const Maybe &k_start, const Maybe &q_len, const Maybe &k_len, bool causal, double scale) {
+  linear_check(q, "q", q);
+  for (const auto &[t, name] : {std::make_pair(&k, "k"), std::make_pair(&v, "v")}) {
+    if (!t->is_cuda()) throw std::runtime_error(std::string("Not implemented on the CPU (") + name + " is on the CPU)");
+    if (t->layout() != at::kStrided) throw std::invalid_argument(std::string(name) + " must be a dense tensor");
+    if (t->device() != q.device()) throw std::runtime_error(std::string(name) + " is on another device than q");
+    if (t->scalar_type() != q.scalar_type()) throw std::invalid_argument(std::string(name) + " dtype differs from q dtype");
+  }
+  if (q.dim() != 3 && q.dim() != 4) throw std::invalid_argument("q must be [tokens, heads, dim] or [items, tokens, heads, dim]");
+  if (k.dim() != q.dim() || k.sizes() != v.sizes()) throw std::invalid_argument("k and v must have one shape, and q's axes");
+  if (k.size(-1) != q.size(-1)) throw std::invalid_argument("q and k differ in their channels");
+  if (q.dim() == 4 && k.size(0) != q.size(0)) throw std::invalid_argument("q and k differ in their items");
+  Attention a{};
+  a.p.dtype = dtype_code(q);
+  a.p.items = q.dim() == 4 ? linear_int(q.size(0), "the number of items") : 1;
+  a.p.q_rows = q.size(-3);
+  a.p.k_rows = k.size(-3);
+  a.p.heads = linear_int(q.size(-2), "the number of heads");
+  a.p.kv_heads = linear_int(k.size(-2), "the number of key heads");
+  a.p.dim = linear_int(q.size(-1), "the number of channels");
+  a.p.causal = causal;
+  a.p.scale = (float)scale;
+  if (q_start || k_start) {
+    if (q.dim() != 3) throw std::invalid_argument("packed sequences need q [tokens, heads, dim]");
+    if (!q_start || !k_start) throw std::invalid_argument("q_start and k_start go together");
+    if (q_len || k_len) throw std::invalid_argument("packed sequences have no q_len and k_len");
+  }
+  a.p.q_start = attention_table(q_start, "q_start", q, a.q_start);
+  a.p.k_start = attention_table(k_start, "k_start", q, a.k_start);
+  a.p.q_len = attention_table(q_len, "q_len", q, a.q_len);
+  a.p.k_len = attention_table(k_len, "k_len", q, a.k_len);
+  for (const Maybe *t : {&q_len, &k_len})
+    if (*t && (*t)->size(0) != a.p.items)
+      throw std::invalid_argument("q_len and k_len must have an entry for each of " + std::to_string(a.p.items) + " items");
+  if (q_start) {
+    const int64_t n = q_start->size(0);
+    if (n < 2 || n != k_start->size(0) || n > OPS3D_ATTENTION_MAX_SEQUENCES + 1)
+      throw std::invalid_argument("q_start and k_start must have an entry for each of 1.." +
+                                  std::to_string(OPS3D_ATTENTION_MAX_SEQUENCES) + " sequences and the last one's end, got " +
+                                  std::to_string(n) + " and " + std::to_string(k_start->size(0)));
+    a.p.q_start_count = a.p.k_start_count = (int)n;
+    a.p.sequences = (int)n - 1;
+  }
+  return a;
+}
+
+ops3d_attention_tensor attention_tensor(const at::Tensor &t) {
+  int64_t s[3];
+  strides_of(t, s);
+  return {ptr(t), s[0], s[1], s[2]};
+}
+
+// [out, lse]; lse (for the backward) when keep.
+std::tuple<at::Tensor, Maybe> attention_forward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                                                const Maybe &q_start, const Maybe &k_start, const Maybe &q_len,
+                                                const Maybe &k_len, bool causal, double scale, bool keep) {
+  const Attention a = attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale);
+  const DeviceGuard guard(q.device());
+  const at::Tensor qd = channels_dense(q), kd = channels_dense(k), vd = channels_dense(v);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  Maybe lse;
+  if (keep) lse = at::empty({a.p.items, a.p.heads, a.p.q_rows}, q.options().dtype(at::kFloat));
+  const size_t n = ops3d_attention_forward_workspace_bytes(&a.p);
+  at::Tensor ws;
+  if (n) ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
+  const auto tq = attention_tensor(qd), tk = attention_tensor(kd), tv = attention_tensor(vd), to = attention_tensor(out);
+  const int rc = ops3d_attention_forward(&a.p, &tq, &tk, &tv, &to, lse ? (float *)ptr(*lse) : nullptr, ptr(ws), n, stream_of(q));
+  if (rc != OPS3D_FDA_OK) raise(rc, "attention_forward failed");
+  return {out, lse};
+}
+
+// [grad_q, grad_k, grad_v], None where not wanted (the latter two together).
+std::tuple<Maybe, Maybe, Maybe> attention_backward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                                                   const Maybe &q_start, const Maybe &k_start, const Maybe &q_len,
+                                                   const Maybe &k_len, bool causal, double scale, const at::Tensor &out,
+                                                   const at::Tensor &lse, const at::Tensor &grad_out, bool need_q, bool need_kv) {
+  const Attention a = attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale);
+  linear_check(grad_out, "grad_output", q);
+  if (grad_out.sizes() != q.sizes()) throw std::invalid_argument("grad_output must have the output's shape");
+  if (out.device() != q.device() || out.scalar_type() != q.scalar_type() || out.sizes() != q.sizes() || !out.is_contiguous() ||
+      lse.device() != q.device() || lse.scalar_type() != at::kFloat || !lse.is_contiguous() ||
+      lse.sizes() != at::IntArrayRef({a.p.items, a.p.heads, a.p.q_rows}))
+    throw std::invalid_argument("out and lse are not a forward's of this shape");
+  const DeviceGuard guard(q.device());
+  const at::Tensor qd = channels_dense(q), kd = channels_dense(k), vd = channels_dense(v), gd = channels_dense(grad_out);
+  Maybe gq, gk, gv;
+  if (need_q) gq = at::empty(q.sizes(), q.options());
+  if (need_kv) gk = at::empty(k.sizes(), q.options()), gv = at::empty(k.sizes(), q.options());
+  const size_t n = ops3d_attention_backward_workspace_bytes(&a.p);
+  at::Tensor ws;
+  if (n) ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
+  const auto some = [](const Maybe &t) { return t ? attention_tensor(*t) : ops3d_attention_tensor{}; };
+  const auto tq = attention_tensor(qd), tk = attention_tensor(kd), tv = attention_tensor(vd), to = attention_tensor(out),
+             tg = attention_tensor(gd), tgq = some(gq), tgk = some(gk), tgv = some(gv);
+  const int rc = ops3d_attention_backward(&a.p, &tq, &tk, &tv, &to, (const float *)ptr(lse), &tg, need_q ? &tgq : nullptr,
+                                          need_kv ? &tgk : nullptr, need_kv ? &tgv : nullptr, ptr(ws), n, stream_of(q));
+  if (rc != OPS3D_FDA_OK) raise(rc, "attention_backward failed");
+  return {gq, gk, gv};
+}
+
+class AttentionNode : public torch::autograd::Function<AttentionNode> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                            const Maybe &q_start, const Maybe &k_start, const Maybe &q_len, const Maybe &k_len, bool causal,
+                            double scale) {
+    auto [out, lse] = attention_forward(q, k, v, q_start, k_start, q_len, k_len, causal, scale, true);
+    const auto some = [](const Maybe &t) { return t ? *t : at::Tensor(); };
+    ctx->save_for_backward({q, k, v, some(q_start), some(k_start), some(q_len), some(k_len), out, *lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["needs"] = std::vector<int64_t>{q.requires_grad(), k.requires_grad(), v.requires_grad()};
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const auto needs = ctx->saved_data["needs"].toIntVector();
+    const auto some = [&](int i) { return s[i].defined() ? Maybe(s[i]) : c10::nullopt; };
+    const bool gq = needs[0] && ctx->needs_input_grad(0), gk = needs[1] && ctx->needs_input_grad(1),
+               gv = needs[2] && ctx->needs_input_grad(2);
+    torch::autograd::variable_list out(9);
+    if (gq || gk || gv) {
+      const at::NoGradGuard no_grad;
+      auto [dq, dk, dv] = attention_backward(s[0], s[1], s[2], some(3), some(4), some(5), some(6), ctx->saved_data["causal"].toBool(),
+                                             ctx->saved_data["scale"].toDouble(), s[7], s[8], grads[0], gq, gk || gv);
+      if (gq) out[0] = *dq;
+      if (gk) out[1] = *dk;
+      if (gv) out[2] = *dv;
+    }
+    const bool given = grads[0].requires_grad();
+    once(out[0], true, "attention");
+    once(out[1], true, "attention");
+    once(out[2], needs[0] || needs[1] || given, "attention");
+    return out;
+  }
+};
+
+at::Tensor attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const Maybe &q_start, const Maybe &k_start,
+                     const Maybe &q_len, const Maybe &k_len, bool causal, double scale) {
+  refuse_trace("packed_attention");
+  for (const at::Tensor *t : {&q, &k, &v}) refuse_tangent(*t, "packed_attention has");
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return AttentionNode::apply(q, k, v, q_start, k_start, q_len, k_len, causal, scale);
+  return std::get<0>(attention_forward(q, k, v, q_start, k_start, q_len, k_len, causal, scale, false));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -981,6 +1147,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_forward", &layer_norm_forward, "layer norm over the last axis, and its statistics");
   m.def("layer_norm", &layer_norm, "layer_norm_forward with its gradients through autograd");
   m.def("layer_norm_backward", &layer_norm_backward, "gradients of layer_norm_forward");
+  m.def("attention_forward", &attention_forward, "attention over all tokens, and its statistics");
+  m.def("attention", &attention, "attention_forward with its gradients through autograd");
+  m.def("attention_backward", &attention_backward, "gradients of attention_forward");
   m.def("rotary_apply", &rotary_apply, "pairs of channels turned by their token's position, or back");
   m.def("rotary", &rotary, "rotary_apply with its gradient through autograd");
   m.def("roi_align_3d_forward", &roi_align_3d_forward, "roi_align_3d_forward");
