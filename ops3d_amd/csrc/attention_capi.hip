@@ -150,6 +150,14 @@ Args args_of(const ops3d_attention_problem *p) {
   return a;
 }
 
+// Whether a stage's rows may go straight to LDS: whole padded rows at 16-byte boundaries, whose places in a stage of
+// 128 and in a group of heads fit 32 bits.
+bool direct(const ops3d_attention_problem *p, const Tensor &t) {
+  const int64_t es = elem_size(p->dtype);
+  return p->dim == padded_dim(p->dim) && !((reinterpret_cast<uintptr_t>(t.p) | (uint64_t)(t.item * es) | (uint64_t)(t.token * es) | (uint64_t)(t.head * es)) & 15u) &&
+         t.token < (1 << 20) && t.head < (1 << 20) && p->heads / p->kv_heads <= 256;   // 2^31 bytes, of 4 an element
+}
+
 template <typename F> int run(int dtype, const char *what, F f) {
   const hipError_t e = dtype == OPS3D_FDA_F32 ? f(float()) : dtype == OPS3D_FDA_F16 ? f(_Float16()) : f(__bf16());
   if (e == hipSuccess) return OPS3D_FDA_OK;
@@ -197,6 +205,7 @@ int ops3d_attention_forward(const ops3d_attention_problem *problem, const ops3d_
   const Plan plan = plan_queries(problem);
   if (!set_plan(a, problem, plan)) return fail(OPS3D_FDA_EINVAL, "attention: 2^31 tiles or more");
   const int dp = padded_dim(problem->dim);
+  a.dma = direct(problem, a.k) && direct(problem, a.v) ? 1 : 0;
   a.part = static_cast<float *>(workspace);
   a.part_ml = a.part + (size_t)a.splits * a.cells * dp;
   return run(problem->dtype, "attention forward",
@@ -235,6 +244,7 @@ int ops3d_attention_backward(const ops3d_attention_problem *problem, const ops3d
   a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + align256((size_t)cells * 4));
   const int dp = padded_dim(problem->dim);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  a.dma = (keys && direct(problem, a.k) && direct(problem, a.v) ? 1 : 0) | (cells && direct(problem, a.q) && direct(problem, a.g) ? 2 : 0);
   if (cells) {
     const Plan plan = plan_queries(problem);
     if (!set_plan(a, problem, plan)) return fail(OPS3D_FDA_EINVAL, "attention: 2^31 tiles or more");

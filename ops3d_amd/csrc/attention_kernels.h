@@ -46,6 +46,7 @@ struct Args {
   uint32_t magic;                     // c / G = 2 c magic >> 32 >> shift
   int shift;
   int causal;
+  int dma;                            // rows go straight to LDS: bit 0 k and v, bit 1 q and grad_out
   float scale, c;                     // c = scale log2 e
   int tiles, tiles_item, splits;      // tiles of all items (a bound), of one, and parts of the other side
   int heads;                          // items Hk
@@ -62,14 +63,13 @@ struct Work {
   int first;             // first owned column
 };
 
-// Tile t of `per` columns.  KEYS: columns are keys, otherwise queries times heads.
-template <bool KEYS> __device__ __forceinline__ bool locate(const Args &p, int t, int per, Work &w) {
+template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, int t, int per, Work &w) {
   const int unit = KEYS ? 1 : p.G;
   if (!p.q_start) {
     const int e = t / p.tiles_item;
     w.item = e;
     w.q0 = w.k0 = 0;
-    const auto held = [](const int64_t *len, int e, int rows) {
+    const auto held = [](const int64_t *len, int e, int rows) __attribute__((always_inline)) {
       if (!len) return rows;
       const int64_t v = len[e];
       return v < 0 ? 0 : (int)(v < rows ? v : rows);
@@ -123,6 +123,16 @@ template <bool KEYS> __device__ __forceinline__ bool locate(const Args &p, int t
   return true;
 }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Tile t of `per` columns, the same for the block.  KEYS: columns are keys, otherwise queries times heads.
+template <bool KEYS> __device__ __forceinline__ bool locate(const Args &p, int t, int per, Work &w) {
+  Work v{};
+  if (!find_work<KEYS>(p, t, per, v)) return false;
+  w = Work{uniform(v.item), uniform(v.q0), uniform(v.k0), uniform(v.nq), uniform(v.nk), uniform(v.rows), uniform(v.first)};
+  return true;
+}
+
 __device__ __forceinline__ int divide(const Args &p, int c) { return (int)(__umulhi((uint32_t)c << 1, p.magic) >> p.shift); }
 
 // A stage of R rows of DP elements in LDS, in 16-byte chunks, XOR-swizzled: 8 rows that follow each other and
@@ -142,14 +152,43 @@ template <typename T, int DP, int R, int NT> struct Stage {
   static __device__ __forceinline__ int row_of(int i) { return (int)(threadIdx.x + i * NT) / RC; }
   static __device__ __forceinline__ int chunk_of(int i) { return (int)(threadIdx.x + i * NT) % RC; }
 
-  // at(row): the row's first element; zeros from row n on and behind D.
+  // at(row): the row's first element; zeros from row n on and behind D.  n > 0.  Whole chunks are loaded without
+  // branches, those outside from the last row's or the row's last place.
   template <typename F> static __device__ __forceinline__ void load(uint4 (&v)[NL], F at, int n, int D) {
+    if (D % CH == 0) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) v[i] = load16(at(min(row_of(i), n - 1)) + min(chunk_of(i) * CH, D - CH));
+      if (n < R || D < DP) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+          if (row_of(i) >= n || chunk_of(i) * CH >= D) v[i] = make_uint4(0, 0, 0, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int row = row_of(i), col = chunk_of(i) * CH;
       v[i] = make_uint4(0, 0, 0, 0);
       if (row < n && col < D) v[i] = fetch(at(row), 0, 0, col, 1, D);
     }
+  }
+  // The same without registers between: an instruction of a wave fills 1024 bytes of LDS in lane order, so the
+  // lane at a place loads the chunk that the swizzle puts there.  For D = DP and rows that start at 16-byte
+  // boundaries.  off: the lanes' places, in bytes, of rows at at(row); rows from n on are the last one again.
+  template <typename F> static __device__ __forceinline__ void places(uint32_t (&off)[NL], F at, int n) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int slot = (wave * NL + i) * 64 + lane, row = slot / RC, chunk = (address(row, slot % RC) >> 4) - row * RC;
+      off[i] = at(min(row, n - 1)) + chunk * 16;
+    }
+  }
+  static __device__ __forceinline__ void load_lds(char *lds, const char *base, const uint32_t (&off)[NL]) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + off[i]),
+                                       (__attribute__((address_space(3))) void *)(lds + (wave * NL + i) * 1024), 16, 0, 0);
   }
   static __device__ __forceinline__ void store(char *lds, const uint4 (&v)[NL]) {
 #pragma unroll
@@ -255,8 +294,8 @@ template <int WK, int N, typename F> __device__ __forceinline__ void add_waves(c
 
 // ---------------------------------------------------------------------------------------------
 // Forward: WC waves of NC x 16 columns side by side, and WK of them that share out each stage's KT keys.
-template <typename T, int DP, int NC, int WC, int WK, int KT>
-__global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
+template <typename T, int DP, int NC, int WC, int WK, int KT, int OCC, bool DMA>
+__global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC))) void forward_kernel(Args p) {
   constexpr int NT = 64 * WC * WK, BM = WC * NC * 16, KW = KT / WK, KN = KW / 16;
   constexpr int STEPS = DP * (int)sizeof(T) / 64, DT = DP / 16, PR = sizeof(T) == 2 ? 2 : 1;   // tiles an operand holds
   typedef Stage<T, DP, KT, NT> ST;
@@ -278,20 +317,17 @@ __global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
 
   typename Type<T>::frag qf[NC][STEPS];
   int limit[NC];   // keys that the column sees; those of columns that do not count are not held back
-  int least = w.nk;
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     const int c = c0 + n * 16 + i, t = divide(p, c);
     load_column<T, STEPS>(qf[n], c < active ? qb + t * p.q.token + (c - t * p.G) * p.q.head : nullptr, p.D, q);
     limit[n] = p.causal && c < active ? min(w.nk, t + off + 1) : w.nk;
-    least = min(least, limit[n]);
   }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
-  least = __builtin_amdgcn_readfirstlane(least);
+  // what every column of the block sees: its first column's keys
+  const int least = uniform(p.causal ? min(w.nk, max(0, divide(p, w.first) + off + 1)) : w.nk);
   // keys that any column of the block sees, and this part of them
   int keys = w.first < active ? w.nk : 0;
-  if (p.causal && keys) keys = max(0, min(keys, divide(p, min(active, w.first + BM) - 1) + off + 1));
+  if (p.causal && keys) keys = uniform(max(0, min(keys, divide(p, min(active, w.first + BM) - 1) + off + 1)));
   int k_begin = 0, k_end = keys;
   if (p.splits > 1) {
     const int per = ((keys + KT - 1) / KT + p.splits - 1) / p.splits * KT;
@@ -299,34 +335,55 @@ __global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
     k_end = min(keys, k_begin + per);
   }
 
-  f32x4 o[NC][DT];
-  float m[NC], mc[NC], l[NC], top[NC];   // reference, the same times c, sum (this lane's rows), what raises it
+  f32x4 o[NC][DT], sum[NC];                // sums of P V and of P (SUMS: by the matrix units, from the rounded P)
+  float m[NC], mc[NC], l[NC], top[NC];     // reference, the same times c, sum of P (this lane's rows), what raises it
+  constexpr bool SUMS = sizeof(T) == 2;
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     m[n] = top[n] = -INFINITY;
     mc[n] = -Range<T>::kShift;
     l[n] = 0.f;
+    sum[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float slack = Range<T>::kSlack / p.c;
 
-  uint4 kv[ST::NL], vv[ST::NL];
-  const auto load = [&](int k0) {
+  uint4 kv[DMA ? 1 : ST::NL], vv[DMA ? 1 : ST::NL];
+  uint32_t k_off[DMA ? ST::NL : 1], v_off[DMA ? ST::NL : 1];
+  if constexpr (DMA) {
+    ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, KT);
+    ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, KT);
+  }
+  const auto load = [&](int k0, int buf) __attribute__((always_inline)) {
     const int left = k_end - k0;
-    ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
-    ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
+    if constexpr (DMA) {
+      char *const lk = lds + buf * 2 * ST::kBytes;
+      if (left < KT) {
+        ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, left);
+        ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, left);
+      }
+      ST::load_lds(lk, reinterpret_cast<const char *>(kb + k0 * p.k.token), k_off);
+      ST::load_lds(lk + ST::kBytes, reinterpret_cast<const char *>(vb + k0 * p.v.token), v_off);
+    } else {
+      ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
+      ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
+    }
   };
-  if (k_begin < k_end) load(k_begin);
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += KT, buf ^= 1) {
+  const int r0 = wk * KW;
+  int k0 = k_begin, buf = 0;
+  const auto stage = [&](auto masked) __attribute__((always_inline)) {
     char *const lk = lds + buf * 2 * ST::kBytes, *const lv = lk + ST::kBytes;
-    ST::store(lk, kv);
-    ST::store(lv, vv);
-    if (k0 + KT < k_end) load(k0 + KT);
-    __syncthreads();   // the other buffer's readers are past the barrier before
+    if constexpr (!DMA) {
+      ST::store(lk, kv);
+      ST::store(lv, vv);
+      if (k0 + KT < k_end) load(k0 + KT, 0);
+      __syncthreads();   // the other buffer's readers are past the barrier before
+    } else {
+      __syncthreads();   // this stage has arrived, and the other buffer's readers are done
+      if (k0 + KT < k_end) load(k0 + KT, buf ^ 1);
+    }
 
-    const int r0 = wk * KW;
     f32x4 s[NC][KN];
 #pragma unroll
     for (int kt = 0; kt < KN; ++kt) {
@@ -339,15 +396,14 @@ __global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
         for (int n = 0; n < NC; ++n) s[n][kt] = Type<T>::mma(kf, qf[n][st], s[n][kt]);
       }
     }
-    const int first = k0 + r0;
-    if (first + KW > least) {   // also keys behind the last
+    if constexpr (decltype(masked)::value) {   // also keys behind the last
 #pragma unroll
       for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int kt = 0; kt < KN; ++kt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (first + kt * 16 + q * 4 + j >= limit[n]) s[n][kt][j] = -INFINITY;
+            if (k0 + r0 + kt * 16 + q * 4 + j >= limit[n]) s[n][kt][j] = -INFINITY;
     }
     bool raise = false;
     float mx[NC];
@@ -367,6 +423,7 @@ __global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
         if (now != m[n]) {
           const float by = m[n] == -INFINITY ? 0.f : exp2_((m[n] - now) * p.c);
           l[n] *= by;
+          sum[n] *= by;
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[n][d] *= by;
           m[n] = now;
@@ -376,19 +433,20 @@ __global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
       }
     }
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-      for (int kt = 0; kt < KN; ++kt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[n][kt][j] = exp2_(fmaf(s[n][kt][j], p.c, -mc[n]));
-          l[n] += s[n][kt][j];
-        }
-#pragma unroll
     for (int kt = 0; kt < KN; kt += PR) {
       typename Type<T>::frag pf[NC];
 #pragma unroll
-      for (int n = 0; n < NC; ++n) pf[n] = operand<T>(&s[n][kt]);
+      for (int n = 0; n < NC; ++n) {
+#pragma unroll
+        for (int u = 0; u < PR; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[n][kt + u][j] = exp2_(fmaf(s[n][kt + u][j], p.c, -mc[n]));
+            if (!SUMS) l[n] += s[n][kt + u][j];
+          }
+        pf[n] = operand<T>(&s[n][kt]);
+        if (SUMS) sum[n] = Type<T>::mma(Type<T>::ones(), pf[n], sum[n]);
+      }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const auto vf = ST::columns(lv, r0 + kt * 16, d, lane);
@@ -396,9 +454,15 @@ __global__ __launch_bounds__(64 * WC *WK) void forward_kernel(Args p) {
         for (int n = 0; n < NC; ++n) o[n][d] = Type<T>::mma(vf, pf[n], o[n][d]);
       }
     }
-  }
+    buf ^= 1;
+    k0 += KT;
+  };
+  if (k_begin < k_end) load(k_begin, 0);
+  while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
+  while (k0 < k_end) stage(std::true_type());
 #pragma unroll
-  for (int n = 0; n < NC; ++n) l[n] = ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(l[n]));
+  for (int n = 0; n < NC; ++n)
+    l[n] = SUMS ? sum[n][0] : ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(l[n]));
 
   if constexpr (WK > 1) {   // the waves' shares, each with its own reference
     f32x4 *x = reinterpret_cast<f32x4 *>(lds);
@@ -488,8 +552,8 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void join_forwar
 
 // ---------------------------------------------------------------------------------------------
 // Gradient of the queries, and delta = sum of o grad_out, which the keys' needs (gq NULL: that alone).
-template <typename T, int DP, int NC, int WC, int WK, int KT>
-__global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
+template <typename T, int DP, int NC, int WC, int WK, int KT, int OCC, bool DMA>
+__global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC))) void grad_q_kernel(Args p) {
   constexpr int NT = 64 * WC * WK, BM = WC * NC * 16, KW = KT / WK, KN = KW / 16;
   constexpr int STEPS = DP * (int)sizeof(T) / 64, DT = DP / 16, PR = sizeof(T) == 2 ? 2 : 1, CH = 16 / (int)sizeof(T);
   typedef Stage<T, DP, KT, NT> ST;
@@ -510,13 +574,13 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
   const int64_t cell0 = ((int64_t)(w.item * p.Hk + h) * p.Sq + w.q0) * p.G;
 
   typename Type<T>::frag qf[NC][STEPS], gf[NC][STEPS];
-  int limit[NC], least = w.nk;
+  int limit[NC];
   float lse[NC], delta[NC];
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     const int c = c0 + n * 16 + i, t = divide(p, c), head = h * p.G + c - t * p.G;
     const bool in = c < active;
-    const auto row = [&](const Tensor &x) {
+    const auto row = [&](const Tensor &x) __attribute__((always_inline)) {
       return in ? static_cast<const T *>(x.p) + w.item * x.item + (w.q0 + t) * x.token + head * x.head : nullptr;
     };
     load_column<T, STEPS>(qf[n], row(p.q), p.D, q);
@@ -532,14 +596,11 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
     lse[n] = in ? p.lse[cell0 + c] : INFINITY;
     if (c < w.rows * p.G && q == 0 && wk == 0 && part == 0) p.delta[cell0 + c] = delta[n];
     limit[n] = p.causal && in ? min(w.nk, t + off + 1) : w.nk;
-    least = min(least, limit[n]);
   }
   if (!p.gq.p) return;
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
-  least = __builtin_amdgcn_readfirstlane(least);
+  const int least = uniform(p.causal ? min(w.nk, max(0, divide(p, w.first) + off + 1)) : w.nk);
   int keys = w.first < active ? w.nk : 0;
-  if (p.causal && keys) keys = max(0, min(keys, divide(p, min(active, w.first + BM) - 1) + off + 1));
+  if (p.causal && keys) keys = uniform(max(0, min(keys, divide(p, min(active, w.first + BM) - 1) + off + 1)));
   int k_begin = 0, k_end = keys;
   if (p.splits > 1) {
     const int per = ((keys + KT - 1) / KT + p.splits - 1) / p.splits * KT;
@@ -552,22 +613,40 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
   for (int n = 0; n < NC; ++n)
 #pragma unroll
     for (int d = 0; d < DT; ++d) a[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  uint4 kv[ST::NL], vv[ST::NL];
-  const auto load = [&](int k0) {
+  uint4 kv[DMA ? 1 : ST::NL], vv[DMA ? 1 : ST::NL];
+  uint32_t k_off[DMA ? ST::NL : 1], v_off[DMA ? ST::NL : 1];
+  if constexpr (DMA) {
+    ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, KT);
+    ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, KT);
+  }
+  const auto load = [&](int k0, int buf) __attribute__((always_inline)) {
     const int left = k_end - k0;
-    ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
-    ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
+    if constexpr (DMA) {
+      char *const lk = lds + buf * 2 * ST::kBytes;
+      if (left < KT) {
+        ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, left);
+        ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, left);
+      }
+      ST::load_lds(lk, reinterpret_cast<const char *>(kb + k0 * p.k.token), k_off);
+      ST::load_lds(lk + ST::kBytes, reinterpret_cast<const char *>(vb + k0 * p.v.token), v_off);
+    } else {
+      ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
+      ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
+    }
   };
-  if (k_begin < k_end) load(k_begin);
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += KT, buf ^= 1) {
+  const int r0 = wk * KW;
+  int k0 = k_begin, buf = 0;
+  const auto stage = [&](auto masked) __attribute__((always_inline)) {
     char *const lk = lds + buf * 2 * ST::kBytes, *const lv = lk + ST::kBytes;
-    ST::store(lk, kv);
-    ST::store(lv, vv);
-    if (k0 + KT < k_end) load(k0 + KT);
-    __syncthreads();
-    const int r0 = wk * KW, first = k0 + r0;
-    const bool mask = first + KW > least;
+    if constexpr (!DMA) {
+      ST::store(lk, kv);
+      ST::store(lv, vv);
+      if (k0 + KT < k_end) load(k0 + KT, 0);
+      __syncthreads();
+    } else {
+      __syncthreads();
+      if (k0 + KT < k_end) load(k0 + KT, buf ^ 1);
+    }
 #pragma unroll
     for (int kt = 0; kt < KN; kt += PR) {
       f32x4 s[NC][PR], dp[NC][PR];
@@ -593,7 +672,7 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float x = exp2_(fmaf(s[n][u][j], p.c, -lse[n])) * (dp[n][u][j] - delta[n]);
-            if (mask && first + (kt + u) * 16 + q * 4 + j >= limit[n]) x = 0.f;
+            if (decltype(masked)::value && k0 + r0 + (kt + u) * 16 + q * 4 + j >= limit[n]) x = 0.f;
             s[n][u][j] = x;
           }
         ds[n] = operand<T>(s[n]);
@@ -605,7 +684,12 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
         for (int n = 0; n < NC; ++n) a[n][d] = Type<T>::mma(kf, ds[n], a[n][d]);
       }
     }
-  }
+    buf ^= 1;
+    k0 += KT;
+  };
+  if (k_begin < k_end) load(k_begin, 0);
+  while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
+  while (k0 < k_end) stage(std::true_type());
   if constexpr (WK > 1) {
     static_assert(WC == 1, "the waves' results lie one behind another");
     add_waves<WK, NC * DT>(lds, wk, lane, [&](int k) -> f32x4 & { return a[k / DT][k % DT]; });
@@ -630,8 +714,8 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_q_kernel(Args p) {
 
 // ---------------------------------------------------------------------------------------------
 // Gradients of keys and values.
-template <typename T, int DP, int NC, int WC, int WK, int QT>
-__global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
+template <typename T, int DP, int NC, int WC, int WK, int QT, int OCC, bool DMA>
+__global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC))) void grad_kv_kernel(Args p) {
   constexpr int NT = 64 * WC * WK, BN = WC * NC * 16, QW = QT / WK, QN = QW / 16;
   constexpr int STEPS = DP * (int)sizeof(T) / 64, DT = DP / 16, PR = sizeof(T) == 2 ? 2 : 1;
   typedef Stage<T, DP, QT, NT> ST;
@@ -648,7 +732,7 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
   const int wc = wave % WC, wk = wave / WC;
   const int active = w.nq * p.G, off = w.nk - w.nq, j0 = w.first + wc * NC * 16;
-  const auto rows_of = [&](const Tensor &x) { return static_cast<const T *>(x.p) + w.item * x.item + w.q0 * x.token + (int64_t)h * p.G * x.head; };
+  const auto rows_of = [&](const Tensor &x) __attribute__((always_inline)) { return static_cast<const T *>(x.p) + w.item * x.item + w.q0 * x.token + (int64_t)h * p.G * x.head; };
   const T *qb = rows_of(p.q), *gb = rows_of(p.g);
   const int64_t cell0 = ((int64_t)(w.item * p.Hk + h) * p.Sq + w.q0) * p.G;
 
@@ -657,17 +741,18 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     const int j = j0 + n * 16 + i;
-    const auto row = [&](const Tensor &x) {
+    const auto row = [&](const Tensor &x) __attribute__((always_inline)) {
       return j < w.nk ? static_cast<const T *>(x.p) + w.item * x.item + (w.k0 + j) * x.token + h * x.head : nullptr;
     };
     load_column<T, STEPS>(kf[n], row(p.k), p.D, q);
     load_column<T, STEPS>(vf[n], row(p.v), p.D, q);
     since[n] = p.causal ? (int)min((int64_t)active, max((int64_t)0, (int64_t)(j - off) * p.G)) : 0;
   }
-  const int last = j0 + NC * 16 - 1;   // of this wave
-  const int all_see = p.causal ? (int)min((int64_t)active, max((int64_t)0, (int64_t)(last - off) * p.G)) : 0;
+  const int last = w.first + BN - 1;   // of this block
+  const int all_see = !p.causal ? 0 : uniform( (int)min((int64_t)active, max((int64_t)0, (int64_t)(last - off) * p.G)));
   int begin = w.first < w.nk ? 0 : active;
   if (p.causal) begin = max(begin, (int)min((int64_t)active, max((int64_t)0, (int64_t)(w.first - off) * p.G)) / QT * QT);
+  begin = uniform(begin);
   int c_begin = begin, c_end = active;
   if (p.splits > 1) {
     const int per = ((active - begin + QT - 1) / QT + p.splits - 1) / p.splits * QT;
@@ -680,38 +765,59 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
   for (int n = 0; n < NC; ++n)
 #pragma unroll
     for (int d = 0; d < DT; ++d) ak[n][d] = av[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  uint4 qv[ST::NL], gv[ST::NL];
+  uint4 qv[DMA ? 1 : ST::NL], gv[DMA ? 1 : ST::NL];
+  uint32_t q_off[ST::NL], g_off[ST::NL];
   float row_lse = INFINITY, row_delta = 0.f;
-  const auto load = [&](int c0) {
-    const int left = c_end - c0;
-    const auto at = [&](const T *base, const Tensor &x, int r) {
-      const int t = divide(p, c0 + r);
-      return base + t * x.token + (c0 + r - t * p.G) * x.head;
+  const bool fixed = QT % p.G == 0;   // each stage starts at a query, and its rows lie as those of the one before
+  const auto place_rows = [&](int c0, int n) __attribute__((always_inline)) {
+    const int t0 = fixed ? 0 : uniform(divide(p, c0)), c = fixed ? 0 : c0 - t0 * p.G;
+    const auto at = [&](const Tensor &x, int r) __attribute__((always_inline)) {
+      const int t = divide(p, c + r);
+      return (uint32_t)((t * (uint32_t)x.token + (c + r - t * p.G) * (uint32_t)x.head) * sizeof(T));
     };
-    ST::load(qv, [&](int r) { return at(qb, p.q, r); }, left, p.D);
-    ST::load(gv, [&](int r) { return at(gb, p.g, r); }, left, p.D);
+    ST::places(q_off, [&](int r) { return at(p.q, r); }, n);
+    ST::places(g_off, [&](int r) { return at(p.g, r); }, n);
+  };
+  const auto load = [&](int c0, int buf) __attribute__((always_inline)) {
+    const int left = c_end - c0;
+    if constexpr (DMA) {
+      char *const lq = lds + buf * kStage;
+      const int t0 = uniform(divide(p, c0));
+      if (!fixed || left < QT) place_rows(c0, min(left, QT));
+      ST::load_lds(lq, reinterpret_cast<const char *>(qb + t0 * p.q.token), q_off);
+      ST::load_lds(lq + ST::kBytes, reinterpret_cast<const char *>(gb + t0 * p.g.token), g_off);
+    } else {
+      const auto at = [&](const T *base, const Tensor &x, int r) __attribute__((always_inline)) {
+        const int t = divide(p, c0 + r);
+        return base + t * x.token + (c0 + r - t * p.G) * x.head;
+      };
+      ST::load(qv, [&](int r) { return at(qb, p.q, r); }, left, p.D);
+      ST::load(gv, [&](int r) { return at(gb, p.g, r); }, left, p.D);
+    }
     if (threadIdx.x < QT) {
       const bool in = (int)threadIdx.x < left;   // P = 0 in the others
       row_lse = in ? p.lse[cell0 + c0 + threadIdx.x] : INFINITY;
       row_delta = in ? p.delta[cell0 + c0 + threadIdx.x] : 0.f;
     }
   };
-  if (c_begin < c_end) load(c_begin);
-  int buf = 0;
+  if constexpr (DMA) place_rows(0, QT);
   constexpr float kDown = sizeof(T) == 2 ? 1.f / (float)(1 << (int)Range<T>::kShift) : 1.f;
-  for (int c0 = c_begin; c0 < c_end; c0 += QT, buf ^= 1) {
+  const int r0 = wk * QW;
+  int c0 = c_begin, buf = 0;
+  const auto stage = [&](auto masked) __attribute__((always_inline)) {
     char *const lq = lds + buf * kStage, *const lg = lq + ST::kBytes;
     float *const ll = reinterpret_cast<float *>(lg + ST::kBytes), *const ld = ll + QT;
-    ST::store(lq, qv);
-    ST::store(lg, gv);
+    if constexpr (!DMA) {
+      ST::store(lq, qv);
+      ST::store(lg, gv);
+    }
     if (threadIdx.x < QT) {
       ll[threadIdx.x] = row_lse - Range<T>::kShift;
       ld[threadIdx.x] = row_delta;
     }
-    if (c0 + QT < c_end) load(c0 + QT);
+    if (!DMA && c0 + QT < c_end) load(c0 + QT, 0);
     __syncthreads();
-    const int r0 = wk * QW, first = c0 + r0;
-    const bool mask = first < all_see;
+    if (DMA && c0 + QT < c_end) load(c0 + QT, buf ^ 1);
 #pragma unroll
     for (int qt = 0; qt < QN; qt += PR) {
       f32x4 s[NC][PR], dp[NC][PR];
@@ -739,7 +845,7 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float x = exp2_(fmaf(s[n][u][j], p.c, -lse[j])), y = x * fmaf(dp[n][u][j], kDown, -kDown * delta[j]);
-            if (mask && c0 + r + j < since[n]) x = y = 0.f;
+            if (decltype(masked)::value && c0 + r + j < since[n]) x = y = 0.f;
             s[n][u][j] = x;
             dp[n][u][j] = y;
           }
@@ -757,7 +863,12 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
         }
       }
     }
-  }
+    buf ^= 1;
+    c0 += QT;
+  };
+  if (c_begin < c_end) load(c_begin, 0);
+  while (c0 < c_end && c0 < all_see) stage(std::true_type());
+  while (c0 < c_end) stage(std::false_type());
   if constexpr (WK > 1) {
     static_assert(WC == 1, "the waves' results lie one behind another");
     add_waves<WK, NC * DT>(lds, wk, lane, [&](int k) -> f32x4 & { return ak[k / DT][k % DT]; });
@@ -780,7 +891,7 @@ __global__ __launch_bounds__(64 * WC *WK) void grad_kv_kernel(Args p) {
       }
       continue;
     }
-    const auto row = [&](const Tensor &x) { return static_cast<T *>(x.p) + w.item * x.item + (w.k0 + j) * x.token + h * x.head; };
+    const auto row = [&](const Tensor &x) __attribute__((always_inline)) { return static_cast<T *>(x.p) + w.item * x.item + (w.k0 + j) * x.token + h * x.head; };
     T *const gk = row(p.gk), *const gv = row(p.gv);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -812,12 +923,24 @@ template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void 
 
 // ---------------------------------------------------------------------------------------------
 // Launches (attention_f32.hip and its like).  dp: the padded number of channels, 32, 64 or 128.
+// Waves a SIMD that a kernel's registers are to leave room for: two of 256 at least, whose results then stay in
+// registers that vector instructions read.
+enum Kernel { kforward, kgrad_q, kgrad_kv };
+template <typename T> constexpr int occupancy(Kernel k, int dp, int wk) {
+  if (dp <= 32) return 3;
+  if (dp <= 64) return 2;
+  return wk > 1 || sizeof(T) == 4 || k == kgrad_kv ? 1 : 2;
+}
+
 enum Shape { kMany = 0, kSome = 1, kFew = 2 };   // columns of a block: 128, 64 or 16
-template <typename T, int DP, typename F> hipError_t with_shape(int shape, F f) {
+template <typename T, int DP, Kernel kKernel, typename F> hipError_t with_shape(int shape, F f) {
+  typedef std::integral_constant<int, 1> one;
   constexpr int E = (int)sizeof(T) / 2;   // stages of as many bytes in each type
-  if (shape == kMany) return f(std::integral_constant<int, 2>(), std::integral_constant<int, 4>(), std::integral_constant<int, 1>(), std::integral_constant<int, 64 / E>());
-  if (shape == kSome) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 4>(), std::integral_constant<int, 1>(), std::integral_constant<int, 64 / E>());
-  return f(std::integral_constant<int, 1>(), std::integral_constant<int, 1>(), std::integral_constant<int, 4>(), std::integral_constant<int, 128 / E>());
+  typedef std::integral_constant<int, 64 / E> rows;
+  typedef std::integral_constant<int, 4> four;
+  if (shape == kMany) return f(std::integral_constant<int, 2>(), four(), one(), std::integral_constant<int, kKernel != kforward && DP == 128 ? 32 : 64 / E>());
+  if (shape == kSome) return f(one(), four(), one(), rows());
+  return f(one(), one(), four(), std::integral_constant<int, 128 / E>());
 }
 template <typename F> hipError_t with_dim(int dp, F f) {
   if (dp == 32) return f(std::integral_constant<int, 32>());
@@ -829,9 +952,11 @@ inline unsigned blocks_of(const Args &p) { return (unsigned)((int64_t)p.tiles * 
 template <typename T> hipError_t forward(const Args &p, int dp, int shape, hipStream_t st) {
   return with_dim(dp, [&](auto d) {
     constexpr int DP = decltype(d)::value;
-    return with_shape<T, DP>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
+    return with_shape<T, DP, kforward>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      forward_kernel<T, DP, NC, WC, WK, KT><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      constexpr int OCC = occupancy<T>(kforward, DP, WK);
+      if (p.dma & 1) forward_kernel<T, DP, NC, WC, WK, KT, OCC, true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      else forward_kernel<T, DP, NC, WC, WK, KT, OCC, false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
       if (p.splits > 1) join_forward_kernel<T, DP><<<(unsigned)((p.cells + 3) / 4), 256, 0, st>>>(p);
       return hipGetLastError();
     });
@@ -840,9 +965,11 @@ template <typename T> hipError_t forward(const Args &p, int dp, int shape, hipSt
 template <typename T> hipError_t grad_q(const Args &p, int dp, int shape, hipStream_t st) {
   return with_dim(dp, [&](auto d) {
     constexpr int DP = decltype(d)::value;
-    return with_shape<T, DP>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
+    return with_shape<T, DP, kgrad_q>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      grad_q_kernel<T, DP, NC, WC, WK, KT><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      constexpr int OCC = occupancy<T>(kgrad_q, DP, WK);
+      if (p.dma & 1) grad_q_kernel<T, DP, NC, WC, WK, KT, OCC, true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      else grad_q_kernel<T, DP, NC, WC, WK, KT, OCC, false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
       if (p.splits > 1) join_sum_kernel<T, DP, false><<<(unsigned)((p.cells + 3) / 4), 256, 0, st>>>(p);
       return hipGetLastError();
     });
@@ -851,9 +978,11 @@ template <typename T> hipError_t grad_q(const Args &p, int dp, int shape, hipStr
 template <typename T> hipError_t grad_kv(const Args &p, int dp, int shape, hipStream_t st) {
   return with_dim(dp, [&](auto d) {
     constexpr int DP = decltype(d)::value;
-    return with_shape<T, DP>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
+    return with_shape<T, DP, kgrad_kv>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      grad_kv_kernel<T, DP, NC, WC, WK, KT><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      constexpr int OCC = occupancy<T>(kgrad_kv, DP, WK);
+      if (p.dma & 2) grad_kv_kernel<T, DP, NC, WC, WK, KT, OCC, true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      else grad_kv_kernel<T, DP, NC, WC, WK, KT, OCC, false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
       const int64_t rows = (int64_t)p.heads * p.Sk * 2;
       if (p.splits > 1) join_sum_kernel<T, DP, true><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(p);
       return hipGetLastError();
