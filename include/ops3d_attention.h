@@ -59,11 +59,12 @@ typedef struct ops3d_attention_problem {
  * keys; 0 for other and for invalid sizes. */
 OPS3D_FDA_API size_t ops3d_attention_forward_workspace_bytes(const ops3d_attention_problem *problem);
 
-/* Writes every channel of out; lse [items, heads, q_rows] fp32 (in an order of the library's own), where
- * not NULL, is for the backward. */
+/* Writes every channel of out.  For the backward, where not NULL: lse [items, heads, q_rows] fp32 (in an order of
+ * the library's own), and out_rest [items, q_rows, heads, dim], contiguous, of dtype: what rounding took from
+ * out. */
 OPS3D_FDA_API int ops3d_attention_forward(const ops3d_attention_problem *problem, const ops3d_attention_tensor *q,
                                           const ops3d_attention_tensor *k, const ops3d_attention_tensor *v,
-                                          const ops3d_attention_tensor *out, float *lse, void *workspace,
+                                          const ops3d_attention_tensor *out, void *out_rest, float *lse, void *workspace,
                                           size_t workspace_bytes, void *stream);
 
 /* Bytes of device workspace (256-byte aligned) of the backward: the products of out with grad_out, and
@@ -71,10 +72,11 @@ OPS3D_FDA_API int ops3d_attention_forward(const ops3d_attention_problem *problem
 OPS3D_FDA_API size_t ops3d_attention_backward_workspace_bytes(const ops3d_attention_problem *problem);
 
 /* Writes every channel of grad_q, grad_k and grad_v; grad_q may be NULL, and grad_k and grad_v together:
- * not wanted.  Results are bitwise repeatable (no atomics). */
+ * not wanted.  out_rest may be NULL; with it, the products of out with grad_out are those of the unrounded
+ * output, and the gradients of logits are closer.  Results are bitwise repeatable (no atomics). */
 OPS3D_FDA_API int ops3d_attention_backward(const ops3d_attention_problem *problem, const ops3d_attention_tensor *q,
                                            const ops3d_attention_tensor *k, const ops3d_attention_tensor *v,
-                                           const ops3d_attention_tensor *out, const float *lse,
+                                           const ops3d_attention_tensor *out, const void *out_rest, const float *lse,
                                            const ops3d_attention_tensor *grad_out, const ops3d_attention_tensor *grad_q,
                                            const ops3d_attention_tensor *grad_k, const ops3d_attention_tensor *grad_v,
                                            void *workspace, size_t workspace_bytes, void *stream);

@@ -175,9 +175,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         size = getattr(lib, f"ops3d_attention_{name}_workspace_bytes")
         size.restype, size.argtypes = _sz, [problem]
     lib.ops3d_attention_forward.restype = _i
-    lib.ops3d_attention_forward.argtypes = [problem] + [tensor] * 4 + [_vp, _vp, _sz, _vp]
+    lib.ops3d_attention_forward.argtypes = [problem] + [tensor] * 4 + [_vp, _vp, _vp, _sz, _vp]
     lib.ops3d_attention_backward.restype = _i
-    lib.ops3d_attention_backward.argtypes = [problem] + [tensor] * 4 + [_vp] + [tensor] * 4 + [_vp, _sz, _vp]
+    lib.ops3d_attention_backward.argtypes = [problem] + [tensor] * 4 + [_vp, _vp] + [tensor] * 4 + [_vp, _sz, _vp]
     lib.ops3d_layer_norm_forward.restype = _i
     lib.ops3d_layer_norm_forward.argtypes = [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i64, _i, ctypes.c_float, _vp]
     lib.ops3d_layer_norm_backward_workspace_bytes.restype = _sz
@@ -653,21 +653,22 @@ class _NativeFDA:
         return self.attention_forward(*args, False)[0]
 
     def attention_forward(self, q, k, v, q_start, k_start, q_len, k_len, causal, scale, keep):
-        """(out, lse); lse (None otherwise) when ``keep``."""
+        """(out, lse, out_rest); the latter two (None otherwise, out_rest in 32 bits too) when ``keep``."""
         p = self._attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale)
         qd, kd, vd = (self._channels_dense(t) for t in (q, k, v))
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty((p.items, p.heads, p.q_rows), dtype=torch.float32, device=q.device) if keep else None
+        rest = torch.empty(q.shape, dtype=q.dtype, device=q.device) if keep and q.dtype != torch.float32 else None
         n = self._lib.ops3d_attention_forward_workspace_bytes(p)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         with torch.cuda.device(q.device):
-            rc = self._lib.ops3d_attention_forward(p, *(self._attention_tensor(t) for t in (qd, kd, vd, out)), _ptr(lse), _ptr(ws),
-                                                   n, torch.cuda.current_stream(q.device).cuda_stream)
+            rc = self._lib.ops3d_attention_forward(p, *(self._attention_tensor(t) for t in (qd, kd, vd, out)), _ptr(rest), _ptr(lse),
+                                                   _ptr(ws), n, torch.cuda.current_stream(q.device).cuda_stream)
         if rc != OPS3D_FDA_OK:
             self._raise(rc, "attention_forward failed")
-        return out, lse
+        return out, lse, rest
 
-    def attention_backward(self, q, k, v, q_start, k_start, q_len, k_len, causal, scale, out, lse, grad_out, need_q, need_kv):
+    def attention_backward(self, q, k, v, q_start, k_start, q_len, k_len, causal, scale, out, lse, rest, grad_out, need_q, need_kv):
         """(grad_q, grad_k, grad_v), None where not wanted (the latter two together)."""
         p = self._attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale)
         self._linear_check("grad_output", grad_out, q)
@@ -675,7 +676,9 @@ class _NativeFDA:
             raise ValueError("grad_output must have the output's shape")
         if (out.device != q.device or out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous()
                 or lse.device != q.device or lse.dtype != torch.float32 or not lse.is_contiguous()
-                or lse.shape != (p.items, p.heads, p.q_rows)):
+                or lse.shape != (p.items, p.heads, p.q_rows)
+                or rest is not None and (rest.device != q.device or rest.dtype != q.dtype or rest.shape != q.shape
+                                         or not rest.is_contiguous())):
             raise ValueError("out and lse are not a forward's of this shape")
         qd, kd, vd, gd = (self._channels_dense(t) for t in (q, k, v, grad_out))
         gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
@@ -684,7 +687,7 @@ class _NativeFDA:
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         with torch.cuda.device(q.device):
             rc = self._lib.ops3d_attention_backward(
-                p, *(self._attention_tensor(t) for t in (qd, kd, vd, out)), _ptr(lse),
+                p, *(self._attention_tensor(t) for t in (qd, kd, vd, out)), _ptr(rest), _ptr(lse),
                 *(self._attention_tensor(t) for t in (gd, gq, gk, gv)), _ptr(ws), n,
                 torch.cuda.current_stream(q.device).cuda_stream)
         if rc != OPS3D_FDA_OK:

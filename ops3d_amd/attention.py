@@ -5,7 +5,8 @@ No counterpart in the reference, whose attention samples a few places of the val
 also needs this one.  The heads of a group share a key head, sequences of different lengths run packed one
 behind another or as items of a batch that use some of their rows, and lengths are read on the device
 only, so no call waits for them.  Logits, statistics and sums are fp32; probabilities and the gradients of
-logits are rounded to the tensors' dtype before they are multiplied; each result is rounded once.
+logits are rounded to the tensors' dtype before they are multiplied; each result is rounded once.  For
+the backward the forward keeps, beside the output, what rounding took from it.
 Results are bitwise repeatable (csrc/attention_kernels.h).
 """
 from __future__ import annotations
@@ -24,18 +25,18 @@ class AttentionFunction(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, q_start, k_start, q_len, k_len, causal, scale, native):
-        out, lse = native.attention_forward(q, k, v, q_start, k_start, q_len, k_len, causal, scale, True)
-        ctx.save_for_backward(q, k, v, q_start, k_start, q_len, k_len, out, lse)
+        out, lse, rest = native.attention_forward(q, k, v, q_start, k_start, q_len, k_len, causal, scale, True)
+        ctx.save_for_backward(q, k, v, q_start, k_start, q_len, k_len, out, lse, rest)
         ctx.rest = causal, scale
         ctx.native = native
         return out
 
     @staticmethod
     def backward(ctx, grad_output):
-        *inputs, out, lse = ctx.saved_tensors
+        *inputs, out, lse, rest = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         with torch.no_grad():
-            gq, gk, gv = ctx.native.attention_backward(*inputs, *ctx.rest, out, lse, grad_output, need_q, need_k or need_v)
+            gq, gk, gv = ctx.native.attention_backward(*inputs, *ctx.rest, out, lse, rest, grad_output, need_q, need_k or need_v)
         given = grad_output.requires_grad
         return (once(gq, True, "attention"), once(gk if need_k else None, True, "attention"),
                 once(gv if need_v else None, need_q or need_k or given, "attention")) + (None,) * 7

@@ -65,17 +65,18 @@ struct Plan {
 };
 
 // columns and others: of an item, or of all packed sequences.
-Plan plan_of(const ops3d_attention_problem *p, int64_t columns, int64_t others) {
+Plan plan_of(const ops3d_attention_problem *p, int64_t columns, int64_t others, int widest) {
   const int64_t runs = p->q_start ? p->sequences : p->items;   // what has tiles of its own
   const int64_t per = p->q_start ? ceil_div(columns, runs) : columns, far = p->q_start ? ceil_div(others, runs) : others;
   const int e = elem_size(p->dtype) / 2;
   Plan best{};
   for (const int shape : {kMany, kSome, kFew}) {
+    if (shape < widest) continue;
     const int width = shape == kMany ? 128 : shape == kSome ? 64 : 16, stage = (shape == kFew ? 128 : 64) / e;
     const int64_t blocks = ceil_div(per, width) * runs * p->kv_heads;
-    // parts of 4 stages at least, for two blocks a CU
-    int64_t splits = blocks ? 512 / blocks : 1;
-    const int64_t most = ceil_div(far, 4 * stage);
+    // two blocks a CU, or four where they differ in what they have to do, in parts of 2 stages at least
+    int64_t splits = blocks ? (p->causal || p->q_start ? 1024 : 512) / blocks : 1;
+    const int64_t most = ceil_div(far, 2 * stage);
     splits = splits > most ? most : splits;
     splits = splits < 1 ? 1 : splits;
     best.shape = shape;
@@ -88,8 +89,12 @@ Plan plan_of(const ops3d_attention_problem *p, int64_t columns, int64_t others) 
   if (!p->q_start) best.tiles = 0;
   return best;
 }
-Plan plan_queries(const ops3d_attention_problem *p) { return plan_of(p, p->q_rows * (p->heads / p->kv_heads), p->k_rows); }
-Plan plan_keys(const ops3d_attention_problem *p) { return plan_of(p, p->k_rows, p->q_rows * (p->heads / p->kv_heads)); }
+Plan plan_queries(const ops3d_attention_problem *p) { return plan_of(p, p->q_rows * (p->heads / p->kv_heads), p->k_rows, kMany); }
+// Keys of 128 channels: two results, K and V for each column are too many registers for tiles of 128 columns
+// (grad k v of 8192 causal tokens, 16/4 heads: 374 us, in tiles of 64 273 us).
+Plan plan_keys(const ops3d_attention_problem *p) {
+  return plan_of(p, p->k_rows, p->q_rows * (p->heads / p->kv_heads), p->dim > 64 ? kSome : kMany);
+}
 
 // false: more blocks than a launch has
 bool set_plan(Args &a, const ops3d_attention_problem *p, const Plan &plan) {
@@ -188,8 +193,8 @@ size_t ops3d_attention_forward_workspace_bytes(const ops3d_attention_problem *pr
 
 int ops3d_attention_forward(const ops3d_attention_problem *problem, const ops3d_attention_tensor *q,
                             const ops3d_attention_tensor *k, const ops3d_attention_tensor *v,
-                            const ops3d_attention_tensor *out, float *lse, void *workspace, size_t workspace_bytes,
-                            void *stream) {
+                            const ops3d_attention_tensor *out, void *out_rest, float *lse, void *workspace,
+                            size_t workspace_bytes, void *stream) {
   ops3d_fda::set_last_error(OPS3D_FDA_OK, "");
   int rc = check(problem);
   if (rc) return rc;
@@ -199,6 +204,9 @@ int ops3d_attention_forward(const ops3d_attention_problem *problem, const ops3d_
   if ((rc = take(a.q, q, es)) || (rc = take(a.o, out, es))) return rc;
   if (problem->k_rows && ((rc = take(a.k, k, es)) || (rc = take(a.v, v, es)))) return rc;
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return fail(OPS3D_FDA_EINVAL, "lse must be 4-byte aligned");
+  if (reinterpret_cast<uintptr_t>(out_rest) & (uintptr_t)(es - 1))
+    return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
+  a.rest = out_rest;
   a.lse = lse;
   const size_t need = forward_bytes(problem);
   if ((rc = check_workspace(workspace, workspace_bytes, need))) return rc;
@@ -218,7 +226,8 @@ size_t ops3d_attention_backward_workspace_bytes(const ops3d_attention_problem *p
 
 int ops3d_attention_backward(const ops3d_attention_problem *problem, const ops3d_attention_tensor *q,
                              const ops3d_attention_tensor *k, const ops3d_attention_tensor *v,
-                             const ops3d_attention_tensor *out, const float *lse, const ops3d_attention_tensor *grad_out,
+                             const ops3d_attention_tensor *out, const void *out_rest, const float *lse,
+                             const ops3d_attention_tensor *grad_out,
                              const ops3d_attention_tensor *grad_q, const ops3d_attention_tensor *grad_k,
                              const ops3d_attention_tensor *grad_v, void *workspace, size_t workspace_bytes, void *stream) {
   ops3d_fda::set_last_error(OPS3D_FDA_OK, "");
@@ -232,6 +241,9 @@ int ops3d_attention_backward(const ops3d_attention_problem *problem, const ops3d
   const int es = elem_size(problem->dtype);
   if (cells) {
     if ((rc = take(a.q, q, es)) || (rc = take(a.o, out, es)) || (rc = take(a.g, grad_out, es))) return rc;
+    if (reinterpret_cast<uintptr_t>(out_rest) & (uintptr_t)(es - 1))
+      return fail(OPS3D_FDA_EINVAL, "data pointers must be aligned to their element size");
+    a.rest = const_cast<void *>(out_rest);
     if (!lse) return fail(OPS3D_FDA_EINVAL, "NULL pointer argument");
     if (reinterpret_cast<uintptr_t>(lse) & 3u) return fail(OPS3D_FDA_EINVAL, "lse must be 4-byte aligned");
   }

@@ -46,11 +46,13 @@ struct Args {
   uint32_t magic;                     // c / G = 2 c magic >> 32 >> shift
   int shift;
   int causal;
+  int pair;                           // see place()
   int dma;                            // rows go straight to LDS: bit 0 k and v, bit 1 q and grad_out
   float scale, c;                     // c = scale log2 e
   int tiles, tiles_item, splits;      // tiles of all items (a bound), of one, and parts of the other side
   int heads;                          // items Hk
   int64_t cells;                      // heads Sq G: queries times heads
+  void *rest;                         // what rounding took from o, [items, Sq, heads, D] contiguous, or nullptr
   float *lse, *delta;                 // [items, Hk, Sq G]; log2 of the sum of exponentials, and sum of o g
   float *part, *part_ml;              // [splits, columns, DP], [splits, columns, 2]
 };
@@ -135,20 +137,24 @@ template <bool KEYS> __device__ __forceinline__ bool locate(const Args &p, int t
 
 __device__ __forceinline__ int divide(const Args &p, int c) { return (int)(__umulhi((uint32_t)c << 1, p.magic) >> p.shift); }
 
-// A stage of R rows of DP elements in LDS, in 16-byte chunks, XOR-swizzled: 8 rows that follow each other and
-// a chunk of each, and 4 rows and two neighbouring chunks of each, fall on different banks.
+// A stage of R rows of DP elements in LDS, in 16-byte chunks, XOR-swizzled within the 16 chunks that the banks
+// hold: 16 rows and a chunk of each, and 8 rows that follow each other and two neighbouring chunks of each, fall on
+// different banks.
 template <typename T, int DP, int R, int NT> struct Stage {
   static constexpr int CH = 16 / (int)sizeof(T), RC = DP / CH, NL = R * RC / NT;
   static constexpr int kBytes = R * DP * (int)sizeof(T);
   static_assert(R * RC % NT == 0 && RC >= 4, "chunks divide over the threads");
+  static_assert((kBytes & (kBytes - 1)) == 0, "buffers are told apart by a bit of the address");
 
-  static __device__ __forceinline__ int address(int row, int chunk) {
-    if (RC == 4) {
-      const int line = row >> 1;
-      return (row * 4 + (chunk ^ (((line & 1) << 1) | ((line >> 1) & 1)))) << 4;
-    }
-    return (row * RC + (chunk ^ (((row & 3) << 1) | ((row >> 2) & 1)))) << 4;
+  // The place of a row among those that share banks (all, every second, every fourth), its upper bit folded
+  // into the next one: two rows whose places differ in the lowest bit alone are read in one cycle, whichever way
+  // the hardware groups lanes.
+  static __device__ __forceinline__ int swizzle(int row) {
+    constexpr int kBits = RC >= 16 ? 3 : RC == 8 ? 2 : 1;   // below the row's bit 3
+    const int low = (row >> (3 - kBits)) & ((1 << kBits) - 1), top = (row >> 3) & 1;
+    return (low ^ (top << (kBits - 1))) << 1 | top;
   }
+  static __device__ __forceinline__ int address(int row, int chunk) { return (row * RC + (chunk ^ swizzle(row))) << 4; }
   static __device__ __forceinline__ int row_of(int i) { return (int)(threadIdx.x + i * NT) / RC; }
   static __device__ __forceinline__ int chunk_of(int i) { return (int)(threadIdx.x + i * NT) % RC; }
 
@@ -195,29 +201,49 @@ template <typename T, int DP, int R, int NT> struct Stage {
     for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4 *>(lds + address(row_of(i), chunk_of(i))) = v[i];
   }
 
-  // MFMA operand: 16 rows from r0 on, step s of the channels
-  static __device__ __forceinline__ typename Type<T>::frag rows(const char *lds, int r0, int s, int lane) {
-    return __builtin_bit_cast(typename Type<T>::frag,
-                              *reinterpret_cast<const uint4 *>(lds + address(r0 + (lane & 15), s * 4 + (lane >> 4))));
+  // A lane's places in the first of two buffers of two stages, or, flipped, in the second: of its row in a
+  // tile of 16 rows at each step of the channels, and of its piece of 4 rows of 16 channels at each 16 channels
+  // (16 bits).
+  struct Lane {
+    int row[DP * (int)sizeof(T) / 64], col[DP / 16];
+    __device__ __forceinline__ void flip() {
+#pragma unroll
+      for (int s = 0; s < DP * (int)sizeof(T) / 64; ++s) row[s] ^= 2 * kBytes;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) col[d] ^= 2 * kBytes;
+    }
+  };
+  static __device__ __forceinline__ Lane lane_places(int lane) {
+    const int i = lane & 15, q = lane >> 4;
+    Lane l;
+#pragma unroll
+    for (int s = 0; s < DP * (int)sizeof(T) / 64; ++s) l.row[s] = address(i, s * 4 + q);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+      l.col[d] = sizeof(T) == 2 ? address(q * 4 + (i >> 2), d * 2 + ((i & 3) >> 1)) + (i & 1) * 8 : 0;   // 32 bits: the buffer
+    return l;
   }
-  // MFMA operand: 16 channels from 16 dt on, summed over rows: in 16 bits rows r0 + 4 q .. + 3 and those 16
+  // MFMA operand: 16 rows from r0 (a multiple of 16) on, step s of the channels
+  static __device__ __forceinline__ typename Type<T>::frag rows(const char *lds, int r0, int s, const Lane &l) {
+    return __builtin_bit_cast(typename Type<T>::frag, *reinterpret_cast<const uint4 *>(lds + r0 * RC * 16 + l.row[s]));
+  }
+  // MFMA operand: 16 channels from 16 d on, summed over rows: in 16 bits rows r0 + 4 q .. + 3 and those 16
   // further, in 32 bits the former.  16 lanes read 4 rows of 16 channels, 4 channels a lane, and get them
   // transposed.
-  static __device__ __forceinline__ typename Type<T>::frag columns(const char *lds, int r0, int dt, int lane) {
-    const int i = lane & 15, q = lane >> 4;
+  static __device__ __forceinline__ typename Type<T>::frag columns(const char *lds, int r0, int d, const Lane &l, int lane) {
     if constexpr (sizeof(T) == 2) {
       s16x4 h[2];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const char *at = lds + address(r0 + p * 16 + q * 4 + (i >> 2), dt * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
-        h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(const_cast<char *>(at)));
-      }
+      for (int p = 0; p < 2; ++p)
+        h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4 *)(const_cast<char *>(lds + (r0 + p * 16) * RC * 16 + l.col[d])));
       return __builtin_bit_cast(typename Type<T>::frag, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
+      const int i = lane & 15, q = lane >> 4;
       f32x4 f;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        f[j] = *reinterpret_cast<const float *>(lds + address(r0 + q * 4 + j, dt * 4 + (i >> 2)) + (i & 3) * 4);
+        f[j] = *reinterpret_cast<const float *>(lds + l.col[d] + address(r0 + q * 4 + j, d * 4 + (i >> 2)) + (i & 3) * 4);
       return __builtin_bit_cast(typename Type<T>::frag, f);
     }
   }
@@ -244,6 +270,15 @@ __device__ __forceinline__ void load_column(typename Type<T>::frag (&f)[STEPS], 
     f[s] = __builtin_bit_cast(typename Type<T>::frag, row ? fetch(row, 0, 0, (s * 4 + q) * CH, 1, D) : make_uint4(0, 0, 0, 0));
 }
 
+__device__ __forceinline__ f32x4 splat(float x) { return f32x4{x, x, x, x}; }
+
+// The output's rounding: what is left of v in T.
+template <typename T> __device__ __forceinline__ f32x4 rest_of(f32x4 v) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] -= (float)(T)v[j];
+  return v;
+}
+
 // 4 consecutive channels of a row; those behind D are left out.
 template <typename T> __device__ __forceinline__ void store4(T *row, int d, const f32x4 &v, int D) {
   if (d + 4 <= D) {
@@ -266,10 +301,12 @@ template <> struct Range<_Float16> { static constexpr float kShift = 10.f, kSlac
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The block's place: key head, part and tile; tiles from the last on, which in causal attention have most to
-// do.
+// do.  Blocks go to XCD block % 8, so with 8 key heads one has a head, whose rows its L2 then keeps; where two
+// heads' rows share 128-byte lines (p.pair), the two take turns on two XCDs.
 __device__ __forceinline__ void place(const Args &p, int &h, int &part, int &tile) {
   const int r = blockIdx.x / p.Hk;
   h = blockIdx.x - r * p.Hk;
+  if (p.pair) h ^= r & 1;
   part = r % p.splits;
   tile = p.tiles - 1 - r / p.splits;
 }
@@ -338,14 +375,15 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   f32x4 o[NC][DT], sum[NC];                // sums of P V and of P (SUMS: by the matrix units, from the rounded P)
   float m[NC], mc[NC], l[NC], top[NC];     // reference, the same times c, sum of P (this lane's rows), what raises it
   constexpr bool SUMS = sizeof(T) == 2;
+  constexpr float kShift = Range<T>::kShift;
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     m[n] = top[n] = -INFINITY;
-    mc[n] = -Range<T>::kShift;
+    mc[n] = -kShift;
     l[n] = 0.f;
-    sum[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    sum[n] = splat(0.f);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DT; ++d) o[n][d] = splat(0.f);
   }
   const float slack = Range<T>::kSlack / p.c;
 
@@ -371,12 +409,13 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     }
   };
   const int r0 = wk * KW;
+  typename ST::Lane at = ST::lane_places(lane);
+  const char *const lk = lds, *const lv = lds + ST::kBytes;
   int k0 = k_begin, buf = 0;
   const auto stage = [&](auto masked) __attribute__((always_inline)) {
-    char *const lk = lds + buf * 2 * ST::kBytes, *const lv = lk + ST::kBytes;
     if constexpr (!DMA) {
-      ST::store(lk, kv);
-      ST::store(lv, vv);
+      ST::store(lds + buf * 2 * ST::kBytes, kv);
+      ST::store(lds + buf * 2 * ST::kBytes + ST::kBytes, vv);
       if (k0 + KT < k_end) load(k0 + KT, 0);
       __syncthreads();   // the other buffer's readers are past the barrier before
     } else {
@@ -388,10 +427,10 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
     for (int kt = 0; kt < KN; ++kt) {
 #pragma unroll
-      for (int n = 0; n < NC; ++n) s[n][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NC; ++n) s[n][kt] = splat(0.f);
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        const auto kf = ST::rows(lk, r0 + kt * 16, st, lane);
+        const auto kf = ST::rows(lk, r0 + kt * 16, st, at);
 #pragma unroll
         for (int n = 0; n < NC; ++n) s[n][kt] = Type<T>::mma(kf, qf[n][st], s[n][kt]);
       }
@@ -427,7 +466,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[n][d] *= by;
           m[n] = now;
-          mc[n] = now * p.c - Range<T>::kShift;
+          mc[n] = now * p.c - kShift;
           top[n] = now + slack;
         }
       }
@@ -449,13 +488,14 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const auto vf = ST::columns(lv, r0 + kt * 16, d, lane);
+        const auto vf = ST::columns(lv, r0 + kt * 16, d, at, lane);
 #pragma unroll
         for (int n = 0; n < NC; ++n) o[n][d] = Type<T>::mma(vf, pf[n], o[n][d]);
       }
     }
-    buf ^= 1;
     k0 += KT;
+    buf ^= 1;
+    at.flip();
   };
   if (k_begin < k_end) load(k_begin, 0);
   while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
@@ -463,6 +503,8 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
   for (int n = 0; n < NC; ++n)
     l[n] = SUMS ? sum[n][0] : ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(l[n]));
+#pragma unroll
+  for (int n = 0; n < NC; ++n) m[n] *= p.c;   // from here on log2
 
   if constexpr (WK > 1) {   // the waves' shares, each with its own reference
     f32x4 *x = reinterpret_cast<f32x4 *>(lds);
@@ -484,7 +526,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       for (int k = 0; k < WK - 1; ++k) {
         const f32x4 *y = x + ((k * WC + wc) * NC + n) * (DT + 1) * 64 + lane;
         const float mk = y[DT * 64][0], now = fmaxf(m[n], mk);
-        const float a = m[n] == -INFINITY ? 0.f : exp2_((m[n] - now) * p.c), b = mk == -INFINITY ? 0.f : exp2_((mk - now) * p.c);
+        const float a = m[n] == -INFINITY ? 0.f : exp2_(m[n] - now), b = mk == -INFINITY ? 0.f : exp2_(mk - now);
         l[n] = l[n] * a + y[DT * 64][1] * b;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[n][d] = o[n][d] * a + y[d * 64] * b;
@@ -498,55 +540,69 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     const int c = c0 + n * 16 + i;
     if (c >= w.rows * p.G) continue;
     if (p.splits > 1) {
-      const int64_t at = part * p.cells + cell0 + c;
+      const int64_t to = part * p.cells + cell0 + c;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + at * DP + d * 16 + q * 4) = o[n][d];
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + to * DP + d * 16 + q * 4) = o[n][d];
       if (q == 0) {   // columns that do not count saw nothing
-        p.part_ml[2 * at] = c < active ? m[n] * p.c : -INFINITY;
-        p.part_ml[2 * at + 1] = c < active ? l[n] : 0.f;
+        p.part_ml[2 * to] = c < active ? m[n] : -INFINITY;
+        p.part_ml[2 * to + 1] = c < active ? l[n] : 0.f;
       }
       continue;
     }
     const bool none = c >= active || l[n] == 0.f;
     const float inv = none ? 0.f : 1.f / l[n];
     const int t = divide(p, c);
-    T *to = static_cast<T *>(p.o.p) + w.item * p.o.item + (w.q0 + t) * p.o.token + ((int64_t)h * p.G + c - t * p.G) * p.o.head;
+    const int head = h * p.G + c - t * p.G;
+    T *const to = static_cast<T *>(p.o.p) + w.item * p.o.item + (w.q0 + t) * p.o.token + head * p.o.head;
+    T *const rest = static_cast<T *>(p.rest) + (((int64_t)w.item * p.Sq + w.q0 + t) * (p.Hk * p.G) + head) * p.D;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) store4(to, d * 16 + q * 4, none ? f32x4{0.f, 0.f, 0.f, 0.f} : o[n][d] * inv, p.D);
-    if (p.lse && q == 0) p.lse[cell0 + c] = none ? INFINITY : m[n] * p.c + __builtin_amdgcn_logf(l[n]) - Range<T>::kShift;
+    for (int d = 0; d < DT; ++d) {
+      const f32x4 v = none ? splat(0.f) : o[n][d] * inv;
+      store4(to, d * 16 + q * 4, v, p.D);
+      if (p.rest) store4(rest, d * 16 + q * 4, rest_of<T>(v), p.D);
+    }
+    if (p.lse && q == 0) p.lse[cell0 + c] = none ? INFINITY : m[n] + __builtin_amdgcn_logf(l[n]) - kShift;
   }
 }
 
-// The parts of a query and head joined: a wave each.
+// The parts of a query and head joined: a wave each, 4 channels a lane, as many parts at a time as that leaves
+// lanes for.
 template <typename T, int DP> __global__ __launch_bounds__(256) void join_forward_kernel(Args p) {
+  constexpr int PER = DP / 4, AT = 64 / PER;   // lanes of a row, parts at a time
   const int64_t cell = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (cell >= p.cells) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, d = lane % PER * 4;
   float m = -INFINITY;
   for (int z = lane; z < p.splits; z += 64) m = fmaxf(m, p.part_ml[2 * (z * p.cells + cell)]);
   m = ops3d_reduce::all<64, ops3d_reduce::Max>(m);
-  float l = 0.f, o[(DP + 63) / 64];
-#pragma unroll
-  for (int k = 0; k < (DP + 63) / 64; ++k) o[k] = 0.f;
+  float l = 0.f;
+  f32x4 o = splat(0.f);
   if (m != -INFINITY) {
-    for (int z = 0; z < p.splits; ++z) {
+#pragma unroll 2
+    for (int z = lane / PER; z < p.splits; z += AT) {
       const int64_t at = z * p.cells + cell;
-      const float mz = p.part_ml[2 * at];
-      const float by = mz == -INFINITY ? 0.f : exp2_(mz - m);
-      if (by == 0.f) continue;
-      l = fmaf(by, p.part_ml[2 * at + 1], l);
-#pragma unroll
-      for (int k = 0; k < (DP + 63) / 64; ++k)
-        if (k * 64 + lane < DP) o[k] = fmaf(by, p.part[at * DP + k * 64 + lane], o[k]);
+      const float mz = p.part_ml[2 * at], lz = p.part_ml[2 * at + 1];
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(p.part + at * DP + d);
+      if (mz == -INFINITY) continue;
+      const float by = exp2_(mz - m);
+      l = fmaf(by, lz, l);
+      o += v * by;
     }
   }
-  const int per = p.Sq * p.G, ih = (int)(cell / per), c = (int)(cell - (int64_t)ih * per);
-  const int item = ih / p.Hk, h = ih - item * p.Hk, t = divide(p, c);
-  const bool none = l == 0.f;
-  T *to = static_cast<T *>(p.o.p) + item * p.o.item + t * p.o.token + ((int64_t)h * p.G + c - t * p.G) * p.o.head;
 #pragma unroll
-  for (int k = 0; k < (DP + 63) / 64; ++k)
-    if (k * 64 + lane < p.D) to[k * 64 + lane] = (T)(none ? 0.f : o[k] / l);
+  for (int s = PER; s < 64; s <<= 1) {
+    l += __shfl_xor(l, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], s);
+  }
+  const int per = p.Sq * p.G, ih = (int)(cell / per), c = (int)(cell - (int64_t)ih * per);
+  const int item = ih / p.Hk, h = ih - item * p.Hk, t = divide(p, c), head = h * p.G + c - t * p.G;
+  const bool none = l == 0.f;
+  const f32x4 v = none ? splat(0.f) : o * (1.f / l);
+  if (lane < PER) {
+    store4(static_cast<T *>(p.o.p) + item * p.o.item + t * p.o.token + head * p.o.head, d, v, p.D);
+    if (p.rest) store4(static_cast<T *>(p.rest) + (((int64_t)item * p.Sq + t) * (p.Hk * p.G) + head) * p.D, d, rest_of<T>(v), p.D);
+  }
   if (p.lse && lane == 0) p.lse[cell] = none ? INFINITY : m + __builtin_amdgcn_logf(l) - Range<T>::kShift;
 }
 
@@ -585,13 +641,14 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     };
     load_column<T, STEPS>(qf[n], row(p.q), p.D, q);
     load_column<T, STEPS>(gf[n], row(p.g), p.D, q);
-    typename Type<T>::frag of[STEPS];
+    typename Type<T>::frag of[STEPS], rf[STEPS];
     load_column<T, STEPS>(of, row(p.o), p.D, q);
+    load_column<T, STEPS>(rf, in && p.rest ? static_cast<const T *>(p.rest) + (((int64_t)w.item * p.Sq + w.q0 + t) * (p.Hk * p.G) + head) * p.D : nullptr, p.D, q);
     float d = 0.f;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-      for (int j = 0; j < CH; ++j) d = fmaf((float)of[s][j], (float)gf[n][s][j], d);
+      for (int j = 0; j < CH; ++j) d = fmaf((float)of[s][j] + (float)rf[s][j], (float)gf[n][s][j], d);
     delta[n] = ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(d));
     lse[n] = in ? p.lse[cell0 + c] : INFINITY;
     if (c < w.rows * p.G && q == 0 && wk == 0 && part == 0) p.delta[cell0 + c] = delta[n];
@@ -612,7 +669,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
   for (int n = 0; n < NC; ++n)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) a[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DT; ++d) a[n][d] = splat(0.f);
   uint4 kv[DMA ? 1 : ST::NL], vv[DMA ? 1 : ST::NL];
   uint32_t k_off[DMA ? ST::NL : 1], v_off[DMA ? ST::NL : 1];
   if constexpr (DMA) {
@@ -635,12 +692,13 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     }
   };
   const int r0 = wk * KW;
+  typename ST::Lane at = ST::lane_places(lane);
+  const char *const lk = lds, *const lv = lds + ST::kBytes;
   int k0 = k_begin, buf = 0;
   const auto stage = [&](auto masked) __attribute__((always_inline)) {
-    char *const lk = lds + buf * 2 * ST::kBytes, *const lv = lk + ST::kBytes;
     if constexpr (!DMA) {
-      ST::store(lk, kv);
-      ST::store(lv, vv);
+      ST::store(lds + buf * 2 * ST::kBytes, kv);
+      ST::store(lds + buf * 2 * ST::kBytes + ST::kBytes, vv);
       if (k0 + KT < k_end) load(k0 + KT, 0);
       __syncthreads();
     } else {
@@ -653,10 +711,10 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
       for (int u = 0; u < PR; ++u) {
 #pragma unroll
-        for (int n = 0; n < NC; ++n) s[n][u] = dp[n][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NC; ++n) s[n][u] = splat(0.f), dp[n][u] = splat(-delta[n]);
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
-          const auto kf = ST::rows(lk, r0 + (kt + u) * 16, st, lane), vf = ST::rows(lv, r0 + (kt + u) * 16, st, lane);
+          const auto kf = ST::rows(lk, r0 + (kt + u) * 16, st, at), vf = ST::rows(lv, r0 + (kt + u) * 16, st, at);
 #pragma unroll
           for (int n = 0; n < NC; ++n) {
             s[n][u] = Type<T>::mma(kf, qf[n][st], s[n][u]);
@@ -671,7 +729,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
         for (int u = 0; u < PR; ++u)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float x = exp2_(fmaf(s[n][u][j], p.c, -lse[n])) * (dp[n][u][j] - delta[n]);
+            float x = exp2_(fmaf(s[n][u][j], p.c, -lse[n])) * dp[n][u][j];
             if (decltype(masked)::value && k0 + r0 + (kt + u) * 16 + q * 4 + j >= limit[n]) x = 0.f;
             s[n][u][j] = x;
           }
@@ -679,13 +737,14 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const auto kf = ST::columns(lk, r0 + kt * 16, d, lane);
+        const auto kf = ST::columns(lk, r0 + kt * 16, d, at, lane);
 #pragma unroll
         for (int n = 0; n < NC; ++n) a[n][d] = Type<T>::mma(kf, ds[n], a[n][d]);
       }
     }
-    buf ^= 1;
     k0 += KT;
+    buf ^= 1;
+    at.flip();
   };
   if (k_begin < k_end) load(k_begin, 0);
   while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
@@ -700,15 +759,15 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     const int c = c0 + n * 16 + i, t = divide(p, c);
     if (c >= w.rows * p.G) continue;
     if (p.splits > 1) {
-      const int64_t at = part * p.cells + cell0 + c;
+      const int64_t to = part * p.cells + cell0 + c;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + at * DP + d * 16 + q * 4) = a[n][d];
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + to * DP + d * 16 + q * 4) = a[n][d];
       continue;
     }
     T *to = static_cast<T *>(p.gq.p) + w.item * p.gq.item + (w.q0 + t) * p.gq.token + ((int64_t)h * p.G + c - t * p.G) * p.gq.head;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      store4(to, d * 16 + q * 4, c < active ? a[n][d] * p.scale : f32x4{0.f, 0.f, 0.f, 0.f}, p.D);
+      store4(to, d * 16 + q * 4, c < active ? a[n][d] * p.scale : splat(0.f), p.D);
   }
 }
 
@@ -720,9 +779,9 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   constexpr int STEPS = DP * (int)sizeof(T) / 64, DT = DP / 16, PR = sizeof(T) == 2 ? 2 : 1;
   typedef Stage<T, DP, QT, NT> ST;
   static_assert(QN % PR == 0 && QT <= NT, "whole operands, a thread a row");
-  constexpr int kStage = 2 * ST::kBytes + QT * 8;   // and the rows' lse and delta
   constexpr int kMerge = (WK - 1) * NC * DT * 1024;
-  constexpr int kLds = 2 * kStage > kMerge ? 2 * kStage : kMerge;
+  constexpr int kStages = 4 * ST::kBytes + 4 * QT * 4;   // and the rows' lse and delta
+  constexpr int kLds = kStages > kMerge ? kStages : kMerge;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
 
   int h, part, tile;
@@ -764,7 +823,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
   for (int n = 0; n < NC; ++n)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) ak[n][d] = av[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DT; ++d) ak[n][d] = av[n][d] = splat(0.f);
   uint4 qv[DMA ? 1 : ST::NL], gv[DMA ? 1 : ST::NL];
   uint32_t q_off[ST::NL], g_off[ST::NL];
   float row_lse = INFINITY, row_delta = 0.f;
@@ -781,7 +840,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   const auto load = [&](int c0, int buf) __attribute__((always_inline)) {
     const int left = c_end - c0;
     if constexpr (DMA) {
-      char *const lq = lds + buf * kStage;
+      char *const lq = lds + buf * 2 * ST::kBytes;
       const int t0 = uniform(divide(p, c0));
       if (!fixed || left < QT) place_rows(c0, min(left, QT));
       ST::load_lds(lq, reinterpret_cast<const char *>(qb + t0 * p.q.token), q_off);
@@ -803,31 +862,35 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   if constexpr (DMA) place_rows(0, QT);
   constexpr float kDown = sizeof(T) == 2 ? 1.f / (float)(1 << (int)Range<T>::kShift) : 1.f;
   const int r0 = wk * QW;
+  typename ST::Lane at = ST::lane_places(lane);
+  const char *const lq = lds, *const lg = lds + ST::kBytes;
   int c0 = c_begin, buf = 0;
   const auto stage = [&](auto masked) __attribute__((always_inline)) {
-    char *const lq = lds + buf * kStage, *const lg = lq + ST::kBytes;
-    float *const ll = reinterpret_cast<float *>(lg + ST::kBytes), *const ld = ll + QT;
+    float *const ll = reinterpret_cast<float *>(lds + 4 * ST::kBytes) + buf * 2 * QT, *const ld = ll + QT;
     if constexpr (!DMA) {
-      ST::store(lq, qv);
-      ST::store(lg, gv);
+      ST::store(lds + buf * 2 * ST::kBytes, qv);
+      ST::store(lds + buf * 2 * ST::kBytes + ST::kBytes, gv);
     }
     if (threadIdx.x < QT) {
-      ll[threadIdx.x] = row_lse - Range<T>::kShift;
-      ld[threadIdx.x] = row_delta;
+      ll[threadIdx.x] = Range<T>::kShift - row_lse;
+      ld[threadIdx.x] = -row_delta;
     }
     if (!DMA && c0 + QT < c_end) load(c0 + QT, 0);
     __syncthreads();
     if (DMA && c0 + QT < c_end) load(c0 + QT, buf ^ 1);
 #pragma unroll
     for (int qt = 0; qt < QN; qt += PR) {
-      f32x4 s[NC][PR], dp[NC][PR];
+      f32x4 s[NC][PR], dp[NC][PR], lse[PR];
 #pragma unroll
       for (int u = 0; u < PR; ++u) {
+        const int r = r0 + (qt + u) * 16 + q * 4;
+        lse[u] = *reinterpret_cast<const f32x4 *>(ll + r);
+        const f32x4 delta = *reinterpret_cast<const f32x4 *>(ld + r);
 #pragma unroll
-        for (int n = 0; n < NC; ++n) s[n][u] = dp[n][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NC; ++n) s[n][u] = splat(0.f), dp[n][u] = delta;
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
-          const auto qf = ST::rows(lq, r0 + (qt + u) * 16, st, lane), gf = ST::rows(lg, r0 + (qt + u) * 16, st, lane);
+          const auto qf = ST::rows(lq, r0 + (qt + u) * 16, st, at), gf = ST::rows(lg, r0 + (qt + u) * 16, st, at);
 #pragma unroll
           for (int n = 0; n < NC; ++n) {
             s[n][u] = Type<T>::mma(qf, kf[n][st], s[n][u]);
@@ -840,12 +903,12 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       for (int n = 0; n < NC; ++n) {
 #pragma unroll
         for (int u = 0; u < PR; ++u) {
-          const int r = r0 + (qt + u) * 16 + q * 4;
-          const f32x4 lse = *reinterpret_cast<const f32x4 *>(ll + r), delta = *reinterpret_cast<const f32x4 *>(ld + r);
+          const int r = c0 + r0 + (qt + u) * 16 + q * 4;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float x = exp2_(fmaf(s[n][u][j], p.c, -lse[j])), y = x * fmaf(dp[n][u][j], kDown, -kDown * delta[j]);
-            if (decltype(masked)::value && c0 + r + j < since[n]) x = y = 0.f;
+            float x = exp2_(fmaf(s[n][u][j], p.c, lse[u][j])), y = x * dp[n][u][j];
+            if (kDown != 1.f) y *= kDown;
+            if (decltype(masked)::value && r + j < since[n]) x = y = 0.f;
             s[n][u][j] = x;
             dp[n][u][j] = y;
           }
@@ -855,7 +918,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const auto gf = ST::columns(lg, r0 + qt * 16, d, lane), qf = ST::columns(lq, r0 + qt * 16, d, lane);
+        const auto gf = ST::columns(lg, r0 + qt * 16, d, at, lane), qf = ST::columns(lq, r0 + qt * 16, d, at, lane);
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
           av[n][d] = Type<T>::mma(gf, pf[n], av[n][d]);
@@ -863,8 +926,9 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
         }
       }
     }
-    buf ^= 1;
     c0 += QT;
+    buf ^= 1;
+    at.flip();
   };
   if (c_begin < c_end) load(c_begin, 0);
   while (c0 < c_end && c0 < all_see) stage(std::true_type());
@@ -883,11 +947,11 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     if (j >= w.rows) continue;
     const bool in = j < w.nk;   // keys that do not count, whose operands are 0, have gathered exp(0) all the same
     if (p.splits > 1) {
-      const int64_t at = (part * keys + key0 + j) * 2;
+      const int64_t to = (part * keys + key0 + j) * 2;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        *reinterpret_cast<f32x4 *>(p.part + at * DP + d * 16 + q * 4) = in ? ak[n][d] : f32x4{0.f, 0.f, 0.f, 0.f};
-        *reinterpret_cast<f32x4 *>(p.part + (at + 1) * DP + d * 16 + q * 4) = in ? av[n][d] * kDown : f32x4{0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<f32x4 *>(p.part + to * DP + d * 16 + q * 4) = in ? ak[n][d] : splat(0.f);
+        *reinterpret_cast<f32x4 *>(p.part + (to + 1) * DP + d * 16 + q * 4) = in ? av[n][d] * kDown : splat(0.f);
       }
       continue;
     }
@@ -895,30 +959,30 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     T *const gk = row(p.gk), *const gv = row(p.gv);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      store4(gk, d * 16 + q * 4, in ? ak[n][d] * p.scale : f32x4{0.f, 0.f, 0.f, 0.f}, p.D);
-      store4(gv, d * 16 + q * 4, in ? av[n][d] * kDown : f32x4{0.f, 0.f, 0.f, 0.f}, p.D);
+      store4(gk, d * 16 + q * 4, in ? ak[n][d] * p.scale : splat(0.f), p.D);
+      store4(gv, d * 16 + q * 4, in ? av[n][d] * kDown : splat(0.f), p.D);
     }
   }
 }
 
-// Sums of parts: of grad q (KEYS false), a row a cell; of grad k and grad v, two rows a key.  A wave each.
+// Sums of parts: of grad q (KEYS false), a row a cell; of grad k and grad v, two rows a key.  4 channels a
+// thread, the parts in order.
 template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void join_sum_kernel(Args p) {
+  constexpr int PER = DP / 4;
   const int per = KEYS ? p.Sk : p.Sq * p.G;
   const int64_t n = (int64_t)p.heads * per * (KEYS ? 2 : 1);
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= n) return;
-  const int lane = threadIdx.x & 63;
+  const int64_t at = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER;
+  const int d = threadIdx.x % PER * 4;
+  if (at >= n || d >= p.D) return;
   const int64_t row = KEYS ? at >> 1 : at;
   const int ih = (int)(row / per), c = (int)(row - (int64_t)ih * per), item = ih / p.Hk, h = ih - item * p.Hk;
   const bool value = KEYS && (at & 1);
   const Tensor &x = KEYS ? (value ? p.gv : p.gk) : p.gq;
   const int t = KEYS ? c : divide(p, c), head = KEYS ? h : h * p.G + c - t * p.G;
-  T *to = static_cast<T *>(x.p) + item * x.item + t * x.token + head * x.head;
-  for (int d = lane; d < p.D; d += 64) {
-    float s = 0.f;
-    for (int z = 0; z < p.splits; ++z) s += p.part[(z * n + at) * DP + d];
-    to[d] = (T)(value ? s : s * p.scale);
-  }
+  f32x4 s = splat(0.f);
+#pragma unroll 4
+  for (int z = 0; z < p.splits; ++z) s += *reinterpret_cast<const f32x4 *>(p.part + (z * n + at) * DP + d);
+  store4(static_cast<T *>(x.p) + item * x.item + t * x.token + head * x.head, d, value ? s : s * p.scale, p.D);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -926,10 +990,10 @@ template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void 
 // Waves a SIMD that a kernel's registers are to leave room for: two of 256 at least, whose results then stay in
 // registers that vector instructions read.
 enum Kernel { kforward, kgrad_q, kgrad_kv };
-template <typename T> constexpr int occupancy(Kernel k, int dp, int wk) {
-  if (dp <= 32) return 3;
+template <typename T> constexpr int occupancy(bool direct, int dp, int wk) {
+  if (dp <= 32) return direct ? 4 : 3;
   if (dp <= 64) return 2;
-  return wk > 1 || sizeof(T) == 4 || k == kgrad_kv ? 1 : 2;
+  return wk > 1 || sizeof(T) == 4 ? 1 : 2;
 }
 
 enum Shape { kMany = 0, kSome = 1, kFew = 2 };   // columns of a block: 128, 64 or 16
@@ -938,7 +1002,9 @@ template <typename T, int DP, Kernel kKernel, typename F> hipError_t with_shape(
   constexpr int E = (int)sizeof(T) / 2;   // stages of as many bytes in each type
   typedef std::integral_constant<int, 64 / E> rows;
   typedef std::integral_constant<int, 4> four;
-  if (shape == kMany) return f(std::integral_constant<int, 2>(), four(), one(), std::integral_constant<int, kKernel != kforward && DP == 128 ? 32 : 64 / E>());
+  if constexpr (kKernel != kgrad_kv || DP < 128)
+    if (shape == kMany)
+      return f(std::integral_constant<int, 2>(), four(), one(), std::integral_constant<int, kKernel == kgrad_q && DP == 128 ? 32 : 64 / E>());
   if (shape == kSome) return f(one(), four(), one(), rows());
   return f(one(), one(), four(), std::integral_constant<int, 128 / E>());
 }
@@ -954,9 +1020,8 @@ template <typename T> hipError_t forward(const Args &p, int dp, int shape, hipSt
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kforward>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      constexpr int OCC = occupancy<T>(kforward, DP, WK);
-      if (p.dma & 1) forward_kernel<T, DP, NC, WC, WK, KT, OCC, true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
-      else forward_kernel<T, DP, NC, WC, WK, KT, OCC, false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      if (p.dma & 1) forward_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      else forward_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
       if (p.splits > 1) join_forward_kernel<T, DP><<<(unsigned)((p.cells + 3) / 4), 256, 0, st>>>(p);
       return hipGetLastError();
     });
@@ -967,10 +1032,9 @@ template <typename T> hipError_t grad_q(const Args &p, int dp, int shape, hipStr
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kgrad_q>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      constexpr int OCC = occupancy<T>(kgrad_q, DP, WK);
-      if (p.dma & 1) grad_q_kernel<T, DP, NC, WC, WK, KT, OCC, true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
-      else grad_q_kernel<T, DP, NC, WC, WK, KT, OCC, false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
-      if (p.splits > 1) join_sum_kernel<T, DP, false><<<(unsigned)((p.cells + 3) / 4), 256, 0, st>>>(p);
+      if (p.dma & 1) grad_q_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      else grad_q_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      if (p.splits > 1) join_sum_kernel<T, DP, false><<<(unsigned)((p.cells * (DP / 4) + 255) / 256), 256, 0, st>>>(p);
       return hipGetLastError();
     });
   });
@@ -980,11 +1044,10 @@ template <typename T> hipError_t grad_kv(const Args &p, int dp, int shape, hipSt
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kgrad_kv>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      constexpr int OCC = occupancy<T>(kgrad_kv, DP, WK);
-      if (p.dma & 2) grad_kv_kernel<T, DP, NC, WC, WK, KT, OCC, true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
-      else grad_kv_kernel<T, DP, NC, WC, WK, KT, OCC, false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      if (p.dma & 2) grad_kv_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      else grad_kv_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
       const int64_t rows = (int64_t)p.heads * p.Sk * 2;
-      if (p.splits > 1) join_sum_kernel<T, DP, true><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(p);
+      if (p.splits > 1) join_sum_kernel<T, DP, true><<<(unsigned)((rows * (DP / 4) + 255) / 256), 256, 0, st>>>(p);
       return hipGetLastError();
     });
   });

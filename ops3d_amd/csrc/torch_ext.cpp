@@ -1029,36 +1029,41 @@ ops3d_attention_tensor attention_tensor(const at::Tensor &t) {
   return {ptr(t), s[0], s[1], s[2]};
 }
 
-// [out, lse]; lse (for the backward) when keep.
-std::tuple<at::Tensor, Maybe> attention_forward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+// [out, lse, out_rest]; the latter two (for the backward; out_rest in 16 bits only) when keep.
+std::tuple<at::Tensor, Maybe, Maybe> attention_forward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
                                                 const Maybe &q_start, const Maybe &k_start, const Maybe &q_len,
                                                 const Maybe &k_len, bool causal, double scale, bool keep) {
   const Attention a = attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale);
   const DeviceGuard guard(q.device());
   const at::Tensor qd = channels_dense(q), kd = channels_dense(k), vd = channels_dense(v);
   at::Tensor out = at::empty(q.sizes(), q.options());
-  Maybe lse;
+  Maybe lse, rest;
   if (keep) lse = at::empty({a.p.items, a.p.heads, a.p.q_rows}, q.options().dtype(at::kFloat));
+  if (keep && q.scalar_type() != at::kFloat) rest = at::empty(q.sizes(), q.options());
   const size_t n = ops3d_attention_forward_workspace_bytes(&a.p);
   at::Tensor ws;
   if (n) ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
   const auto tq = attention_tensor(qd), tk = attention_tensor(kd), tv = attention_tensor(vd), to = attention_tensor(out);
-  const int rc = ops3d_attention_forward(&a.p, &tq, &tk, &tv, &to, lse ? (float *)ptr(*lse) : nullptr, ptr(ws), n, stream_of(q));
+  const int rc = ops3d_attention_forward(&a.p, &tq, &tk, &tv, &to, rest ? ptr(*rest) : nullptr,
+                                         lse ? (float *)ptr(*lse) : nullptr, ptr(ws), n, stream_of(q));
   if (rc != OPS3D_FDA_OK) raise(rc, "attention_forward failed");
-  return {out, lse};
+  return {out, lse, rest};
 }
 
 // [grad_q, grad_k, grad_v], None where not wanted (the latter two together).
 std::tuple<Maybe, Maybe, Maybe> attention_backward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
                                                    const Maybe &q_start, const Maybe &k_start, const Maybe &q_len,
                                                    const Maybe &k_len, bool causal, double scale, const at::Tensor &out,
-                                                   const at::Tensor &lse, const at::Tensor &grad_out, bool need_q, bool need_kv) {
+                                                   const at::Tensor &lse, const Maybe &rest, const at::Tensor &grad_out, bool need_q,
+                                                   bool need_kv) {
   const Attention a = attention_problem(q, k, v, q_start, k_start, q_len, k_len, causal, scale);
   linear_check(grad_out, "grad_output", q);
   if (grad_out.sizes() != q.sizes()) throw std::invalid_argument("grad_output must have the output's shape");
   if (out.device() != q.device() || out.scalar_type() != q.scalar_type() || out.sizes() != q.sizes() || !out.is_contiguous() ||
       lse.device() != q.device() || lse.scalar_type() != at::kFloat || !lse.is_contiguous() ||
-      lse.sizes() != at::IntArrayRef({a.p.items, a.p.heads, a.p.q_rows}))
+      lse.sizes() != at::IntArrayRef({a.p.items, a.p.heads, a.p.q_rows}) ||
+      (rest && (rest->device() != q.device() || rest->scalar_type() != q.scalar_type() || rest->sizes() != q.sizes() ||
+                !rest->is_contiguous())))
     throw std::invalid_argument("out and lse are not a forward's of this shape");
   const DeviceGuard guard(q.device());
   const at::Tensor qd = channels_dense(q), kd = channels_dense(k), vd = channels_dense(v), gd = channels_dense(grad_out);
@@ -1071,7 +1076,7 @@ std::tuple<Maybe, Maybe, Maybe> attention_backward(const at::Tensor &q, const at
   const auto some = [](const Maybe &t) { return t ? attention_tensor(*t) : ops3d_attention_tensor{}; };
   const auto tq = attention_tensor(qd), tk = attention_tensor(kd), tv = attention_tensor(vd), to = attention_tensor(out),
              tg = attention_tensor(gd), tgq = some(gq), tgk = some(gk), tgv = some(gv);
-  const int rc = ops3d_attention_backward(&a.p, &tq, &tk, &tv, &to, (const float *)ptr(lse), &tg, need_q ? &tgq : nullptr,
+  const int rc = ops3d_attention_backward(&a.p, &tq, &tk, &tv, &to, rest ? ptr(*rest) : nullptr, (const float *)ptr(lse), &tg, need_q ? &tgq : nullptr,
                                           need_kv ? &tgk : nullptr, need_kv ? &tgv : nullptr, ptr(ws), n, stream_of(q));
   if (rc != OPS3D_FDA_OK) raise(rc, "attention_backward failed");
   return {gq, gk, gv};
@@ -1082,9 +1087,9 @@ class AttentionNode : public torch::autograd::Function<AttentionNode> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
                             const Maybe &q_start, const Maybe &k_start, const Maybe &q_len, const Maybe &k_len, bool causal,
                             double scale) {
-    auto [out, lse] = attention_forward(q, k, v, q_start, k_start, q_len, k_len, causal, scale, true);
+    auto [out, lse, rest] = attention_forward(q, k, v, q_start, k_start, q_len, k_len, causal, scale, true);
     const auto some = [](const Maybe &t) { return t ? *t : at::Tensor(); };
-    ctx->save_for_backward({q, k, v, some(q_start), some(k_start), some(q_len), some(k_len), out, *lse});
+    ctx->save_for_backward({q, k, v, some(q_start), some(k_start), some(q_len), some(k_len), out, *lse, some(rest)});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["needs"] = std::vector<int64_t>{q.requires_grad(), k.requires_grad(), v.requires_grad()};
@@ -1100,7 +1105,7 @@ class AttentionNode : public torch::autograd::Function<AttentionNode> {
     if (gq || gk || gv) {
       const at::NoGradGuard no_grad;
       auto [dq, dk, dv] = attention_backward(s[0], s[1], s[2], some(3), some(4), some(5), some(6), ctx->saved_data["causal"].toBool(),
-                                             ctx->saved_data["scale"].toDouble(), s[7], s[8], grads[0], gq, gk || gv);
+                                             ctx->saved_data["scale"].toDouble(), s[7], s[8], some(9), grads[0], gq, gk || gv);
       if (gq) out[0] = *dq;
       if (gk) out[1] = *dk;
       if (gv) out[2] = *dv;

@@ -13,7 +13,7 @@ count roundings (U = 2^-24, u half a step of dtype):
 * fp16: P is held 2^10 up, so that one below 2^-14 is off by 2^-35 at most; dS is not: by 2^-25;
 * every type: a power, and a product in fp32 or an operand of bf16, below 2^-126 may count as 0, so that a P is off by
   2^-125 more, and a dS by that times its factor and once more;
-* the sum of out grad_out is formed from the rounded out.
+* the sum of out grad_out is formed from the rounded out and what rounding took from it, itself rounded.
 """
 from __future__ import annotations
 
@@ -72,7 +72,7 @@ def sequence(q, k, v, causal, scale, grad=None):
         mean_d = (p * d).sum(1, keepdim=True)
         y = p @ vh
         e_y = (p * (d + u + hk)) @ vh.abs() + low_p * (seen.double() @ vh.abs()) + y.abs() * (mean_d + hk + 4 * U)
-        e_y = e_y + _round(y, dtype)
+        e_o, e_y = e_y + u * _round(y, dtype), e_y + _round(y, dtype)
         out["y"][0][:, h], out["y"][1][:, h] = y, torch.where(some, e_y, 0.0)
         if grad is None:
             continue
@@ -82,7 +82,7 @@ def sequence(q, k, v, causal, scale, grad=None):
         dp = g @ vh.t()
         e_dp = (D + 2) * U * (g.abs() @ vh.abs().t())
         delta = (y * g).sum(1, keepdim=True)
-        e_delta = (e_y * g.abs()).sum(1, keepdim=True) + (D + 2) * U * (y * g).abs().sum(1, keepdim=True)
+        e_delta = (e_o * g.abs()).sum(1, keepdim=True) + (D + 2) * U * (y * g).abs().sum(1, keepdim=True)
         ds = p * (dp - delta)
         e_ds = ds.abs() * (d + u + 3 * U) + p * (e_dp + e_delta + 2 * U * (dp.abs() + delta.abs()))
         e_ds = e_ds + seen.double() * (low_ds + tiny * (dp.abs() + delta.abs()))

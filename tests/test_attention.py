@@ -131,8 +131,8 @@ def test_c_refusals_before_device_work(lib):
     def tensor(data=16, item=0, token=8, head=8):
         return _extension._AttentionTensor(data, item, token, head)
 
-    def forward(p, q=tensor(), k=tensor(), v=tensor(), o=tensor(), lse=None, ws=None, n=0):
-        return lib.ops3d_attention_forward(p, q, k, v, o, lse, ws, n, None)
+    def forward(p, q=tensor(), k=tensor(), v=tensor(), o=tensor(), rest=None, lse=None, ws=None, n=0):
+        return lib.ops3d_attention_forward(p, q, k, v, o, rest, lse, ws, n, None)
 
     packed = {"q_start": 16, "k_start": 16, "items": 1, "sequences": 3, "q_start_count": 4, "k_start_count": 3}
     bad = [{"dtype": 3}, {"heads": 3}, {"heads": 0}, {"kv_heads": 0}, {"dim": 0}, {"dim": 129}, {"scale": 0.0}, {"scale": -1.0},
@@ -143,18 +143,18 @@ def test_c_refusals_before_device_work(lib):
     for kw in bad:
         assert forward(problem(**kw), ws=256, n=2 ** 60) == 1, kw
         assert lib.ops3d_fda_last_error()
-    for kw in ({"q": tensor(None)}, {"k": tensor(None)}, {"v": tensor(18)}, {"o": tensor(None)}, {"q": None}, {"lse": 18}, {"q": tensor(token=-1)}):
-        assert forward(problem(), **kw) == 1, kw
-    assert lib.ops3d_attention_forward(None, None, None, None, None, None, None, 0, None) == 1
+    for kw in ({"q": tensor(None)}, {"k": tensor(None)}, {"v": tensor(18)}, {"o": tensor(None)}, {"q": None}, {"lse": 18}, {"rest": 19, "p": problem(dtype=1)}, {"q": tensor(token=-1)}):
+        assert forward(**{"p": problem(), **kw}) == 1, kw
+    assert lib.ops3d_attention_forward(None, None, None, None, None, None, None, None, 0, None) == 1
     assert forward(problem(items=0)) == forward(problem(q_rows=0)) == 0
     few = problem(q_rows=1, k_rows=100000, items=1)
     need = lib.ops3d_attention_forward_workspace_bytes(few)
     assert need > 0
     assert forward(few, ws=None, n=need) == forward(few, ws=256, n=need - 1) == forward(few, ws=264, n=need) == 1
 
-    def backward(p, q=tensor(), k=tensor(), v=tensor(), o=tensor(), lse=16, g=tensor(), gq=tensor(), gk=tensor(), gv=tensor(), ws=256, n=None):
+    def backward(p, q=tensor(), k=tensor(), v=tensor(), o=tensor(), rest=None, lse=16, g=tensor(), gq=tensor(), gk=tensor(), gv=tensor(), ws=256, n=None):
         n = lib.ops3d_attention_backward_workspace_bytes(p) if n is None else n
-        return lib.ops3d_attention_backward(p, q, k, v, o, lse, g, gq, gk, gv, ws, n, None)
+        return lib.ops3d_attention_backward(p, q, k, v, o, rest, lse, g, gq, gk, gv, ws, n, None)
 
     for kw in ({"lse": None}, {"lse": 18}, {"gk": None}, {"gv": None}, {"g": None}, {"o": tensor(None)}, {"ws": None}, {"n": 16}, {"gq": tensor(17)}):
         assert backward(problem(), **kw) == 1, kw
