@@ -75,7 +75,7 @@ Plan plan_of(const ops3d_attention_problem *p, int64_t columns, int64_t others, 
     const int width = shape == kMany ? 128 : shape == kSome ? 64 : 16, stage = (shape == kFew ? 128 : 64) / e;
     const int64_t blocks = ceil_div(per, width) * runs * p->kv_heads;
     // two blocks a CU, or four where they differ in what they have to do, in parts of 2 stages at least
-    int64_t splits = blocks ? (p->causal || p->q_start ? 1024 : 512) / blocks : 1;
+    int64_t splits = blocks ? ((p->causal || p->q_start ? 1024 : 512) + blocks / 2) / blocks : 1;
     const int64_t most = ceil_div(far, 2 * stage);
     splits = splits > most ? most : splits;
     splits = splits < 1 ? 1 : splits;
@@ -155,11 +155,11 @@ Args args_of(const ops3d_attention_problem *p) {
   return a;
 }
 
-// Whether a stage's rows may go straight to LDS: whole padded rows at 16-byte boundaries, whose places in a stage of
+// Whether a stage's rows may go straight to LDS: whole chunks at 16-byte boundaries, whose places in a stage of
 // 128 and in a group of heads fit 32 bits.
 bool direct(const ops3d_attention_problem *p, const Tensor &t) {
   const int64_t es = elem_size(p->dtype);
-  return p->dim == padded_dim(p->dim) && !((reinterpret_cast<uintptr_t>(t.p) | (uint64_t)(t.item * es) | (uint64_t)(t.token * es) | (uint64_t)(t.head * es)) & 15u) &&
+  return p->dim * es % 16 == 0 && !((reinterpret_cast<uintptr_t>(t.p) | (uint64_t)(t.item * es) | (uint64_t)(t.token * es) | (uint64_t)(t.head * es)) & 15u) &&
          t.token < (1 << 20) && t.head < (1 << 20) && p->heads / p->kv_heads <= 256;   // 2^31 bytes, of 4 an element
 }
 

@@ -88,21 +88,20 @@ template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, in
   const int64_t *own = KEYS ? p.k_start : p.q_start, *other = KEYS ? p.q_start : p.k_start;
   const int own_count = KEYS ? p.k_count : p.q_count, other_count = KEYS ? p.q_count : p.k_count;
   const int own_rows = KEYS ? p.Sk : p.Sq, other_rows = KEYS ? p.Sq : p.Sk;
-  int carry = 0, before = 0, j = -1, lower = 0;
-  for (int base = 0; base < p.E + 2; base += 64) {
+  int carry = 0, before = 0, j = -1, lower = 0, rows = 0, first = 0;
+  for (int base = 0; base < p.E + 2 && j < 0; base += 64) {
     const Segment s = segment_at(own, own_count, own_rows, base + lane, carry);
     const int tiles = base + lane < p.E + 2 ? (int)(((int64_t)(s.upper - s.lower) * unit + per - 1) / per) : 0;
     const int incl = before + ops3d_segments::scan_add(tiles);
     const uint64_t m = __ballot(incl > t);
+    before = __builtin_amdgcn_readlane(incl, 63);
     if (m) {
       const int src = __builtin_ctzll(m);
       j = base + src;
       lower = __builtin_amdgcn_readlane(s.lower, src);
-      w.rows = __builtin_amdgcn_readlane(s.upper, src) - lower;
-      w.first = (t - (__builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane(tiles, src))) * per;
-      break;
+      rows = __builtin_amdgcn_readlane(s.upper, src) - lower;
+      first = (t - (__builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane(tiles, src))) * per;
     }
-    before = __builtin_amdgcn_readlane(incl, 63);
   }
   if (j < 0) return false;
   int o_lower = 0, o_rows = 0;
@@ -120,8 +119,10 @@ template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, in
   w.item = 0;
   w.q0 = KEYS ? o_lower : lower;
   w.k0 = KEYS ? lower : o_lower;
-  w.nq = KEYS ? o_rows : (in ? w.rows : 0);
-  w.nk = KEYS ? (in ? w.rows : 0) : o_rows;
+  w.nq = KEYS ? o_rows : (in ? rows : 0);
+  w.nk = KEYS ? (in ? rows : 0) : o_rows;
+  w.rows = rows;
+  w.first = first;
   return true;
 }
 
@@ -179,22 +180,27 @@ template <typename T, int DP, int R, int NT> struct Stage {
     }
   }
   // The same without registers between: an instruction of a wave fills 1024 bytes of LDS in lane order, so the
-  // lane at a place loads the chunk that the swizzle puts there.  For D = DP and rows that start at 16-byte
+  // lane at a place loads the chunk that the swizzle puts there.  For whole chunks, and rows that start at 16-byte
   // boundaries.  off: the lanes' places, in bytes, of rows at at(row); rows from n on are the last one again.
-  template <typename F> static __device__ __forceinline__ void places(uint32_t (&off)[NL], F at, int n) {
+  // Chunks behind D stay as they are: 0 from clear() on.
+  template <typename F> static __device__ __forceinline__ void places(uint32_t (&off)[NL], F at, int n, int D) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int slot = (wave * NL + i) * 64 + lane, row = slot / RC, chunk = (address(row, slot % RC) >> 4) - row * RC;
-      off[i] = at(min(row, n - 1)) + chunk * 16;
+      off[i] = chunk * CH < D ? at(min(row, n - 1)) + chunk * 16 : ~0u;
     }
   }
-  static __device__ __forceinline__ void load_lds(char *lds, const char *base, const uint32_t (&off)[NL]) {
+  static __device__ __forceinline__ void load_lds(char *lds, const char *base, const uint32_t (&off)[NL], int D) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + off[i]),
+      if (D == DP || off[i] != ~0u) __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + off[i]),
                                        (__attribute__((address_space(3))) void *)(lds + (wave * NL + i) * 1024), 16, 0, 0);
+  }
+  static __device__ __forceinline__ void clear(char *lds, int bytes) {
+    for (int i = threadIdx.x * 16; i < bytes; i += NT * 16) *reinterpret_cast<uint4 *>(lds + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
   }
   static __device__ __forceinline__ void store(char *lds, const uint4 (&v)[NL]) {
 #pragma unroll
@@ -390,19 +396,19 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   uint4 kv[DMA ? 1 : ST::NL], vv[DMA ? 1 : ST::NL];
   uint32_t k_off[DMA ? ST::NL : 1], v_off[DMA ? ST::NL : 1];
   if constexpr (DMA) {
-    ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, KT);
-    ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, KT);
+    ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, KT, p.D);
+    ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, KT, p.D);
   }
   const auto load = [&](int k0, int buf) __attribute__((always_inline)) {
     const int left = k_end - k0;
     if constexpr (DMA) {
       char *const lk = lds + buf * 2 * ST::kBytes;
       if (left < KT) {
-        ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, left);
-        ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, left);
+        ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, left, p.D);
+        ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, left, p.D);
       }
-      ST::load_lds(lk, reinterpret_cast<const char *>(kb + k0 * p.k.token), k_off);
-      ST::load_lds(lk + ST::kBytes, reinterpret_cast<const char *>(vb + k0 * p.v.token), v_off);
+      ST::load_lds(lk, reinterpret_cast<const char *>(kb + k0 * p.k.token), k_off, p.D);
+      ST::load_lds(lk + ST::kBytes, reinterpret_cast<const char *>(vb + k0 * p.v.token), v_off, p.D);
     } else {
       ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
       ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
@@ -497,6 +503,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     buf ^= 1;
     at.flip();
   };
+  if (DMA && p.D < DP) ST::clear(lds, 4 * ST::kBytes);
   if (k_begin < k_end) load(k_begin, 0);
   while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
   while (k0 < k_end) stage(std::true_type());
@@ -673,19 +680,19 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   uint4 kv[DMA ? 1 : ST::NL], vv[DMA ? 1 : ST::NL];
   uint32_t k_off[DMA ? ST::NL : 1], v_off[DMA ? ST::NL : 1];
   if constexpr (DMA) {
-    ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, KT);
-    ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, KT);
+    ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, KT, p.D);
+    ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, KT, p.D);
   }
   const auto load = [&](int k0, int buf) __attribute__((always_inline)) {
     const int left = k_end - k0;
     if constexpr (DMA) {
       char *const lk = lds + buf * 2 * ST::kBytes;
       if (left < KT) {
-        ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, left);
-        ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, left);
+        ST::places(k_off, [&](int r) { return r * (uint32_t)(p.k.token * sizeof(T)); }, left, p.D);
+        ST::places(v_off, [&](int r) { return r * (uint32_t)(p.v.token * sizeof(T)); }, left, p.D);
       }
-      ST::load_lds(lk, reinterpret_cast<const char *>(kb + k0 * p.k.token), k_off);
-      ST::load_lds(lk + ST::kBytes, reinterpret_cast<const char *>(vb + k0 * p.v.token), v_off);
+      ST::load_lds(lk, reinterpret_cast<const char *>(kb + k0 * p.k.token), k_off, p.D);
+      ST::load_lds(lk + ST::kBytes, reinterpret_cast<const char *>(vb + k0 * p.v.token), v_off, p.D);
     } else {
       ST::load(kv, [&](int r) { return kb + (k0 + r) * p.k.token; }, left, p.D);
       ST::load(vv, [&](int r) { return vb + (k0 + r) * p.v.token; }, left, p.D);
@@ -746,6 +753,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     buf ^= 1;
     at.flip();
   };
+  if (DMA && p.D < DP) ST::clear(lds, 4 * ST::kBytes);
   if (k_begin < k_end) load(k_begin, 0);
   while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
   while (k0 < k_end) stage(std::true_type());
@@ -834,8 +842,8 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       const int t = divide(p, c + r);
       return (uint32_t)((t * (uint32_t)x.token + (c + r - t * p.G) * (uint32_t)x.head) * sizeof(T));
     };
-    ST::places(q_off, [&](int r) { return at(p.q, r); }, n);
-    ST::places(g_off, [&](int r) { return at(p.g, r); }, n);
+    ST::places(q_off, [&](int r) { return at(p.q, r); }, n, p.D);
+    ST::places(g_off, [&](int r) { return at(p.g, r); }, n, p.D);
   };
   const auto load = [&](int c0, int buf) __attribute__((always_inline)) {
     const int left = c_end - c0;
@@ -843,8 +851,8 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       char *const lq = lds + buf * 2 * ST::kBytes;
       const int t0 = uniform(divide(p, c0));
       if (!fixed || left < QT) place_rows(c0, min(left, QT));
-      ST::load_lds(lq, reinterpret_cast<const char *>(qb + t0 * p.q.token), q_off);
-      ST::load_lds(lq + ST::kBytes, reinterpret_cast<const char *>(gb + t0 * p.g.token), g_off);
+      ST::load_lds(lq, reinterpret_cast<const char *>(qb + t0 * p.q.token), q_off, p.D);
+      ST::load_lds(lq + ST::kBytes, reinterpret_cast<const char *>(gb + t0 * p.g.token), g_off, p.D);
     } else {
       const auto at = [&](const T *base, const Tensor &x, int r) __attribute__((always_inline)) {
         const int t = divide(p, c0 + r);
@@ -930,6 +938,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     buf ^= 1;
     at.flip();
   };
+  if (DMA && p.D < DP) ST::clear(lds, 4 * ST::kBytes);
   if (c_begin < c_end) load(c_begin, 0);
   while (c0 < c_end && c0 < all_see) stage(std::true_type());
   while (c0 < c_end) stage(std::false_type());

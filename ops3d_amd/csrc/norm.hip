@@ -86,6 +86,29 @@ template <int L> __device__ __forceinline__ float row_sum(float v, float *lds) {
   }
 }
 
+// Two sums at once.
+template <int L> __device__ __forceinline__ float2 row_sums(float u, float v, float *lds) {
+  if constexpr (L <= 64) {
+    return make_float2(sum<L>(u), sum<L>(v));
+  } else {
+    u = sum<64>(u);
+    v = sum<64>(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      lds[(threadIdx.x >> 6) * 2] = u;
+      lds[(threadIdx.x >> 6) * 2 + 1] = v;
+    }
+    __syncthreads();
+    float2 s = make_float2(lds[0], lds[1]);
+#pragma unroll
+    for (int i = 1; i < L / 64; ++i) {
+      s.x += lds[2 * i];
+      s.y += lds[2 * i + 1];
+    }
+    return s;
+  }
+}
+
 // The product, rounded: not one with a difference that it goes into, which would then be another mean than
 // the one that is stored.
 __device__ __forceinline__ float rounded(float a, float b) {
@@ -97,7 +120,7 @@ __device__ __forceinline__ float rounded(float a, float b) {
 // L lanes a row, NCH chunks a lane: chunk j of lane i is chunk j L + i of the row.
 template <typename T, typename W, int NCH, int L, int NT> __global__ __launch_bounds__(NT) void forward_kernel(Args p) {
   constexpr int CH = 16 / (int)sizeof(T), G = NT / L;
-  __shared__ float lds[L > 64 ? L / 64 : 1];
+  __shared__ float lds[L > 64 ? L / 32 : 1];
   const int lane = threadIdx.x % L;
   const T *x = static_cast<const T *>(p.x);
   float w[NCH][CH], b[NCH][CH];
@@ -140,8 +163,9 @@ template <typename T, typename W, int NCH, int L, int NT> __global__ __launch_bo
         dd = fmaf(u, u, dd);
       }
     }
-    const float rest = rounded(row_sum<L>(d, lds), inv);
-    const float var = fmaf(-rest, rest, row_sum<L>(dd, lds) * inv);
+    const float2 sums = row_sums<L>(d, dd, lds);
+    const float rest = rounded(sums.x, inv);
+    const float var = fmaf(-rest, rest, sums.y * inv);
     const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + p.eps);
     if (p.stats && lane == 0) {
       p.stats[3 * row] = mean;
@@ -163,7 +187,7 @@ template <typename T, typename W, int NCH, int L, int NT> __global__ __launch_bo
 // The same for rows that no block's registers hold.
 template <typename T, typename W> __global__ __launch_bounds__(256) void forward_long_kernel(Args p) {
   constexpr int CH = 16 / (int)sizeof(T), L = 256;
-  __shared__ float lds[L / 64];
+  __shared__ float lds[L / 32];
   const float inv = 1.f / (float)p.C;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T *x = static_cast<const T *>(p.x) + row * p.ldx;
@@ -185,8 +209,9 @@ template <typename T, typename W> __global__ __launch_bounds__(256) void forward
         dd = fmaf(u, u, dd);
       }
     }
-    const float rest = rounded(row_sum<L>(d, lds), inv);
-    const float var = fmaf(-rest, rest, row_sum<L>(dd, lds) * inv);
+    const float2 sums = row_sums<L>(d, dd, lds);
+    const float rest = rounded(sums.x, inv);
+    const float var = fmaf(-rest, rest, sums.y * inv);
     const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + p.eps);
     if (p.stats && threadIdx.x == 0) {
       p.stats[3 * row] = mean;
@@ -243,7 +268,7 @@ __device__ __forceinline__ void store_partial(float *part, float (&v)[NCH][CH], 
 
 template <typename T, typename W, int NCH, int L, int NT> __global__ __launch_bounds__(NT) void backward_kernel(Args p) {
   constexpr int CH = 16 / (int)sizeof(T), G = NT / L;
-  __shared__ float lds[L >= NT ? L / 64 : NT / 64 * NCH * CH * (L < 64 ? L : 64)];
+  __shared__ float lds[L >= NT ? L / 32 : NT / 64 * NCH * CH * (L < 64 ? L : 64)];
   const int lane = threadIdx.x % L;
   const T *x = static_cast<const T *>(p.x), *g = static_cast<const T *>(p.g);
   float w[NCH][CH], aw[NCH][CH], ab[NCH][CH];
@@ -290,8 +315,9 @@ template <typename T, typename W, int NCH, int L, int NT> __global__ __launch_bo
     }
     if (row + step < p.rows) load(row + step);
     if (!p.out) continue;
-    s = row_sum<L>(s, lds) * inv;
-    sn = row_sum<L>(sn, lds) * inv;
+    const float2 sums = row_sums<L>(s, sn, lds);
+    s = sums.x * inv;
+    sn = sums.y * inv;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
       const int col = (j * L + lane) * CH;
@@ -309,7 +335,7 @@ template <typename T, typename W, int NCH, int L, int NT> __global__ __launch_bo
 // Rows that no block's registers hold: grad_x, a block a row ...
 template <typename T, typename W> __global__ __launch_bounds__(256) void backward_long_kernel(Args p) {
   constexpr int CH = 16 / (int)sizeof(T), L = 256;
-  __shared__ float lds[L / 64];
+  __shared__ float lds[L / 32];
   const float inv = 1.f / (float)p.C;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T *x = static_cast<const T *>(p.x) + row * p.ldx, *g = static_cast<const T *>(p.g) + row * p.ldg;
@@ -335,8 +361,9 @@ template <typename T, typename W> __global__ __launch_bounds__(256) void backwar
         if (step) store_chunk<T>(static_cast<T *>(p.out) + row * p.C + col, pack<T>(dx), p.C - col);
       }
       if (step == 0) {
-        s = row_sum<L>(s, lds) * inv;
-        sn = row_sum<L>(sn, lds) * inv;
+        const float2 sums = row_sums<L>(s, sn, lds);
+        s = sums.x * inv;
+        sn = sums.y * inv;
       }
     }
   }
@@ -448,7 +475,7 @@ template <typename T, typename W> hipError_t forward(const Args &a, int dtype, h
   }
   return with_plan<T>(plan, [&](auto l, auto c) {
     constexpr int L = decltype(l)::value, NT = L < 256 ? 256 : L;
-    forward_kernel<T, W, decltype(c)::value, L, NT><<<grid_for((a.rows + NT / L - 1) / (NT / L), 2048), NT, 0, st>>>(a);
+    forward_kernel<T, W, decltype(c)::value, L, NT><<<grid_for((a.rows + NT / L - 1) / (NT / L), 2048 * 256 / NT), NT, 0, st>>>(a);
     return hipGetLastError();
   });
 }
