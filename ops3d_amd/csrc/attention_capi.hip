@@ -64,30 +64,44 @@ struct Plan {
   int shape, tiles, tiles_item, splits;
 };
 
-// columns and others: of an item, or of all packed sequences.
+// columns and others: of an item, or of all packed sequences.  Measured in bf16 (us):
+//   wide tiles read the rows that come by least often, if there are two blocks a CU: 8192 x 8192, 8 heads of 32
+//     channels, forward: 141 in tiles of 128, 151 of 64, 298 of 16; 4096 x 4096: 51, 47, 81
+//   narrow tiles, where there are few columns and few rows: 1024 x 1024: 15, 12, 10
+//   parts, where few columns see many rows: 200 x 37376, 2 items: 360 in one, 54 in 8, 42 in 16; one query of 32/8
+//     heads of 128 over 8 caches of 8192: 42 in 8, 39 in 16, 50 in narrow tiles
+//   twice the blocks, where sequences or a causal mask give them different amounts to do: grad k v of 8192 causal
+//     tokens, 16/4 heads of 128: 273 in one part, 189 + 16 for the join in 2
 Plan plan_of(const ops3d_attention_problem *p, int64_t columns, int64_t others, int widest) {
   const int64_t runs = p->q_start ? p->sequences : p->items;   // what has tiles of its own
-  const int64_t per = p->q_start ? ceil_div(columns, runs) : columns, far = p->q_start ? ceil_div(others, runs) : others;
-  const int e = elem_size(p->dtype) / 2;
-  Plan best{};
-  for (const int shape : {kMany, kSome, kFew}) {
-    if (shape < widest) continue;
-    const int width = shape == kMany ? 128 : shape == kSome ? 64 : 16, stage = (shape == kFew ? 128 : 64) / e;
-    const int64_t blocks = ceil_div(per, width) * runs * p->kv_heads;
-    // two blocks a CU, or four where they differ in what they have to do, in parts of 2 stages at least
-    int64_t splits = blocks ? ((p->causal || p->q_start ? 1024 : 512) + blocks / 2) / blocks : 1;
-    const int64_t most = ceil_div(far, 2 * stage);
-    splits = splits > most ? most : splits;
-    splits = splits < 1 ? 1 : splits;
-    best.shape = shape;
-    best.splits = (int)splits;
-    best.tiles_item = (int)ceil_div(columns, width);
-    // packed: each segment may end inside a tile
-    best.tiles = (int)(p->q_start ? columns / width + p->sequences + 2 : 0);
-    if ((per > width / 2 || shape == kFew) && (blocks * splits >= 256 || shape == kFew)) break;
+  const int64_t per = p->q_start ? ceil_div(columns, runs) : columns;
+  // of packed sequences the largest count, of which the sizes here say little
+  const int64_t mean = p->q_start ? ceil_div(others, runs) : others, far = p->q_start && 4 * mean < others ? 4 * mean : others;
+  const int64_t stages = far / (elem_size(p->dtype) == 4 ? 32 : 64);
+  const bool uneven = p->causal || p->q_start;
+  const auto blocks = [&](int width) { return ceil_div(per, width) * runs * p->kv_heads; };
+  const auto parts = [&](int64_t target, int64_t blocks) {
+    const int64_t n = blocks ? (target + blocks / 2) / blocks : 1, most = stages / 2;
+    return (int)(n < 2 || most < 2 ? 1 : n < most ? n : most);
+  };
+  Plan plan{};
+  plan.splits = 1;
+  if (widest == kMany && blocks(128) >= 512) {
+    plan.shape = kMany;
+    plan.splits = uneven ? parts(1024, blocks(128)) : 1;
+  } else if (blocks(64) >= 256) {
+    plan.shape = kSome;
+    plan.splits = uneven ? parts(1024, blocks(64)) : 1;
+  } else if (stages >= 32) {
+    plan.shape = widest == kMany && per > 64 ? kMany : kSome;
+    plan.splits = plan.shape == kMany ? parts(uneven ? 1024 : 512, blocks(128)) : parts(1024, blocks(64));
+  } else {
+    plan.shape = kFew;
   }
-  if (!p->q_start) best.tiles = 0;
-  return best;
+  const int width = plan.shape == kMany ? 128 : plan.shape == kSome ? 64 : 16;
+  plan.tiles_item = (int)ceil_div(columns, width);
+  plan.tiles = p->q_start ? (int)(columns / width + p->sequences + 2) : 0;   // packed: each segment may end inside a tile
+  return plan;
 }
 Plan plan_queries(const ops3d_attention_problem *p) { return plan_of(p, p->q_rows * (p->heads / p->kv_heads), p->k_rows, kMany); }
 // Keys of 128 channels: two results, K and V for each column are too many registers for tiles of 128 columns

@@ -1005,7 +1005,8 @@ template <typename T> constexpr int occupancy(bool direct, int dp, int wk) {
   return wk > 1 || sizeof(T) == 4 ? 1 : 2;
 }
 
-enum Shape { kMany = 0, kSome = 1, kFew = 2 };   // columns of a block: 128, 64 or 16
+// Columns of a block: 128, 64, or 16, of which each of 4 waves takes a quarter of a stage's rows.
+enum Shape { kMany = 0, kSome = 1, kFew = 2 };
 template <typename T, int DP, Kernel kKernel, typename F> hipError_t with_shape(int shape, F f) {
   typedef std::integral_constant<int, 1> one;
   constexpr int E = (int)sizeof(T) / 2;   // stages of as many bytes in each type
