@@ -9,6 +9,9 @@ it to ``FlashDeformAttnFromOffsets``, which forms the locations inside the kerne
 divide, cat or split pass on either side of the op.  With ``level_value_proj`` the values of each
 level have a projection of their own (``GroupedLinear`` over the flattened levels), and a ``residual``
 given to the forward is added in the output projection's epilogue.
+
+``SelfAttention3D`` is the layer beside it in which every token sees all others: object queries among
+themselves, the tokens of a coarse level, or crops of different sizes packed one behind another.
 """
 from __future__ import annotations
 
@@ -17,8 +20,11 @@ import math
 import torch
 from torch import nn
 
+from .attention import packed_attention
 from .flash_deform_attn import FlashDeformAttnFromOffsets
 from .linear import fused_linear, grouped_linear
+from .norm import layer_norm
+from .rotary import rotary_positions
 
 
 class GroupedLinear(nn.Module):
@@ -120,3 +126,73 @@ class FlashDeformAttn3D(nn.Module):
         if _plain_linear(self.output_proj):
             return fused_linear(out, self.output_proj.weight, self.output_proj.bias, residual=residual)
         return self.output_proj(out) + residual
+
+
+class LayerNorm(nn.Module):
+    """layer_norm over the last axis with a weight and a bias.  Kept in float32 beside 16-bit inputs, they get
+    float32 gradients, and no input is cast."""
+
+    def __init__(self, width: int, eps: float = 1e-5, bias: bool = True):
+        super().__init__()
+        self.width, self.eps = width, eps
+        self.weight = nn.Parameter(torch.ones(width))
+        self.bias = nn.Parameter(torch.zeros(width)) if bias else None
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class SelfAttention3D(nn.Module):
+    """norm -> qkv -> rotary positions of queries and keys -> attention over all tokens -> output_proj, and x added.
+
+    forward(x [B,S,C] or [S,C], positions [S,A] or [B,S,A] (float32 or int64), start, lengths) -> x's shape:
+    x + output_proj(attention).  start [E + 1] int64 on x's device: the rows of x [S,C] are E packed
+    sequences (see ``packed_attention``).  lengths [B] int64: how many rows of each item of x [B,S,C] count;
+    the others see nothing and are seen by none.
+
+    num_kv_heads key and value heads are shared by num_heads query heads.  sections: how many channel pairs
+    of a head turn along each of the A axes; by default head_dim / 2 over three axes (depth, height, width), as
+    evenly as they go, None of them with an empty tuple (positions are then not looked at).  The residual is
+    added in output_proj's epilogue, where that is a plain nn.Linear without hooks.
+    """
+
+    def __init__(self, embed_dim: int = 256, num_heads: int = 8, num_kv_heads: int | None = None, sections=None,
+                 theta: float = 10000.0, causal: bool = False, eps: float = 1e-5):
+        super().__init__()
+        num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+        if embed_dim % num_heads:
+            raise ValueError(f"embed_dim ({embed_dim}) must be divisible by num_heads ({num_heads})")
+        if num_kv_heads < 1 or num_heads % num_kv_heads:
+            raise ValueError(f"num_heads ({num_heads}) must be divisible by num_kv_heads ({num_kv_heads})")
+        self.embed_dim, self.num_heads, self.num_kv_heads = embed_dim, num_heads, num_kv_heads
+        self.head_dim = embed_dim // num_heads
+        pairs = self.head_dim // 2
+        self.sections = tuple((pairs + a) // 3 for a in range(3)) if sections is None else tuple(sections)
+        if sum(self.sections) > pairs:
+            raise ValueError(f"sections {self.sections} do not fit heads of {self.head_dim} channels")
+        self.theta, self.causal = theta, causal
+        self.norm = LayerNorm(embed_dim, eps)
+        self.qkv = nn.Linear(embed_dim, (num_heads + 2 * num_kv_heads) * self.head_dim)
+        self.output_proj = nn.Linear(embed_dim, embed_dim)
+        self.reset_parameters()
+
+    @torch.no_grad()
+    def reset_parameters(self) -> None:
+        for m in (self.qkv, self.output_proj):
+            nn.init.xavier_uniform_(m.weight)
+            nn.init.zeros_(m.bias)
+
+    def forward(self, x, positions=None, start=None, lengths=None):
+        H, Hk = self.num_heads, self.num_kv_heads
+        y = self.norm(x)
+        y = fused_linear(y, self.qkv.weight, self.qkv.bias) if _plain_linear(self.qkv) else self.qkv(y)
+        qk, v = y.unflatten(-1, (H + 2 * Hk, self.head_dim)).split([H + Hk, Hk], dim=-2)
+        if self.sections:
+            if positions is None:
+                raise ValueError("positions are needed for the sections")
+            qk = rotary_positions(qk, positions, self.sections, self.theta)
+        q, k = qk.split([H, Hk], dim=-2)
+        out = packed_attention(q, k, v, q_start=start, q_len=lengths, k_len=lengths, causal=self.causal).flatten(-2)
+        if _plain_linear(self.output_proj):
+            return fused_linear(out, self.output_proj.weight, self.output_proj.bias, residual=x)
+        return self.output_proj(out) + x
