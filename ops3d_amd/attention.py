@@ -56,8 +56,8 @@ def packed_attention(q, k, v, q_start=None, k_start=None, q_len=None, k_len=None
     many of an item's rows count (a cache's filled part, a padded batch).  Queries see the keys of their
     own sequence; causal, query i sees key j where ``j <= i + keys - queries``: the last query sees all, and
     one new token its whole cache.  A query that sees no key gives 0.  Rows that do not count or are in no
-    sequence are not read; their outputs and gradients are 0.  Among those that count, a key that a causal
-    mask hides is multiplied by 0, so NaN or infinity in it may reach queries before it.
+    sequence are not read; their outputs and gradients are 0.  NaN and infinities in keys and values reach
+    the queries that see them, and no others.
 
     q, k and v may be strided between items, tokens and heads (parts of one projection, a transposed
     cache); with strided channels they are copied.  Under autocast they are cast to its dtype.

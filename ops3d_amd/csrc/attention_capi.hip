@@ -68,7 +68,7 @@ struct Plan {
 //   wide tiles read the rows that come by least often, if there are two blocks a CU: 8192 x 8192, 8 heads of 32
 //     channels, forward: 141 in tiles of 128, 151 of 64, 298 of 16; 4096 x 4096: 51, 47, 81
 //   narrow tiles, where there are few columns and few rows: 1024 x 1024: 15, 12, 10
-//   parts, where few columns see many rows: 200 x 37376, 2 items: 360 in one, 54 in 8, 42 in 16; one query of 32/8
+//   parts, where few columns see many rows: 200 x 37376, 2 items: 360 in one, 49 in 8, 42 in 16; one query of 32/8
 //     heads of 128 over 8 caches of 8192: 42 in 8, 39 in 16, 50 in narrow tiles
 //   twice the blocks, where sequences or a causal mask give them different amounts to do: grad k v of 8192 causal
 //     tokens, 16/4 heads of 128: 273 in one part, 189 + 16 for the join in 2
@@ -93,8 +93,8 @@ Plan plan_of(const ops3d_attention_problem *p, int64_t columns, int64_t others, 
     plan.shape = kSome;
     plan.splits = uneven ? parts(1024, blocks(64)) : 1;
   } else if (stages >= 32) {
-    plan.shape = widest == kMany && per > 64 ? kMany : kSome;
-    plan.splits = plan.shape == kMany ? parts(uneven ? 1024 : 512, blocks(128)) : parts(1024, blocks(64));
+    plan.shape = kSome;
+    plan.splits = parts(1024, blocks(64));
   } else {
     plan.shape = kFew;
   }

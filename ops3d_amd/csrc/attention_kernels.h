@@ -276,7 +276,6 @@ __device__ __forceinline__ void load_column(typename Type<T>::frag (&f)[STEPS], 
     f[s] = __builtin_bit_cast(typename Type<T>::frag, row ? fetch(row, 0, 0, (s * 4 + q) * CH, 1, D) : make_uint4(0, 0, 0, 0));
 }
 
-__device__ __forceinline__ f32x4 splat(float x) { return f32x4{x, x, x, x}; }
 
 // The output's rounding: what is left of v in T.
 template <typename T> __device__ __forceinline__ f32x4 rest_of(f32x4 v) {
@@ -296,6 +295,43 @@ template <typename T> __device__ __forceinline__ void store4(T *row, int d, cons
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (d + j < D) row[d + j] = (T)v[j];
+  }
+}
+
+__device__ __forceinline__ f32x4 splat(float x) { return f32x4{x, x, x, x}; }
+
+// A causal mask's 0 times an infinity or NaN of a hidden row would be NaN.  Stages with hidden rows are looked over: by
+// their results, where each row has some, or else by the operand times 0, which is NaN where one of its rows is not
+// finite.
+template <int N> __device__ __forceinline__ bool finite_results(const f32x4 *s) {
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z = fmaf(s[i][j], 0.f, z);
+  return !__ballot(z != z);
+}
+template <typename T, int DP, int ROWS, typename ST>
+__device__ __forceinline__ bool all_finite(const char *lds, int r0, const typename ST::Lane &at, int lane) {
+  f32x4 z = splat(0.f);
+#pragma unroll
+  for (int r = 0; r < ROWS; r += sizeof(T) == 2 ? 32 : 16)
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) z = Type<T>::mma(ST::columns(lds, r0 + r, d, at, lane), typename Type<T>::frag{}, z);
+  return !__ballot(z[0] != z[0] || z[1] != z[1] || z[2] != z[2] || z[3] != z[3]);
+}
+// acc += a b row by row of the sum, for the columns that see the row: seen(row).
+template <typename T, typename F>
+__device__ __forceinline__ void add_seen(f32x4 &acc, const typename Type<T>::frag &a, const typename Type<T>::frag &b, int q, F seen) {
+  constexpr int N = 16 / (int)sizeof(T);
+#pragma unroll 1
+  for (int e = 0; e < 4 * N; ++e) {
+    const int owner = e / N, j = e % N;
+    typename Type<T>::frag one;
+#pragma unroll
+    for (int k = 0; k < N; ++k) one[k] = k == j && q == owner ? a[k] : (T)0.f;
+    const f32x4 x = Type<T>::mma(one, b, splat(0.f));
+    if (seen((j >> 2) * 16 + owner * 4 + (j & 3))) acc += x;
   }
 }
 
@@ -450,6 +486,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
           for (int j = 0; j < 4; ++j)
             if (k0 + r0 + kt * 16 + q * 4 + j >= limit[n]) s[n][kt][j] = -INFINITY;
     }
+    const bool finite = !decltype(masked)::value || !p.causal || all_finite<T, DP, KW, ST>(lv, r0, at, lane);
     bool raise = false;
     float mx[NC];
 #pragma unroll
@@ -496,7 +533,10 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       for (int d = 0; d < DT; ++d) {
         const auto vf = ST::columns(lv, r0 + kt * 16, d, at, lane);
 #pragma unroll
-        for (int n = 0; n < NC; ++n) o[n][d] = Type<T>::mma(vf, pf[n], o[n][d]);
+        for (int n = 0; n < NC; ++n) {
+          if (!decltype(masked)::value || finite) o[n][d] = Type<T>::mma(vf, pf[n], o[n][d]);
+          else add_seen<T>(o[n][d], vf, pf[n], q, [&](int r) { return k0 + r0 + kt * 16 + r < limit[n]; });
+        }
       }
     }
     k0 += KT;
@@ -729,6 +769,8 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
           }
         }
       }
+      // a key that is not finite has no finite logit
+      const bool finite = !decltype(masked)::value || !p.causal || finite_results<NC * PR>(s[0]);
       typename Type<T>::frag ds[NC];
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
@@ -746,7 +788,10 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       for (int d = 0; d < DT; ++d) {
         const auto kf = ST::columns(lk, r0 + kt * 16, d, at, lane);
 #pragma unroll
-        for (int n = 0; n < NC; ++n) a[n][d] = Type<T>::mma(kf, ds[n], a[n][d]);
+        for (int n = 0; n < NC; ++n) {
+          if (!decltype(masked)::value || finite) a[n][d] = Type<T>::mma(kf, ds[n], a[n][d]);
+          else add_seen<T>(a[n][d], kf, ds[n], q, [&](int r) { return k0 + r0 + kt * 16 + r < limit[n]; });
+        }
       }
     }
     k0 += KT;
@@ -906,6 +951,8 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
           }
         }
       }
+      // a query or an output gradient that is not finite has no finite logit or no finite product with a value
+      const bool finite = !decltype(masked)::value || (finite_results<NC * PR>(s[0]) && finite_results<NC * PR>(dp[0]));
       typename Type<T>::frag pf[NC], ds[NC];
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
@@ -929,8 +976,14 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
         const auto gf = ST::columns(lg, r0 + qt * 16, d, at, lane), qf = ST::columns(lq, r0 + qt * 16, d, at, lane);
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-          av[n][d] = Type<T>::mma(gf, pf[n], av[n][d]);
-          ak[n][d] = Type<T>::mma(qf, ds[n], ak[n][d]);
+          if (!decltype(masked)::value || finite) {
+            av[n][d] = Type<T>::mma(gf, pf[n], av[n][d]);
+            ak[n][d] = Type<T>::mma(qf, ds[n], ak[n][d]);
+          } else {
+            const auto seen = [&](int r) { return c0 + r0 + qt * 16 + r >= since[n]; };
+            add_seen<T>(av[n][d], gf, pf[n], q, seen);
+            add_seen<T>(ak[n][d], qf, ds[n], q, seen);
+          }
         }
       }
     }
@@ -997,12 +1050,12 @@ template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void 
 // ---------------------------------------------------------------------------------------------
 // Launches (attention_f32.hip and its like).  dp: the padded number of channels, 32, 64 or 128.
 // Waves a SIMD that a kernel's registers are to leave room for: two of 256 at least, whose results then stay in
-// registers that vector instructions read.
+// registers that vector instructions read, where they fit.
 enum Kernel { kforward, kgrad_q, kgrad_kv };
 template <typename T> constexpr int occupancy(bool direct, int dp, int wk) {
   if (dp <= 32) return direct ? 4 : 3;
   if (dp <= 64) return 2;
-  return wk > 1 || sizeof(T) == 4 ? 1 : 2;
+  return wk > 1 || sizeof(T) == 4 || !direct ? 1 : 2;
 }
 
 // Columns of a block: 128, 64, or 16, of which each of 4 waves takes a quarter of a stage's rows.

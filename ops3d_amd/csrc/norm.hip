@@ -475,7 +475,10 @@ template <typename T, typename W> hipError_t forward(const Args &a, int dtype, h
   }
   return with_plan<T>(plan, [&](auto l, auto c) {
     constexpr int L = decltype(l)::value, NT = L < 256 ? 256 : L;
-    forward_kernel<T, W, decltype(c)::value, L, NT><<<grid_for((a.rows + NT / L - 1) / (NT / L), 2048 * 256 / NT), NT, 0, st>>>(a);
+    // as many blocks as the CUs hold: each loads its next row while it sums one (2053 x 4101 fp32: 17.6 us, with twice as
+    // many 21.2)
+    constexpr int kMost = L > 64 ? 512 * 512 / NT : 2048;
+    forward_kernel<T, W, decltype(c)::value, L, NT><<<grid_for((a.rows + NT / L - 1) / (NT / L), kMost), NT, 0, st>>>(a);
     return hipGetLastError();
   });
 }

@@ -309,6 +309,40 @@ def test_not_finite_values_reach_those_that_see_them(gpu_device):
 
 @gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nq,nk,H,Hk,D", [(150, 150, 4, 2, 32), (150, 170, 2, 2, 36), (700, 700, 2, 1, 64), (300, 300, 2, 2, 128), (2100, 2100, 8, 8, 32),
+                                          (4200, 4200, 8, 8, 32), (2300, 2300, 16, 4, 128), (3, 5000, 2, 1, 64)])
+def test_hidden_values_that_are_not_finite(gpu_device, nq, nk, H, Hk, D, dtype):
+    """Causal: NaN and infinities in keys and values reach no query before them, and in queries and output gradients
+    no key behind them, in the same tile or another."""
+    gen = torch.Generator(device="cuda").manual_seed(nq)
+    dt = DTYPES[dtype]
+    q, k, v, u = (make(gen, s, dt) for s in ((nq, H, D), (nk, Hk, D), (nk, Hk, D), (nq, H, D)))
+    want = ref.sequence(q, k, v, True, D ** -0.5, u)
+    off = nk - nq
+    late, early = max(off + 1, nk - 60), nq // 3   # a key, and a query, counted among their own
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        kk, vv = k.clone(), v.clone()
+        kk[late, 0, D // 2], vv[late, :, 0], vv[late + (late + 1 < nk), 0, D - 1] = bad, bad, bad
+        leaves = [t.detach().requires_grad_(True) for t in (q, kk, vv)]
+        y = packed_attention(*leaves, causal=True)
+        gq, _, _ = torch.autograd.grad(y, leaves, u)
+        clean = slice(0, late - off)   # the queries before the key
+        for name, got in (("y", y), ("dq", gq)):
+            check(name, got[clean], tuple(t[clean] for t in want[name]))
+        assert not torch.isfinite(y[late - off:, :, 0]).any()
+        qq, uu = q.clone(), u.clone()
+        qq[early, 0, 0], uu[early, :, D - 1] = bad, bad
+        leaves = [t.detach().requires_grad_(True) for t in (qq, k, v)]
+        y = packed_attention(*leaves, causal=True)
+        _, gk, gv = torch.autograd.grad(y, leaves, uu)
+        clean = slice(early + off + 1, nk)   # the keys that the query does not see
+        for name, got in (("dk", gk), ("dv", gv)):
+            check(name, got[clean], tuple(t[clean] for t in want[name]))
+        assert not torch.isfinite(gv[:early + off + 1, :, D - 1]).any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("dim", [32, 36])
 def test_strides(gpu_device, dim, dtype):
     """Parts of one projection, unaligned rows, heads before tokens, shared and strided ones, and gradients so."""
