@@ -67,7 +67,7 @@ struct Plan {
 // columns and others: of an item, or of all packed sequences.  Measured in bf16 (us):
 //   wide tiles read the rows that come by least often, if there are two blocks a CU: 8192 x 8192, 8 heads of 32
 //     channels, forward: 141 in tiles of 128, 151 of 64, 298 of 16; 4096 x 4096: 51, 47, 81
-//   narrow tiles, where there are few columns and few rows: 1024 x 1024: 15, 12, 10
+//   narrow tiles, where there are few columns and few rows: 1024 x 1024: 15, 12, 10; and where sequences are short
 //   parts, where few columns see many rows: 200 x 37376, 2 items: 360 in one, 49 in 8, 42 in 16; one query of 32/8
 //     heads of 128 over 8 caches of 8192: 42 in 8, 39 in 16, 50 in narrow tiles
 //   twice the blocks, where sequences or a causal mask give them different amounts to do: grad k v of 8192 causal
@@ -86,10 +86,10 @@ Plan plan_of(const ops3d_attention_problem *p, int64_t columns, int64_t others, 
   };
   Plan plan{};
   plan.splits = 1;
-  if (widest == kMany && blocks(128) >= 512) {
+  if (widest == kMany && per > 64 && blocks(128) >= 512) {
     plan.shape = kMany;
     plan.splits = uneven ? parts(1024, blocks(128)) : 1;
-  } else if (blocks(64) >= 256) {
+  } else if (per > 16 && blocks(64) >= 256) {
     plan.shape = kSome;
     plan.splits = uneven ? parts(1024, blocks(64)) : 1;
   } else if (stages >= 32) {
@@ -120,18 +120,28 @@ bool set_plan(Args &a, const ops3d_attention_problem *p, const Plan &plan) {
   return true;
 }
 
+// Bytes of the table of a plan's tiles, where sequences are many.
+size_t table_bytes(const ops3d_attention_problem *p, const Plan &plan) {
+  return p->q_start && p->sequences > kWalk ? align256((size_t)plan.tiles * 32) : 0;
+}
+
 int64_t cells_of(const ops3d_attention_problem *p) { return (int64_t)p->items * p->heads * p->q_rows; }
 int64_t keys_of(const ops3d_attention_problem *p) { return (int64_t)p->items * p->kv_heads * p->k_rows; }
 
 size_t forward_bytes(const ops3d_attention_problem *p) {
   const Plan plan = plan_queries(p);
-  return plan.splits > 1 ? align256((size_t)plan.splits * cells_of(p) * (padded_dim(p->dim) + 2) * 4) : 0;
+  return table_bytes(p, plan) + (plan.splits > 1 ? align256((size_t)plan.splits * cells_of(p) * (padded_dim(p->dim) + 2) * 4) : 0);
+}
+// The larger of the two kernels' tables, then delta, then the larger of their parts.
+size_t backward_table(const ops3d_attention_problem *p) {
+  const size_t q = table_bytes(p, plan_queries(p)), k = table_bytes(p, plan_keys(p));
+  return q > k ? q : k;
 }
 size_t backward_bytes(const ops3d_attention_problem *p) {
   const size_t row = (size_t)padded_dim(p->dim) * 4;
   const int q = plan_queries(p).splits, k = plan_keys(p).splits;
   const size_t a = q > 1 ? q * cells_of(p) * row : 0, b = k > 1 ? 2 * k * keys_of(p) * row : 0;
-  return align256((size_t)cells_of(p) * 4) + align256(a > b ? a : b);
+  return backward_table(p) + align256((size_t)cells_of(p) * 4) + align256(a > b ? a : b);
 }
 
 int take(Tensor &t, const ops3d_attention_tensor *x, int es) {
@@ -228,7 +238,9 @@ int ops3d_attention_forward(const ops3d_attention_problem *problem, const ops3d_
   if (!set_plan(a, problem, plan)) return fail(OPS3D_FDA_EINVAL, "attention: 2^31 tiles or more");
   const int dp = padded_dim(problem->dim);
   a.dma = direct(problem, a.k) && direct(problem, a.v) ? 1 : 0;
-  a.part = static_cast<float *>(workspace);
+  const size_t table = table_bytes(problem, plan);
+  a.table = table ? static_cast<const int4 *>(workspace) : nullptr;
+  a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + table);
   a.part_ml = a.part + (size_t)a.splits * a.cells * dp;
   return run(problem->dtype, "attention forward",
              [&](auto t) { return ops3d_attention::forward<decltype(t)>(a, dp, plan.shape, static_cast<hipStream_t>(stream)); });
@@ -266,8 +278,10 @@ int ops3d_attention_backward(const ops3d_attention_problem *problem, const ops3d
   if (wants_k && ((rc = take(a.gk, grad_k, es)) || (rc = take(a.gv, grad_v, es)))) return rc;
   a.lse = const_cast<float *>(lse);
   if ((rc = check_workspace(workspace, workspace_bytes, backward_bytes(problem)))) return rc;
-  a.delta = static_cast<float *>(workspace);
-  a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + align256((size_t)cells * 4));
+  const size_t table = backward_table(problem);
+  a.table = table ? static_cast<const int4 *>(workspace) : nullptr;
+  a.delta = reinterpret_cast<float *>(static_cast<char *>(workspace) + table);
+  a.part = a.delta + align256((size_t)cells * 4) / 4;
   const int dp = padded_dim(problem->dim);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   a.dma = (keys && direct(problem, a.k) && direct(problem, a.v) ? 1 : 0) | (cells && direct(problem, a.q) && direct(problem, a.g) ? 2 : 0);

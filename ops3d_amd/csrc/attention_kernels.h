@@ -46,12 +46,12 @@ struct Args {
   uint32_t magic;                     // c / G = 2 c magic >> 32 >> shift
   int shift;
   int causal;
-  int pair;                           // see place()
   int dma;                            // rows go straight to LDS: bit 0 k and v, bit 1 q and grad_out
   float scale, c;                     // c = scale log2 e
   int tiles, tiles_item, splits;      // tiles of all items (a bound), of one, and parts of the other side
   int heads;                          // items Hk
   int64_t cells;                      // heads Sq G: queries times heads
+  const int4 *table;                  // two for each tile of packed sequences (see table_kernel), or nullptr
   void *rest;                         // what rounding took from o, [items, Sq, heads, D] contiguous, or nullptr
   float *lse, *delta;                 // [items, Hk, Sq G]; log2 of the sum of exponentials, and sum of o g
   float *part, *part_ml;              // [splits, columns, DP], [splits, columns, 2]
@@ -81,6 +81,11 @@ template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, in
     w.rows = KEYS ? p.Sk : p.Sq;
     w.first = (t - e * p.tiles_item) * per;
     return true;
+  }
+  if (p.table) {
+    const int4 a = p.table[2 * t], b = p.table[2 * t + 1];
+    w = Work{0, a.x, a.y, a.z, a.w, b.x, b.y};
+    return b.y >= 0;
   }
   using ops3d_segments::Segment;
   using ops3d_segments::segment_at;
@@ -124,6 +129,71 @@ template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, in
   w.rows = rows;
   w.first = first;
   return true;
+}
+
+// The work of each of n tiles of many sequences (more than a wave looks over in a step or two), for a kernel's blocks to
+// look up: {q0, k0, nq, nk}, {rows, first, 0, 0}, first -1 where there is none.  One block: each thread has a run of
+// segments, whose bounds and tiles depend on the runs before, scanned in LDS.
+constexpr int kWalk = 64;   // sequences that blocks find by themselves (64 steps of a walk cost a block about 30 us)
+template <bool KEYS> __global__ __launch_bounds__(1024) void table_kernel(Args p, int per, int4 *table, int n) {
+  __shared__ int scan[3][1024];
+  const int64_t *own = KEYS ? p.k_start : p.q_start, *other = KEYS ? p.q_start : p.k_start;
+  const int own_count = KEYS ? p.k_count : p.q_count, other_count = KEYS ? p.q_count : p.k_count;
+  const int own_rows = KEYS ? p.Sk : p.Sq, other_rows = KEYS ? p.Sq : p.Sk;
+  const int unit = KEYS ? 1 : p.G, t = threadIdx.x, run = (p.E + 2 + 1023) / 1024;
+  const int begin = min(p.E + 2, t * run), end = min(p.E + 2, begin + run);
+  const auto entry = [](const int64_t *start, int count, int rows, int j) __attribute__((always_inline)) {
+    const int64_t v = j < count ? start[j] : (int64_t)rows;
+    return v < 0 ? 0 : (int)(v < rows ? v : rows);
+  };
+  int most[2] = {0, 0};   // of the run's entries
+  for (int j = begin; j < end; ++j) {
+    most[0] = max(most[0], entry(own, own_count, own_rows, j));
+    most[1] = max(most[1], entry(other, other_count, other_rows, j));
+  }
+  scan[0][t] = most[0];
+  scan[1][t] = most[1];
+  __syncthreads();
+  for (int o = 1; o < 1024; o <<= 1) {
+    const int a = t >= o ? scan[0][t - o] : 0, b = t >= o ? scan[1][t - o] : 0;
+    __syncthreads();
+    scan[0][t] = max(scan[0][t], a);
+    scan[1][t] = max(scan[1][t], b);
+    __syncthreads();
+  }
+  const int lower = t ? scan[0][t - 1] : 0, o_lower = t ? scan[1][t - 1] : 0;   // where the run's first segment starts
+  int tiles = 0, from = lower;
+  for (int j = begin; j < end; ++j) {
+    const int to = max(from, entry(own, own_count, own_rows, j));
+    tiles += (int)(((int64_t)(to - from) * unit + per - 1) / per);
+    from = to;
+  }
+  scan[2][t] = tiles;
+  __syncthreads();
+  for (int o = 1; o < 1024; o <<= 1) {
+    const int a = t >= o ? scan[2][t - o] : 0;
+    __syncthreads();
+    scan[2][t] += a;
+    __syncthreads();
+  }
+  int at = t ? scan[2][t - 1] : 0, o_from = o_lower;
+  from = lower;
+  for (int j = begin; j < end; ++j) {
+    const int to = max(from, entry(own, own_count, own_rows, j)), o_to = max(o_from, entry(other, other_count, other_rows, j));
+    const bool in = j >= 1 && j <= p.E;   // rows of no sequence: none that count
+    const int rows = to - from, o_rows = in ? o_to - o_from : 0, o_at = in ? o_from : 0, counted = in ? rows : 0;
+    const int4 a = KEYS ? make_int4(o_at, from, o_rows, counted) : make_int4(from, o_at, counted, o_rows);
+    for (int64_t first = 0; first < (int64_t)rows * unit && at < n; first += per, ++at) {
+      table[2 * at] = a;
+      table[2 * at + 1] = make_int4(rows, (int)first, 0, 0);
+    }
+    from = to;
+    o_from = o_to;
+  }
+  for (int i = scan[2][1023] + t; i < n; i += 1024) {
+    table[2 * i] = make_int4(0, 0, 0, 0);
+    table[2 * i + 1] = make_int4(0, -1, 0, 0);
+  }
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -197,6 +267,11 @@ template <typename T, int DP, int R, int NT> struct Stage {
     for (int i = 0; i < NL; ++i)
       if (D == DP || off[i] != ~0u) __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + off[i]),
                                        (__attribute__((address_space(3))) void *)(lds + (wave * NL + i) * 1024), 16, 0, 0);
+  }
+  // A barrier behind which what the block's waves have loaded is in LDS: the compiler waits for no such load.
+  static __device__ __forceinline__ void arrived() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    __syncthreads();
   }
   static __device__ __forceinline__ void clear(char *lds, int bytes) {
     for (int i = threadIdx.x * 16; i < bytes; i += NT * 16) *reinterpret_cast<uint4 *>(lds + i) = make_uint4(0, 0, 0, 0);
@@ -343,12 +418,10 @@ template <> struct Range<_Float16> { static constexpr float kShift = 10.f, kSlac
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The block's place: key head, part and tile; tiles from the last on, which in causal attention have most to
-// do.  Blocks go to XCD block % 8, so with 8 key heads one has a head, whose rows its L2 then keeps; where two
-// heads' rows share 128-byte lines (p.pair), the two take turns on two XCDs.
+// do.  Blocks go to XCD block % 8, so with 8 key heads one has a head, whose rows its L2 then keeps.
 __device__ __forceinline__ void place(const Args &p, int &h, int &part, int &tile) {
   const int r = blockIdx.x / p.Hk;
   h = blockIdx.x - r * p.Hk;
-  if (p.pair) h ^= r & 1;
   part = r % p.splits;
   tile = p.tiles - 1 - r / p.splits;
 }
@@ -461,7 +534,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       if (k0 + KT < k_end) load(k0 + KT, 0);
       __syncthreads();   // the other buffer's readers are past the barrier before
     } else {
-      __syncthreads();   // this stage has arrived, and the other buffer's readers are done
+      ST::arrived();     // this stage, everywhere; and the other buffer's readers are done
       if (k0 + KT < k_end) load(k0 + KT, buf ^ 1);
     }
 
@@ -749,7 +822,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       if (k0 + KT < k_end) load(k0 + KT, 0);
       __syncthreads();
     } else {
-      __syncthreads();
+      ST::arrived();
       if (k0 + KT < k_end) load(k0 + KT, buf ^ 1);
     }
 #pragma unroll
@@ -929,7 +1002,8 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       ld[threadIdx.x] = -row_delta;
     }
     if (!DMA && c0 + QT < c_end) load(c0 + QT, 0);
-    __syncthreads();
+    if (DMA) ST::arrived();
+    else __syncthreads();
     if (DMA && c0 + QT < c_end) load(c0 + QT, buf ^ 1);
 #pragma unroll
     for (int qt = 0; qt < QN; qt += PR) {
@@ -1071,6 +1145,11 @@ template <typename T, int DP, Kernel kKernel, typename F> hipError_t with_shape(
   if (shape == kSome) return f(one(), four(), one(), rows());
   return f(one(), one(), four(), std::integral_constant<int, 128 / E>());
 }
+// The table of a kernel's tiles, where the sequences are many.
+template <bool KEYS> Args with_table(Args p, int shape, hipStream_t st) {
+  if (p.table) table_kernel<KEYS><<<1, 1024, 0, st>>>(p, shape == kMany ? 128 : shape == kSome ? 64 : 16, const_cast<int4 *>(p.table), p.tiles);
+  return p;
+}
 template <typename F> hipError_t with_dim(int dp, F f) {
   if (dp == 32) return f(std::integral_constant<int, 32>());
   if (dp == 64) return f(std::integral_constant<int, 64>());
@@ -1078,7 +1157,8 @@ template <typename F> hipError_t with_dim(int dp, F f) {
 }
 inline unsigned blocks_of(const Args &p) { return (unsigned)((int64_t)p.tiles * p.splits * p.Hk); }
 
-template <typename T> hipError_t forward(const Args &p, int dp, int shape, hipStream_t st) {
+template <typename T> hipError_t forward(const Args &args, int dp, int shape, hipStream_t st) {
+  const Args p = with_table<false>(args, shape, st);
   return with_dim(dp, [&](auto d) {
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kforward>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
@@ -1090,7 +1170,8 @@ template <typename T> hipError_t forward(const Args &p, int dp, int shape, hipSt
     });
   });
 }
-template <typename T> hipError_t grad_q(const Args &p, int dp, int shape, hipStream_t st) {
+template <typename T> hipError_t grad_q(const Args &args, int dp, int shape, hipStream_t st) {
+  const Args p = with_table<false>(args, shape, st);
   return with_dim(dp, [&](auto d) {
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kgrad_q>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
@@ -1102,7 +1183,8 @@ template <typename T> hipError_t grad_q(const Args &p, int dp, int shape, hipStr
     });
   });
 }
-template <typename T> hipError_t grad_kv(const Args &p, int dp, int shape, hipStream_t st) {
+template <typename T> hipError_t grad_kv(const Args &args, int dp, int shape, hipStream_t st) {
+  const Args p = with_table<true>(args, shape, st);
   return with_dim(dp, [&](auto d) {
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kgrad_kv>(shape, [&](auto nc, auto wc, auto wk, auto kt) {

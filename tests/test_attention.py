@@ -241,6 +241,19 @@ def test_many_sequences(gpu_device, dtype):
     other = [0] + sizes.flip(0).cumsum(0).tolist()
     case(dtype, rows + 3, rows + 3, 2, 1, 16, True, q_start=start)
     case(dtype, rows, rows, 1, 1, 32, False, q_start=start, k_start=other)
+    odd = list(start)
+    odd[7], odd[300], odd[2000] = rows + 900, -5, 3   # the largest so far counts, held to the rows
+    case(dtype, rows, rows, 2, 2, 32, False, q_start=[5] + odd[1:], k_start=other)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("sequences,rows", [(63, 900), (64, 900), (65, 900), (66, 3000), (130, 20000), (1022, 5000), (1023, 5000), (4097, 4200)])
+def test_sequences_found_and_looked_up(gpu_device, sequences, rows, dtype):
+    """Around the numbers of sequences where blocks stop finding their own, and where a thread gets more of them."""
+    gen = torch.Generator().manual_seed(sequences)
+    start = [2] + sorted(torch.randint(2, rows - 3, (sequences - 1,), generator=gen).tolist()) + [rows - 3]
+    case(dtype, rows, rows, 2, 1, 32, sequences % 2 == 0, q_start=start)
 
 
 @gpu
