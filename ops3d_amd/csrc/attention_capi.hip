@@ -130,7 +130,7 @@ int64_t keys_of(const ops3d_attention_problem *p) { return (int64_t)p->items * p
 
 size_t forward_bytes(const ops3d_attention_problem *p) {
   const Plan plan = plan_queries(p);
-  return table_bytes(p, plan) + (plan.splits > 1 ? align256((size_t)plan.splits * cells_of(p) * (padded_dim(p->dim) + 2) * 4) : 0);
+  return table_bytes(p, plan) + (plan.splits > 1 ? align256((size_t)plan.splits * cells_of(p) * (padded_dim(p->dim) + 4) * 4) : 0);
 }
 // The larger of the two kernels' tables, then delta, then the larger of their parts.
 size_t backward_table(const ops3d_attention_problem *p) {
@@ -241,7 +241,7 @@ int ops3d_attention_forward(const ops3d_attention_problem *problem, const ops3d_
   const size_t table = table_bytes(problem, plan);
   a.table = table ? static_cast<const int4 *>(workspace) : nullptr;
   a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + table);
-  a.part_ml = a.part + (size_t)a.splits * a.cells * dp;
+  a.part_ml = reinterpret_cast<f32x4 *>(a.part + (size_t)a.splits * a.cells * dp);
   return run(problem->dtype, "attention forward",
              [&](auto t) { return ops3d_attention::forward<decltype(t)>(a, dp, plan.shape, static_cast<hipStream_t>(stream)); });
 }

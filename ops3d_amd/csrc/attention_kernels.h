@@ -54,7 +54,8 @@ struct Args {
   const int4 *table;                  // two for each tile of packed sequences (see table_kernel), or nullptr
   void *rest;                         // what rounding took from o, [items, Sq, heads, D] contiguous, or nullptr
   float *lse, *delta;                 // [items, Hk, Sq G]; log2 of the sum of exponentials, and sum of o g
-  float *part, *part_ml;              // [splits, columns, DP], [splits, columns, 2]
+  float *part;                        // [splits, columns, DP]
+  f32x4 *part_ml;                     // [splits, columns]: reference, sum of rounded P, sum of P
 };
 
 // What a block works on.
@@ -132,9 +133,10 @@ template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, in
 }
 
 // The work of each of n tiles of many sequences (more than a wave looks over in a step or two), for a kernel's blocks to
-// look up: {q0, k0, nq, nk}, {rows, first, 0, 0}, first -1 where there is none.  One block: each thread has a run of
+// look up: {q0, k0, nq, nk}, {rows, first, 0, 0}, first -1 where there is none (4096 sequences of 16 tokens, forward: 156 us;
+// 2487 where each block walks over them).  One block: each thread has a run of
 // segments, whose bounds and tiles depend on the runs before, scanned in LDS.
-constexpr int kWalk = 64;   // sequences that blocks find by themselves (64 steps of a walk cost a block about 30 us)
+constexpr int kWalk = 64;   // sequences that blocks find by themselves
 template <bool KEYS> __global__ __launch_bounds__(1024) void table_kernel(Args p, int per, int4 *table, int n) {
   __shared__ int scan[3][1024];
   const int64_t *own = KEYS ? p.k_start : p.q_start, *other = KEYS ? p.q_start : p.k_start;
@@ -487,9 +489,12 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     k_end = min(keys, k_begin + per);
   }
 
-  f32x4 o[NC][DT], sum[NC];                // sums of P V and of P (SUMS: by the matrix units, from the rounded P)
+  // sums of P V and of P; in 16 bits the latter by the matrix units, from the rounded P, and where the backward is to
+  // have its logarithm, of P as it is too: the rounded sum's would put the same error into all of a row's gradients
+  f32x4 o[NC][DT], sum[NC];
   float m[NC], mc[NC], l[NC], top[NC];     // reference, the same times c, sum of P (this lane's rows), what raises it
   constexpr bool SUMS = sizeof(T) == 2;
+  const bool exact = !SUMS || p.lse;
   constexpr float kShift = Range<T>::kShift;
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
@@ -595,10 +600,13 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
         for (int u = 0; u < PR; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[n][kt + u][j] = exp2_(fmaf(s[n][kt + u][j], p.c, -mc[n]));
-            if (!SUMS) l[n] += s[n][kt + u][j];
-          }
+          for (int j = 0; j < 4; ++j) s[n][kt + u][j] = exp2_(fmaf(s[n][kt + u][j], p.c, -mc[n]));
+        if (exact) {
+#pragma unroll
+          for (int u = 0; u < PR; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[n] += s[n][kt + u][j];
+        }
         pf[n] = operand<T>(&s[n][kt]);
         if (SUMS) sum[n] = Type<T>::mma(Type<T>::ones(), pf[n], sum[n]);
       }
@@ -620,11 +628,13 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   if (k_begin < k_end) load(k_begin, 0);
   while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
   while (k0 < k_end) stage(std::true_type());
+  float whole[NC];   // what the output is divided by
 #pragma unroll
-  for (int n = 0; n < NC; ++n)
-    l[n] = SUMS ? sum[n][0] : ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(l[n]));
-#pragma unroll
-  for (int n = 0; n < NC; ++n) m[n] *= p.c;   // from here on log2
+  for (int n = 0; n < NC; ++n) {
+    l[n] = ops3d_reduce::across32<ops3d_reduce::Add>(ops3d_reduce::across16<ops3d_reduce::Add>(l[n]));
+    whole[n] = SUMS ? sum[n][0] : l[n];
+    m[n] *= p.c;   // from here on log2
+  }
 
   if constexpr (WK > 1) {   // the waves' shares, each with its own reference
     f32x4 *x = reinterpret_cast<f32x4 *>(lds);
@@ -635,7 +645,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
         f32x4 *y = x + (((wk - 1) * WC + wc) * NC + n) * (DT + 1) * 64 + lane;
 #pragma unroll
         for (int d = 0; d < DT; ++d) y[d * 64] = o[n][d];
-        y[DT * 64] = f32x4{m[n], l[n], 0.f, 0.f};
+        y[DT * 64] = f32x4{m[n], whole[n], l[n], 0.f};
       }
     }
     __syncthreads();
@@ -647,7 +657,8 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
         const f32x4 *y = x + ((k * WC + wc) * NC + n) * (DT + 1) * 64 + lane;
         const float mk = y[DT * 64][0], now = fmaxf(m[n], mk);
         const float a = m[n] == -INFINITY ? 0.f : exp2_(m[n] - now), b = mk == -INFINITY ? 0.f : exp2_(mk - now);
-        l[n] = l[n] * a + y[DT * 64][1] * b;
+        whole[n] = whole[n] * a + y[DT * 64][1] * b;
+        l[n] = l[n] * a + y[DT * 64][2] * b;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[n][d] = o[n][d] * a + y[d * 64] * b;
         m[n] = now;
@@ -663,14 +674,12 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
       const int64_t to = part * p.cells + cell0 + c;
 #pragma unroll
       for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + to * DP + d * 16 + q * 4) = o[n][d];
-      if (q == 0) {   // columns that do not count saw nothing
-        p.part_ml[2 * to] = c < active ? m[n] : -INFINITY;
-        p.part_ml[2 * to + 1] = c < active ? l[n] : 0.f;
-      }
+      if (q == 0)   // columns that do not count saw nothing
+        p.part_ml[to] = c < active ? f32x4{m[n], whole[n], l[n], 0.f} : f32x4{-INFINITY, 0.f, 0.f, 0.f};
       continue;
     }
-    const bool none = c >= active || l[n] == 0.f;
-    const float inv = none ? 0.f : 1.f / l[n];
+    const bool none = c >= active || whole[n] == 0.f;
+    const float inv = none ? 0.f : 1.f / whole[n];
     const int t = divide(p, c);
     const int head = h * p.G + c - t * p.G;
     T *const to = static_cast<T *>(p.o.p) + w.item * p.o.item + (w.q0 + t) * p.o.token + head * p.o.head;
@@ -693,32 +702,33 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void join_forwar
   if (cell >= p.cells) return;
   const int lane = threadIdx.x & 63, d = lane % PER * 4;
   float m = -INFINITY;
-  for (int z = lane; z < p.splits; z += 64) m = fmaxf(m, p.part_ml[2 * (z * p.cells + cell)]);
+  for (int z = lane; z < p.splits; z += 64) m = fmaxf(m, p.part_ml[z * p.cells + cell][0]);
   m = ops3d_reduce::all<64, ops3d_reduce::Max>(m);
-  float l = 0.f;
+  float whole = 0.f, l = 0.f;
   f32x4 o = splat(0.f);
   if (m != -INFINITY) {
 #pragma unroll 2
     for (int z = lane / PER; z < p.splits; z += AT) {
       const int64_t at = z * p.cells + cell;
-      const float mz = p.part_ml[2 * at], lz = p.part_ml[2 * at + 1];
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(p.part + at * DP + d);
-      if (mz == -INFINITY) continue;
-      const float by = exp2_(mz - m);
-      l = fmaf(by, lz, l);
+      const f32x4 ml = p.part_ml[at], v = *reinterpret_cast<const f32x4 *>(p.part + at * DP + d);
+      if (ml[0] == -INFINITY) continue;
+      const float by = exp2_(ml[0] - m);
+      whole = fmaf(by, ml[1], whole);
+      l = fmaf(by, ml[2], l);
       o += v * by;
     }
   }
 #pragma unroll
   for (int s = PER; s < 64; s <<= 1) {
+    whole += __shfl_xor(whole, s);
     l += __shfl_xor(l, s);
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], s);
   }
   const int per = p.Sq * p.G, ih = (int)(cell / per), c = (int)(cell - (int64_t)ih * per);
   const int item = ih / p.Hk, h = ih - item * p.Hk, t = divide(p, c), head = h * p.G + c - t * p.G;
-  const bool none = l == 0.f;
-  const f32x4 v = none ? splat(0.f) : o * (1.f / l);
+  const bool none = whole == 0.f;
+  const f32x4 v = none ? splat(0.f) : o * (1.f / whole);
   if (lane < PER) {
     store4(static_cast<T *>(p.o.p) + item * p.o.item + t * p.o.token + head * p.o.head, d, v, p.D);
     if (p.rest) store4(static_cast<T *>(p.rest) + (((int64_t)item * p.Sq + t) * (p.Hk * p.G) + head) * p.D, d, rest_of<T>(v), p.D);

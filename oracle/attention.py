@@ -8,8 +8,8 @@ count roundings (U = 2^-24, u half a step of dtype):
 * a logit is off by (D + 2) U sum |q k|; as an exponent of 2 it and the reference are rounded three times
   more, and the power is good to 2^-22.  The reference is at most the largest logit's size, or its
   logarithm's.  The relative error of a probability is the sum of these, natural logarithm times;
-* in 16 bits the probabilities are summed as rounded, as they are multiplied: each term of the sum is off by u of itself, and
-  so is the sum, in the output's denominator and in the logarithm that the backward's probabilities come from;
+* in 16 bits the output's denominator is the sum of the rounded probabilities: each term is off by u of itself, and so is the
+  sum (the logarithm that the backward's probabilities come from is of the sum as it is);
 * a sum of n products is off by (n / 4 + 40) U of the sum of their sizes: four at least are added at a time,
   a sum is rescaled some times, and parts are joined;
 * fp16: P is held 2^10 up, so that one below 2^-14 is off by 2^-35 at most; dS is not: by 2^-25;
@@ -80,7 +80,7 @@ def sequence(q, k, v, causal, scale, grad=None):
             continue
         g = grad[:, h]
         lse = (top + torch.log(torch.where(some, total, 1.0))).abs()
-        d = e_s + 4 * U * (s.abs() + lse + size) + 2.0 ** -22 + mean_d + u + hk + 4 * U
+        d = e_s + 4 * U * (s.abs() + lse + size) + 2.0 ** -22 + mean_d + hk + 4 * U
         dp = g @ vh.t()
         e_dp = (D + 2) * U * (g.abs() @ vh.abs().t())
         delta = (y * g).sum(1, keepdim=True)
