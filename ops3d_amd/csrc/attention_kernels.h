@@ -377,7 +377,8 @@ template <typename T> __device__ __forceinline__ void store4(T *row, int d, cons
 
 __device__ __forceinline__ f32x4 splat(float x) { return f32x4{x, x, x, x}; }
 
-// A causal mask's 0 times an infinity or NaN of a hidden row would be NaN.  Stages with hidden rows are looked over: by
+// A mask's 0 times an infinity or NaN of a hidden row (or of the last row, which stands in for those behind it) would be
+// NaN.  Stages with hidden rows are looked over: by
 // their results, where each row has some, or else by the operand times 0, which is NaN where one of its rows is not
 // finite.
 template <int N> __device__ __forceinline__ bool finite_results(const f32x4 *s) {
@@ -564,7 +565,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
           for (int j = 0; j < 4; ++j)
             if (k0 + r0 + kt * 16 + q * 4 + j >= limit[n]) s[n][kt][j] = -INFINITY;
     }
-    const bool finite = !decltype(masked)::value || !p.causal || all_finite<T, DP, KW, ST>(lv, r0, at, lane);
+    const bool finite = !decltype(masked)::value || all_finite<T, DP, KW, ST>(lv, r0, at, lane);
     bool raise = false;
     float mx[NC];
 #pragma unroll

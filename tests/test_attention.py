@@ -356,6 +356,22 @@ def test_hidden_values_that_are_not_finite(gpu_device, nq, nk, H, Hk, D, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nq,nk", [(5, 1), (5, 70), (9000, 70), (40000, 70), (3, 5001)])
+def test_infinity_in_the_last_value(gpu_device, nq, nk, dtype):
+    """The last row stands in for those behind it in its tile, whose weight is 0: an infinity there stays one."""
+    gen = torch.Generator(device="cuda").manual_seed(nq)
+    q, k, v = (make(gen, s, DTYPES[dtype]) for s in ((nq, 2, 32), (nk, 2, 32), (nk, 2, 32)))
+    value, bound = ref.sequence(q, k, v, False, 32 ** -0.5)["y"]
+    v[-1, 0, 3], v[-1, 1, 4] = math.inf, -math.inf
+    y = packed_attention(q, k, v)
+    assert (y[:, 0, 3] == math.inf).all() and (y[:, 1, 4] == -math.inf).all()
+    keep = torch.isfinite(y)
+    assert keep.sum() == y.numel() - 2 * nq
+    check("y", y[keep], (value[keep], bound[keep]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("dim", [32, 36])
 def test_strides(gpu_device, dim, dtype):
     """Parts of one projection, unaligned rows, heads before tokens, shared and strided ones, and gradients so."""
