@@ -16,6 +16,14 @@
 //
 // Softmax runs along: a column's reference m is raised, and its sums are rescaled, only when a logit passes
 // it by 2^kSlack; P is at most that.  Statistics are kept in log2 units.
+//
+// What bounds them (one MI355X, bf16, 8 heads; a large library product reaches 1184 TFLOP/s): with 32 channels a logit
+// is 128 operations on the matrix units and, beside them, an exponential, a multiply-add, a comparison and a rounding, and
+// the vector units are the bound; with 128 channels the matrix units and the LDS reads that feed them.
+//   forward  4096 x 4096     32 / 64 / 96 / 128 channels   47 / 58 / 86 / 88 us   367 / 594 / 597 / 782 TFLOP/s
+//            32768 x 32768   32                            1700 us                647
+//   backward 4096 x 4096     32 / 64 / 96 / 128            124 / 158 / 250 / 263  347 / 543 / 515 / 653 (10 D a logit; 14 D
+//                                                          are done, as both kernels form S and dP)
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -66,8 +74,13 @@ struct Work {
   int first;             // first owned column
 };
 
+// Tile t in the order of the launch, which starts with those that have most to do: of a causal mask's queries the last
+// ones, of its keys the first; of up to 62 packed sequences those that see most (16411 tokens in 7 sequences, 8 heads of
+// 32, bf16: forward 165 -> 154 us, grad q 166 -> 155, grad k v 203 -> 191).
 template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, int t, int per, Work &w) {
   const int unit = KEYS ? 1 : p.G;
+  const bool sorted = p.q_start && p.E + 2 <= 64;
+  if (!KEYS && !sorted) t = p.tiles - 1 - t;
   if (!p.q_start) {
     const int e = t / p.tiles_item;
     w.item = e;
@@ -95,6 +108,27 @@ template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, in
   const int own_count = KEYS ? p.k_count : p.q_count, other_count = KEYS ? p.q_count : p.k_count;
   const int own_rows = KEYS ? p.Sk : p.Sq, other_rows = KEYS ? p.Sq : p.Sk;
   int carry = 0, before = 0, j = -1, lower = 0, rows = 0, first = 0;
+  if (sorted) {   // a lane a segment
+    const Segment s = segment_at(own, own_count, own_rows, lane, carry);
+    carry = 0;
+    const Segment o = segment_at(other, other_count, other_rows, lane, carry);
+    const int own_n = lane < p.E + 2 ? s.upper - s.lower : 0, other_n = lane >= 1 && lane <= p.E ? o.upper - o.lower : 0;
+    const int tiles = (int)(((int64_t)own_n * unit + per - 1) / per);
+    for (int l = 0; l < p.E + 2; ++l) {
+      const int most = __builtin_amdgcn_readlane(other_n, l), n = __builtin_amdgcn_readlane(tiles, l);
+      if (most > other_n || (most == other_n && l < lane)) before += n;
+    }
+    const uint64_t m = __ballot(t >= before && t < before + tiles);
+    if (!m) return false;
+    const int src = __builtin_ctzll(m), nth = t - __builtin_amdgcn_readlane(before, src), n = __builtin_amdgcn_readlane(tiles, src);
+    lower = __builtin_amdgcn_readlane(s.lower, src);
+    rows = __builtin_amdgcn_readlane(own_n, src);
+    const int o_lower = __builtin_amdgcn_readlane(o.lower, src), o_rows = __builtin_amdgcn_readlane(other_n, src);
+    const int counted = src >= 1 && src <= p.E ? rows : 0;   // rows of no sequence: none that count
+    w = Work{0, KEYS ? o_lower : lower, KEYS ? lower : o_lower, KEYS ? o_rows : counted, KEYS ? counted : o_rows, rows,
+             (p.causal && !KEYS ? n - 1 - nth : nth) * per};
+    return true;
+  }
   for (int base = 0; base < p.E + 2 && j < 0; base += 64) {
     const Segment s = segment_at(own, own_count, own_rows, base + lane, carry);
     const int tiles = base + lane < p.E + 2 ? (int)(((int64_t)(s.upper - s.lower) * unit + per - 1) / per) : 0;
@@ -132,10 +166,10 @@ template <bool KEYS> __device__ __forceinline__ bool find_work(const Args &p, in
   return true;
 }
 
-// The work of each of n tiles of many sequences (more than a wave looks over in a step or two), for a kernel's blocks to
-// look up: {q0, k0, nq, nk}, {rows, first, 0, 0}, first -1 where there is none (4096 sequences of 16 tokens, forward: 156 us;
-// 2487 where each block walks over them).  One block: each thread has a run of
-// segments, whose bounds and tiles depend on the runs before, scanned in LDS.
+// The work of each of n tiles of many sequences (more than a wave looks over in a step or two), for a kernel's blocks
+// to look up: {q0, k0, nq, nk}, {rows, first, 0, 0}, first -1 where there is none.  One block: each thread has a run of
+// segments, whose bounds and tiles depend on the runs before, scanned in LDS.  Forward, bf16, 8 heads of 32: 4096
+// sequences of 16 tokens 156 us (2487 where each block walks over them), 1000 of 50: 40 (135), 16384 of 4: 534 (22188).
 constexpr int kWalk = 64;   // sequences that blocks find by themselves
 template <bool KEYS> __global__ __launch_bounds__(1024) void table_kernel(Args p, int per, int4 *table, int n) {
   __shared__ int scan[3][1024];
@@ -251,7 +285,8 @@ template <typename T, int DP, int R, int NT> struct Stage {
       if (row < n && col < D) v[i] = fetch(at(row), 0, 0, col, 1, D);
     }
   }
-  // The same without registers between: an instruction of a wave fills 1024 bytes of LDS in lane order, so the
+  // The same without registers between (32768 x 32768 forward, 8 heads of 32, bf16: 1680 us for 2004; the registers let
+  // four waves a SIMD run): an instruction of a wave fills 1024 bytes of LDS in lane order, so the
   // lane at a place loads the chunk that the swizzle puts there.  For whole chunks, and rows that start at 16-byte
   // boundaries.  off: the lanes' places, in bytes, of rows at at(row); rows from n on are the last one again.
   // Chunks behind D stay as they are: 0 from clear() on.
@@ -353,7 +388,6 @@ __device__ __forceinline__ void load_column(typename Type<T>::frag (&f)[STEPS], 
     f[s] = __builtin_bit_cast(typename Type<T>::frag, row ? fetch(row, 0, 0, (s * 4 + q) * CH, 1, D) : make_uint4(0, 0, 0, 0));
 }
 
-
 // The output's rounding: what is left of v in T.
 template <typename T> __device__ __forceinline__ f32x4 rest_of(f32x4 v) {
 #pragma unroll
@@ -420,13 +454,12 @@ template <> struct Range<_Float16> { static constexpr float kShift = 10.f, kSlac
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The block's place: key head, part and tile; tiles from the last on, which in causal attention have most to
-// do.  Blocks go to XCD block % 8, so with 8 key heads one has a head, whose rows its L2 then keeps.
+// The block's place: key head, part and tile.  Blocks go to XCD block % 8, so with 8 key heads one has a head, whose rows its L2 then keeps.
 __device__ __forceinline__ void place(const Args &p, int &h, int &part, int &tile) {
   const int r = blockIdx.x / p.Hk;
   h = blockIdx.x - r * p.Hk;
   part = r % p.splits;
-  tile = p.tiles - 1 - r / p.splits;
+  tile = r / p.splits;
 }
 
 // Adds the waves' results of a block whose WK waves had each a share of the rows: lane by lane through LDS,
@@ -449,6 +482,14 @@ template <int WK, int N, typename F> __device__ __forceinline__ void add_waves(c
 
 // ---------------------------------------------------------------------------------------------
 // Forward: WC waves of NC x 16 columns side by side, and WK of them that share out each stage's KT keys.
+// Vector instructions issue in 79 % of the cycles and the matrix units are busy in 37 % at 32 channels (32768 x
+// 32768, 8 heads, bf16: 1700 us); where sequences differ, blocks that end early leave fewer waves: 64 and 23 % (16411
+// tokens in 7 sequences: 154 us), at 128 channels 36 and 31 % (8192 causal tokens in 5 sequences, 16/4 heads: 143 us).  LDS
+// is read without bank conflicts, two buffers of KT keys and values hide the loads.  One query of 32/8 heads over 8
+// caches of 8192 tokens, 128 channels: 41 us of which 33 are its bytes.
+// Tried: 4 x 16 columns a wave 1700 us beside 1745 then (and less to share out among the CUs), 128 keys a stage 1990,
+// the sums of P by fp32 additions alone 1835, the scale multiplied into Q beforehand (as two 16-bit terms, to be exact)
+// 1820 beside 1720.
 template <typename T, int DP, int NC, int WC, int WK, int KT, int OCC, bool DMA>
 __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC))) void forward_kernel(Args p) {
   constexpr int NT = 64 * WC * WK, BM = WC * NC * 16, KW = KT / WK, KN = KW / 16;
@@ -739,6 +780,11 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void join_forwar
 
 // ---------------------------------------------------------------------------------------------
 // Gradient of the queries, and delta = sum of o grad_out, which the keys' needs (gq NULL: that alone).
+// The keys' gradient is a kernel of its own, which forms S and dP again: one kernel for both would have to add up
+// grad q over the blocks of keys, by atomics in an order that changes results, or in a workspace of one grad q a block.
+// 16411 tokens in 7 sequences, 8 heads of 32: 155 us (three products of 30 GF: 583 TFLOP/s; vector units 57 %, matrix units
+// 28 % of the cycles); 8192 causal tokens in 5 sequences, 16/4 heads of 128: 165 us (35 and 38 %).  At 128 channels stages are 32 keys
+// long: Q, dO and dQ of 128 columns leave registers for no more.
 template <typename T, int DP, int NC, int WC, int WK, int KT, int OCC, bool DMA>
 __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC))) void grad_q_kernel(Args p) {
   constexpr int NT = 64 * WC * WK, BM = WC * NC * 16, KW = KT / WK, KN = KW / 16;
@@ -909,7 +955,12 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 }
 
 // ---------------------------------------------------------------------------------------------
-// Gradients of keys and values.
+// Gradients of keys and values.  A block owns keys, and queries, output gradients and their two statistics come by: the
+// heads of a group are rows like any other, so their sum is part of the product's.
+// 16411 tokens in 7 sequences, 8 heads of 32: 191 us (four products of 30 GF: 631 TFLOP/s; vector units 48 %, matrix units
+// 29 % of the cycles); 8192 causal tokens in 5 sequences, 16/4 heads of 128: 256 us and 16 for the join (25 and 32 %, LDS
+// 36 %: the operands of four products pass through it for 16 columns a wave, since K, V, dK and dV of 32 columns need
+// more registers than two waves a SIMD have; with them 374 us where these tiles took 273 in one part).
 template <typename T, int DP, int NC, int WC, int WK, int QT, int OCC, bool DMA>
 __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC))) void grad_kv_kernel(Args p) {
   constexpr int NT = 64 * WC * WK, BN = WC * NC * 16, QW = QT / WK, QN = QW / 16;
@@ -924,7 +975,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   int h, part, tile;
   place(p, h, part, tile);
   Work w;
-  if (!locate<true>(p, p.tiles - 1 - tile, BN, w)) return;   // the first keys have most queries
+  if (!locate<true>(p, tile, BN, w)) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
   const int wc = wave % WC, wk = wave / WC;
   const int active = w.nq * p.G, off = w.nk - w.nq, j0 = w.first + wc * NC * 16;
