@@ -22,7 +22,7 @@
  * with sequences or sequences + 1 entries each; with sequences entries the last one ends with the rows.
  * Entries are read on the device only: each counts as the largest of itself and those before it, held to
  * [0, rows].  Sequences may be empty.  Rows that do not count or are in no sequence are not read; their
- * outputs and gradients are 0.
+ * outputs and gradients are 0.  Outputs and workspace must overlap neither each other nor an input.
  */
 #ifndef OPS3D_ATTENTION_H
 #define OPS3D_ATTENTION_H

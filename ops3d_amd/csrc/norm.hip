@@ -14,6 +14,10 @@
 // Backward: the gradients of weight and bias are sums over rows.  A lane keeps them for its columns over
 // all rows it sees, the block adds its waves' in LDS and stores one row of partial sums, and a second
 // kernel adds those in order.
+//
+// 73728 x 256 bf16: forward 16.8 us (75.5 MB at 4.5 TB/s), backward 22.2 + 4.0 for the join (113 MB at 5.1); 2053 x 4101
+// fp32, rows that start anywhere: 17.7 (67 MB, 3.8) and 28.0 + 6.0 (101 MB, 3.6); 400 x 256: 3.2, a launch.  (A copy of
+// 256 MB reaches 5.4 TB/s.)
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
 #include <stdint.h>

@@ -4,6 +4,9 @@
 // LDS first, one pair of a token a thread at a time, since every head of a token turns by the same ones, then
 // streams the heads in 16-byte chunks.  The angle in turns is a 64-bit product, and its whole turns are dropped
 // there: positions far out lose nothing.
+//
+// 73728 tokens, 16 heads of 32, three axes, bf16: 31.6 us (151 MB at 4.8 TB/s; a copy of 256 MB reaches 5.4); 2 x 1551
+// tokens, 20 heads of 128, pairs, fp16: 10.3 (31.8 MB, 3.1).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdarg.h>
