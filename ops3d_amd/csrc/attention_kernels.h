@@ -748,17 +748,15 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void join_forwar
   m = ops3d_reduce::all<64, ops3d_reduce::Max>(m);
   float whole = 0.f, l = 0.f;
   f32x4 o = splat(0.f);
-  if (m != -INFINITY) {
 #pragma unroll 2
-    for (int z = lane / PER; z < p.splits; z += AT) {
-      const int64_t at = z * p.cells + cell;
-      const f32x4 ml = p.part_ml[at], v = *reinterpret_cast<const f32x4 *>(p.part + at * DP + d);
-      if (ml[0] == -INFINITY) continue;
-      const float by = exp2_(ml[0] - m);
-      whole = fmaf(by, ml[1], whole);
-      l = fmaf(by, ml[2], l);
-      o += v * by;
-    }
+  for (int z = lane / PER; z < p.splits; z += AT) {
+    const int64_t at = z * p.cells + cell;
+    const f32x4 ml = p.part_ml[at], v = *reinterpret_cast<const f32x4 *>(p.part + at * DP + d);
+    // without a reference the sums are 0, or NaN where the part's logits are: both count
+    const float by = ml[0] == -INFINITY ? 1.f : exp2_(ml[0] - m);
+    whole = fmaf(by, ml[1], whole);
+    l = fmaf(by, ml[2], l);
+    o += v * by;
   }
 #pragma unroll
   for (int s = PER; s < 64; s <<= 1) {

@@ -1,0 +1,72 @@
+"""packed_attention where inputs are not finite, rows do not count, sums are cut into parts, numbers are small
+or large for their type, and calls are many: against oracle/attention.py, or against the definition where a
+result is not finite."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import attention as ref
+from ops3d_amd import _extension, packed_attention
+from test_attention import DTYPES, check, gpu, make, table
+
+
+def inputs(dtype, nq, nk, H, Hk, D, lead=(), seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return [make(gen, (*lead, *s), DTYPES[dtype]) for s in ((nq, H, D), (nk, Hk, D), (nk, Hk, D), (nq, H, D))]
+
+
+def step(q, k, v, u, **kw):
+    """[y, dq, dk, dv]"""
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    y = packed_attention(*leaves, **kw)
+    return [y.detach(), *torch.autograd.grad(y, leaves, u)]
+
+
+def parts(dtype, nq, nk, H, Hk, D, items=1, causal=False, sequences=0):
+    """Whether the forward of this problem is cut into parts: its workspace holds them (and, of more than 64
+    sequences, the table of tiles)."""
+    p = _extension._AttentionProblem()
+    for name, value in {"q_rows": nq, "k_rows": nk, "items": items, "heads": H, "kv_heads": Hk, "dim": D, "scale": 1.0, "causal": causal,
+                        "dtype": list(DTYPES).index(dtype), "sequences": sequences}.items():
+        setattr(p, name, value)
+    if sequences:
+        p.q_start = p.k_start = 256
+        p.q_start_count = p.k_start_count = sequences + 1
+    return _extension.load_library().ops3d_attention_forward_workspace_bytes(p) > 0
+
+
+IN_PARTS = [(1, 8192, 4, 1, 64, False), (3, 5000, 2, 2, 32, False), (200, 9000, 8, 8, 32, False), (4200, 4200, 8, 8, 32, True), (3, 5000, 2, 1, 128, True)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nq,nk,H,Hk,D,causal", IN_PARTS)
+def test_nan_reaches_queries_whose_keys_are_cut_into_parts(gpu_device, nq, nk, H, Hk, D, causal, dtype):
+    """A part whose logits are all NaN has no largest one, and counts all the same."""
+    assert parts(dtype, nq, nk, H, Hk, D, causal=causal)
+    q, k, v, u = inputs(dtype, nq, nk, H, Hk, D, seed=nq)
+    want = ref.sequence(q, k, v, causal, D ** -0.5, u)
+    other = slice(H // Hk, H) if Hk > 1 else slice(0, 0)   # query heads of other key heads than the first
+    bad = q.clone()
+    bad[nq // 2, 0, 1] = math.nan
+    y, dq, _, _ = step(bad, k, v, u, causal=causal)
+    keep = torch.ones(nq, H, dtype=torch.bool, device="cuda")
+    keep[nq // 2, 0] = False
+    assert y[nq // 2, 0].isnan().all() and dq[nq // 2, 0].isnan().all()
+    for name, got in (("y", y), ("dq", dq)):
+        check(name, got[keep], tuple(t[keep] for t in want[name]))
+    for keys in (slice(0, nk), slice(0, nk - nk // 3), slice(nk // 3, nk), slice(128, 1024)):
+        bad = k.clone()
+        bad[keys, 0, D - 1] = math.nan
+        y, dq, dk, dv = step(q, bad, v, u, causal=causal)
+        first = max(0, keys.start - (nk - nq)) if causal else 0   # the first query that sees one of them
+        assert y[first:, :H // Hk].isnan().all() and dq[first:, :H // Hk].isnan().all()
+        assert dk[keys, 0].isnan().all() and dv[keys, 0].isnan().all()
+        for name, got in (("y", y), ("dq", dq)):
+            check(name, got[:first], tuple(t[:first] for t in want[name]))
+            check(name, got[:, other], tuple(t[:, other] for t in want[name]))
+        with torch.no_grad():
+            assert torch.equal(packed_attention(q, bad, v, causal=causal).isnan(), y.isnan())
