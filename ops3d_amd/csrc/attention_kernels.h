@@ -942,7 +942,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     if (p.splits > 1) {
       const int64_t to = part * p.cells + cell0 + c;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + to * DP + d * 16 + q * 4) = a[n][d];
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + to * DP + d * 16 + q * 4) = c < active ? a[n][d] : splat(0.f);
       continue;
     }
     T *to = static_cast<T *>(p.gq.p) + w.item * p.gq.item + (w.q0 + t) * p.gq.token + ((int64_t)h * p.G + c - t * p.G) * p.gq.head;

@@ -70,3 +70,21 @@ def test_nan_reaches_queries_whose_keys_are_cut_into_parts(gpu_device, nq, nk, H
             check(name, got[:, other], tuple(t[:, other] for t in want[name]))
         with torch.no_grad():
             assert torch.equal(packed_attention(q, bad, v, causal=causal).isnan(), y.isnan())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("nq,nk,H,Hk,D", [(3, 5000, 2, 1, 64), (5, 4000, 4, 4, 128), (70, 6000, 4, 2, 32), (70, 90, 4, 2, 32)])
+def test_gradients_of_rows_that_do_not_count(gpu_device, nq, nk, H, Hk, D, value, dtype):
+    """Zeros, also beside keys and values that are not finite, in parts or not."""
+    q, k, v, u = inputs(dtype, nq, nk, H, Hk, D, lead=(2,), seed=nq)
+    k[0, 7, 0, 0], v[0, nk - 1, Hk - 1, 1], k[1, nk // 2, 0, 0], v[1, 5, 0, 1] = value, value, value, value
+    lens = [nq - 1, nq // 3]
+    q_len = table(lens)
+    y, dq, _, _ = step(q, k, v, u, q_len=q_len)
+    for i, n in enumerate(lens):
+        assert not y[i, n:].any() and not dq[i, n:].any()
+    y, dq, _, _ = step(q[0], k[0], v[0], u[0], q_start=table([1, lens[0]]), k_start=table([0, nk]))
+    for t in (y, dq):
+        assert not t[:1].any() and not t[lens[0]:].any()
