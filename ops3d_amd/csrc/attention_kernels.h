@@ -314,6 +314,10 @@ template <typename T, int DP, int R, int NT> struct Stage {
     for (int i = threadIdx.x * 16; i < bytes; i += NT * 16) *reinterpret_cast<uint4 *>(lds + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
+  // Zeros in rows from n on.  Called by all threads, between barriers.
+  static __device__ __forceinline__ void clear_rows(char *lds, int n) {
+    for (int i = n * RC + threadIdx.x; i < R * RC; i += NT) *reinterpret_cast<uint4 *>(lds + i * 16) = make_uint4(0, 0, 0, 0);
+  }
   static __device__ __forceinline__ void store(char *lds, const uint4 (&v)[NL]) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4 *>(lds + address(row_of(i), chunk_of(i))) = v[i];
@@ -1065,6 +1069,11 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     if (DMA) ST::arrived();
     else __syncthreads();
     if (DMA && c0 + QT < c_end) load(c0 + QT, buf ^ 1);
+    if (DMA && c_end - c0 < QT) {   // copies of the last row, whose infinities times P = 0 would be NaN
+      ST::clear_rows(lds + buf * 2 * ST::kBytes, c_end - c0);
+      ST::clear_rows(lds + buf * 2 * ST::kBytes + ST::kBytes, c_end - c0);
+      __syncthreads();
+    }
 #pragma unroll
     for (int qt = 0; qt < QN; qt += PR) {
       f32x4 s[NC][PR], dp[NC][PR], lse[PR];

@@ -88,3 +88,20 @@ def test_gradients_of_rows_that_do_not_count(gpu_device, nq, nk, H, Hk, D, value
     y, dq, _, _ = step(q[0], k[0], v[0], u[0], q_start=table([1, lens[0]]), k_start=table([0, nk]))
     for t in (y, dq):
         assert not t[:1].any() and not t[lens[0]:].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nq,nk,H,Hk,D", [(1, 70, 2, 2, 32), (5, 70, 2, 2, 32), (70, 70, 4, 2, 32), (9000, 70, 2, 2, 32), (333, 8000, 6, 2, 64), (70, 300, 2, 2, 128),
+                                          (70, 300, 2, 2, 36), (5000, 20000, 6, 2, 32)])
+def test_infinity_in_the_last_output_gradient(gpu_device, nq, nk, H, Hk, D, dtype):
+    """Rows behind the last one in its tile have no weight: an infinity in the last one stays one in the values'
+    gradients, and the other channels know nothing of it."""
+    q, k, v, u = inputs(dtype, nq, nk, H, Hk, D, seed=nq)
+    value, bound = ref.sequence(q, k, v, False, D ** -0.5, u)["dv"]
+    u[-1, H // Hk - 1, 3], u[-1, H - 1, 4] = math.inf, -math.inf
+    _, _, _, dv = step(q, k, v, u)
+    assert (dv[:, 0, 3] == math.inf).all() and (dv[:, Hk - 1, 4] == -math.inf).all()
+    keep = torch.isfinite(dv)
+    assert keep.sum() == dv.numel() - 2 * nk
+    check("dv", dv[keep], (value[keep], bound[keep]))
