@@ -63,7 +63,7 @@ struct Args {
   void *rest;                         // what rounding took from o, [items, Sq, heads, D] contiguous, or nullptr
   float *lse, *delta;                 // [items, Hk, Sq G]; log2 of the sum of exponentials, and sum of o g
   float *part;                        // [splits, columns, DP]
-  f32x4 *part_ml;                     // [splits, columns]: reference, sum of rounded P, sum of P
+  f32x4 *part_ml;                     // [splits, columns]: reference, sum of rounded P, sum of P, whether the column sees a key
 };
 
 // What a block works on.
@@ -716,15 +716,16 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   for (int n = 0; n < NC; ++n) {
     const int c = c0 + n * 16 + i;
     if (c >= w.rows * p.G) continue;
+    // 0 for columns that do not count or see no key.  By what they see: a sum of 0 is also that of logits of minus
+    // infinity, whose softmax is NaN.
+    const bool none = c >= active || limit[n] <= 0;
     if (p.splits > 1) {
       const int64_t to = part * p.cells + cell0 + c;
 #pragma unroll
       for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + to * DP + d * 16 + q * 4) = o[n][d];
-      if (q == 0)   // columns that do not count saw nothing
-        p.part_ml[to] = c < active ? f32x4{m[n], whole[n], l[n], 0.f} : f32x4{-INFINITY, 0.f, 0.f, 0.f};
+      if (q == 0) p.part_ml[to] = none ? f32x4{-INFINITY, 0.f, 0.f, 0.f} : f32x4{m[n], whole[n], l[n], 1.f};
       continue;
     }
-    const bool none = c >= active || whole[n] == 0.f;
     const float inv = none ? 0.f : 1.f / whole[n];
     const int t = divide(p, c);
     const int head = h * p.G + c - t * p.G;
@@ -771,7 +772,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void join_forwar
   }
   const int per = p.Sq * p.G, ih = (int)(cell / per), c = (int)(cell - (int64_t)ih * per);
   const int item = ih / p.Hk, h = ih - item * p.Hk, t = divide(p, c), head = h * p.G + c - t * p.G;
-  const bool none = whole == 0.f;
+  const bool none = p.part_ml[cell][3] == 0.f;   // the same in all parts
   const f32x4 v = none ? splat(0.f) : o * (1.f / whole);
   if (lane < PER) {
     store4(static_cast<T *>(p.o.p) + item * p.o.item + t * p.o.token + head * p.o.head, d, v, p.D);

@@ -105,3 +105,42 @@ def test_infinity_in_the_last_output_gradient(gpu_device, nq, nk, H, Hk, D, dtyp
     keep = torch.isfinite(dv)
     assert keep.sum() == dv.numel() - 2 * nk
     check("dv", dv[keep], (value[keep], bound[keep]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nq,nk,H,Hk,D", [(5, 9, 2, 1, 32), (70, 150, 4, 2, 36), (1, 600, 2, 1, 64), (1, 8192, 4, 1, 64), (200, 9000, 8, 8, 32), (2600, 2600, 8, 8, 32)])
+def test_logits_that_are_all_minus_infinity(gpu_device, nq, nk, H, Hk, D, dtype):
+    """Softmax of them is NaN, as their keys are: a query is only 0 where it sees no key."""
+    q, k, v, u = inputs(dtype, nq, nk, H, Hk, D, seed=nk)
+    q[..., 0] = 1
+    k[:, 0, 0] = -math.inf
+    y, dq, dk, dv = step(q, k, v, u)
+    own = slice(0, H // Hk)   # the first key head's queries
+    for t in (y[:, own], dq[:, own], dk[:, 0], dv[:, 0]):
+        assert t.isnan().all()
+    assert torch.isfinite(y[:, H // Hk:]).all() and torch.isfinite(dq[:, H // Hk:]).all()
+    with torch.no_grad():
+        assert torch.equal(packed_attention(q, k, v).isnan(), y.isnan())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n,H,Hk,D", [(90, 2, 1, 32), (700, 2, 2, 64), (4200, 8, 8, 32), (2300, 8, 2, 128)])
+def test_one_logit_of_minus_infinity(gpu_device, n, H, Hk, D, dtype):
+    """Causal: the first key has it.  The first query sees no other and gives NaN, the rest as without that key; queries
+    before the keys see none and give 0."""
+    q, k, v, u = inputs(dtype, n, n, H, Hk, D, seed=n)
+    q[..., 0] = 1
+    bad = k.clone()
+    bad[0, :, 0] = -math.inf
+    y, dq, dk, dv = step(q, bad, v, u, causal=True)
+    assert y[0].isnan().all() and dq[0].isnan().all() and dk[0].isnan().all() and dv[0].isnan().all()
+    want = ref.sequence(q[1:], k[1:], v[1:], True, D ** -0.5, u[1:])
+    check("y", y[1:], want["y"])
+    check("dq", dq[1:, :, 1:], tuple(t[..., 1:] for t in want["dq"]))   # 0 times the infinity in the first channel
+    check("dk", dk[1:], want["dk"])
+    check("dv", dv[1:], want["dv"])
+    y, dq, dk, dv = step(q, k[:n // 2], v[:n // 2], u, causal=True)
+    first = n - n // 2
+    assert not y[:first].any() and not dq[:first].any() and y[first:].any(-1).all()
