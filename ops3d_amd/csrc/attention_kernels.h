@@ -392,10 +392,10 @@ __device__ __forceinline__ void load_column(typename Type<T>::frag (&f)[STEPS], 
     f[s] = __builtin_bit_cast(typename Type<T>::frag, row ? fetch(row, 0, 0, (s * 4 + q) * CH, 1, D) : make_uint4(0, 0, 0, 0));
 }
 
-// The output's rounding: what is left of v in T.
+// The output's rounding: what is left of v in T; nothing of an infinity, which would be NaN.
 template <typename T> __device__ __forceinline__ f32x4 rest_of(f32x4 v) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] -= (float)(T)v[j];
+  for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) == INFINITY ? 0.f : v[j] - (float)(T)v[j];
   return v;
 }
 

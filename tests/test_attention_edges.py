@@ -144,3 +144,18 @@ def test_one_logit_of_minus_infinity(gpu_device, n, H, Hk, D, dtype):
     y, dq, dk, dv = step(q, k[:n // 2], v[:n // 2], u, causal=True)
     first = n - n // 2
     assert not y[:first].any() and not dq[:first].any() and y[first:].any(-1).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nk", [9, 300, 5000])
+def test_infinite_outputs_and_their_gradients(gpu_device, nk, dtype):
+    """An infinite value makes the output's product with its gradient infinite, and the other keys' gradients with it."""
+    q, k, v, u = inputs(dtype, 1, nk, 1, 1, 32, seed=nk)
+    v[4, 0, 2] = math.inf
+    y, dq, dk, dv = step(q, k, v, u)
+    assert y[0, 0, 2] == math.inf and torch.isfinite(y).sum() == 31
+    others = torch.arange(nk, device="cuda") != 4
+    sign = -torch.sign(u[0, 0, 2]) * torch.sign(q[0])   # logits' gradients are P (dP - delta)
+    assert torch.equal(dk[others], (sign * math.inf)[None].expand(nk - 1, 1, 32))
+    assert dk[4].isnan().all() and dq.isnan().all() and torch.isfinite(dv).all()
