@@ -453,10 +453,62 @@ __device__ __forceinline__ void add_seen(f32x4 &acc, const typename Type<T>::fra
 
 // 16-bit fractions as fp16 numbers lose precision below 2^-14, so that of P is kept 2^kShift up; with the
 // slack below, P stays under 2^15.
-template <typename T> struct Range { static constexpr float kShift = 0.f, kSlack = 8.f; };
-template <> struct Range<_Float16> { static constexpr float kShift = 10.f, kSlack = 4.f; };
+template <typename T> struct Range {
+  static constexpr float kShift = 0.f, kSlack = 8.f;
+  static constexpr bool kScaled = false;
+};
+template <> struct Range<_Float16> {
+  static constexpr float kShift = 10.f, kSlack = 4.f;
+  static constexpr bool kScaled = true;   // see Scale
+};
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// fp16: dS has no bounds of its own (grad_out may be scaled, and P is small where keys are many), so a column's is held
+// times a power of two, chosen like the softmax's reference: the first that are not 0 come to 2^9 at most, and so do, with
+// the sums so far, those of which one would pass 2^15.  The maxima and the branch cost 2 to 18 % of the backward (16411 tokens
+// in 7 sequences, 8 heads of 32: 309 -> 342 us; 8192 causal tokens in 5, 16/4 heads of 128: 355 -> 361).
+struct Scale {
+  float top = 0.f;   // what raises it: 2^15 over the power, or 0 where there is none yet
+  __device__ __forceinline__ float power() const { return __uint_as_float(0x86800000u - __float_as_uint(top)); }   // finite for 0 too
+  __device__ __forceinline__ float inverse() const { return top * 0x1p-15f; }
+  // most: the largest size of the lane's new ones
+  template <int N> __device__ __forceinline__ void raise(float most, f32x4 (&sums)[N]) {
+    most = ops3d_reduce::across32<ops3d_reduce::Max>(ops3d_reduce::across16<ops3d_reduce::Max>(most));
+    if (!(most > top)) return;
+    const int e = 9 - __builtin_amdgcn_frexp_expf(fminf(most, 0x1p127f));   // the power's exponent
+    const float now = __uint_as_float((uint32_t)(127 + 15 - max(-112, min(100, e))) << 23), change = top * __uint_as_float(0x7f000000u - __float_as_uint(now));   // powers of two, or 0
+#pragma unroll
+    for (int i = 0; i < N; ++i) sums[i] *= change;
+    top = now;
+  }
+};
+
+// dS as operands of products that are summed to sums, NC columns of PR tiles.
+template <typename F, int NC, int PR, int N>
+__device__ __forceinline__ void scaled(F (&f)[NC], f32x4 (&ds)[NC][PR], Scale (&scale)[NC], f32x4 (&sums)[NC][N]) {
+  float most[NC];
+  bool raise = false;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    most[n] = 0.f;
+#pragma unroll
+    for (int u = 0; u < PR; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most[n] = fmaxf(most[n], fabsf(ds[n][u][j]));
+    raise |= most[n] > scale[n].top;
+  }
+  if (__ballot(raise)) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) scale[n].raise(most[n], sums[n]);
+  }
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+#pragma unroll
+    for (int u = 0; u < PR; ++u) ds[n][u] *= scale[n].power();
+    f[n] = operand<_Float16>(ds[n]);
+  }
+}
 
 // The block's place: key head, part and tile.  Blocks go to XCD block % 8, so with 8 key heads one has a head, whose rows its L2 then keeps.
 __device__ __forceinline__ void place(const Args &p, int &h, int &part, int &tile) {
@@ -846,6 +898,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   }
 
   f32x4 a[NC][DT];
+  Scale scale[NC];
 #pragma unroll
   for (int n = 0; n < NC; ++n)
 #pragma unroll
@@ -915,8 +968,9 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
             if (decltype(masked)::value && k0 + r0 + (kt + u) * 16 + q * 4 + j >= limit[n]) x = 0.f;
             s[n][u][j] = x;
           }
-        ds[n] = operand<T>(s[n]);
+        if (!Range<T>::kScaled) ds[n] = operand<T>(s[n]);
       }
+      if constexpr (Range<T>::kScaled) scaled(ds, s, scale, a);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const auto kf = ST::columns(lk, r0 + kt * 16, d, at, lane);
@@ -935,6 +989,12 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   if (k_begin < k_end) load(k_begin, 0);
   while (k0 < k_end && k0 + KT <= least) stage(std::false_type());
   while (k0 < k_end) stage(std::true_type());
+  if constexpr (Range<T>::kScaled) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) a[n][d] *= scale[n].inverse();
+  }
   if constexpr (WK > 1) {
     static_assert(WC == 1, "the waves' results lie one behind another");
     add_waves<WK, NC * DT>(lds, wk, lane, [&](int k) -> f32x4 & { return a[k / DT][k % DT]; });
@@ -1011,6 +1071,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   }
 
   f32x4 ak[NC][DT], av[NC][DT];
+  Scale scale[NC];
 #pragma unroll
   for (int n = 0; n < NC; ++n)
 #pragma unroll
@@ -1106,15 +1167,15 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float x = exp2_(fmaf(s[n][u][j], p.c, lse[u][j])), y = x * dp[n][u][j];
-            if (kDown != 1.f) y *= kDown;
             if (decltype(masked)::value && r + j < since[n]) x = y = 0.f;
             s[n][u][j] = x;
             dp[n][u][j] = y;
           }
         }
         pf[n] = operand<T>(s[n]);
-        ds[n] = operand<T>(dp[n]);
+        if (!Range<T>::kScaled) ds[n] = operand<T>(dp[n]);
       }
+      if constexpr (Range<T>::kScaled) scaled(ds, dp, scale, ak);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const auto gf = ST::columns(lg, r0 + qt * 16, d, at, lane), qf = ST::columns(lq, r0 + qt * 16, d, at, lane);
@@ -1139,6 +1200,12 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   if (c_begin < c_end) load(c_begin, 0);
   while (c0 < c_end && c0 < all_see) stage(std::true_type());
   while (c0 < c_end) stage(std::false_type());
+  if constexpr (Range<T>::kScaled) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) ak[n][d] *= scale[n].inverse() * kDown;
+  }
   if constexpr (WK > 1) {
     static_assert(WC == 1, "the waves' results lie one behind another");
     add_waves<WK, NC * DT>(lds, wk, lane, [&](int k) -> f32x4 & { return ak[k / DT][k % DT]; });

@@ -12,7 +12,8 @@ count roundings (U = 2^-24, u half a step of dtype):
   sum (the logarithm that the backward's probabilities come from is of the sum as it is);
 * a sum of n products is off by (n / 4 + 40) U of the sum of their sizes: four at least are added at a time,
   a sum is rescaled some times, and parts are joined;
-* fp16: P is held 2^10 up, so that one below 2^-14 is off by 2^-35 at most; dS is not: by 2^-25;
+* fp16: P is held 2^10 up, so that one below 2^-14 is off by 2^-35 at most; dS is held so that the largest of what is
+  summed, for a query's gradient or for a key's, is 2^8 at least: one far below it is off by 2^-33 of that largest;
 * every type: a power, and a product in fp32 or an operand of bf16, below 2^-126 may count as 0, so that a P is off by
   2^-125 more, and a dS by that times its factor and once more;
 * the sum of out grad_out is formed from the rounded out and what rounding took from it, itself rounded.
@@ -45,7 +46,7 @@ def sequence(q, k, v, causal, scale, grad=None):
     G = H // Hk
     u = 0.0 if dtype == torch.float32 else _half(dtype)
     tiny = 2.0 ** -125
-    low_p, low_ds = (2.0 ** -35, 2.0 ** -25) if dtype == torch.float16 else (tiny, tiny)
+    low_p, low_ds = (2.0 ** -35, 2.0 ** -33) if dtype == torch.float16 else (tiny, 0.0)
     q, k, v = q.double(), k.double(), v.double()
     grad = None if grad is None else grad.double()
     out = {"y": [torch.zeros_like(q), torch.zeros_like(q)]}
@@ -59,7 +60,7 @@ def sequence(q, k, v, causal, scale, grad=None):
         seen = torch.arange(nk, device=q.device)[None] <= torch.arange(nq, device=q.device)[:, None] + nk - nq
     some = seen.any(1, keepdim=True)
     hk, hq = (nk / 4 + 40) * U, (nq * G / 4 + 40) * U
-    log2e = 1 / LN2
+    most, weight = torch.zeros(nk, Hk, 1, dtype=q.dtype, device=q.device), torch.zeros_like(k)   # of a key's dS, and of what it meets
     for h in range(H):
         qh, kh, vh = q[:, h], k[:, h // G], v[:, h // G]
         s = (qh @ kh.t()) * scale
@@ -87,13 +88,19 @@ def sequence(q, k, v, causal, scale, grad=None):
         e_delta = (e_o * g.abs()).sum(1, keepdim=True) + (D + 2) * U * (y * g).abs().sum(1, keepdim=True)
         ds = p * (dp - delta)
         e_ds = ds.abs() * (d + u + 3 * U) + p * (e_dp + e_delta + 2 * U * (dp.abs() + delta.abs()))
-        e_ds = e_ds + seen.double() * (low_ds + tiny * (dp.abs() + delta.abs()))
+        e_ds = e_ds + seen.double() * tiny * (1 + dp.abs() + delta.abs())
+        size = ds.abs() + e_ds
+        low_q = low_ds * size.amax(1, keepdim=True) * seen.double()
+        most[:, h // G] = torch.maximum(most[:, h // G], size.amax(0)[:, None])
+        weight[:, h // G] += seen.double().t() @ qh.abs()
         out["dq"][0][:, h] = scale * (ds @ kh)
-        out["dq"][1][:, h] = scale * ((e_ds + hk * ds.abs()) @ kh.abs())
+        out["dq"][1][:, h] = scale * ((e_ds + low_q + hk * ds.abs()) @ kh.abs())
         out["dk"][0][:, h // G] += scale * (ds.t() @ qh)
         out["dk"][1][:, h // G] += scale * ((e_ds + hq * ds.abs()).t() @ qh.abs())
         out["dv"][0][:, h // G] += p.t() @ g
         out["dv"][1][:, h // G] += (p * (d + u + hq)).t() @ g.abs() + low_p * (seen.double().t() @ g.abs())
+    if grad is not None:
+        out["dk"][1] += scale * low_ds * most * weight
     for name in ("dq", "dk", "dv"):
         if grad is not None:
             value, bound = out[name]

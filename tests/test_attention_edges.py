@@ -159,3 +159,37 @@ def test_infinite_outputs_and_their_gradients(gpu_device, nk, dtype):
     sign = -torch.sign(u[0, 0, 2]) * torch.sign(q[0])   # logits' gradients are P (dP - delta)
     assert torch.equal(dk[others], (sign * math.inf)[None].expand(nk - 1, 1, 32))
     assert dk[4].isnan().all() and dq.isnan().all() and torch.isfinite(dv).all()
+
+
+@gpu
+@pytest.mark.parametrize("nq,nk,H,Hk,D,causal", [(50, 6000, 2, 1, 32, False), (700, 700, 4, 2, 64, True), (6000, 50, 2, 2, 32, False), (300, 300, 2, 1, 128, False),
+                                                 (300, 400, 3, 1, 36, True), (9000, 9000, 8, 8, 32, True), (1, 8192, 8, 2, 128, False)])
+@pytest.mark.parametrize("size", [1e-4, 1.0, 2000.0])
+def test_fp16_gradients_of_small_and_large_ones(gpu_device, size, nq, nk, H, Hk, D, causal):
+    """Logits' gradients are held in fp16 times a power of two of their query's or key's own."""
+    q, k, v, u = inputs("fp16", nq, nk, H, Hk, D, seed=nq)
+    if size > 1:   # products of v and grad_out pass fp16, what is made of them does not
+        q, k, v = q * 0.01, k * 0.01, v * 100
+    u = (u.float() * size).half()
+    want = ref.sequence(q, k, v, causal, D ** -0.5, u)
+    for name, got in zip(("y", "dq", "dk", "dv"), step(q, k, v, u, causal=causal)):
+        value, bound = want[name]
+        fits = value.abs() + bound < 65504
+        assert fits.float().mean() > 0.9, name
+        check(name, got[fits], (value[fits], bound[fits]))
+
+
+@gpu
+def test_fp16_gradients_that_grow_along_the_sum(gpu_device):
+    """Each query's and each key's largest comes last, or first, over many powers of two; zeros first."""
+    q, k, v, u = inputs("fp16", 600, 700, 2, 1, 32, seed=3)
+    for flip in (False, True):
+        up = torch.exp2(torch.linspace(-20, 9, 600, device="cuda"))[:, None, None]
+        down = torch.exp2(torch.linspace(-14, 5, 700, device="cuda"))[:, None, None]
+        if flip:
+            up, down = up.flip(0), down.flip(0)
+        uu, vv = (u * up).half(), (v * down).half()
+        uu[:40] = 0
+        want = ref.sequence(q, k, vv, False, 32 ** -0.5, uu)
+        for name, got in zip(("y", "dq", "dk", "dv"), step(q, k, vv, uu)):
+            check(name, got, want[name])
