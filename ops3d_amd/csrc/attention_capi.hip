@@ -110,7 +110,7 @@ Plan plan_keys(const ops3d_attention_problem *p) {
   return plan_of(p, p->k_rows, p->q_rows * (p->heads / p->kv_heads), p->dim > 64 ? kSome : kMany);
 }
 
-// false: more blocks than a launch has
+// false: 2^31 blocks or more, which are counted in 32 bits
 bool set_plan(Args &a, const ops3d_attention_problem *p, const Plan &plan) {
   const int64_t tiles = p->q_start ? plan.tiles : (int64_t)plan.tiles_item * p->items;
   if (tiles * p->kv_heads > 0x7fffffff / plan.splits) return false;

@@ -33,6 +33,7 @@
 #include <type_traits>
 
 #include "elements.h"
+#include "launch.h"
 #include "reduce.h"
 #include "segments.h"
 
@@ -57,6 +58,7 @@ struct Args {
   int dma;                            // rows go straight to LDS: bit 0 k and v, bit 1 q and grad_out
   float scale, c;                     // c = scale log2 e
   int tiles, tiles_item, splits;      // tiles of all items (a bound), of one, and parts of the other side
+  unsigned block0;                    // blocks in launches before this one
   int heads;                          // items Hk
   int64_t cells;                      // heads Sq G: queries times heads
   const int4 *table;                  // two for each tile of packed sequences (see table_kernel), or nullptr
@@ -512,8 +514,8 @@ __device__ __forceinline__ void scaled(F (&f)[NC], f32x4 (&ds)[NC][PR], Scale (&
 
 // The block's place: key head, part and tile.  Blocks go to XCD block % 8, so with 8 key heads one has a head, whose rows its L2 then keeps.
 __device__ __forceinline__ void place(const Args &p, int &h, int &part, int &tile) {
-  const int r = blockIdx.x / p.Hk;
-  h = blockIdx.x - r * p.Hk;
+  const int block = blockIdx.x + p.block0, r = block / p.Hk;
+  h = block - r * p.Hk;
   part = r % p.splits;
   tile = r / p.splits;
 }
@@ -1292,7 +1294,10 @@ template <typename F> hipError_t with_dim(int dp, F f) {
   if (dp == 64) return f(std::integral_constant<int, 64>());
   return f(std::integral_constant<int, 128>());
 }
-inline unsigned blocks_of(const Args &p) { return (unsigned)((int64_t)p.tiles * p.splits * p.Hk); }
+// The launch itself, and its errors.  Those of joins are small: what is cut into parts has few columns.
+template <typename K> hipError_t start(K kernel, const Args &p, int threads, hipStream_t st) {
+  return ops3d_launch::launch(kernel, (int64_t)p.tiles * p.splits * p.Hk, threads, st, p);
+}
 
 template <typename T> hipError_t forward(const Args &args, int dp, int shape, hipStream_t st) {
   const Args p = with_table<false>(args, shape, st);
@@ -1300,8 +1305,9 @@ template <typename T> hipError_t forward(const Args &args, int dp, int shape, hi
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kforward>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      if (p.dma & 1) forward_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
-      else forward_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      const hipError_t e = p.dma & 1 ? start(forward_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true>, p, 64 * WC * WK, st)
+                                     : start(forward_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false>, p, 64 * WC * WK, st);
+      if (e != hipSuccess) return e;
       if (p.splits > 1) join_forward_kernel<T, DP><<<(unsigned)((p.cells + 3) / 4), 256, 0, st>>>(p);
       return hipGetLastError();
     });
@@ -1313,8 +1319,9 @@ template <typename T> hipError_t grad_q(const Args &args, int dp, int shape, hip
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kgrad_q>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      if (p.dma & 1) grad_q_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
-      else grad_q_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      const hipError_t e = p.dma & 1 ? start(grad_q_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true>, p, 64 * WC * WK, st)
+                                     : start(grad_q_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false>, p, 64 * WC * WK, st);
+      if (e != hipSuccess) return e;
       if (p.splits > 1) join_sum_kernel<T, DP, false><<<(unsigned)((p.cells * (DP / 4) + 255) / 256), 256, 0, st>>>(p);
       return hipGetLastError();
     });
@@ -1326,8 +1333,9 @@ template <typename T> hipError_t grad_kv(const Args &args, int dp, int shape, hi
     constexpr int DP = decltype(d)::value;
     return with_shape<T, DP, kgrad_kv>(shape, [&](auto nc, auto wc, auto wk, auto kt) {
       constexpr int NC = decltype(nc)::value, WC = decltype(wc)::value, WK = decltype(wk)::value, KT = decltype(kt)::value;
-      if (p.dma & 2) grad_kv_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
-      else grad_kv_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false><<<blocks_of(p), 64 * WC * WK, 0, st>>>(p);
+      const hipError_t e = p.dma & 2 ? start(grad_kv_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(true, DP, WK), true>, p, 64 * WC * WK, st)
+                                     : start(grad_kv_kernel<T, DP, NC, WC, WK, KT, occupancy<T>(false, DP, WK), false>, p, 64 * WC * WK, st);
+      if (e != hipSuccess) return e;
       const int64_t rows = (int64_t)p.heads * p.Sk * 2;
       if (p.splits > 1) join_sum_kernel<T, DP, true><<<(unsigned)((rows * (DP / 4) + 255) / 256), 256, 0, st>>>(p);
       return hipGetLastError();

@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "elements.h"
+#include "launch.h"
 #include "segments.h"
 
 namespace ops3d_linear {
@@ -1213,18 +1214,7 @@ inline int64_t max_row_tiles(const Groups &g, int BM) {
   return (int64_t)g.B * (tiles < g.S ? tiles : g.S);
 }
 
-// A launch holds less than 2^32 threads; more go in several, each a multiple of the XCDs' 8 blocks.
-template <typename K, typename A> inline hipError_t launch(K kernel, int64_t grid, int threads, hipStream_t st, A p) {
-  if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
-  const int64_t most = 0xffffffff / threads & ~(int64_t)7;
-  for (int64_t at = 0; at < grid; at += most) {
-    p.block0 = (unsigned)at;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(grid - at < most ? grid - at : most)), dim3(threads), 0, st, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
-}
+using ops3d_launch::launch;
 
 template <typename T, int BM, int BN, int WR, int WC, int U, bool DMA, int OCC, bool WSTR, bool SCALE, bool EPI, bool SPLIT = false>
 inline hipError_t launch_rows(RowsArgs p, hipStream_t st) {

@@ -193,3 +193,13 @@ def test_fp16_gradients_that_grow_along_the_sum(gpu_device):
         want = ref.sequence(q, k, vv, False, 32 ** -0.5, uu)
         for name, got in zip(("y", "dq", "dk", "dv"), step(q, k, vv, uu)):
             check(name, got, want[name])
+
+
+@gpu
+def test_more_blocks_than_one_launch_has(gpu_device):
+    """2^24 blocks of 256 threads and some: items of one token, whose result is the value."""
+    items = (1 << 21) + 5
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    q, k, v, u = (torch.randint(-3, 4, (items, 1, 8, 8), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16) for _ in range(4))
+    y, dq, dk, dv = step(q, k, v, u)
+    assert torch.equal(y, v) and torch.equal(dv, u) and not dq.any() and not dk.any()
