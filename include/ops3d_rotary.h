@@ -15,7 +15,8 @@
  *
  * positions [items or 1, tokens, axes], contiguous, on the device; position_item is the distance between
  * items in elements (0: the same for all).  frequencies and axis_of [pairs] are HOST memory, read before
- * the call returns.
+ * the call returns.  A call has at most OPS3D_ROTARY_MAX_ITEMS items of less than 2^31 tokens, and a token at
+ * most 65536 heads, 65536 channels a head and 2^24 channels.
  */
 #ifndef OPS3D_ROTARY_H
 #define OPS3D_ROTARY_H
@@ -35,6 +36,7 @@ extern "C" {
 #define OPS3D_ROTARY_POSITION_I64 1
 #define OPS3D_ROTARY_MAX_PAIRS 128
 #define OPS3D_ROTARY_MAX_AXES 8
+#define OPS3D_ROTARY_MAX_ITEMS 65535 /* of a call */
 
 /* Writes every channel of y.  strides: {item, token, head}. */
 OPS3D_FDA_API int ops3d_rotary(const void *x, const int64_t *x_strides, const void *positions, int position_type,

@@ -95,6 +95,7 @@ class _AttentionProblem(ctypes.Structure):
 
 
 MAX_SEQUENCES = 65536   # OPS3D_ATTENTION_MAX_SEQUENCES
+MAX_ROTARY_ITEMS = 65535   # OPS3D_ROTARY_MAX_ITEMS
 
 
 def _declare(lib: ctypes.CDLL) -> None:
@@ -574,14 +575,19 @@ class _NativeFDA:
             raise ValueError("there must be a frequency for each pair")
         xr, pos, n = self._channels_dense(x), positions.resolve_neg().contiguous(), len(axis_of)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        with torch.cuda.device(x.device):
-            rc = self._lib.ops3d_rotary(
-                _ptr(xr), self._strides(xr), _ptr(pos), int(pos.dtype == torch.int64),
-                tokens * pos.shape[-1] if pos.dim() == 3 else 0, (ctypes.c_double * n)(*frequencies), (_i * n)(*axis_of),
-                n, pos.shape[-1], int(layout), int(inverse), _ptr(y), self._strides(y), _DTYPE_CODE[x.dtype], items, tokens,
-                heads, dim, torch.cuda.current_stream(x.device).cuda_stream)
-        if rc != OPS3D_FDA_OK:
-            self._raise(rc, "rotary positions failed")
+        for at in range(0, max(1, items), MAX_ROTARY_ITEMS):   # some items a call
+            some = slice(at, at + MAX_ROTARY_ITEMS)
+            xi, yi, pi = xr, y, pos
+            if x.dim() == 4:
+                xi, yi, pi = xr[some], y[some], pos[some] if pos.dim() == 3 else pos
+            with torch.cuda.device(x.device):
+                rc = self._lib.ops3d_rotary(
+                    _ptr(xi), self._strides(xi), _ptr(pi), int(pos.dtype == torch.int64),
+                    tokens * pos.shape[-1] if pos.dim() == 3 else 0, (ctypes.c_double * n)(*frequencies), (_i * n)(*axis_of),
+                    n, pos.shape[-1], int(layout), int(inverse), _ptr(yi), self._strides(yi), _DTYPE_CODE[x.dtype],
+                    xi.shape[0] if x.dim() == 4 else 1, tokens, heads, dim, torch.cuda.current_stream(x.device).cuda_stream)
+            if rc != OPS3D_FDA_OK:
+                self._raise(rc, "rotary positions failed")
         return y
 
     # -- attention over all tokens (include/ops3d_attention.h) ----------------------------------

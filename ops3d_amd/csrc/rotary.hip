@@ -144,7 +144,7 @@ extern "C" int ops3d_rotary(const void *x, const int64_t *x_strides, const void 
   if (position_type != OPS3D_ROTARY_POSITION_F32 && position_type != OPS3D_ROTARY_POSITION_I64)
     return fail(OPS3D_FDA_EINVAL, "unknown position type %d", position_type);
   if (layout != OPS3D_ROTARY_HALVES && layout != OPS3D_ROTARY_PAIRS) return fail(OPS3D_FDA_EINVAL, "unknown layout %d", layout);
-  if (items < 0 || tokens < 0 || heads < 0 || items > 65535 || tokens > 0x7fffffff || heads > 65536)
+  if (items < 0 || tokens < 0 || heads < 0 || items > OPS3D_ROTARY_MAX_ITEMS || tokens > 0x7fffffff || heads > 65536)
     return fail(OPS3D_FDA_EINVAL, "invalid or too many items, tokens or heads: %d, %lld, %d", items, (long long)tokens, heads);
   if (dim < 1 || dim > 65536) return fail(OPS3D_FDA_EINVAL, "heads must have 1..65536 channels, got %d", dim);
   if ((int64_t)heads * dim > 1 << 24)

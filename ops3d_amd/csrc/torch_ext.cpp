@@ -16,6 +16,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -915,12 +916,19 @@ at::Tensor rotary_apply(const at::Tensor &x, const at::Tensor &positions, const 
   strides_of(xr, xs);
   strides_of(y, ys);
   const std::vector<int> axis(axis_of.begin(), axis_of.end());
-  const int rc = ops3d_rotary(ptr(xr), xs, ptr(pos), pos.scalar_type() == at::kFloat ? OPS3D_ROTARY_POSITION_F32 : OPS3D_ROTARY_POSITION_I64,
-                              pos.dim() == 3 ? tokens * pos.size(-1) : 0, frequencies.data(), axis.data(), (int)axis.size(),
-                              linear_int(pos.size(-1), "the number of axes"), (int)layout, inverse, ptr(y), ys, code,
-                              linear_int(items, "the number of items"), tokens, linear_int(heads, "the number of heads"),
-                              linear_int(dim, "the number of channels"), stream_of(x));
-  if (rc != OPS3D_FDA_OK) raise(rc, "rotary positions failed");
+  const int position_type = pos.scalar_type() == at::kFloat ? OPS3D_ROTARY_POSITION_F32 : OPS3D_ROTARY_POSITION_I64;
+  const int64_t pos_item = pos.dim() == 3 ? tokens * pos.size(-1) : 0, size = x.element_size();
+  const auto from = [](const at::Tensor &t, int64_t bytes) { return t.numel() ? static_cast<char *>(t.data_ptr()) + bytes : nullptr; };
+  int64_t item = 0;
+  do {   // some items a call
+    const int64_t n = std::min<int64_t>(items - item, OPS3D_ROTARY_MAX_ITEMS);
+    const int rc = ops3d_rotary(from(xr, item * xs[0] * size), xs, from(pos, item * pos_item * pos.element_size()), position_type, pos_item,
+                                frequencies.data(), axis.data(), (int)axis.size(), linear_int(pos.size(-1), "the number of axes"),
+                                (int)layout, inverse, from(y, item * ys[0] * size), ys, code, (int)n, tokens,
+                                linear_int(heads, "the number of heads"), linear_int(dim, "the number of channels"), stream_of(x));
+    if (rc != OPS3D_FDA_OK) raise(rc, "rotary positions failed");
+    item += n;
+  } while (item < items);
   return y;
 }
 

@@ -253,3 +253,20 @@ def test_refusals(gpu_device):
         torch.jit.trace(lambda t: rotary_positions(t, pos, (2, 2)), (x,), check_trace=False)
     with pytest.raises(Exception):
         torch.func.vmap(lambda t: rotary_positions(t, pos, (2, 2)))(x[None])
+
+
+@gpu
+@pytest.mark.parametrize("binding", ["module", "ctypes"])
+def test_more_items_than_a_call_takes(gpu_device, binding):
+    """Windows of a volume as a batch: more than the 65535 items that the C entry takes at once."""
+    native = _extension._C if binding == "module" else _extension._NativeFDA(_extension.load_library(), _extension.LIB_PATH)
+
+    def turn(x, positions, sections, layout):
+        from ops3d_amd.rotary import LAYOUTS, _pairs
+
+        return native.rotary(x, positions, *_pairs(sections, 10000.0), LAYOUTS[layout])
+
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = make(gen, (140000, 3, 9), torch.bfloat16)[:, :, :8].unflatten(-1, (1, 8))
+    compare(x, torch.randint(0, 99, (3, 2), generator=gen, device="cuda"), (2, 1), turn=turn)
+    compare(x, torch.randint(0, 99, (140000, 3, 2), generator=gen, device="cuda"), (2, 2), "pairs", turn=turn)
