@@ -203,3 +203,76 @@ def test_more_blocks_than_one_launch_has(gpu_device):
     q, k, v, u = (torch.randint(-3, 4, (items, 1, 8, 8), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16) for _ in range(4))
     y, dq, dk, dv = step(q, k, v, u)
     assert torch.equal(y, v) and torch.equal(dv, u) and not dq.any() and not dk.any()
+
+
+def wide(dtype, rows, runs, H, Hk):
+    """Blocks of 128 columns of queries, and of keys: from 512 on attention_capi.hip takes these tiles."""
+    return [-(-rows * g // 128) * runs * Hk for g in (H // Hk, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim,group", [(32, 1), (32, 3), (36, 1), (64, 4), (128, 1), (128, 3)])
+def test_tiles_of_128_columns(gpu_device, dim, group, causal, dtype):
+    """Many items of more than 128 tokens, with lengths and without."""
+    items, n, Hk = 32, 150, 8
+    assert min(wide(dtype, n, items, group * Hk, Hk)) >= 512
+    q, k, v, u = inputs(dtype, n, n, group * Hk, Hk, dim, lead=(items,), seed=dim)
+    for lens in (None, [(41 * i) % (n + 1) for i in range(items)]):
+        got = step(q, k, v, u, causal=causal, q_len=table(lens), k_len=table(lens))
+        want = ref.items(q, k, v, lens, lens, causal, dim ** -0.5, u)
+        for name, t in zip(("y", "dq", "dk", "dv"), got):
+            check(name, t, want[name])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sequences,dim,group,cross", [(40, 32, 3, True), (40, 64, 4, False), (40, 128, 1, True), (70, 32, 1, False), (70, 128, 1, True)])
+def test_packed_tiles_of_128_columns(gpu_device, sequences, dim, group, cross, causal, dtype):
+    """Sequences in the order of what they see, and looked up in a table."""
+    Hk, rows = 8, sequences * 150
+    assert min(wide(dtype, 150, sequences, group * Hk, Hk)) >= 512
+    gen = torch.Generator().manual_seed(dim)
+
+    def starts():
+        return [3] + sorted(torch.randint(3, rows - 5, (sequences - 1,), generator=gen).tolist()) + [rows - 5]
+
+    q_start = starts()
+    k_start = starts() if cross else q_start
+    q, k, v, u = inputs(dtype, rows, rows, group * Hk, Hk, dim, seed=dim)
+    got = step(q, k, v, u, causal=causal, q_start=table(q_start), k_start=table(k_start))
+    want = ref.packed(q, k, v, q_start, k_start, causal, dim ** -0.5, u)
+    for name, t in zip(("y", "dq", "dk", "dv"), got):
+        check(name, t, want[name])
+
+
+@gpu
+@pytest.mark.parametrize("sequences", [5, 70])
+def test_c_starts_without_the_last_end(gpu_device, sequences):
+    """From C: with `sequences` entries the last sequence ends with the rows."""
+    rows, H, D = 900, 2, 32
+    gen = torch.Generator().manual_seed(sequences)
+    start = [0] + sorted(torch.randint(0, rows, (sequences - 1,), generator=gen).tolist())
+    q, k, v, u = inputs("bf16", rows, rows, H, H, D)
+    native = _extension._NativeFDA(_extension.load_library(), _extension.LIB_PATH)
+    outs = []
+    for count in (sequences, sequences + 1):
+        at = table(start + [rows])[:count].clone()
+        p = native._attention_problem(q, k, v, table(start + [rows]), table(start + [rows]), None, None, True, 0.2)
+        assert p.sequences == sequences
+        p.q_start = p.k_start = at.data_ptr()
+        p.q_start_count = p.k_start_count = count
+        y, dq, dk, dv = (torch.full_like(q, math.nan) for _ in range(4))
+        lse, n = torch.empty(1, H, rows, device="cuda"), native._lib.ops3d_attention_forward_workspace_bytes(p)
+        m = native._lib.ops3d_attention_backward_workspace_bytes(p)
+        ws = torch.empty(max(n, m, 1), dtype=torch.uint8, device="cuda")
+        tq, tk, tv, ty, tu, tgq, tgk, tgv = (native._attention_tensor(t) for t in (q, k, v, y, u, dq, dk, dv))
+        stream = torch.cuda.current_stream().cuda_stream
+        assert native._lib.ops3d_attention_forward(p, tq, tk, tv, ty, None, lse.data_ptr(), ws.data_ptr(), n, stream) == 0
+        assert native._lib.ops3d_attention_backward(p, tq, tk, tv, ty, None, lse.data_ptr(), tu, tgq, tgk, tgv, ws.data_ptr(), m, stream) == 0
+        torch.cuda.synchronize()
+        outs.append((y, dq, dk, dv))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert torch.equal(outs[0][0], packed_attention(q, k, v, q_start=table(start + [rows]), causal=True, scale=0.2))
