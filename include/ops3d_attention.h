@@ -23,6 +23,13 @@
  * Entries are read on the device only: each counts as the largest of itself and those before it, held to
  * [0, rows].  Sequences may be empty.  Rows that do not count or are in no sequence are not read; their
  * outputs and gradients are 0.  Outputs and workspace must overlap neither each other nor an input.
+ *
+ * A query whose visible logits are all minus infinity, or of which one is NaN, gives NaN.  In fp16 probabilities and
+ * the gradients of logits are held times powers of two, the latter's chosen for each query and each key, so that they keep
+ * their precision where they are small and do not overflow where they are large.
+ *
+ * Limits: OPS3D_ATTENTION_MAX_DIM channels, OPS3D_ATTENTION_MAX_SEQUENCES packed sequences or 2^24 items, less than
+ * 2^31 - 65536 keys, and queries times the heads of a group, of an item.
  */
 #ifndef OPS3D_ATTENTION_H
 #define OPS3D_ATTENTION_H
@@ -55,8 +62,9 @@ typedef struct ops3d_attention_problem {
   float scale; /* positive */
 } ops3d_attention_problem;
 
-/* Bytes of device workspace (256-byte aligned) of the forward: partial results where few queries see many
- * keys; 0 for other and for invalid sizes. */
+/* Bytes of device workspace (256-byte aligned) of the forward, to be asked for each problem: partial results where
+ * the keys are cut into parts (few queries that see many keys; causal or packed problems of middling size), and the
+ * table of tiles of more than 64 packed sequences.  0 where neither is needed, and for invalid sizes. */
 OPS3D_FDA_API size_t ops3d_attention_forward_workspace_bytes(const ops3d_attention_problem *problem);
 
 /* Writes every channel of out.  For the backward, where not NULL: lse [items, heads, q_rows] fp32 (in an order of
@@ -67,8 +75,8 @@ OPS3D_FDA_API int ops3d_attention_forward(const ops3d_attention_problem *problem
                                           const ops3d_attention_tensor *out, void *out_rest, float *lse, void *workspace,
                                           size_t workspace_bytes, void *stream);
 
-/* Bytes of device workspace (256-byte aligned) of the backward: the products of out with grad_out, and
- * partial sums where few rows depend on many. */
+/* Bytes of device workspace (256-byte aligned) of the backward: the products of out with grad_out, partial sums
+ * where a side is cut into parts, and the table of tiles of more than 64 packed sequences. */
 OPS3D_FDA_API size_t ops3d_attention_backward_workspace_bytes(const ops3d_attention_problem *problem);
 
 /* Writes every channel of grad_q, grad_k and grad_v; grad_q may be NULL, and grad_k and grad_v together:

@@ -5,8 +5,8 @@ No counterpart in the reference, whose attention samples a few places of the val
 also needs this one.  The heads of a group share a key head, sequences of different lengths run packed one
 behind another or as items of a batch that use some of their rows, and lengths are read on the device
 only, so no call waits for them.  Logits, statistics and sums are fp32; probabilities and the gradients of
-logits are rounded to the tensors' dtype before they are multiplied; each result is rounded once.  For
-the backward the forward keeps, beside the output, what rounding took from it.
+logits are rounded to the tensors' dtype before they are multiplied (in float16 times powers of two, which keep
+them in its range); each result is rounded once.  For the backward the forward keeps, beside the output, what rounding took from it.
 Results are bitwise repeatable (csrc/attention_kernels.h).
 """
 from __future__ import annotations

@@ -19,7 +19,9 @@
 //
 // What bounds them (one MI355X, bf16, 8 heads; a large library product reaches 1184 TFLOP/s): with 32 channels a logit
 // is 128 operations on the matrix units and, beside them, an exponential, a multiply-add, a comparison and a rounding, and
-// the vector units are the bound; with 128 channels the matrix units and the LDS reads that feed them.
+// where all blocks are alike the vector units are the bound (79 % of the cycles).  Elsewhere nothing is full: with 128
+// channels the registers leave two waves a SIMD, which wait for their own loads and products (matrix units 33 to 39 % of the
+// cycles, vector units 26 to 39, LDS 38 at most).
 //   forward  4096 x 4096     32 / 64 / 96 / 128 channels   47 / 58 / 86 / 88 us   367 / 594 / 597 / 782 TFLOP/s
 //            32768 x 32768   32                            1700 us                647
 //   backward 4096 x 4096     32 / 64 / 96 / 128            124 / 158 / 250 / 263  347 / 543 / 515 / 653 (10 D a logit; 14 D
@@ -1022,9 +1024,9 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 // ---------------------------------------------------------------------------------------------
 // Gradients of keys and values.  A block owns keys, and queries, output gradients and their two statistics come by: the
 // heads of a group are rows like any other, so their sum is part of the product's.
-// 16411 tokens in 7 sequences, 8 heads of 32: 191 us (four products of 30 GF: 631 TFLOP/s; vector units 48 %, matrix units
-// 29 % of the cycles); 8192 causal tokens in 5 sequences, 16/4 heads of 128: 256 us and 16 for the join (25 and 32 %, LDS
-// 36 %: the operands of four products pass through it for 16 columns a wave, since K, V, dK and dV of 32 columns need
+// 16411 tokens in 7 sequences, 8 heads of 32: 185 us (four products of 30 GF: 650 TFLOP/s; vector units 55 %, matrix units
+// 32 % of the cycles); 8192 causal tokens in 5 sequences, 16/4 heads of 128: 257 us and 16 for the join (26 and 33 %, LDS
+// 38 %: the operands of four products pass through it for 16 columns a wave, since K, V, dK and dV of 32 columns need
 // more registers than two waves a SIMD have; with them 374 us where these tiles took 273 in one part).
 template <typename T, int DP, int NC, int WC, int WK, int QT, int OCC, bool DMA>
 __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC))) void grad_kv_kernel(Args p) {
