@@ -318,10 +318,6 @@ template <typename T, int DP, int R, int NT> struct Stage {
     for (int i = threadIdx.x * 16; i < bytes; i += NT * 16) *reinterpret_cast<uint4 *>(lds + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
-  // Zeros in rows from n on.  Called by all threads, between barriers.
-  static __device__ __forceinline__ void clear_rows(char *lds, int n) {
-    for (int i = n * RC + threadIdx.x; i < R * RC; i += NT) *reinterpret_cast<uint4 *>(lds + i * 16) = make_uint4(0, 0, 0, 0);
-  }
   static __device__ __forceinline__ void store(char *lds, const uint4 (&v)[NL]) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4 *>(lds + address(row_of(i), chunk_of(i))) = v[i];
@@ -1135,11 +1131,6 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
     if (DMA) ST::arrived();
     else __syncthreads();
     if (DMA && c0 + QT < c_end) load(c0 + QT, buf ^ 1);
-    if (DMA && c_end - c0 < QT) {   // copies of the last row, whose infinities times P = 0 would be NaN
-      ST::clear_rows(lds + buf * 2 * ST::kBytes, c_end - c0);
-      ST::clear_rows(lds + buf * 2 * ST::kBytes + ST::kBytes, c_end - c0);
-      __syncthreads();
-    }
 #pragma unroll
     for (int qt = 0; qt < QN; qt += PR) {
       f32x4 s[NC][PR], dp[NC][PR], lse[PR];
@@ -1171,7 +1162,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float x = exp2_(fmaf(s[n][u][j], p.c, lse[u][j])), y = x * dp[n][u][j];
-            if (decltype(masked)::value && r + j < since[n]) x = y = 0.f;
+            if (decltype(masked)::value && (r + j < since[n] || r + j >= c_end)) x = y = 0.f;
             s[n][u][j] = x;
             dp[n][u][j] = y;
           }
@@ -1189,7 +1180,7 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
             av[n][d] = Type<T>::mma(gf, pf[n], av[n][d]);
             ak[n][d] = Type<T>::mma(qf, ds[n], ak[n][d]);
           } else {
-            const auto seen = [&](int r) { return c0 + r0 + qt * 16 + r >= since[n]; };
+            const auto seen = [&](int r) { return c0 + r0 + qt * 16 + r >= since[n] && c0 + r0 + qt * 16 + r < c_end; };
             add_seen<T>(av[n][d], gf, pf[n], q, seen);
             add_seen<T>(ak[n][d], qf, ds[n], q, seen);
           }
@@ -1202,8 +1193,10 @@ __global__ __launch_bounds__(64 * WC *WK) __attribute__((amdgpu_waves_per_eu(OCC
   };
   if (DMA && p.D < DP) ST::clear(lds, 4 * ST::kBytes);
   if (c_begin < c_end) load(c_begin, 0);
-  while (c0 < c_end && c0 < all_see) stage(std::true_type());
-  while (c0 < c_end) stage(std::false_type());
+  while (c0 < c_end) {   // rows behind the last are hidden too: an infinite key times their zeros is NaN
+    while (c0 < c_end && (c0 < all_see || c_end - c0 < QT)) stage(std::true_type());
+    while (c0 >= all_see && c0 + QT <= c_end) stage(std::false_type());
+  }
   if constexpr (Range<T>::kScaled) {
 #pragma unroll
     for (int n = 0; n < NC; ++n)

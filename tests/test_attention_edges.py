@@ -109,6 +109,26 @@ def test_infinity_in_the_last_output_gradient(gpu_device, nq, nk, H, Hk, D, dtyp
 
 @gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nq,nk,H,Hk,D", [(1, 70, 2, 2, 32), (5, 70, 2, 1, 36), (70, 300, 6, 2, 64), (70, 300, 2, 2, 128), (9000, 70, 2, 2, 32), (333, 5000, 2, 2, 33)])
+def test_keys_whose_logits_are_all_minus_infinity(gpu_device, nq, nk, H, Hk, D, dtype):
+    """Such keys have no weight, and gradients of 0: rows behind the last query, zeros or not, are no queries of theirs."""
+    q, k, v, u = inputs(dtype, nq, nk, H, Hk, D, seed=nq)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    gone = [0, nk // 2, nk - 1]
+    k[gone, :, 0] = -math.inf
+    y, dq, dk, dv = step(q, k, v, u)
+    left = torch.ones(nk, dtype=torch.bool, device="cuda")
+    left[gone] = False
+    want = ref.sequence(q, k[left], v[left], False, D ** -0.5, u)
+    assert not dk[gone].any() and not dv[gone].any()
+    check("y", y, want["y"])
+    check("dq", dq[..., 1:], tuple(t[..., 1:] for t in want["dq"]))   # 0 times the infinity in the first channel
+    check("dk", dk[left], want["dk"])
+    check("dv", dv[left], want["dv"])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("nq,nk,H,Hk,D", [(5, 9, 2, 1, 32), (70, 150, 4, 2, 36), (1, 600, 2, 1, 64), (1, 8192, 4, 1, 64), (200, 9000, 8, 8, 32), (2600, 2600, 8, 8, 32)])
 def test_logits_that_are_all_minus_infinity(gpu_device, nq, nk, H, Hk, D, dtype):
     """Softmax of them is NaN, as their keys are: a query is only 0 where it sees no key."""
