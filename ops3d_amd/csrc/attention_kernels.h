@@ -443,10 +443,13 @@ __device__ __forceinline__ void add_seen(f32x4 &acc, const typename Type<T>::fra
 #pragma unroll 1
   for (int e = 0; e < 4 * N; ++e) {
     const int owner = e / N, j = e % N;
-    typename Type<T>::frag one;
+    typename Type<T>::frag one_a, one_b;   // this row's alone: another's infinity times 0 would be NaN
 #pragma unroll
-    for (int k = 0; k < N; ++k) one[k] = k == j && q == owner ? a[k] : (T)0.f;
-    const f32x4 x = Type<T>::mma(one, b, splat(0.f));
+    for (int k = 0; k < N; ++k) {
+      one_a[k] = k == j && q == owner ? a[k] : (T)0.f;
+      one_b[k] = k == j && q == owner ? b[k] : (T)0.f;
+    }
+    const f32x4 x = Type<T>::mma(one_a, one_b, splat(0.f));
     if (seen((j >> 2) * 16 + owner * 4 + (j & 3))) acc += x;
   }
 }

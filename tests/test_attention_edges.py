@@ -182,6 +182,25 @@ def test_infinite_outputs_and_their_gradients(gpu_device, nk, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("nq,nk,D,causal", [(1, 20, 32, False), (5, 90, 33, False), (70, 70, 32, True), (300, 400, 64, True), (300, 300, 128, True), (5, 5000, 32, True)])
+def test_infinite_gradients_beside_finite_ones(gpu_device, nq, nk, D, causal, dtype):
+    """One head of one query has an infinite output gradient, that of the first key's logit is minus infinity: the key's
+    gradient is an infinity of the query's sign, whatever the other rows of the tile are, hidden ones among them."""
+    q, k, v, u = inputs(dtype, nq, nk, 2, 1, D, seed=nq)
+    row = nq // 2
+    last = nk - nq + row if causal else nk - 1   # the last key that it sees
+    v[:, 0, 1] = v[:, 0, 1].abs() + 0.25
+    v[0, 0, 1] = -0.01
+    u[row, 1, 1] = math.inf
+    _, dq, dk, dv = step(q, k, v, u, causal=causal)
+    assert torch.equal(dk[0, 0], -torch.sign(q[row, 1]) * math.inf)
+    assert dk[1:last + 1].isnan().all() and torch.isfinite(dk[last + 1:]).all()
+    assert (dv[:last + 1, 0, 1] == math.inf).all() and torch.isfinite(dv[last + 1:]).all() and torch.isfinite(dv[:, 0, 2:]).all()
+    assert dq[row, 1].isnan().all() and torch.isfinite(dq).sum() == dq.numel() - D
+
+
+@gpu
 @pytest.mark.parametrize("nq,nk,H,Hk,D,causal", [(50, 6000, 2, 1, 32, False), (700, 700, 4, 2, 64, True), (6000, 50, 2, 2, 32, False), (300, 300, 2, 1, 128, False),
                                                  (300, 400, 3, 1, 36, True), (9000, 9000, 8, 8, 32, True), (1, 8192, 8, 2, 128, False)])
 @pytest.mark.parametrize("size", [1e-4, 1.0, 2000.0])
