@@ -480,7 +480,7 @@ struct Scale {
     most = ops3d_reduce::across32<ops3d_reduce::Max>(ops3d_reduce::across16<ops3d_reduce::Max>(most));
     if (!(most > top)) return;
     const int e = 9 - __builtin_amdgcn_frexp_expf(fminf(most, 0x1p127f));   // the power's exponent
-    const float now = __uint_as_float((uint32_t)(127 + 15 - max(-112, min(100, e))) << 23), change = top * __uint_as_float(0x7f000000u - __float_as_uint(now));   // powers of two, or 0
+    const float now = __uint_as_float((uint32_t)(127 + 15 - max(-111, min(100, e))) << 23), change = top * __uint_as_float(0x7f000000u - __float_as_uint(now));   // powers of two, 1 over now not 0
 #pragma unroll
     for (int i = 0; i < N; ++i) sums[i] *= change;
     top = now;

@@ -235,6 +235,23 @@ def test_fp16_gradients_that_grow_along_the_sum(gpu_device):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n,D", [(70, 33), (200, 36), (700, 64), (300, 128)])
+def test_infinite_gradients_again_and_again(gpu_device, n, D, dtype):
+    """Of several queries far apart: the sums, infinities by then, are scaled no further."""
+    q, k, v, u = inputs(dtype, n, n, 1, 1, D, seed=n)
+    q = q.abs() + 0.25
+    v[:, 0, 1] = v[:, 0, 1].abs() + 0.25
+    v[0, 0, 1] = -0.01
+    rows = [2, n // 2, n - 1]
+    u[rows, 0, 1] = math.inf
+    _, dq, dk, dv = step(q, k, v, u)
+    assert (dk[0] == -math.inf).all() and dk[1:].isnan().all()
+    assert (dv[:, 0, 1] == math.inf).all() and torch.isfinite(dv).sum() == dv.numel() - n
+    assert dq[rows].isnan().all() and torch.isfinite(dq).sum() == dq.numel() - 3 * D
+
+
+@gpu
 def test_more_blocks_than_one_launch_has(gpu_device):
     """2^24 blocks of 256 threads and some: items of one token, whose result is the value."""
     items = (1 << 21) + 5
